@@ -50,6 +50,9 @@ typedef enum {                     /* ggml_type ids */
     MI_TYPE_Q4_K = 12,             /* 144 B / 256 values, convert/q4k.py:9-10  */
     MI_TYPE_Q6_K = 14,             /* 210 B / 256 values, convert/q6k.py:10-11 */
     MI_TYPE_I32  = 26,
+    MI_TYPE_MXFP4 = 39,            /*  17 B / 32 values: e E8M0 | qs[16] E2M1 codes (value j: low nibble of
+                                       qs[j], 16 + j: high); x = 2^(e - 127) +-{0, .5, 1, 1.5, 2, 3, 4, 6};
+                                       e = 255: NaN */
 } mi_type;
 
 typedef enum {                     /* activation between the two expert products */
@@ -79,7 +82,8 @@ typedef enum {
 
 /* Expert tables of one layer come from one family: the k-quants (Q4_K, Q6_K),
  * the 32-value formats with F16 (Q4_0, Q5_0, Q8_0, F16; rows of a multiple
- * of 32 values, F16 tables 16-byte aligned), or F32.
+ * of 32 values, F16 tables 16-byte aligned), MXFP4 (rows of a multiple of 32
+ * values, any alignment and strides), or F32.
  * ggml_tensor stand-in: data on the device, ne fastest-first, nb in bytes. */
 typedef struct {
     void    *data;
@@ -289,9 +293,13 @@ int mi_top_k(mi_moe_ctx *ctx, const mi_tensor *a, int32_t k, mi_tensor *dst, mi_
  * ids I32 ne=[n_used, T]) -> F32 ne=[N, n_used, T]
  * (moondream.cpp:519,537; qwen3omni_model.cpp:769-774; moe_compute.cpp:124-130).
  * dst[:, k, t] = as[:, :, ids[k,t]] . b[:, k % ne11, t].  as types: Q4_K,
- * Q6_K, Q4_0, Q5_0, Q8_0, F16, F32.  b is first converted to the type's ggml
- * vec_dot_type, like ggml-cpu: Q8_K for k-quants, Q8_0 for the 32-value
- * formats, fp16 for F16 (F32 tables take b as given).
+ * Q6_K, Q4_0, Q5_0, Q8_0, F16, MXFP4, F32.  b is first converted to the type's
+ * ggml vec_dot_type, like ggml-cpu: Q8_K for k-quants, Q8_0 for the 32-value
+ * formats and MXFP4, fp16 for F16 (F32 tables take b as given).  MXFP4: the
+ * products of the codes are exact and summed in fp64 (few rows per expert) or
+ * fp32; a dst value is NaN where its table row holds a NaN block or its b row
+ * a NaN, an infinity or a block whose Q8_0 scale leaves the fp16 range (|x|
+ * above 8.3e6).
  * Ids must lie in [0, E): the dst row of an id outside is written as zeros
  * and the id is counted for mi_moe_ctx_take_errors. */
 int mi_mul_mat_id(mi_moe_ctx *ctx, const mi_tensor *as, const mi_tensor *b, const mi_tensor *ids,
@@ -305,9 +313,20 @@ int mi_mul_mat_id(mi_moe_ctx *ctx, const mi_tensor *as, const mi_tensor *b, cons
  * quantizers, convert/_lib.py:120-130).  src: F32 [nrows][n_per_row] device
  * (n_per_row a multiple of 256 for k-quants, of 32 otherwise), dst: nrows *
  * row_size bytes device.  Byte-identical to the CPU restatement of ggml's
- * reference quantizers. */
+ * reference quantizers.
+ * MXFP4: a block's scale byte is the exponent of its largest |x| less 2 (0
+ * where that is below 2^-125 or zero), a value's code the nearest step, the
+ * smaller of two that are equally near, 6 above 6; a block that holds an
+ * infinity or a NaN is a NaN block (scale byte 255, codes 0). */
 int mi_quantize(mi_moe_ctx *ctx, int32_t type, const float *src, void *dst, int64_t nrows,
                 int64_t n_per_row, mi_stream_t stream);
+
+/* The values that rows of a table stand for (ggml's to_float of the type):
+ * src: nrows rows of row_size bytes device, dst: F32 [nrows][n_per_row] device,
+ * not overlapping src.  Types MXFP4, Q4_0, Q5_0, Q8_0 and F16 (n_per_row a
+ * multiple of 32); others MI_MOE_ERR_TYPE. */
+int mi_dequantize(mi_moe_ctx *ctx, int32_t type, const void *src, float *dst, int64_t nrows,
+                  int64_t n_per_row, mi_stream_t stream);
 
 /* ---- tiled copies of expert tables ------------------------------------------
  * Load-time copies of Q4_K and Q6_K expert tables in the grouped GEMMs' order,
@@ -369,8 +388,8 @@ int  mi_gguf_tensor_info(const mi_gguf *gguf, const char *name, int32_t *type, i
 /* block `block`'s MoE layer uploaded to the current device in one allocation
  * (*device_buffer; free it with mi_dev_free when the layer is no longer
  * used): router (F32), bias if present, expert tables as stored (Q4_K,
- * Q6_K, Q8_0, Q5_0, Q4_0, F16 or F32: one family per layer, the k-quants,
- * the 32-value formats with F16, or F32), K from
+ * Q6_K, Q8_0, Q5_0, Q4_0, F16, MXFP4 or F32: one family per layer, the
+ * k-quants, the 32-value formats with F16, MXFP4, or F32), K from
  * <general.architecture>.expert_used_count, fused
  * [h | g] when the block has no ffn_gate_exps.  act: mi_act (the
  * architecture's choice: moondream3 MI_ACT_GELU_ERF_GP1, qwen3omni
@@ -396,7 +415,7 @@ int mi_moe_ctx_stage_clock(mi_moe_ctx *ctx, const char *stage, double *ghz, int 
  * k-quant layers the GEMM when 2 * T * K >= E (from half a dispatched row
  * per expert); for Q4_0 / Q5_0 layers and mi_mul_mat_id when 4 * T * K > 5 * E
  * (more than 1.25 rows per expert), for Q8_0 / F16 layers when 2 * T * K >
- * 3 * E (more than 1.5). */
+ * 3 * E (more than 1.5), for MXFP4 when T * K > 2 * E. */
 int mi_moe_ctx_set_gemm_threshold(mi_moe_ctx *ctx, int64_t min_tokens_for_gemm);
 /* Row tiles of the grouped GEMMs.  Of Q4_K gate/up layers: 0 (the default) by
  * shape, 32-row tiles when the call dispatches at most 8 rows per expert on

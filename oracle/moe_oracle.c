@@ -634,6 +634,56 @@ float orc_vec_dot_q8_0_q8_0(int n, const void *vx, const void *vy) {
     return sumf;
 }
 
+/* MXFP4: the E2M1 steps, doubled */
+static const int mxfp4_twice[16] = {0, 1, 2, 3, 4, 6, 8, 12, 0, -1, -2, -3, -4, -6, -8, -12};
+
+void orc_quantize_row_mxfp4(const float *x, void *vy, int64_t k) {
+    orc_block_mxfp4 *y = (orc_block_mxfp4 *)vy;
+    for (int64_t i = 0; i < k / ORC_QK32; i++, x += ORC_QK32) {
+        float amax = 0.0f;
+        int finite = 1;
+        for (int j = 0; j < ORC_QK32; j++) {
+            if (!isfinite(x[j])) finite = 0;
+            if (fabsf(x[j]) > amax) amax = fabsf(x[j]);
+        }
+        memset(y[i].qs, 0, sizeof(y[i].qs));
+        int ex = 0;
+        if (amax > 0.0f) (void)frexpf(amax, &ex);   /* amax = f 2^ex, f in [1/2, 1) */
+        int e = amax > 0.0f ? ex - 1 - 2 + 127 : 0;
+        y[i].e = (uint8_t)(!finite ? 255 : e < 0 ? 0 : e);
+        if (!finite) continue;
+        const double step = ldexp(0.5, (int)y[i].e - 127);
+        for (int j = 0; j < ORC_QK32; j++) {
+            int best = 0;
+            for (int c = 1; c < 8; c++)
+                if (fabs(fabs((double)x[j]) - mxfp4_twice[c] * step) < fabs(fabs((double)x[j]) - mxfp4_twice[best] * step)) best = c;
+            if (best && x[j] < 0.0f) best |= 8;
+            y[i].qs[j & 15] |= (uint8_t)(best << (j >= 16 ? 4 : 0));
+        }
+    }
+}
+
+void orc_dequantize_row_mxfp4(const void *vx, float *y, int64_t k) {
+    const orc_block_mxfp4 *x = (const orc_block_mxfp4 *)vx;
+    for (int64_t i = 0; i < k / ORC_QK32; i++)
+        for (int j = 0; j < ORC_QK32; j++) {
+            const int c = (x[i].qs[j & 15] >> (j >= 16 ? 4 : 0)) & 15;
+            y[i * ORC_QK32 + j] = x[i].e == 255 ? NAN : (float)ldexp(0.5 * mxfp4_twice[c], (int)x[i].e - 127);
+        }
+}
+
+float orc_vec_dot_mxfp4_q8_0(int n, const void *vx, const void *vy) {
+    const orc_block_mxfp4 *x = (const orc_block_mxfp4 *)vx;
+    const orc_block_q8_0 *y = (const orc_block_q8_0 *)vy;
+    double sum = 0.0;
+    for (int ib = 0; ib < n / ORC_QK32; ++ib) {
+        int s = 0;
+        for (int j = 0; j < ORC_QK32; j++) s += mxfp4_twice[(x[ib].qs[j & 15] >> (j >= 16 ? 4 : 0)) & 15] * y[ib].qs[j];
+        sum += (x[ib].e == 255 ? NAN : ldexp(0.5 * s, (int)x[ib].e - 127)) * (double)orc_fp16_to_fp32(y[ib].d);
+    }
+    return (float)sum;
+}
+
 float orc_vec_dot_f16(int n, const uint16_t *x, const uint16_t *y) {
     double sumf = 0.0;
     for (int i = 0; i < n; ++i) sumf += (double)(orc_fp16_to_fp32(x[i]) * orc_fp16_to_fp32(y[i]));
@@ -650,6 +700,7 @@ size_t orc_row_size(int type, int64_t k) {
     case ORC_TYPE_Q4_0: return (size_t)(k / ORC_QK32) * sizeof(orc_block_q4_0);
     case ORC_TYPE_Q5_0: return (size_t)(k / ORC_QK32) * sizeof(orc_block_q5_0);
     case ORC_TYPE_Q8_0: return (size_t)(k / ORC_QK32) * sizeof(orc_block_q8_0);
+    case ORC_TYPE_MXFP4: return (size_t)(k / ORC_QK32) * sizeof(orc_block_mxfp4);
     default: return 0;
     }
 }
@@ -666,6 +717,7 @@ void orc_quantize_rows(int type, const float *x, void *y, int64_t nrows, int64_t
         else if (type == ORC_TYPE_Q4_0) orc_quantize_row_q4_0(xr, yr, k);
         else if (type == ORC_TYPE_Q5_0) orc_quantize_row_q5_0(xr, yr, k);
         else if (type == ORC_TYPE_Q8_0) orc_quantize_row_q8_0(xr, yr, k);
+        else if (type == ORC_TYPE_MXFP4) orc_quantize_row_mxfp4(xr, yr, k);
         else if (type == ORC_TYPE_F16) {
             uint16_t *h = (uint16_t *)yr;
             for (int64_t i = 0; i < k; i++) h[i] = orc_fp32_to_fp16(xr[i]);
@@ -1181,6 +1233,7 @@ static void dequant_row_any(int type, const void *row, float *out, int64_t k) {
     else if (type == ORC_TYPE_Q4_0) orc_dequantize_row_q4_0(row, out, k);
     else if (type == ORC_TYPE_Q5_0) orc_dequantize_row_q5_0(row, out, k);
     else if (type == ORC_TYPE_Q8_0) orc_dequantize_row_q8_0(row, out, k);
+    else if (type == ORC_TYPE_MXFP4) orc_dequantize_row_mxfp4(row, out, k);
     else if (type == ORC_TYPE_F16) {
         const uint16_t *h = (const uint16_t *)row;
         for (int64_t i = 0; i < k; i++) out[i] = orc_fp16_to_fp32(h[i]);
@@ -1194,7 +1247,8 @@ int orc_mul_mat_id(int type, const void *as, int64_t Kin, int64_t N, int E,
         return -1;
     if (ne11 != 1 && ne11 != n_used) return -1;
     const int kq = (type == ORC_TYPE_Q4_K || type == ORC_TYPE_Q6_K);
-    const int b32 = (type == ORC_TYPE_Q4_0 || type == ORC_TYPE_Q5_0 || type == ORC_TYPE_Q8_0);
+    const int b32 = (type == ORC_TYPE_Q4_0 || type == ORC_TYPE_Q5_0 || type == ORC_TYPE_Q8_0 ||
+                     type == ORC_TYPE_MXFP4);
     const int f16 = type == ORC_TYPE_F16;
     if (kq && (Kin % QK_K)) return -1;
     if (b32 && (Kin % ORC_QK32)) return -1;
@@ -1268,6 +1322,7 @@ int orc_mul_mat_id(int type, const void *as, int64_t Kin, int64_t N, int E,
                         } else if (b32) {
                             const void *yb = bq0 + brow * (Kin / ORC_QK32);
                             v = type == ORC_TYPE_Q8_0   ? orc_vec_dot_q8_0_q8_0((int)Kin, wr, yb)
+                                : type == ORC_TYPE_MXFP4 ? orc_vec_dot_mxfp4_q8_0((int)Kin, wr, yb)
                                 : type == ORC_TYPE_Q5_0 ? orc_vec_dot_q5_0_q8_0((int)Kin, wr, yb)
                                                         : orc_vec_dot_q4_0_q8_0((int)Kin, wr, yb);
                         } else if (f16) {

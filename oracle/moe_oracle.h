@@ -54,6 +54,7 @@ enum {
     ORC_TYPE_Q6_K = 14,
     ORC_TYPE_Q8_K = 15,
     ORC_TYPE_I32  = 26,
+    ORC_TYPE_MXFP4 = 39,
 };
 
 /* block layouts: convert/q4k.py:9-10, convert/q6k.py:10-11 */
@@ -98,6 +99,11 @@ typedef struct {
     uint16_t d;          /* fp16 scale */
     int8_t   qs[32];     /* x = d q */
 } orc_block_q8_0;        /* 34 bytes */
+
+typedef struct {
+    uint8_t  e;          /* E8M0 scale 2^(e - 127), 255: NaN */
+    uint8_t  qs[16];     /* E2M1 codes: value j low nibble of qs[j], value j+16 high nibble */
+} orc_block_mxfp4;       /* 17 bytes */
 #pragma pack(pop)
 
 enum {                    /* activation applied between the two expert products */
@@ -178,6 +184,12 @@ int orc_set_simd(int on);
 float orc_vec_dot_q4_0_q8_0(int n, const void *x, const void *y);
 float orc_vec_dot_q5_0_q8_0(int n, const void *x, const void *y);
 float orc_vec_dot_q8_0_q8_0(int n, const void *x, const void *y);
+/* MXFP4 (ggml type 39).  Quantizer: scale exponent floor(log2 amax) - 2, nearest
+ * step with ties to the smaller; a block with a non-finite value: e = 255, codes
+ * 0.  Dot with Q8_0: the exact block sums added in double, rounded once. */
+void orc_quantize_row_mxfp4(const float *x, void *y, int64_t k);
+void orc_dequantize_row_mxfp4(const void *x, float *y, int64_t k);
+float orc_vec_dot_mxfp4_q8_0(int n, const void *x, const void *y);
 float orc_vec_dot_f16(int n, const uint16_t *x, const uint16_t *y);
 
 /* ---- seeded synthetic data ----------------------------------------------

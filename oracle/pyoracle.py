@@ -17,17 +17,18 @@ HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "_build" / "liboracle.so"
 
 TYPE_F32, TYPE_F16, TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_K, TYPE_I32 = 0, 1, 12, 14, 15, 26
-TYPE_Q4_0, TYPE_Q5_0, TYPE_Q8_0 = 2, 6, 8
+TYPE_Q4_0, TYPE_Q5_0, TYPE_Q8_0, TYPE_MXFP4 = 2, 6, 8, 39
 ACT_SILU, ACT_GELU_ERF_GP1, ACT_GELU_TANH, ACT_GELU_ERF = 0, 1, 2, 3
 QK_K = 256
 QK32 = 32
-BLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q6_K: 210, TYPE_Q8_K: 292, TYPE_Q4_0: 18, TYPE_Q5_0: 22, TYPE_Q8_0: 34}
+BLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q6_K: 210, TYPE_Q8_K: 292, TYPE_Q4_0: 18, TYPE_Q5_0: 22, TYPE_Q8_0: 34,
+               TYPE_MXFP4: 17}
 B32_TYPES = (TYPE_Q4_0, TYPE_Q5_0, TYPE_Q8_0)
 
 
 def block_values(type_: int) -> int:
     """values per block of a quantized type (1 for F32 / F16)"""
-    return QK32 if type_ in B32_TYPES else QK_K if type_ in (TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_K) else 1
+    return QK32 if type_ in B32_TYPES + (TYPE_MXFP4,) else QK_K if type_ in (TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_K) else 1
 
 _lib = None
 
@@ -64,9 +65,9 @@ def _declare(L: C.CDLL) -> None:
     L.orc_quantize_row_q6_K.argtypes = [P, P, i64, C.c_int]
     L.orc_quantize_row_q8_K.argtypes = [P, P, i64]
     L.orc_quantize_rows.argtypes = [C.c_int, P, P, i64, i64, C.c_int]
-    for n in ("q4_K", "q6_K", "q8_K", "q4_0", "q5_0", "q8_0"):
+    for n in ("q4_K", "q6_K", "q8_K", "q4_0", "q5_0", "q8_0", "mxfp4"):
         getattr(L, f"orc_dequantize_row_{n}").argtypes = [P, P, i64]
-    for n in ("q4_0", "q5_0", "q8_0"):
+    for n in ("q4_0", "q5_0", "q8_0", "mxfp4"):
         getattr(L, f"orc_quantize_row_{n}").argtypes = [P, P, i64]
         getattr(L, f"orc_vec_dot_{n}_q8_0").argtypes = [C.c_int, P, P]
         getattr(L, f"orc_vec_dot_{n}_q8_0").restype = C.c_float
@@ -159,7 +160,8 @@ def dequantize(type_: int, q: np.ndarray, k: int) -> np.ndarray:
         return rows.view(np.float16).astype(np.float32).reshape(*q.shape[:-1], k)
     fn = {TYPE_Q4_K: lib().orc_dequantize_row_q4_K, TYPE_Q6_K: lib().orc_dequantize_row_q6_K,
           TYPE_Q8_K: lib().orc_dequantize_row_q8_K, TYPE_Q4_0: lib().orc_dequantize_row_q4_0,
-          TYPE_Q5_0: lib().orc_dequantize_row_q5_0, TYPE_Q8_0: lib().orc_dequantize_row_q8_0}[type_]
+          TYPE_Q5_0: lib().orc_dequantize_row_q5_0, TYPE_Q8_0: lib().orc_dequantize_row_q8_0,
+          TYPE_MXFP4: lib().orc_dequantize_row_mxfp4}[type_]
     for r in range(rows.shape[0]):
         fn(_p(rows[r]), _p(out[r]), k)
     return out.reshape(*q.shape[:-1], k)
@@ -171,7 +173,8 @@ def vec_dot(type_: int, wrow: np.ndarray, q8row: np.ndarray, k: int) -> float:
     fp16 values for F16)"""
     fn = {TYPE_Q4_K: lib().orc_vec_dot_q4_K_q8_K, TYPE_Q6_K: lib().orc_vec_dot_q6_K_q8_K,
           TYPE_Q4_0: lib().orc_vec_dot_q4_0_q8_0, TYPE_Q5_0: lib().orc_vec_dot_q5_0_q8_0,
-          TYPE_Q8_0: lib().orc_vec_dot_q8_0_q8_0, TYPE_F16: lib().orc_vec_dot_f16}[type_]
+          TYPE_Q8_0: lib().orc_vec_dot_q8_0_q8_0, TYPE_F16: lib().orc_vec_dot_f16,
+          TYPE_MXFP4: lib().orc_vec_dot_mxfp4_q8_0}[type_]
     return fn(k, _p(np.ascontiguousarray(wrow)), _p(np.ascontiguousarray(q8row)))
 
 

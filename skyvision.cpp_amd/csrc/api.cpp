@@ -25,6 +25,7 @@
 #include "../../include/mi_moe_util.h"
 #include "common.hpp"
 #include "launch.hpp"
+#include "mx.hpp"
 #include "wave_ops.hpp"
 
 namespace mimoe {
@@ -165,8 +166,10 @@ bool is_kquant(int t) { return t == MI_TYPE_Q4_K || t == MI_TYPE_Q6_K; }
 // 32-value block formats and F16: the k_b32.hip kernels
 bool is_b32(int t) { return t == MI_TYPE_Q4_0 || t == MI_TYPE_Q5_0 || t == MI_TYPE_Q8_0; }
 bool is_b32f(int t) { return is_b32(t) || t == MI_TYPE_F16; }
-// the table families one layer's products may mix: 0 F32, 1 k-quants, 2 the b32 / F16 family
-int type_family(int t) { return is_kquant(t) ? 1 : is_b32f(t) ? 2 : 0; }
+// MXFP4: the k_mx.hip / k_mxg.hip kernels
+bool is_mx(int t) { return t == MI_TYPE_MXFP4; }
+// the table families one layer's products may mix: 0 F32, 1 k-quants, 2 the b32 / F16 family, 3 MXFP4
+int type_family(int t) { return is_kquant(t) ? 1 : is_b32f(t) ? 2 : is_mx(t) ? 3 : 0; }
 
 size_t type_row_size(int32_t type, int64_t n) {
     switch (type) {
@@ -177,6 +180,7 @@ size_t type_row_size(int32_t type, int64_t n) {
     case MI_TYPE_Q4_0: return n % 32 ? 0 : (size_t)(n / 32) * 18;
     case MI_TYPE_Q5_0: return n % 32 ? 0 : (size_t)(n / 32) * 22;
     case MI_TYPE_Q8_0: return n % 32 ? 0 : (size_t)(n / 32) * 34;
+    case MI_TYPE_MXFP4: return n % 32 ? 0 : (size_t)(n / 32) * MX_BYTES;
     default: return 0;
     }
 }
@@ -184,8 +188,8 @@ size_t type_row_size(int32_t type, int64_t n) {
 // an expert table ne=[K, N, E] with ggml strides
 int check_table(const mi_tensor &t, int64_t K, int64_t N, int64_t E) {
     if (!t.data) return MI_MOE_ERR_NULL;
-    if (!is_kquant(t.type) && !is_b32f(t.type) && t.type != MI_TYPE_F32) return MI_MOE_ERR_TYPE;
-    if (is_b32f(t.type) && K % 32) return MI_MOE_ERR_UNSUPPORTED;   // whole 32-value blocks (F16: the kernels' unit)
+    if (!is_kquant(t.type) && !is_b32f(t.type) && !is_mx(t.type) && t.type != MI_TYPE_F32) return MI_MOE_ERR_TYPE;
+    if ((is_b32f(t.type) || is_mx(t.type)) && K % 32) return MI_MOE_ERR_UNSUPPORTED;   // whole 32-value blocks (F16: the kernels' unit)
     if (t.ne[0] != K || t.ne[1] != N || t.ne[2] < E || t.ne[3] != 1) return MI_MOE_ERR_SHAPE;
     const size_t rs = type_row_size(t.type, K);
     if (rs == 0) return MI_MOE_ERR_SHAPE;
@@ -758,6 +762,95 @@ int run_experts_b32(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_
     return MI_MOE_OK;
 }
 
+// The operand rows (mx.hpp) of `rows` rows of K values in an activation set:
+// its code, scale, block-sum and fp16 arrays are one run of 1 + 1/64 + 1/8 + 2
+// bytes per value (carve_workspace), the operand takes 3 + 1/8.
+MxRows mx_rows(void *base, int64_t rows, int64_t K) {
+    MxRows m;
+    m.xb = (uint8_t *)base;
+    m.xs = (uint32_t *)(m.xb + rows * (K / 32) * MX_XB);
+    return m;
+}
+
+// MXFP4: the grouped GEMM above two dispatched rows per expert
+bool use_gemm_mx(const mi_moe_ctx *c, int64_t T, int K, int E) {
+    if (c->gemm_threshold > 0) return T >= c->gemm_threshold;
+    return T * K > 2 * (int64_t)E;
+}
+// The shared expert in the routed experts' launches of few rows: the same
+// table type and activation.
+bool mx_shared_ok(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
+    return is_mx(L->gate.type) && is_mx(L->sh_gate.type) && is_mx(L->sh_down.type) && L->sh_act == L->act &&
+           !use_gemm_mx(c, T, L->n_expert_used, L->n_expert) && T <= GV_SHARED_T;
+}
+
+// routed FFN body of a layer with MXFP4 tables: Q8_0 operand rows (mx.hpp),
+// fp32 slot rows into the combine.  Few rows per expert (k_mx.hip), else the
+// grouped GEMM (k_mxg.hip); the gate/up launch of either writes the down
+// product's operand rows itself.  Arguments as run_experts_b32.
+int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T, const int32_t *ids_gu,
+                   const int32_t *ids_dn, const float *w, const float *res, float *out, hipStream_t st, bool check_ids,
+                   const float *add, bool disp_out, bool sh_here, const float *sh_w) {
+    const int D = L->n_embd, E = L->n_expert, K = L->n_expert_used, I = L->n_ff;
+    const int64_t rows = T * K;
+    const int max_active = (int)std::min<int64_t>(E, rows);
+    const bool same_ids = ids_gu == ids_dn;
+    const bool gated = act_gated(L->act);
+    const bool gemm = use_gemm_mx(c, T, K, E);
+    // few rows: the work-groups find their rows from the router's ids
+    // themselves, unless the caller wants the dispatch's outputs
+    const bool self_disp = !gemm && same_ids && !check_ids && !disp_out && rows <= MXV_IDS;
+    if (!self_disp) {
+        TRY(launch_dispatch(ids_gu, T, K, E, MXG_BM, 1, c->disp[0].view(), st));
+        if (!same_ids) TRY(launch_dispatch(ids_dn, T, K, E, MXG_BM, 1, c->disp[1].view(), st));
+    }
+    const DispBuf &dg = c->disp[0];
+    const DispBuf &dd = same_ids ? c->disp[0] : c->disp[1];
+    stage_end(c, "dispatch", st);
+    const MxRows mx = mx_rows(c->ax.q8, T, D), ma = mx_rows(c->aact.q8, rows, I);
+    TRY(launch_prep_mx(x, D, T, D, mx, st));
+    stage_end(c, "q8_x", st);
+    auto args_for = [&](const ExpertMat &t, const DispBuf &d, int ne11) {
+        MxArgs g = {};
+        g.a = t; g.ne11 = ne11; g.K = K; g.act = L->act;
+        g.perm = d.perm; g.counts = d.counts; g.offsets = d.offsets; g.active_e = d.active_e; g.n_active = d.n_active;
+        g.max_active = max_active;
+        g.tile_e = d.tile_e; g.tile_start = d.tile_start; g.tile_rows = d.tile_rows; g.n_tiles = d.n_tiles;
+        g.max_tiles = (int)((rows + MXG_BM - 1) / MXG_BM + max_active);
+        if (self_disp) { g.ids = ids_gu; g.rows = rows; g.n_expert = E; }
+        return g;
+    };
+    MxArgs a = args_for(as_mat(L->gate), dg, 1);
+    if (gated && !L->fused_gate_up) a.b = as_mat(L->up);
+    a.epi = gated ? MX_GLU : MX_RELU_SQR; a.fused = L->fused_gate_up; a.I = I;
+    a.x = mx; a.o = ma; a.ncols = I;
+    a.bad_total = c->bad_total;   // (with ids: once per call, here)
+    MxArgs d = args_for(as_mat(L->down), dd, K);
+    d.epi = MX_STORE; d.x = ma; d.y = c->z; d.ldy = D; d.ncols = D;
+    if (sh_here) {
+        const int64_t S = L->sh_n_ff;
+        a.sh_rows = d.sh_rows = T;
+        a.sh.a = as_mat(L->sh_gate);
+        if (gated) a.sh.b = as_mat(L->sh_up);
+        a.sh.I = a.sh.ncols = S;
+        a.sh.x = mx;
+        a.sh.o = d.sh.x = mx_rows(c->f1, T, S);   // (f1 is free on this path, and holds 2 cap_I floats per slot)
+        d.sh.a = as_mat(L->sh_down);
+        d.sh.y = c->sh_out; d.sh.ldy = d.sh.ncols = D;
+        d.sh_w = sh_w;
+        add = c->sh_out;
+    }
+    TRY(gemm ? launch_mxg(a, st) : launch_mxv(a, st));
+    stage_end(c, "gate_up", st);
+    TRY(gemm ? launch_mxg(d, st) : launch_mxv(d, st));
+    stage_end(c, "down", st);
+    CombineIds ci;
+    if (check_ids) { ci.a = ids_gu; ci.b = ids_dn; ci.E = E; }
+    TRY(launch_combine(c->z, w, res, out, T, K, D, st, ci, add));
+    stage_end(c, "combine", st);
+    return MI_MOE_OK;
+}
+
 // routed FFN body: ids (device [T][K]; gate/up and down may differ) and
 // weights w [T][K]; x_done: x is already in the x_q8_spec form; check_ids:
 // the ids come from the caller (dead slots are left out of the combine);
@@ -769,6 +862,8 @@ int run_experts(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T,
                 bool disp_out = true, bool sh_here = false, const float *sh_w = nullptr) {
     if (is_b32f(L->gate.type))
         return run_experts_b32(c, L, x, T, ids_gu, ids_dn, w, res, out, st, x_done, check_ids, add, disp_out, sh_here, sh_w);
+    if (is_mx(L->gate.type))
+        return run_experts_mx(c, L, x, T, ids_gu, ids_dn, w, res, out, st, check_ids, add, disp_out, sh_here, sh_w);
     const int D = L->n_embd, E = L->n_expert, K = L->n_expert_used, I = L->n_ff;
     const int64_t rows = T * K;
     const int max_active = (int)std::min<int64_t>(E, rows);
@@ -1333,7 +1428,7 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
     // the shared expert first (its own Q8_K of x; the routed block's follows),
     // unless it rides in the routed launches
     const float *add = nullptr;
-    const bool sh_here = L->sh_n_ff > 0 && b32_shared_ok(c, L, T);
+    const bool sh_here = L->sh_n_ff > 0 && (b32_shared_ok(c, L, T) || mx_shared_ok(c, L, T));
     if (sh_here) {
         if (L->sh_gate_inp) TRY(shared_weights(c, L, x, T, st));
     } else if (L->sh_n_ff > 0) {
@@ -1606,7 +1701,8 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
         return MI_MOE_OK;
     }
     const int max_active = (int)std::min<int64_t>(E, rows);
-    const int bm = !gb ? G4_BM : gf_tiles(c, as->type, rows, (int)E, Kin, N) ? GF_BM : gb_bm(c, rows, (int)E, N);
+    const bool mx = is_mx(as->type);
+    const int bm = mx ? MXG_BM : !gb ? G4_BM : gf_tiles(c, as->type, rows, (int)E, Kin, N) ? GF_BM : gb_bm(c, rows, (int)E, N);
     const int max_tiles = (int)((rows + bm - 1) / bm + max_active);
     const DispBuf &dsp = c->disp[0];
     Dispatch dv = dsp.view();
@@ -1616,6 +1712,18 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
     TRY(launch_dispatch((const int32_t *)ids->data, T, (int)n_used, (int)E, bm, 1, dv, st));
     const ExpertMat M = as_mat(*as);
     const float *bp = (const float *)b->data;
+    if (mx) {
+        MxArgs a = {};
+        a.a = M; a.epi = MX_STORE; a.ne11 = (int)ne11; a.K = (int)n_used;
+        a.x = mx_rows(c->ax.q8, T * ne11, Kin);
+        TRY(launch_prep_mx(bp, Kin, T * ne11, Kin, a.x, st));
+        a.perm = dsp.perm; a.counts = dsp.counts; a.offsets = dsp.offsets; a.active_e = dsp.active_e;
+        a.n_active = dsp.n_active; a.max_active = max_active;
+        a.tile_e = dsp.tile_e; a.tile_start = dsp.tile_start; a.tile_rows = dsp.tile_rows; a.n_tiles = dsp.n_tiles;
+        a.max_tiles = max_tiles;
+        a.y = (float *)dst->data; a.ldy = N; a.ncols = N;
+        return use_gemm_mx(c, T, (int)n_used, (int)E) ? launch_mxg(a, st) : launch_mxv(a, st);
+    }
     if (is_b32f(as->type)) {
         // b in the table type's vec_dot_type (Q8_0 or fp16), then the grouped GEMV or GEMM
         B32Prep o;
@@ -1682,12 +1790,28 @@ int mi_quantize(mi_moe_ctx *c, int32_t type, const float *src, void *dst, int64_
         HIP_TRY(hipSetDevice(c->device));
         return launch_quantize_b32(type, src, dst, nrows * (n_per_row / 32), (hipStream_t)stream);
     }
+    if (is_mx(type)) {
+        if (nrows < 0 || n_per_row <= 0 || n_per_row % 32) return MI_MOE_ERR_SHAPE;
+        if ((uintptr_t)src % 4) return MI_MOE_ERR_UNSUPPORTED;
+        HIP_TRY(hipSetDevice(c->device));
+        return launch_quantize_mx(src, dst, nrows * (n_per_row / 32), (hipStream_t)stream);
+    }
     if (type != MI_TYPE_Q4_K && type != MI_TYPE_Q6_K) return MI_MOE_ERR_TYPE;
     if (nrows < 0 || n_per_row <= 0 || n_per_row % QK) return MI_MOE_ERR_SHAPE;
     if (type == MI_TYPE_Q4_K && ((uintptr_t)dst % 4)) return MI_MOE_ERR_UNSUPPORTED;
     if ((uintptr_t)src % 4) return MI_MOE_ERR_UNSUPPORTED;
     HIP_TRY(hipSetDevice(c->device));
     return launch_quantize(type, src, dst, nrows * (n_per_row / QK), (hipStream_t)stream);
+}
+
+int mi_dequantize(mi_moe_ctx *c, int32_t type, const void *src, float *dst, int64_t nrows, int64_t n_per_row,
+                  mi_stream_t stream) {
+    if (!c || !src || !dst) return MI_MOE_ERR_NULL;
+    if (!is_b32f(type) && !is_mx(type)) return MI_MOE_ERR_TYPE;
+    if (nrows < 0 || n_per_row <= 0 || n_per_row % 32) return MI_MOE_ERR_SHAPE;
+    if ((uintptr_t)dst % 4) return MI_MOE_ERR_UNSUPPORTED;
+    HIP_TRY(hipSetDevice(c->device));
+    return launch_dequantize(type, src, dst, nrows * (n_per_row / 32), (hipStream_t)stream);
 }
 
 int64_t mi_moe_tiled_bytes(const mi_tensor *src) {

@@ -299,11 +299,11 @@ int mi_gguf_load_moe_layer(const mi_gguf *g, int32_t blk, int32_t act, mi_moe_la
         return MI_MOE_ERR_SHAPE;
     if (down->ne[1] != D || down->ne[2] != E) return MI_MOE_ERR_SHAPE;
     // expert tables as the converters write them: k-quants, the 32-value block
-    // formats (Q8_0 by default, Q5_0, Q4_0), F16 or F32 (one family per layer:
+    // formats (Q8_0 by default, Q5_0, Q4_0), F16, MXFP4 or F32 (one family per layer:
     // the forward's validation refuses a mix)
     auto table_type = [](int32_t t) {
         return t == MI_TYPE_Q4_K || t == MI_TYPE_Q6_K || t == MI_TYPE_Q4_0 || t == MI_TYPE_Q5_0 ||
-               t == MI_TYPE_Q8_0 || t == MI_TYPE_F16 || t == MI_TYPE_F32;
+               t == MI_TYPE_Q8_0 || t == MI_TYPE_F16 || t == MI_TYPE_MXFP4 || t == MI_TYPE_F32;
     };
     for (const TensorInfo *t : {up, down, fused ? up : gate})
         if (!table_type(t->type)) return MI_MOE_ERR_TYPE;

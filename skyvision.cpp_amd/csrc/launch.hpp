@@ -350,6 +350,59 @@ constexpr int64_t GB_MAX_X = 0xF0000000ll;          // bytes of xh (32-bit buffe
 constexpr int64_t GB_MAX_ROW_BYTES = 1ll << 25;
 int launch_gb(const GBArgs &g, hipStream_t st);
 
+// ---- MXFP4 expert tables (39; k_mx.hip, k_mxg.hip; format and operand: mx.hpp)
+int launch_quantize_mx(const float *src, void *dst, int64_t nblocks, hipStream_t st);
+// rows of 32-value blocks (F16: 32 values per "block") of types 1, 2, 6, 8, 39 as fp32
+int launch_dequantize(int type, const void *src, float *dst, int64_t nblocks, hipStream_t st);
+// operand rows: [rows][K/32] blocks of MX_XB = 96 bytes and [rows][K/32] scale words
+struct MxRows {
+    uint8_t *xb = nullptr;   // 16-byte aligned
+    uint32_t *xs = nullptr;
+};
+int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, hipStream_t st);
+// Grouped products.  MX_STORE: fp32 rows y; MX_GLU / MX_RELU_SQR: the
+// activation rows leave as the next product's operand o (rows of ncols
+// values, ncols % 32 == 0).  A shared expert (sh_rows > 0) rides in the same
+// launch: sh_rows rows (its operand rows in order, no dispatch) through the
+// tables and operands of sh, of the same epilogue and act; sh_w: weights of its
+// rows (MX_STORE; NULL: 1).
+enum { MX_STORE = 0, MX_GLU = 1, MX_RELU_SQR = 2 };
+struct MxSide {
+    ExpertMat a, b;            // b: up table (separate gate/up GLU), else unused
+    int fused;
+    int64_t I;
+    MxRows x;                  // operand rows of a.K values
+    MxRows o;
+    float *y;                  // rows p, stride ldy
+    int64_t ldy, ncols;
+};
+struct MxArgs : MxSide {
+    int epi, act;
+    int ne11, K;
+    const int32_t *perm;
+    // few rows (launch_mxv): the dispatch's lists, or the rows' expert ids, at
+    // most MXV_IDS of them; a row whose id lies outside [0, n_expert) is not
+    // computed, its output row is not written, and it is counted in bad_total
+    // (NULL: not counted), as by the dispatch
+    const int32_t *counts, *offsets, *active_e, *n_active;
+    int max_active;
+    const int32_t *ids;
+    int64_t rows;
+    int n_expert;              // with ids
+    int32_t *bad_total;
+    // launch_mxg: balanced tiles of at most MXG_BM rows
+    const int32_t *tile_e, *tile_start, *tile_rows, *n_tiles;
+    int max_tiles;
+    MxSide sh;
+    int64_t sh_rows;
+    const float *sh_w;
+    int ncb, sh_wgs;           // (set by the launchers)
+};
+constexpr int MXV_IDS = 512;
+constexpr int MXG_BM = 128;
+int launch_mxv(const MxArgs &g, hipStream_t st);
+int launch_mxg(const MxArgs &g, hipStream_t st);
+
 // Single-token MoE block in one kernel (k_decode.hip).
 struct DecArgs {
     const float *rw, *rb, *x;     // router W [E][D], bias [E] or NULL, tokens [T][D]

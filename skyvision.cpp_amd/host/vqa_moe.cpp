@@ -81,7 +81,8 @@ Tensor *Session::new_tensor(int type, int64_t ne0, int64_t ne1, int64_t ne2) {
     Tensor *t = new Tensor;
     t->type = type;
     t->ne[0] = ne0; t->ne[1] = ne1; t->ne[2] = ne2; t->ne[3] = 1;
-    t->nb[0] = type == MI_TYPE_F32 || type == MI_TYPE_I32 ? 4 : type == MI_TYPE_F16 ? 2 : row / (size_t)(ne0 / 256);
+    t->nb[0] = type == MI_TYPE_F32 || type == MI_TYPE_I32 ? 4 : type == MI_TYPE_F16 ? 2 :
+               type == MI_TYPE_Q4_K || type == MI_TYPE_Q6_K ? row / (size_t)(ne0 / 256) : row / (size_t)(ne0 / 32);
     t->nb[1] = row;
     t->nb[2] = row * (size_t)ne1;
     t->nb[3] = t->nb[2] * (size_t)ne2;

@@ -18,7 +18,7 @@ DECODE_CHAIN, DECODE_FUSED_COOPERATIVE, DECODE_FUSED = 0, 1, 2
 DECODE_FUSED_EXCLUSIVE = DECODE_FUSED   # former name
 
 TYPE_F32, TYPE_F16, TYPE_Q4_K, TYPE_Q6_K, TYPE_I32 = 0, 1, 12, 14, 26
-TYPE_Q4_0, TYPE_Q5_0, TYPE_Q8_0 = 2, 6, 8
+TYPE_Q4_0, TYPE_Q5_0, TYPE_Q8_0, TYPE_MXFP4 = 2, 6, 8, 39
 ACT_SILU, ACT_GELU_ERF_GP1, ACT_GELU_TANH, ACT_GELU_ERF, ACT_RELU_SQR = 0, 1, 2, 3, 4
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 GATING_SOFTMAX_TOPK, GATING_SIGMOID_BIAS, GATING_SOFTMAX_ALL = 0, 1, 2
@@ -27,7 +27,8 @@ ABI_VERSION = 3
 OK, ERR_NULL, ERR_SHAPE, ERR_TYPE, ERR_CAPACITY, ERR_HIP = 0, -1, -2, -3, -4, -5
 ERR_UNSUPPORTED, ERR_DEVICE, ERR_ARG, ERR_FORMAT = -6, -7, -8, -9
 QK_K = 256
-BLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q6_K: 210, TYPE_Q4_0: 18, TYPE_Q5_0: 22, TYPE_Q8_0: 34}
+BLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q6_K: 210, TYPE_Q4_0: 18, TYPE_Q5_0: 22, TYPE_Q8_0: 34,
+               TYPE_MXFP4: 17}
 STATUS = {0: "ok", -1: "null", -2: "shape", -3: "type", -4: "capacity", -5: "hip",
           -6: "unsupported", -7: "device", -8: "arg"}
 
@@ -95,6 +96,7 @@ SYMBOLS = {
     "mi_mul_mat_id": ([P, C.POINTER(Tensor), C.POINTER(Tensor), C.POINTER(Tensor),
                        C.POINTER(Tensor), P], C.c_int),
     "mi_quantize": ([P, i32, P, P, i64, i64, P], C.c_int),
+    "mi_dequantize": ([P, i32, P, P, i64, i64, P], C.c_int),
     "mi_moe_tiled_bytes": ([C.POINTER(Tensor)], i64),
     "mi_moe_tile": ([P, C.POINTER(Tensor), P, C.POINTER(Tensor), P], C.c_int),
     "mi_fill_normal": ([P, P, i64, C.c_uint64, C.c_uint64, C.c_float, C.c_float, P], C.c_int),
@@ -248,7 +250,7 @@ def tensor(buf, type_: int, ne, nb=None, offset: int = 0) -> Tensor:
     """ggml-style descriptor; default strides are ggml's contiguous ones."""
     ne = list(ne) + [1] * (4 - len(ne))
     if nb is None:
-        if type_ in (TYPE_Q4_K, TYPE_Q6_K, TYPE_Q4_0, TYPE_Q5_0, TYPE_Q8_0):
+        if type_ in (TYPE_Q4_K, TYPE_Q6_K, TYPE_Q4_0, TYPE_Q5_0, TYPE_Q8_0, TYPE_MXFP4):
             nb0 = BLOCK_BYTES[type_]
             nb1 = row_size(type_, ne[0])
         else:
@@ -354,6 +356,10 @@ class Context:
     def quantize(self, type_: int, src, dst, nrows: int, n_per_row: int, stream=None) -> int:
         return load().mi_quantize(self.h, type_, _addr(src), _addr(dst), nrows, n_per_row,
                                   _addr(stream))
+
+    def dequantize(self, type_: int, src, dst, nrows: int, n_per_row: int, stream=None) -> int:
+        """dst = the float32 values of rows of an MXFP4, Q4_0, Q5_0, Q8_0 or F16 table"""
+        return load().mi_dequantize(self.h, type_, _addr(src), _addr(dst), nrows, n_per_row, _addr(stream))
 
     def tile(self, src: Tensor, dst, desc: Tensor | None = None, stream=None) -> int:
         """dst = src (a Q4_K or Q6_K table) in the grouped GEMMs' tiled order;

@@ -1,0 +1,448 @@
+"""MXFP4 expert tables through the C ABI against float64 forms (_mxfp4.py) and the CPU oracle.
+
+Tolerances.  mi_quantize and mi_dequantize: exact.  Products of few rows per expert: exact block sums added in fp64
+(error 2^-53 times the number of blocks), rounded to float32 once: 2^-24 of the value, and 2^-50 of the sum of the
+terms' sizes where they cancel.  The GEMM adds a block pair's digit sum to a float32 accumulator, four per 64 values:
+n / 16 additions, each off by at most a step (2^-23, whether the matrix unit rounds or cuts) of the largest partial
+sum, so a value is off by at most n / 16 * 2^-23 of its terms' sizes (|x| . |w|); the digits' partial sums are at most
+2 |x| . |w| together (a balanced digit's part overshoots what it stands for by at most a half), so twice that.
+Layers of few rows: the products as above, the GLU in fp64 rounded to float32, Q8_0 codes equal; z, z w and the
+result rounded to float32: (K + 3) 2^-24 of the terms' sizes; the weights (softmax in float32: exp and sum within 4
+steps) add 2^-21.
+Layers on the GEMM: an error of the gate/up products can move a code of the activation rows by a step (1 / 127 of its
+block's largest) and an fp16 scale by a step (2^-10): held to 1e-2 as the other 32-value types are, and 1e-3 measured
+by the root of the mean square."""
+import numpy as np
+import pytest
+
+import _mxfp4 as X
+import mimoe as M
+import pyoracle as O
+from test_oracle_mxfp4 import rows_of_all_kinds
+
+pytestmark = pytest.mark.gpu
+MX = M.TYPE_MXFP4
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = M.Context(0)
+    c.reserve(640, 2816, 1856, 64, 8)
+    yield c
+    c.close()
+
+
+def table(rng, E, N, n, std=0.02):
+    return O.quantize(O.TYPE_MXFP4, (rng.standard_normal((E, N, n)) * std).astype(np.float32))
+
+
+def rows(rng, *shape):
+    x = rng.standard_normal(shape).astype(np.float32) * np.exp(rng.standard_normal(shape[-1])).astype(np.float32)
+    return x
+
+
+# ------------------------------------------------------------------ quantize, dequantize
+@pytest.mark.parametrize("offset", [0, 4, 1, 3])
+def test_quantize_exact(ctx, offset):
+    x = rows_of_all_kinds()
+    for nrows in (1, 3, len(x)):
+        src = M.DeviceBuffer(x.nbytes + 16).upload(x[:nrows], 4 if offset else 0)
+        n = nrows * M.row_size(MX, x.shape[1])
+        dst = M.to_device(np.full(n + 64, 0xA5, np.uint8))
+        M.check("quantize", ctx.quantize(MX, src.addr + (4 if offset else 0), dst.addr + offset, nrows, x.shape[1]))
+        got = dst.download(np.uint8, (n + 64,))
+        assert np.array_equal(got[offset:offset + n].reshape(nrows, -1), X.quantize(x[:nrows]))
+        assert (got[:offset] == 0xA5).all() and (got[offset + n:] == 0xA5).all()
+
+
+def test_quantize_many_blocks(ctx):
+    x = rows(np.random.default_rng(3), 700, 1056)
+    dst = M.DeviceBuffer(700 * M.row_size(MX, 1056))
+    M.check("quantize", ctx.quantize(MX, M.to_device(x), dst, 700, 1056))
+    assert np.array_equal(dst.download(np.uint8, (700, 561)), O.quantize(O.TYPE_MXFP4, x))
+
+
+@pytest.mark.parametrize("type_", [MX, M.TYPE_Q4_0, M.TYPE_Q5_0, M.TYPE_Q8_0, M.TYPE_F16])
+@pytest.mark.parametrize("nrows,n", [(1, 32), (5, 96), (129, 32), (67, 2816)])
+def test_dequantize_exact(ctx, type_, nrows, n):
+    rng = np.random.default_rng(nrows + n)
+    raw = O.quantize(type_, rows(rng, nrows, n))
+    if type_ == MX:
+        raw = rng.integers(0, 256, raw.shape, dtype=np.uint8)      # every scale byte and code
+    ref = O.dequantize(type_, raw, n)
+    for so, do in ((0, 0), (1 if type_ == MX else 2, 4)):
+        src = M.DeviceBuffer(raw.nbytes + 8).upload(raw, so)
+        dst = M.to_device(np.full(nrows * n + 8, 7.0, np.float32))
+        M.check("dequantize", ctx.dequantize(type_, src.addr + so, dst.addr + do, nrows, n))
+        got = dst.download(np.float32, (nrows * n + 8,))
+        assert np.array_equal(got[do // 4:do // 4 + nrows * n].reshape(nrows, n), ref, equal_nan=True)
+        assert (got[:do // 4] == 7.0).all() and (got[do // 4 + nrows * n:] == 7.0).all()
+
+
+def test_refusals(ctx):
+    b = M.DeviceBuffer(1 << 16)
+    assert ctx.quantize(MX, b, b, 1, 48) == M.ERR_SHAPE and ctx.quantize(MX, b, b, -1, 32) == M.ERR_SHAPE
+    assert ctx.quantize(MX, b.addr + 2, b, 1, 32) == M.ERR_UNSUPPORTED and ctx.quantize(MX, None, b, 1, 32) == M.ERR_NULL
+    assert ctx.quantize(MX, b, b, 0, 32) == 0 and ctx.dequantize(MX, b, b, 0, 32) == 0
+    assert ctx.dequantize(M.TYPE_Q4_K, b, b, 1, 256) == M.ERR_TYPE and ctx.dequantize(M.TYPE_F32, b, b, 1, 32) == M.ERR_TYPE
+    assert ctx.dequantize(MX, b, b, 1, 33) == M.ERR_SHAPE and ctx.dequantize(MX, b, b.addr + 2, 1, 32) == M.ERR_UNSUPPORTED
+    assert ctx.dequantize(MX, b, None, 1, 32) == M.ERR_NULL
+    t = lambda ty, ne, nb=None: M.tensor(b, ty, ne, nb)
+    f, i = M.TYPE_F32, M.TYPE_I32
+    ok = (t(MX, [64, 8, 2]), t(f, [64, 1, 1]), t(i, [2, 1]), t(f, [8, 2, 1]))
+    assert ctx.mul_mat_id(t(MX, [48, 8, 2]), t(f, [48, 1, 1]), ok[2], ok[3]) == M.ERR_UNSUPPORTED
+    assert ctx.mul_mat_id(ok[0], t(f, [96, 1, 1]), ok[2], ok[3]) == M.ERR_SHAPE
+    assert ctx.mul_mat_id(t(MX, [64, 8, 2], [17, 33, 272, 544]), ok[1], ok[2], ok[3]) == M.ERR_SHAPE
+    assert ctx.mul_mat_id(ok[0], ok[1], ok[2], t(M.TYPE_F16, [8, 2, 1])) == M.ERR_TYPE
+    # one family per layer; no tiled copies of MXFP4
+    lay = M.make_layer(64, 2, 1, 32, b, None, t(MX, [64, 64, 2]), None, t(M.TYPE_Q8_0, [32, 64, 2]), True, M.ACT_SILU)
+    assert ctx.forward(lay, b, 1, None, b) == M.ERR_UNSUPPORTED
+    lay = M.make_layer(64, 2, 1, 32, b, None, t(MX, [64, 64, 2]), None, t(MX, [32, 64, 2]), True, M.ACT_SILU)
+    lay.gate_tiled = lay.gate
+    assert ctx.forward(lay, b, 1, None, b) == M.ERR_TYPE and M.tiled_bytes(lay.gate) == M.ERR_TYPE
+
+
+# ------------------------------------------------------------------ products
+def run_product(ctx, raw, b, ids, pad=0, offset=0, stream=None):
+    """raw [E, N, row]; rows pad bytes apart, the table at a byte offset; dst starts as 9s"""
+    E, N, rb = raw.shape
+    T, K = ids.shape
+    n = b.shape[-1]
+    wide = np.full((E, N, rb + pad), 0xFF, np.uint8)
+    wide[..., :rb] = raw
+    w = M.DeviceBuffer(wide.nbytes + 16).upload(wide, offset)
+    nb1 = rb + pad
+    dst = M.to_device(np.full((T, K, N), 9.0, np.float32))
+    bd, idd = M.to_device(b.astype(np.float32)), M.to_device(ids.astype(np.int32))
+    rc = ctx.mul_mat_id(M.tensor(w, MX, [n, N, E], [17, nb1, nb1 * N, nb1 * N * E], offset=offset), M.tensor(bd, M.TYPE_F32, [n, b.shape[1], T]),
+                        M.tensor(idd, M.TYPE_I32, [K, T]), M.tensor(dst, M.TYPE_F32, [N, K, T]), stream)
+    M.check("mul_mat_id", rc)
+    M.synchronize()
+    return dst.download(np.float32, (T, K, N))
+
+
+def check_product(got, raw, b, ids, few):
+    ref = X.product(raw, b, ids)
+    size = X.product_sizes(raw, b, ids)
+    n = b.shape[-1]
+    tol = 2.0 ** -24 * np.abs(ref) + 2.0 ** -50 * size if few else 2.0 ** -24 * np.abs(ref) + n / 16 * 2.0 ** -23 * 2 * size
+    assert np.array_equal(np.isnan(got), np.isnan(ref))
+    off = np.abs(got - ref)
+    assert not (off > tol)[~np.isnan(ref)].any(), (np.nanmax(off / np.maximum(tol, 1e-300)), np.argwhere(off > tol)[:4])
+
+
+SHAPES = [(32, 1), (32, 16), (64, 33), (96, 64), (704, 70), (2048, 160), (2112, 48), (2816, 257), (1056, 129)]
+
+
+@pytest.mark.parametrize("path", ["few", "gemm"])
+@pytest.mark.parametrize("n,N", SHAPES)
+@pytest.mark.parametrize("own_rows", [False, True])
+def test_product_shapes(ctx, path, n, N, own_rows):
+    rng = np.random.default_rng(n * 1000 + N)
+    E, K = 6, 3
+    raw = table(rng, E, N, n)
+    ctx.set_gemm_threshold(1 if path == "gemm" else 1 << 40)
+    try:
+        for T in (1, 2, 5, 47, 150):
+            b = rows(rng, T, K if own_rows else 1, n)
+            ids = np.stack([rng.permutation(E)[:K] for _ in range(T)])
+            check_product(run_product(ctx, raw, b, ids), raw, b, ids, path == "few")
+    finally:
+        ctx.set_gemm_threshold(0)
+
+
+@pytest.mark.parametrize("path", ["few", "gemm"])
+@pytest.mark.parametrize("pad,offset", [(0, 1), (1, 0), (2, 3), (7, 2), (15, 5)])
+def test_product_any_alignment(ctx, path, pad, offset):
+    rng = np.random.default_rng(pad + 16 * offset)
+    raw = table(rng, 4, 50, 352)
+    b, ids = rows(rng, 9, 1, 352), rng.integers(0, 4, (9, 2))
+    ctx.set_gemm_threshold(1 if path == "gemm" else 1 << 40)
+    try:
+        check_product(run_product(ctx, raw, b, ids, pad, offset), raw, b, ids, path == "few")
+    finally:
+        ctx.set_gemm_threshold(0)
+
+
+@pytest.mark.parametrize("path", ["few", "gemm"])
+def test_product_hot_expert_and_bad_ids(ctx, path):
+    """every slot on one expert, the same expert twice in a token, ids outside: zero rows, counted"""
+    rng = np.random.default_rng(11)
+    raw = table(rng, 5, 96, 320)
+    b = rows(rng, 300, 2, 320)
+    ids = np.full((300, 2), 3)
+    ctx.set_gemm_threshold(1 if path == "gemm" else 1 << 40)
+    try:
+        check_product(run_product(ctx, raw, b, ids), raw, b, ids, path == "few")
+        ids = rng.integers(-2, 7, (300, 2))
+        ctx.take_errors()
+        check_product(run_product(ctx, raw, b, ids), raw, b, ids, path == "few")
+        assert ctx.take_errors()[0] == int(((ids < 0) | (ids >= 5)).sum())
+        ids[:] = 99
+        assert not run_product(ctx, raw, b, ids).any()
+    finally:
+        ctx.take_errors()
+        ctx.set_gemm_threshold(0)
+
+
+@pytest.mark.parametrize("path", ["few", "gemm"])
+def test_product_values_at_the_edges(ctx, path):
+    """NaN blocks, the smallest and largest scales, rows with NaN, infinities, zeros, 1e30 and 1e-30"""
+    rng = np.random.default_rng(12)
+    raw = table(rng, 3, 40, 160)
+    raw[0, 3, 17] = 255                    # row 3, block 1: NaN
+    raw[1, :, 0] = 0                       # 2^-127
+    raw[1, 5, 34] = 200                    # 2^73 in one block of a row
+    raw[2, :, 51] = 230
+    b = rows(rng, 12, 1, 160)
+    b[0] = 0.0
+    b[1, 0, 70], b[2, 0, 0], b[3, 0, 159] = np.nan, np.inf, -np.inf
+    b[4, 0, :32], b[5, 0] = 1e30, b[5, 0] * 1e-30
+    b[6, 0, 32:64], b[7, 0, 5] = 0.0, 8.0e6
+    ids = np.tile(np.array([[0, 1, 2]]), (12, 1))
+    ctx.set_gemm_threshold(1 if path == "gemm" else 1 << 40)
+    try:
+        got = run_product(ctx, raw, b, ids)
+        ref = X.product(raw, b, ids)
+        assert np.array_equal(np.isnan(got), np.isnan(ref))
+        size = X.product_sizes(raw, b, ids)
+        # (products of the smallest scales may flush below the smallest normal number)
+        tol = 2.0 ** -24 * np.abs(ref) + (2.0 ** -50 if path == "few" else 2 * 160 / 16 * 2.0 ** -23) * size + 160 * 2.0 ** -126
+        assert (np.abs(got - ref) <= tol)[~np.isnan(ref)].all()
+    finally:
+        ctx.set_gemm_threshold(0)
+
+
+def test_product_of_no_tokens(ctx):
+    raw = table(np.random.default_rng(1), 2, 16, 32)
+    w = M.to_device(raw)
+    rc = ctx.mul_mat_id(M.tensor(w, MX, [32, 16, 2]), M.tensor(w, M.TYPE_F32, [32, 1, 0]), M.tensor(w, M.TYPE_I32, [2, 0]),
+                        M.tensor(w, M.TYPE_F32, [16, 2, 0]))
+    assert rc == 0
+
+
+# ------------------------------------------------------------------ layers
+class Layer:
+    def __init__(self, D, E, K, I, fused, act, seed, gating=0, shared=0, sh_gate_inp=False, bias=False):
+        rng = np.random.default_rng(seed)
+        self.D, self.E, self.K, self.I, self.gating = D, E, K, I, gating
+        self.host = dict(D=D, E=E, K=K, I=I, fused=fused, act=act, gate_type=MX, down_type=MX,
+                         router_w=(rng.standard_normal((E, D)) * 0.05).astype(np.float32), router_b=None)
+        self.host["gate"] = table(rng, E, 2 * I if fused else I, D)
+        self.host["up"] = None if fused or act == 4 else table(rng, E, I, D)
+        self.host["down"] = table(rng, E, D, I)
+        self.keep = keep = {k: M.to_device(v) for k, v in self.host.items() if isinstance(v, np.ndarray)}
+        up = None if self.host["up"] is None else M.tensor(keep["up"], MX, [D, I, E])
+        L = M.make_layer(D, E, K, I, keep["router_w"], None, M.tensor(keep["gate"], MX, [D, 2 * I if fused else I, E]), up,
+                         M.tensor(keep["down"], MX, [I, D, E]), fused, act)
+        L.gating = gating
+        self.scale = self.sel_bias = None
+        if gating == 1:
+            self.sel_bias = (rng.standard_normal(E) * 0.05).astype(np.float32)
+            keep["sel_bias"] = M.to_device(self.sel_bias)
+            L.sel_bias, L.routed_scaling, L.gate_eps = keep["sel_bias"].addr, 2.5, 1e-20
+        if gating == 2:
+            self.scale = rng.uniform(0.5, 1.5, E).astype(np.float32)
+            keep["scale"] = M.to_device(self.scale)
+            L.expert_scale = keep["scale"].addr
+        self.shared = None
+        if shared:
+            sh = self.shared = dict(I=shared, fused=False, act=act, gate=table(rng, 1, shared, D), up=None if act == 4 else table(rng, 1, shared, D),
+                                    down=table(rng, 1, D, shared))
+            for k in ("gate", "up", "down"):
+                if sh[k] is not None:
+                    keep["sh_" + k] = M.to_device(sh[k])
+                    setattr(L, "sh_" + k, M.tensor(keep["sh_" + k], MX, [shared, D] if k == "down" else [D, shared]))
+            L.sh_n_ff, L.sh_act = shared, act
+            if sh_gate_inp:
+                sh["inp"] = (rng.standard_normal((1, D)) * 0.05).astype(np.float32)
+                keep["sh_inp"] = M.to_device(sh["inp"])
+                L.sh_gate_inp = keep["sh_inp"].addr
+        self.L = L
+
+    def route(self, x):
+        """the oracle's ids and weights (logits, ids: bit for bit the library's)"""
+        return O.route_gated(O.router_logits(self.host["router_w"], None, x), self.K, self.gating, self.sel_bias, self.scale,
+                             2.5 if self.gating == 1 else 1.0, 1e-20 if self.gating == 1 else 0.0)
+
+    def reference(self, x, res, xr=None):
+        sel, w = self.route(x if xr is None else xr)
+        y = X.ffn(self.host, x, sel, sel, w)
+        if self.shared:
+            T = len(x)
+            s = 1.0 / (1.0 + np.exp(-(x.astype(np.float64) @ self.shared["inp"][0].astype(np.float64)))) if "inp" in self.shared else np.ones(T)
+            z = np.zeros((T, 1), np.int32)
+            y = y + X.ffn(self.shared, x, z, z, s[:, None].astype(np.float32))
+        return y + (0 if res is None else res)
+
+
+def check_layer(got, ref, moe_size, few):
+    e = float(np.linalg.norm(got - ref) / np.linalg.norm(ref))
+    if few:
+        assert (np.abs(got - ref) <= 2.0 ** -20 * moe_size + 2.0 ** -23 * np.abs(ref)).all(), e
+    else:
+        assert e <= 1e-3, e
+    return e
+
+
+def sizes(lay, x, xr=None):
+    """a bound of the terms' sizes: the slots' weighted outputs by their absolute values"""
+    sel, w = lay.route(x if xr is None else xr)
+    with np.errstate(all="ignore"):
+        y = X.ffn_slots(lay.host, x, sel, sel)
+    s = (np.abs(y) * np.abs(w[..., None])).sum(1)
+    if lay.shared:
+        z = np.zeros((len(x), 1), np.int32)
+        s = s + np.abs(X.ffn_slots(lay.shared, x, z, z))[:, 0]
+    return s
+
+
+LAYERS = {
+    "moondream_like": dict(D=512, E=16, K=4, I=256, fused=True, act=1),
+    "qwen_like": dict(D=512, E=16, K=8, I=96, fused=False, act=0),
+    "gemma_like": dict(D=352, E=8, K=2, I=160, fused=False, act=2, gating=2),
+    "nemotron_like": dict(D=672, E=12, K=6, I=224, fused=False, act=4, gating=1, shared=448),
+    "talker_like": dict(D=512, E=8, K=3, I=128, fused=False, act=0, shared=256, sh_gate_inp=True),
+    "erf": dict(D=64, E=4, K=1, I=32, fused=True, act=3),
+    "wide": dict(D=2816, E=64, K=8, I=704, fused=False, act=2),
+}
+
+
+@pytest.mark.parametrize("name", LAYERS)
+@pytest.mark.parametrize("path", ["default", "few", "gemm"])
+def test_layer(ctx, name, path):
+    lay = Layer(seed=len(name), **LAYERS[name])
+    rng = np.random.default_rng(21)
+    ctx.set_gemm_threshold({"default": 0, "few": 1 << 40, "gemm": 1}[path])
+    try:
+        for T in (1, 2, 3, 8, 16) + ((70,) if name != "wide" else ()):
+            few = path == "few" or (path == "default" and T * lay.K <= 2 * lay.E)
+            x, res = rows(rng, T, lay.D), rows(rng, T, lay.D)
+            out = M.DeviceBuffer(4 * T * lay.D)
+            sel = M.DeviceBuffer(4 * T * lay.K)
+            r = M.Routing()
+            r.sel = sel.addr
+            M.check("forward", ctx.forward(lay.L, M.to_device(x), T, M.to_device(res), out, r))
+            M.synchronize()
+            assert np.array_equal(sel.download(np.int32, (T, lay.K)), lay.route(x)[0])
+            e = check_layer(out.download(np.float32, (T, lay.D)), lay.reference(x, res), sizes(lay, x), few)
+            print(f"{name} {path} T={T}: rel-L2 {e:.2e}", flush=True)
+    finally:
+        ctx.set_gemm_threshold(0)
+
+
+@pytest.mark.parametrize("kind", [M.NORM_RMS, M.NORM_LAYER])
+def test_layer_norm_equals_norm_then_forward(ctx, kind):
+    lay = Layer(seed=3, **LAYERS["qwen_like"])
+    rng = np.random.default_rng(kind)
+    w, b = M.to_device(rows(rng, 512)), M.to_device(rows(rng, 512))
+    norm = M.make_norm(kind, 1e-6, w, b if kind == M.NORM_LAYER else None)
+    for T in (1, 5, 16, 90):
+        h = M.to_device(rows(rng, T, 512))
+        hn, a, c = (M.DeviceBuffer(4 * T * 512) for _ in range(3))
+        M.check("norm", ctx.norm(norm, h, T, 512, hn))
+        M.check("forward", ctx.forward(lay.L, hn, T, h, a))
+        M.check("forward_norm", ctx.forward_norm(lay.L, norm, h, T, h, c))
+        M.synchronize()
+        assert np.array_equal(a.download(np.uint8, (4 * T * 512,)), c.download(np.uint8, (4 * T * 512,)))
+
+
+def test_router_input_and_in_place(ctx):
+    lay = Layer(seed=4, **LAYERS["gemma_like"])
+    rng = np.random.default_rng(8)
+    for T in (1, 7, 60):
+        x, xr, res = rows(rng, T, 352), rows(rng, T, 352), rows(rng, T, 352)
+        out = M.to_device(res)
+        M.check("router_input", ctx.forward_router_input(lay.L, M.to_device(x), M.to_device(xr), T, out, out))
+        M.synchronize()
+        check_layer(out.download(np.float32, (T, 352)), lay.reference(x, res, xr), sizes(lay, x, xr), T * lay.K <= 2 * lay.E)
+
+
+def test_expert_ffn_caller_ids(ctx):
+    """two id sets, ids outside in each: their slots add nothing and are counted"""
+    lay = Layer(seed=5, **LAYERS["moondream_like"])
+    rng = np.random.default_rng(9)
+    for T in (1, 2, 6, 40):
+        x = rows(rng, T, 512)
+        gu, dn = rng.integers(-1, 18, (T, 4)), rng.integers(-1, 18, (T, 4))
+        w = rng.uniform(0, 1, (T, 4)).astype(np.float32)
+        out = M.DeviceBuffer(4 * T * 512)
+        ctx.take_errors()
+        M.check("expert_ffn", ctx.expert_ffn(lay.L, M.to_device(x), T, None, M.to_device(gu.astype(np.int32)), M.to_device(dn.astype(np.int32)),
+                                             M.to_device(w), out))
+        assert ctx.take_errors()[0] == int(((gu < 0) | (gu >= 16)).sum() + ((dn < 0) | (dn >= 16)).sum())
+        ref = X.ffn(lay.host, x, gu, dn, w)
+        got = out.download(np.float32, (T, 512))
+        assert np.linalg.norm(got - ref) <= 1e-3 * np.linalg.norm(ref) + 1e-20
+        dead = ~(((gu >= 0) & (gu < 16)) & ((dn >= 0) & (dn < 16))).any(1)
+        assert not got[dead].any()
+
+
+def test_noalloc_equals_chain(ctx):
+    lay = Layer(seed=6, **LAYERS["qwen_like"])
+    rng = np.random.default_rng(10)
+    c = M.Context(0)
+    c.reserve(64, 512, 96, 16, 8)
+    c.set_fused_decode(M.DECODE_CHAIN)
+    for T in (1, 6, 64):
+        x = M.to_device(rows(rng, T, 512))
+        a, b = M.DeviceBuffer(4 * T * 512), M.DeviceBuffer(4 * T * 512)
+        M.check("noalloc", M.forward_noalloc(lay.L, x, T, x, a))
+        M.check("forward", c.forward(lay.L, x, T, x, b))
+        M.synchronize()
+        assert np.array_equal(a.download(np.uint8, (4 * T * 512,)), b.download(np.uint8, (4 * T * 512,)))
+    c.close()
+
+
+def test_graph_replays(ctx):
+    """a decode step captured and replayed on rewritten inputs, eager work between the replays"""
+    lay = Layer(seed=7, **LAYERS["qwen_like"])
+    rng = np.random.default_rng(13)
+    st = M.Stream()
+    for T in (1, 9, 80):
+        x, out, eager = (M.DeviceBuffer(4 * T * 512) for _ in range(3))
+        x.upload(rows(rng, T, 512))
+        g = M.Graph(st, lambda s: M.check("forward", ctx.forward(lay.L, x, T, x, out, None, s.addr)))
+        for _ in range(4):
+            x.upload(rows(rng, T, 512))
+            M.synchronize()
+            g.launch(st)
+            st.synchronize()
+            M.check("forward", ctx.forward(lay.L, x, T, x, eager))
+            M.synchronize()
+            assert np.array_equal(out.download(np.uint8, (4 * T * 512,)), eager.download(np.uint8, (4 * T * 512,)))
+        g.destroy()
+    st.destroy()
+
+
+def test_quantize_then_layer_run_together(ctx):
+    """as a program uses them: tables quantized on the GPU, a prefill and decode steps of the layer on a stream"""
+    rng = np.random.default_rng(14)
+    D, E, K, I = 512, 16, 4, 256
+    wf = {"gate": (rng.standard_normal((E, 2 * I, D)) * 0.02).astype(np.float32), "down": (rng.standard_normal((E, D, I)) * 0.02).astype(np.float32)}
+    dev, host = {}, dict(D=D, E=E, K=K, I=I, fused=True, act=1, up=None)
+    st = M.Stream()
+    for k, v in wf.items():
+        n = v.shape[-1]
+        dev[k] = M.DeviceBuffer(v.size // 32 * 17)
+        M.check("quantize", ctx.quantize(MX, M.to_device(v), dev[k], v.size // n, n, st.addr))
+        st.synchronize()
+        host[k] = dev[k].download(np.uint8, (*v.shape[:-1], n // 32 * 17))
+        back = M.DeviceBuffer(v.nbytes)
+        M.check("dequantize", ctx.dequantize(MX, dev[k], back, v.size // n, n, st.addr))
+        st.synchronize()
+        assert np.array_equal(back.download(np.float32, v.shape), X.values(host[k]).astype(np.float32))
+    rw = (rng.standard_normal((E, D)) * 0.05).astype(np.float32)
+    rd = M.to_device(rw)
+    L = M.make_layer(D, E, K, I, rd, None, M.tensor(dev["gate"], MX, [D, 2 * I, E]), None, M.tensor(dev["down"], MX, [I, D, E]), True, 1)
+    for T in (200, 1, 1, 3):
+        x = rows(rng, T, D)
+        out = M.DeviceBuffer(4 * T * D)
+        xd = M.to_device(x)
+        M.check("forward", ctx.forward(L, xd, T, None, out, None, st.addr))
+        st.synchronize()
+        sel, w = O.route_gated(O.router_logits(rw, None, x), K, 0)
+        ref = X.ffn(host, x, sel, sel, w)
+        got = out.download(np.float32, (T, D))
+        assert np.linalg.norm(got - ref) <= (1e-3 if T * K > 2 * E else 1e-6) * np.linalg.norm(ref)
+    st.destroy()
