@@ -777,6 +777,11 @@ bool use_gemm_mx(const mi_moe_ctx *c, int64_t T, int K, int E) {
     if (c->gemm_threshold > 0) return T >= c->gemm_threshold;
     return T * K > 2 * (int64_t)E;
 }
+// Row tiles of its GEMM: 128 rows above 32 dispatched rows per expert, else 32
+int mx_bm(const mi_moe_ctx *c, int64_t rows, int E) {
+    if (c->gemm_tiles == 1 || c->gemm_tiles == 2) return c->gemm_tiles == 1 ? MXG_BM : MXG_BM_SMALL;
+    return rows > 32 * (int64_t)E ? MXG_BM : MXG_BM_SMALL;
+}
 // The shared expert in the routed experts' launches of few rows: the same
 // table type and activation.
 bool mx_shared_ok(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
@@ -797,12 +802,13 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
     const bool same_ids = ids_gu == ids_dn;
     const bool gated = act_gated(L->act);
     const bool gemm = use_gemm_mx(c, T, K, E);
+    const int bm = mx_bm(c, rows, E);
     // few rows: the work-groups find their rows from the router's ids
     // themselves, unless the caller wants the dispatch's outputs
     const bool self_disp = !gemm && same_ids && !check_ids && !disp_out && rows <= MXV_IDS;
     if (!self_disp) {
-        TRY(launch_dispatch(ids_gu, T, K, E, MXG_BM, 1, c->disp[0].view(), st));
-        if (!same_ids) TRY(launch_dispatch(ids_dn, T, K, E, MXG_BM, 1, c->disp[1].view(), st));
+        TRY(launch_dispatch(ids_gu, T, K, E, bm, 1, c->disp[0].view(), st));
+        if (!same_ids) TRY(launch_dispatch(ids_dn, T, K, E, bm, 1, c->disp[1].view(), st));
     }
     const DispBuf &dg = c->disp[0];
     const DispBuf &dd = same_ids ? c->disp[0] : c->disp[1];
@@ -816,7 +822,7 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
         g.perm = d.perm; g.counts = d.counts; g.offsets = d.offsets; g.active_e = d.active_e; g.n_active = d.n_active;
         g.max_active = max_active;
         g.tile_e = d.tile_e; g.tile_start = d.tile_start; g.tile_rows = d.tile_rows; g.n_tiles = d.n_tiles;
-        g.max_tiles = (int)((rows + MXG_BM - 1) / MXG_BM + max_active);
+        g.max_tiles = (int)((rows + bm - 1) / bm + max_active); g.bm = bm;
         if (self_disp) { g.ids = ids_gu; g.rows = rows; g.n_expert = E; }
         return g;
     };
@@ -1702,7 +1708,7 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
     }
     const int max_active = (int)std::min<int64_t>(E, rows);
     const bool mx = is_mx(as->type);
-    const int bm = mx ? MXG_BM : !gb ? G4_BM : gf_tiles(c, as->type, rows, (int)E, Kin, N) ? GF_BM : gb_bm(c, rows, (int)E, N);
+    const int bm = mx ? mx_bm(c, rows, (int)E) : !gb ? G4_BM : gf_tiles(c, as->type, rows, (int)E, Kin, N) ? GF_BM : gb_bm(c, rows, (int)E, N);
     const int max_tiles = (int)((rows + bm - 1) / bm + max_active);
     const DispBuf &dsp = c->disp[0];
     Dispatch dv = dsp.view();
@@ -1720,7 +1726,7 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
         a.perm = dsp.perm; a.counts = dsp.counts; a.offsets = dsp.offsets; a.active_e = dsp.active_e;
         a.n_active = dsp.n_active; a.max_active = max_active;
         a.tile_e = dsp.tile_e; a.tile_start = dsp.tile_start; a.tile_rows = dsp.tile_rows; a.n_tiles = dsp.n_tiles;
-        a.max_tiles = max_tiles;
+        a.max_tiles = max_tiles; a.bm = bm;
         a.y = (float *)dst->data; a.ldy = N; a.ncols = N;
         return use_gemm_mx(c, T, (int)n_used, (int)E) ? launch_mxg(a, st) : launch_mxv(a, st);
     }

@@ -390,7 +390,8 @@ struct MxArgs : MxSide {
     int64_t rows;
     int n_expert;              // with ids
     int32_t *bad_total;
-    // launch_mxg: balanced tiles of at most MXG_BM rows
+    // launch_mxg: balanced tiles of at most bm rows (MXG_BM or MXG_BM_SMALL)
+    int bm;
     const int32_t *tile_e, *tile_start, *tile_rows, *n_tiles;
     int max_tiles;
     MxSide sh;
@@ -399,7 +400,7 @@ struct MxArgs : MxSide {
     int ncb, sh_wgs;           // (set by the launchers)
 };
 constexpr int MXV_IDS = 512;
-constexpr int MXG_BM = 128;
+constexpr int MXG_BM = 128, MXG_BM_SMALL = 32;
 int launch_mxv(const MxArgs &g, hipStream_t st);
 int launch_mxg(const MxArgs &g, hipStream_t st);
 
