@@ -772,10 +772,17 @@ MxRows mx_rows(void *base, int64_t rows, int64_t K) {
     return m;
 }
 
-// MXFP4: the grouped GEMM above two dispatched rows per expert
-bool use_gemm_mx(const mi_moe_ctx *c, int64_t T, int K, int E) {
+// MXFP4: the grouped GEMM above two dispatched rows per expert (rows further
+// apart than it addresses keep the other kernel)
+bool use_gemm_mx(const mi_moe_ctx *c, int64_t T, int K, int E, size_t row_bytes) {
+    if ((int64_t)row_bytes > MXG_MAX_ROW_BYTES) return false;
     if (c->gemm_threshold > 0) return T >= c->gemm_threshold;
     return T * K > 2 * (int64_t)E;
+}
+bool mx_layer_gemm(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
+    size_t rb = std::max(L->gate.nb[1], L->down.nb[1]);
+    if (act_gated(L->act) && !L->fused_gate_up) rb = std::max(rb, L->up.nb[1]);
+    return use_gemm_mx(c, T, L->n_expert_used, L->n_expert, rb);
 }
 // Row tiles of its GEMM: 128 rows above 32 dispatched rows per expert, else 32
 int mx_bm(const mi_moe_ctx *c, int64_t rows, int E) {
@@ -786,7 +793,7 @@ int mx_bm(const mi_moe_ctx *c, int64_t rows, int E) {
 // table type and activation.
 bool mx_shared_ok(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
     return is_mx(L->gate.type) && is_mx(L->sh_gate.type) && is_mx(L->sh_down.type) && L->sh_act == L->act &&
-           !use_gemm_mx(c, T, L->n_expert_used, L->n_expert) && T <= GV_SHARED_T;
+           !mx_layer_gemm(c, L, T) && T <= GV_SHARED_T;
 }
 
 // routed FFN body of a layer with MXFP4 tables: Q8_0 operand rows (mx.hpp),
@@ -801,7 +808,7 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
     const int max_active = (int)std::min<int64_t>(E, rows);
     const bool same_ids = ids_gu == ids_dn;
     const bool gated = act_gated(L->act);
-    const bool gemm = use_gemm_mx(c, T, K, E);
+    const bool gemm = mx_layer_gemm(c, L, T);
     const int bm = mx_bm(c, rows, E);
     // few rows: the work-groups find their rows from the router's ids
     // themselves, unless the caller wants the dispatch's outputs
@@ -1728,7 +1735,7 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
         a.tile_e = dsp.tile_e; a.tile_start = dsp.tile_start; a.tile_rows = dsp.tile_rows; a.n_tiles = dsp.n_tiles;
         a.max_tiles = max_tiles; a.bm = bm;
         a.y = (float *)dst->data; a.ldy = N; a.ncols = N;
-        return use_gemm_mx(c, T, (int)n_used, (int)E) ? launch_mxg(a, st) : launch_mxv(a, st);
+        return use_gemm_mx(c, T, (int)n_used, (int)E, as->nb[1]) ? launch_mxg(a, st) : launch_mxv(a, st);
     }
     if (is_b32f(as->type)) {
         // b in the table type's vec_dot_type (Q8_0 or fp16), then the grouped GEMV or GEMM

@@ -9,12 +9,19 @@
 // column tile, two blocks), one per digit.  Lane half h of the MFMA takes block
 // 2 step + h.
 //
-// The K loop runs over granules of four blocks (two steps).  Weights: each
-// lane loads the blocks of its own weight rows into registers, a granule ahead
-// (34 bytes of a row per step and 68 per granule lie together).  Activations:
-// through two LDS buffers, a granule ahead, 400 bytes per row (four blocks of
-// 96 and their scale words; 100 dwords apart, the rows of 8 lanes start on
-// different banks), 8 threads to a row's 128 bytes.
+// The K loop runs over stages of eight blocks, two granules of four.
+//  * weights: the 256 weight rows' runs of a stage (136 bytes) reach LDS by
+//    buffer loads that write LDS directly, each row as nine 16-byte pieces from
+//    the dword at or below its first byte (blocks start at any byte, and rows
+//    may be misaligned); the lanes then take their blocks out into registers,
+//    which frees the buffer for the next stage's loads while this one is
+//    computed.  (Each lane loading its own blocks from memory: a wave's load
+//    touches 64 lines, and the load path takes them one by one, 375 us against
+//    MXG_T us at K 2048, N 2048, 64 experts, 16384 rows.)
+//  * activations: through registers and two LDS buffers, a granule ahead, 400
+//    bytes per row (four blocks of 96 and their scale words; 100 dwords apart,
+//    the rows of 8 lanes start on different banks), 8 threads to a row's 128
+//    bytes.
 #include "act.hpp"
 #include "common.hpp"
 #include "launch.hpp"
@@ -25,7 +32,17 @@ namespace mimoe {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int MXG_ROW = 4 * MX_XB + 16;   // LDS bytes of a row's granule
+constexpr int MXG_ROW = 4 * MX_XB + 16;   // LDS bytes of an activation row's granule
+constexpr int MXG_WROWS = 256, MXG_WROW = 144, MXG_WSTAGE = 8 * MX_BYTES;   // weight rows of a work-group, LDS bytes of one's stage, bytes of its run
+constexpr int MXG_WLD = 64 * MXG_WROW / 1024;   // a wave's loads of 64 rows
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+// this wave's vector-memory loads and LDS accesses complete, then the barrier
+__device__ __forceinline__ void mxg_sync() {
+    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0), lgkmcnt(0)
+    asm volatile("s_barrier" ::: "memory");
+}
 
 template <int DIG>
 __device__ __forceinline__ f32x16 mxg_mfma(const i32x8 &a, const i32x8 &b, const f32x16 &c, int sa, int sb) {
@@ -38,7 +55,9 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
     constexpr bool GLU = EPI == MX_GLU;
     constexpr int RG = BM / (NT / 8);   // row groups of a granule's loads (NT / 8 rows each)
     static_assert(BM % (NT / 8) == 0 && BM <= NT, "whole row groups, a row per thread");
-    __shared__ __attribute__((aligned(16))) uint8_t sx[2][BM * MXG_ROW];
+    __shared__ __attribute__((aligned(16))) uint8_t sx0[BM * MXG_ROW];
+    __shared__ __attribute__((aligned(16))) uint8_t sx1[BM * MXG_ROW];
+    __shared__ __attribute__((aligned(16))) uint8_t sw[MXG_WROWS * MXG_WROW];
     __shared__ int s_p[BM];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31, h = lane >> 5;
     const MxSide s = g;
@@ -52,21 +71,44 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
     const int e = g.tile_e[tile], start = g.tile_start[tile], mrows = g.tile_rows[tile];
     const int nb = (int)(s.a.K / 32), ng = (nb + 3) / 4;
     const int wr = wave / WN, wc = wave - wr * WN;
-    // the lane's weight rows (past the matrix: row 0, not stored); GLU: even
-    // column tiles gate rows, odd ones the matching up rows
-    constexpr int CW = GLU ? 16 * C : 32 * C;   // columns of y (of the activation rows) per wave
-    const int64_t n0 = ((int64_t)cb * WN + wc) * CW;
-    const uint8_t *rowp[C];
+    // Columns of y (of the activation rows) of a work-group and a wave.  The
+    // 256 weight rows in LDS: those of the columns in order (GLU: 128 gate
+    // rows, then the 128 matching up rows); wave w loads rows 64 w .. 64 w + 63.
+    constexpr int CB = GLU ? MXG_WROWS / 2 : MXG_WROWS, CW = CB / WN;
+    static_assert(WM * WN == 4 && 32 * C * WN == MXG_WROWS, "four waves, 256 weight rows");
+    const int64_t c0 = (int64_t)cb * CB, n0 = c0 + CW * wc;
+    __amdgpu_buffer_rsrc_t wr_rsrc;
+    uint32_t woff[MXG_WLD];
+    {
+        const bool up = GLU && wave >= 2;
+        const ExpertMat &m = up && !s.fused ? s.b : s.a;
+        const int64_t r0 = c0 + 64 * (GLU ? wave & 1 : wave), left = s.ncols - r0, row0 = (left > 0 ? r0 : 0) + (up && s.fused ? s.I : 0);
+        const uint8_t *p = m.data + (int64_t)e * m.mat_bytes + row0 * m.row_bytes;
+        const uint32_t mis = (uint32_t)(uintptr_t)p & 3u, rb = (uint32_t)m.row_bytes;
+        // (a dword past the last row's bytes reads as zero, as do the rows past the matrix)
+        const uint32_t bytes = left > 0 ? (mis + ((left < 64 ? (uint32_t)left : 64u) - 1) * rb + (uint32_t)nb * MX_BYTES + 3) & ~3u : 0u;
+        wr_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p - mis), (short)0, (int)bytes, 0x00020000);
+#pragma unroll
+        for (int j = 0; j < MXG_WLD; ++j) {
+            const uint32_t q = 64u * (uint32_t)j + (uint32_t)lane, r = q / 9u, k = q - 9u * r;
+            woff[j] = ((mis + r * rb) & ~3u) + 16u * k;
+        }
+    }
+    auto load_w = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < MXG_WLD; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr_rsrc, (lds_void_t *)(sw + 64 * MXG_WROW * wave + 1024 * j), 16, (int)woff[j],
+                                                     MXG_WSTAGE * st, 0, 0);
+    };
+    // where the lane's weight rows start in the buffer: their first byte's place
+    uint32_t wat[C];
 #pragma unroll
     for (int ct = 0; ct < C; ++ct) {
-        const int64_t col = n0 + 32 * (GLU ? ct / 2 : ct) + l32;
-        int64_t row = col < s.ncols ? col : 0;
-        if (GLU && (ct & 1) && !s.fused) {
-            rowp[ct] = s.b.data + (int64_t)e * s.b.mat_bytes + row * s.b.row_bytes;
-        } else {
-            if (GLU && (ct & 1)) row += s.I;
-            rowp[ct] = s.a.data + (int64_t)e * s.a.mat_bytes + row * s.a.row_bytes;
-        }
+        const int lr = GLU ? 128 * (ct & 1) + CW * wc + 32 * (ct / 2) + l32 : CW * wc + 32 * ct + l32;   // its row in LDS
+        const bool up = GLU && (ct & 1);
+        const ExpertMat &m = up && !s.fused ? s.b : s.a;
+        const int64_t row = c0 + (GLU ? lr & 127 : lr) + (up && s.fused ? s.I : 0);
+        wat[ct] = (uint32_t)(MXG_WROW * lr) + ((uint32_t)((uintptr_t)m.data + (uintptr_t)((int64_t)e * m.mat_bytes + row * m.row_bytes)) & 3u);
     }
     // the rows of this thread's activation loads (past the tile: its first row, not stored)
     const int kdiv = g.ne11 == 1 ? g.K : 1, l8 = tid & 7;
@@ -84,15 +126,6 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
         if (tid < BM) s_p[tid] = p;
         xsc = s.x.xs + (int64_t)(kdiv > 1 ? p / kdiv : p) * nb;
     }
-    MxRaw raw[2][C];
-    auto load_w = [&](int gr) __attribute__((always_inline)) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int b = 4 * gr + 2 * t + h;
-#pragma unroll
-            for (int ct = 0; ct < C; ++ct) mx_load(rowp[ct] + MX_BYTES * (b < nb ? b : nb - 1), raw[t][ct]);
-        }
-    };
     uint4 areg[RG][3];
     uint32_t asc[SW];
     auto load_a = [&](int gr) __attribute__((always_inline)) {
@@ -126,37 +159,24 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
         for (int ct = 0; ct < C; ++ct)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[rt][ct][i] = 0.f;
-    load_w(0);
-    load_a(0);
-    store_a(sx[0]);
-    lds_barrier();
     const int nrt = (mrows - 32 * R * wr + 31) >> 5;   // row tiles of this wave that hold rows
-    for (int gr = 0; gr < ng; ++gr) {
-        const bool more = gr + 1 < ng;
-        // the granule's weight operands out of the loaded dwords, whose registers take the next granule's
-        i32x8 B[2][C];
-        int sb[2][C];
+    // the granule gr's products: weight blocks raw, activations at X
+    auto granule = [&](int gr, const MxRaw (&raw)[2][C], const uint8_t *X) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int b = 4 * gr + 2 * t + h;
             const bool in = b < nb;
+            i32x8 B[C];
+            int sb[C];
 #pragma unroll
             for (int ct = 0; ct < C; ++ct) {
-                const uint32_t mis = (uint32_t)((uintptr_t)rowp[ct] + (uint32_t)(MX_BYTES * (in ? b : nb - 1))) & 3u;
+                const uint32_t mis = (wat[ct] + (uint32_t)(MX_BYTES * (b & 7))) & 3u;
                 uint32_t c[4];
                 mx_codes(raw[t][ct], mis, c);
                 // (a block past the row: the operand's digits are zero, the scale any number)
-                sb[t][ct] = in ? (int)mx_scale(raw[t][ct], mis) : (int)MX_ONE;
-                B[t][ct] = i32x8{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+                sb[ct] = in ? (int)mx_scale(raw[t][ct], mis) : (int)MX_ONE;
+                B[ct] = i32x8{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
             }
-        }
-        if (more) {
-            load_w(gr + 1);
-            load_a(gr + 1);
-        }
-        const uint8_t *X = sx[gr & 1];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int rt = 0; rt < R; ++rt) {
                 if (rt >= nrt) break;
@@ -171,17 +191,47 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
                     A[i] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, 0, 0};
                 }
 #pragma unroll
-                for (int ct = 0; ct < C; ++ct) acc[rt][ct] = mxg_mfma<0>(A[0], B[t][ct], acc[rt][ct], sa, sb[t][ct]);
+                for (int ct = 0; ct < C; ++ct) acc[rt][ct] = mxg_mfma<0>(A[0], B[ct], acc[rt][ct], sa, sb[ct]);
 #pragma unroll
-                for (int ct = 0; ct < C; ++ct) acc[rt][ct] = mxg_mfma<1>(A[1], B[t][ct], acc[rt][ct], sa, sb[t][ct]);
+                for (int ct = 0; ct < C; ++ct) acc[rt][ct] = mxg_mfma<1>(A[1], B[ct], acc[rt][ct], sa, sb[ct]);
 #pragma unroll
-                for (int ct = 0; ct < C; ++ct) acc[rt][ct] = mxg_mfma<2>(A[2], B[t][ct], acc[rt][ct], sa, sb[t][ct]);
+                for (int ct = 0; ct < C; ++ct) acc[rt][ct] = mxg_mfma<2>(A[2], B[ct], acc[rt][ct], sa, sb[ct]);
 #pragma unroll
-                for (int ct = 0; ct < C; ++ct) acc[rt][ct] = mxg_mfma<3>(A[3], B[t][ct], acc[rt][ct], sa, sb[t][ct]);
+                for (int ct = 0; ct < C; ++ct) acc[rt][ct] = mxg_mfma<3>(A[3], B[ct], acc[rt][ct], sa, sb[ct]);
             }
-        if (more) store_a(sx[(gr + 1) & 1]);
+        }
+    };
+    load_a(0);
+    asm volatile("" ::: "memory");   // (the activations' loads first: waiting for them leaves the weights' in flight)
+    load_w(0);
+    store_a(sx0);
+    const int nst = (ng + 1) / 2;
+    for (int st = 0; st < nst; ++st) {
+        const bool second = 2 * st + 1 < ng, next = st + 1 < nst;
+        mxg_sync();   // the stage's weights and its first granule's activations are in LDS
+        MxRaw raw[2][2][C];
+#pragma unroll
+        for (int gg = 0; gg < 2; ++gg)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int ct = 0; ct < C; ++ct) {
+                    const uint32_t at = (wat[ct] + (uint32_t)(MX_BYTES * (4 * gg + 2 * t + h))) & ~3u;
+#pragma unroll
+                    for (int i = 0; i < 5; ++i) raw[gg][t][ct].w[i] = *(const uint32_t *)(sw + at + 4 * i);
+                }
+        if (second) load_a(2 * st + 1);
+        lds_barrier();   // the blocks are in registers
+        if (next) load_w(st + 1);
+        granule(2 * st, raw[0], sx0);
+        if (!second) break;
+        store_a(sx1);
         lds_barrier();
+        if (next) load_a(2 * st + 2);
+        granule(2 * st + 1, raw[1], sx1);
+        if (next) store_a(sx0);
     }
+    lds_barrier();
     // accumulator i of the lane: row 8 (i / 4) + 4 h + i % 4 of the row tile, column l32
     if constexpr (EPI == MX_STORE) {
 #pragma unroll
@@ -198,9 +248,8 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
                 }
             }
     } else {
-        // (4 KB of the wave's own: no wave reads the activations any more)
-        float *v = (float *)(sx[0] + 4096 * wave);
-        static_assert(4096 * WM * WN <= 2 * BM * MXG_ROW, "LDS of the epilogue");
+        // (4 KB of the wave's own in the weights' buffer, which no wave reads or loads any more)
+        float *v = (float *)(sw + 4096 * wave);
 #pragma unroll
         for (int rt = 0; rt < R; ++rt)
 #pragma unroll
@@ -228,7 +277,7 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
 template <int EPI>
 static int mxg_launch(const MxArgs &a, hipStream_t st) {
     MxArgs g = a;
-    constexpr int COLS = EPI == MX_GLU ? 128 : 256;   // per work-group
+    constexpr int COLS = EPI == MX_GLU ? MXG_WROWS / 2 : MXG_WROWS;   // per work-group
     g.ncb = (int)((g.ncols + COLS - 1) / COLS);
     const int64_t wgs = 8 * (int64_t)g.ncb * ((g.max_tiles + 7) / 8);
     if (wgs > 0x7fffffff) return -6;
@@ -240,6 +289,7 @@ static int mxg_launch(const MxArgs &a, hipStream_t st) {
 int launch_mxg(const MxArgs &g, hipStream_t st) {
     if (g.max_tiles <= 0) return 0;
     if (g.bm != MXG_BM && g.bm != MXG_BM_SMALL) return -6;
+    if (g.a.row_bytes > MXG_MAX_ROW_BYTES || (g.epi == MX_GLU && !g.fused && g.b.row_bytes > MXG_MAX_ROW_BYTES)) return -6;
     if (g.a.type != 39 || g.a.K % 32 || g.a.K > 0x7fffffff || (g.epi != MX_STORE && g.ncols % 32)) return -6;
     switch (g.epi) {
     case MX_STORE: return mxg_launch<MX_STORE>(g, st);
