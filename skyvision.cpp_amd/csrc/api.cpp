@@ -784,7 +784,7 @@ bool mx_layer_gemm(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
     if (act_gated(L->act) && !L->fused_gate_up) rb = std::max(rb, L->up.nb[1]);
     return use_gemm_mx(c, T, L->n_expert_used, L->n_expert, rb);
 }
-// Row tiles of its GEMM: 128 rows above 32 dispatched rows per expert, else 32
+// Row tiles of its GEMM: 64 rows above 32 dispatched rows per expert, else 32
 int mx_bm(const mi_moe_ctx *c, int64_t rows, int E) {
     if (c->gemm_tiles == 1 || c->gemm_tiles == 2) return c->gemm_tiles == 1 ? MXG_BM : MXG_BM_SMALL;
     return rows > 32 * (int64_t)E ? MXG_BM : MXG_BM_SMALL;

@@ -9,19 +9,17 @@
 // column tile, two blocks), one per digit.  Lane half h of the MFMA takes block
 // 2 step + h.
 //
-// The K loop runs over stages of eight blocks, two granules of four.
-//  * weights: the 256 weight rows' runs of a stage (136 bytes) reach LDS by
-//    buffer loads that write LDS directly, each row as nine 16-byte pieces from
-//    the dword at or below its first byte (blocks start at any byte, and rows
-//    may be misaligned); the lanes then take their blocks out into registers,
-//    which frees the buffer for the next stage's loads while this one is
-//    computed.  (Each lane loading its own blocks from memory: a wave's load
-//    touches 64 lines, and the load path takes them one by one, 375 us against
-//    MXG_T us at K 2048, N 2048, 64 experts, 16384 rows.)
-//  * activations: through registers and two LDS buffers, a granule ahead, 400
-//    bytes per row (four blocks of 96 and their scale words; 100 dwords apart,
-//    the rows of 8 lanes start on different banks), 8 threads to a row's 128
-//    bytes.
+// The K loop runs over granules of four blocks (two steps).
+//  * weights: the 256 weight rows' runs of a granule (68 bytes) reach one of
+//    two LDS buffers by buffer loads that write LDS directly, a granule ahead,
+//    each row as five 16-byte pieces from the dword at or below its first byte
+//    (blocks start at any byte, and rows may be misaligned; rows 20 dwords
+//    apart start on 16 different banks).
+//  * activations: a granule ahead in registers, one LDS buffer, 400 bytes per
+//    row (four blocks of 96 and their scale words; 100 dwords apart, the rows
+//    of 8 lanes start on different banks), 8 threads to a row's 128 bytes.
+// Two work-groups to a CU (three with 32-row tiles), one's waits and stores
+// beside the other's MFMAs.
 #include "act.hpp"
 #include "common.hpp"
 #include "launch.hpp"
@@ -33,7 +31,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int MXG_ROW = 4 * MX_XB + 16;   // LDS bytes of an activation row's granule
-constexpr int MXG_WROWS = 256, MXG_WROW = 144, MXG_WSTAGE = 8 * MX_BYTES;   // weight rows of a work-group, LDS bytes of one's stage, bytes of its run
+constexpr int MXG_WROWS = 256, MXG_WROW = 80, MXG_WRUN = 4 * MX_BYTES;   // weight rows of a work-group, LDS bytes of one's granule, bytes of its run
 constexpr int MXG_WLD = 64 * MXG_WROW / 1024;   // a wave's loads of 64 rows
 
 typedef __attribute__((address_space(3))) void lds_void_t;
@@ -50,14 +48,14 @@ __device__ __forceinline__ f32x16 mxg_mfma(const i32x8 &a, const i32x8 &b, const
 }
 
 template <int EPI, int R, int C, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) {
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM == 1 ? 3 : 2))) k_mxg(MxArgs g) {
     constexpr int BM = 32 * R * WM, NT = 64 * WM * WN;
     constexpr bool GLU = EPI == MX_GLU;
     constexpr int RG = BM / (NT / 8);   // row groups of a granule's loads (NT / 8 rows each)
     static_assert(BM % (NT / 8) == 0 && BM <= NT, "whole row groups, a row per thread");
-    __shared__ __attribute__((aligned(16))) uint8_t sx0[BM * MXG_ROW];
-    __shared__ __attribute__((aligned(16))) uint8_t sx1[BM * MXG_ROW];
-    __shared__ __attribute__((aligned(16))) uint8_t sw[MXG_WROWS * MXG_WROW];
+    __shared__ __attribute__((aligned(16))) uint8_t sx[BM * MXG_ROW];
+    __shared__ __attribute__((aligned(16))) uint8_t sw0[MXG_WROWS * MXG_WROW];
+    __shared__ __attribute__((aligned(16))) uint8_t sw1[MXG_WROWS * MXG_WROW];
     __shared__ int s_p[BM];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31, h = lane >> 5;
     const MxSide s = g;
@@ -90,15 +88,15 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
         wr_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p - mis), (short)0, (int)bytes, 0x00020000);
 #pragma unroll
         for (int j = 0; j < MXG_WLD; ++j) {
-            const uint32_t q = 64u * (uint32_t)j + (uint32_t)lane, r = q / 9u, k = q - 9u * r;
+            const uint32_t q = 64u * (uint32_t)j + (uint32_t)lane, r = q / 5u, k = q - 5u * r;
             woff[j] = ((mis + r * rb) & ~3u) + 16u * k;
         }
     }
-    auto load_w = [&](int st) __attribute__((always_inline)) {
+    auto load_w = [&](int gr, uint8_t *sw) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < MXG_WLD; ++j)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(wr_rsrc, (lds_void_t *)(sw + 64 * MXG_WROW * wave + 1024 * j), 16, (int)woff[j],
-                                                     MXG_WSTAGE * st, 0, 0);
+                                                     MXG_WRUN * gr, 0, 0);
     };
     // where the lane's weight rows start in the buffer: their first byte's place
     uint32_t wat[C];
@@ -160,27 +158,29 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[rt][ct][i] = 0.f;
     const int nrt = (mrows - 32 * R * wr + 31) >> 5;   // row tiles of this wave that hold rows
-    // the granule gr's products: weight blocks raw, activations at X
-    auto granule = [&](int gr, const MxRaw (&raw)[2][C], const uint8_t *X) __attribute__((always_inline)) {
+    // the products of granule gr, its weights at sw
+    auto granule = [&](int gr, const uint8_t *sw) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int b = 4 * gr + 2 * t + h;
-            const bool in = b < nb;
+            const bool in = 4 * gr + 2 * t + h < nb;
             i32x8 B[C];
             int sb[C];
 #pragma unroll
             for (int ct = 0; ct < C; ++ct) {
-                const uint32_t mis = (wat[ct] + (uint32_t)(MX_BYTES * (b & 7))) & 3u;
+                const uint32_t at = wat[ct] + (uint32_t)(MX_BYTES * (2 * t + h));
+                MxRaw raw;
+#pragma unroll
+                for (int i = 0; i < 5; ++i) raw.w[i] = *(const uint32_t *)(sw + (at & ~3u) + 4 * i);
                 uint32_t c[4];
-                mx_codes(raw[t][ct], mis, c);
+                mx_codes(raw, at & 3u, c);
                 // (a block past the row: the operand's digits are zero, the scale any number)
-                sb[ct] = in ? (int)mx_scale(raw[t][ct], mis) : (int)MX_ONE;
+                sb[ct] = in ? (int)mx_scale(raw, at & 3u) : (int)MX_ONE;
                 B[ct] = i32x8{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
             }
 #pragma unroll
             for (int rt = 0; rt < R; ++rt) {
                 if (rt >= nrt) break;
-                const uint8_t *xr = X + (32 * (R * wr + rt) + l32) * MXG_ROW;
+                const uint8_t *xr = sx + (32 * (R * wr + rt) + l32) * MXG_ROW;
                 const uint8_t *x = xr + (2 * t + h) * MX_XB;
                 const int sa = *(const int *)(xr + 4 * MX_XB + 4 * (2 * t + h));
                 i32x8 A[4];
@@ -201,37 +201,27 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
             }
         }
     };
+    auto turn = [&](int gr, const uint8_t *cur, uint8_t *nxt) __attribute__((always_inline)) {
+        const bool more = gr + 1 < ng;
+        if (more) {
+            load_a(gr + 1);
+            load_w(gr + 1, nxt);
+        }
+        granule(gr, cur);
+        mxg_sync();   // the next granule has come, and no wave reads this one's activations
+        if (more) {
+            store_a(sx);
+            lds_barrier();
+        }
+    };
+    load_w(0, sw0);
     load_a(0);
-    asm volatile("" ::: "memory");   // (the activations' loads first: waiting for them leaves the weights' in flight)
-    load_w(0);
-    store_a(sx0);
-    const int nst = (ng + 1) / 2;
-    for (int st = 0; st < nst; ++st) {
-        const bool second = 2 * st + 1 < ng, next = st + 1 < nst;
-        mxg_sync();   // the stage's weights and its first granule's activations are in LDS
-        MxRaw raw[2][2][C];
-#pragma unroll
-        for (int gg = 0; gg < 2; ++gg)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int ct = 0; ct < C; ++ct) {
-                    const uint32_t at = (wat[ct] + (uint32_t)(MX_BYTES * (4 * gg + 2 * t + h))) & ~3u;
-#pragma unroll
-                    for (int i = 0; i < 5; ++i) raw[gg][t][ct].w[i] = *(const uint32_t *)(sw + at + 4 * i);
-                }
-        if (second) load_a(2 * st + 1);
-        lds_barrier();   // the blocks are in registers
-        if (next) load_w(st + 1);
-        granule(2 * st, raw[0], sx0);
-        if (!second) break;
-        store_a(sx1);
-        lds_barrier();
-        if (next) load_a(2 * st + 2);
-        granule(2 * st + 1, raw[1], sx1);
-        if (next) store_a(sx0);
+    store_a(sx);
+    mxg_sync();
+    for (int gr = 0; gr < ng; gr += 2) {
+        turn(gr, sw0, sw1);
+        if (gr + 1 < ng) turn(gr + 1, sw1, sw0);
     }
-    lds_barrier();
     // accumulator i of the lane: row 8 (i / 4) + 4 h + i % 4 of the row tile, column l32
     if constexpr (EPI == MX_STORE) {
 #pragma unroll
@@ -248,8 +238,8 @@ __global__ void __launch_bounds__(64 * WM * WN, R == 1 ? 2 : 1) k_mxg(MxArgs g) 
                 }
             }
     } else {
-        // (4 KB of the wave's own in the weights' buffer, which no wave reads or loads any more)
-        float *v = (float *)(sw + 4096 * wave);
+        // (4 KB of the wave's own in a weights' buffer, which no wave reads or loads any more)
+        float *v = (float *)(sw0 + 4096 * wave);
 #pragma unroll
         for (int rt = 0; rt < R; ++rt)
 #pragma unroll
@@ -281,7 +271,7 @@ static int mxg_launch(const MxArgs &a, hipStream_t st) {
     g.ncb = (int)((g.ncols + COLS - 1) / COLS);
     const int64_t wgs = 8 * (int64_t)g.ncb * ((g.max_tiles + 7) / 8);
     if (wgs > 0x7fffffff) return -6;
-    if (g.bm == MXG_BM) hipLaunchKernelGGL((k_mxg<EPI, 2, 4, 2, 2>), dim3((unsigned)wgs), dim3(256), 0, st, g);
+    if (g.bm == MXG_BM) hipLaunchKernelGGL((k_mxg<EPI, 1, 4, 2, 2>), dim3((unsigned)wgs), dim3(256), 0, st, g);
     else hipLaunchKernelGGL((k_mxg<EPI, 1, 2, 1, 4>), dim3((unsigned)wgs), dim3(256), 0, st, g);
     return hip_check_launch();
 }

@@ -400,7 +400,7 @@ struct MxArgs : MxSide {
     int ncb, sh_wgs;           // (set by the launchers)
 };
 constexpr int MXV_IDS = 512;
-constexpr int MXG_BM = 128, MXG_BM_SMALL = 32;
+constexpr int MXG_BM = 64, MXG_BM_SMALL = 32;
 constexpr int64_t MXG_MAX_ROW_BYTES = 1ll << 22;   // of launch_mxg (64 rows within 32-bit offsets)
 int launch_mxv(const MxArgs &g, hipStream_t st);
 int launch_mxg(const MxArgs &g, hipStream_t st);
