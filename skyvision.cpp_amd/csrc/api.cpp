@@ -762,20 +762,22 @@ int run_experts_b32(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_
     return MI_MOE_OK;
 }
 
-// The operand rows (mx.hpp) of `rows` rows of K values in an activation set:
-// its code, scale, block-sum and fp16 arrays are one run of 1 + 1/64 + 1/8 + 2
-// bytes per value (carve_workspace), the operand takes 3 + 1/8.
-MxRows mx_rows(void *base, int64_t rows, int64_t K) {
-    MxRows m;
-    m.xb = (uint8_t *)base;
-    m.xs = (uint32_t *)(m.xb + rows * (K / 32) * MX_XB);
-    return m;
+// The operand rows (mx.hpp) of an activation set lie over its code, scale,
+// block-sum and fp16 arrays: those are one run of 1 + 1/64 + 1/8 + 2 bytes per
+// value of rows filled up to 256 values (carve_workspace), the operand takes 3 +
+// 1/8 per value of rows filled up to 128.
+uint8_t *mx_rows(const ActBuf &a) { return (uint8_t *)a.q8; }
+// tokens per pass of its grouped GEMM, which reads the rows through 32-bit
+// offsets; row_bytes: a token's operand bytes
+int64_t mx_max_tokens(int64_t row_bytes) { return MXG_MAX_X / row_bytes; }
+int64_t mx_layer_tokens(const mi_moe_layer *L) {
+    return mx_max_tokens(std::max(mx_row(L->n_embd / 32), L->n_expert_used * mx_row(L->n_ff / 32)));
 }
 
 // MXFP4: the grouped GEMM above two dispatched rows per expert (rows further
 // apart than it addresses keep the other kernel)
 bool use_gemm_mx(const mi_moe_ctx *c, int64_t T, int K, int E, size_t row_bytes) {
-    if ((int64_t)row_bytes > MXG_MAX_ROW_BYTES) return false;
+    if ((int64_t)row_bytes > MXG_MAX_ROW_BYTES) return false;   // (then a token's operand row is far below MXG_MAX_X)
     if (c->gemm_threshold > 0) return T >= c->gemm_threshold;
     return T * K > 2 * (int64_t)E;
 }
@@ -792,8 +794,10 @@ int mx_bm(const mi_moe_ctx *c, int64_t rows, int E) {
 // The shared expert in the routed experts' launches of few rows: the same
 // table type and activation.
 bool mx_shared_ok(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
+    // (its activation rows go to f1, which holds cap_kmax and 2 cap_I floats per slot)
+    if (mx_row(L->sh_n_ff / 32) > 4 * (int64_t)L->n_expert_used * std::max(L->n_embd, 2 * L->n_ff)) return false;
     return is_mx(L->gate.type) && is_mx(L->sh_gate.type) && is_mx(L->sh_down.type) && L->sh_act == L->act &&
-           !mx_layer_gemm(c, L, T) && T <= GV_SHARED_T;
+           !(mx_layer_gemm(c, L, T) && mx_layer_tokens(L) > 0) && T <= GV_SHARED_T;
 }
 
 // routed FFN body of a layer with MXFP4 tables: Q8_0 operand rows (mx.hpp),
@@ -808,8 +812,20 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
     const int max_active = (int)std::min<int64_t>(E, rows);
     const bool same_ids = ids_gu == ids_dn;
     const bool gated = act_gated(L->act);
-    const bool gemm = mx_layer_gemm(c, L, T);
+    const bool gemm = mx_layer_gemm(c, L, T) && mx_layer_tokens(L) > 0;
     const int bm = mx_bm(c, rows, E);
+    const int64_t tmax = mx_layer_tokens(L);
+    if (gemm && T > tmax) {
+        // in passes; then the dispatch of the whole call, whose counts, offsets and lists the caller may read
+        for (int64_t t0 = 0; t0 < T; t0 += tmax) {
+            const int64_t n = std::min(tmax, T - t0);
+            TRY(run_experts_mx(c, L, x + t0 * D, n, ids_gu + t0 * K, ids_dn + t0 * K, w + t0 * K, res ? res + t0 * D : nullptr,
+                               out + t0 * D, st, check_ids, add ? add + t0 * D : nullptr, disp_out, false, nullptr));
+        }
+        DispBuf whole = c->disp[0];
+        whole.bad_total = nullptr;   // (counted by the passes)
+        return launch_dispatch(ids_gu, T, K, E, bm, 1, whole.view(), st);
+    }
     // few rows: the work-groups find their rows from the router's ids
     // themselves, unless the caller wants the dispatch's outputs
     const bool self_disp = !gemm && same_ids && !check_ids && !disp_out && rows <= MXV_IDS;
@@ -820,7 +836,7 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
     const DispBuf &dg = c->disp[0];
     const DispBuf &dd = same_ids ? c->disp[0] : c->disp[1];
     stage_end(c, "dispatch", st);
-    const MxRows mx = mx_rows(c->ax.q8, T, D), ma = mx_rows(c->aact.q8, rows, I);
+    uint8_t *mx = mx_rows(c->ax), *ma = mx_rows(c->aact);
     TRY(launch_prep_mx(x, D, T, D, mx, st));
     stage_end(c, "q8_x", st);
     auto args_for = [&](const ExpertMat &t, const DispBuf &d, int ne11) {
@@ -836,10 +852,10 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
     MxArgs a = args_for(as_mat(L->gate), dg, 1);
     if (gated && !L->fused_gate_up) a.b = as_mat(L->up);
     a.epi = gated ? MX_GLU : MX_RELU_SQR; a.fused = L->fused_gate_up; a.I = I;
-    a.x = mx; a.o = ma; a.ncols = I;
+    a.x = mx; a.xrows = T; a.o = ma; a.ncols = I;
     a.bad_total = c->bad_total;   // (with ids: once per call, here)
     MxArgs d = args_for(as_mat(L->down), dd, K);
-    d.epi = MX_STORE; d.x = ma; d.y = c->z; d.ldy = D; d.ncols = D;
+    d.epi = MX_STORE; d.x = ma; d.xrows = rows; d.y = c->z; d.ldy = D; d.ncols = D;
     if (sh_here) {
         const int64_t S = L->sh_n_ff;
         a.sh_rows = d.sh_rows = T;
@@ -847,7 +863,8 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
         if (gated) a.sh.b = as_mat(L->sh_up);
         a.sh.I = a.sh.ncols = S;
         a.sh.x = mx;
-        a.sh.o = d.sh.x = mx_rows(c->f1, T, S);   // (f1 is free on this path, and holds 2 cap_I floats per slot)
+        a.sh.o = (uint8_t *)c->f1;   // (free on this path)
+        d.sh.x = a.sh.o;
         d.sh.a = as_mat(L->sh_down);
         d.sh.y = c->sh_out; d.sh.ldy = d.sh.ncols = D;
         d.sh_w = sh_w;
@@ -1700,9 +1717,11 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
     const int64_t rows = T * n_used;
     // the grouped GEMM of the 32-value types and F16, in passes past its 32-bit
     // offsets (a single token's rows past them: the GEMV)
-    const int64_t ldx = round_up(Kin, 64), tmax = gb_max_tokens(ne11 * ldx);
+    const bool mx = is_mx(as->type);
+    const int64_t ldx = round_up(Kin, 64), tmax = mx ? mx_max_tokens(ne11 * mx_row(Kin / 32)) : gb_max_tokens(ne11 * ldx);
+    const bool mxg = mx && use_gemm_mx(c, T, (int)n_used, (int)E, as->nb[1]) && tmax > 0;
     const bool gb = is_b32f(as->type) && use_gemm_wide(c, T, (int)n_used, (int)E) && gb_strides_ok(*as) && tmax > 0;
-    if (gb && T > tmax) {
+    if ((gb || mxg) && T > tmax) {
         for (int64_t t0 = 0; t0 < T; t0 += tmax) {
             const int64_t n = std::min(tmax, T - t0);
             mi_tensor bt = *b, it = *ids, dt = *dst;
@@ -1714,7 +1733,6 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
         return MI_MOE_OK;
     }
     const int max_active = (int)std::min<int64_t>(E, rows);
-    const bool mx = is_mx(as->type);
     const int bm = mx ? mx_bm(c, rows, (int)E) : !gb ? G4_BM : gf_tiles(c, as->type, rows, (int)E, Kin, N) ? GF_BM : gb_bm(c, rows, (int)E, N);
     const int max_tiles = (int)((rows + bm - 1) / bm + max_active);
     const DispBuf &dsp = c->disp[0];
@@ -1728,14 +1746,14 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
     if (mx) {
         MxArgs a = {};
         a.a = M; a.epi = MX_STORE; a.ne11 = (int)ne11; a.K = (int)n_used;
-        a.x = mx_rows(c->ax.q8, T * ne11, Kin);
-        TRY(launch_prep_mx(bp, Kin, T * ne11, Kin, a.x, st));
+        a.x = mx_rows(c->ax); a.xrows = T * ne11;
+        TRY(launch_prep_mx(bp, Kin, T * ne11, Kin, mx_rows(c->ax), st));
         a.perm = dsp.perm; a.counts = dsp.counts; a.offsets = dsp.offsets; a.active_e = dsp.active_e;
         a.n_active = dsp.n_active; a.max_active = max_active;
         a.tile_e = dsp.tile_e; a.tile_start = dsp.tile_start; a.tile_rows = dsp.tile_rows; a.n_tiles = dsp.n_tiles;
         a.max_tiles = max_tiles; a.bm = bm;
         a.y = (float *)dst->data; a.ldy = N; a.ncols = N;
-        return use_gemm_mx(c, T, (int)n_used, (int)E, as->nb[1]) ? launch_mxg(a, st) : launch_mxv(a, st);
+        return mxg ? launch_mxg(a, st) : launch_mxv(a, st);
     }
     if (is_b32f(as->type)) {
         // b in the table type's vec_dot_type (Q8_0 or fp16), then the grouped GEMV or GEMM

@@ -163,23 +163,25 @@ int launch_dequantize(int type, const void *src, float *dst, int64_t nblocks, hi
 // (mx.hpp): four threads per block.  Memory-bound.
 template <bool VEC>
 __global__ void __launch_bounds__(256) k_prep_mx(const float *__restrict__ src, int64_t ld, int64_t nrows, int nb,
-                                                 uint8_t *__restrict__ xb, uint32_t *__restrict__ xs) {
+                                                 uint8_t *__restrict__ rows) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, blk = i >> 2;
     const bool live = blk < nrows * nb;
     const int64_t r = live ? blk / nb : 0, b = live ? blk - r * nb : 0;
     float v[8];
     mx_load8<VEC>(src + r * ld + 32 * b, (int)(i & 3), v);
-    mx_store_block(v, xb + blk * MX_XB, xs + blk, (int)(i & 3), live);
+    uint8_t *row = rows + r * mx_row(nb);
+    mx_store_block(v, row, b, (int)(i & 3), live);
+    if (live && b == nb - 1) mx_store_pad(row, nb, (int)(i & 3));
 }
 
-int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, hipStream_t st) {
+int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, uint8_t *rows, hipStream_t st) {
     if (nrows <= 0) return 0;
     if (K % 32 || K > 0x7fffffff) return -6;
     const int64_t wgs = (nrows * (K / 8) + 255) / 256;
     if (wgs > 0x7fffffff) return -6;
     if (ld % 4 == 0 && (uintptr_t)src % 16 == 0)
-        hipLaunchKernelGGL(k_prep_mx<true>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), o.xb, o.xs);
-    else hipLaunchKernelGGL(k_prep_mx<false>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), o.xb, o.xs);
+        hipLaunchKernelGGL(k_prep_mx<true>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), rows);
+    else hipLaunchKernelGGL(k_prep_mx<false>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), rows);
     return hip_check_launch();
 }
 
@@ -220,8 +222,7 @@ constexpr int MXV_KB = 4 * 2 * MXV_U;                 // blocks of a pass over K
 
 template <int EPI, bool SH>
 __global__ void __launch_bounds__(64 * MXV_WAVES) k_mxv(MxArgs g) {
-    __shared__ __attribute__((aligned(16))) uint8_t sx[MXV_NT][MXV_KB * MX_XB];
-    __shared__ uint32_t ss[MXV_NT][MXV_KB];
+    __shared__ __attribute__((aligned(16))) uint8_t sx[MXV_NT][MXV_KB / 4 * MX_XG];
     __shared__ double s_sum[MXV_NT][128];
     __shared__ float s_v[MXV_NT][64];
     __shared__ int s_p[MXV_IDS];
@@ -313,10 +314,8 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) k_mxv(MxArgs g) {
                 if (k0 || n0 || q0) __syncthreads();   // (the activations before are read)
                 for (int n = 0; n < nt; ++n) {
                     const int p = s_p[n0 + n];
-                    const int64_t r = (int64_t)(kdiv > 1 ? p / kdiv : p) * nb + k0;
-                    const uint4 *src = (const uint4 *)(s.x.xb + r * MX_XB);
-                    for (int i = tid; i < kn * (MX_XB / 16); i += 64 * MXV_WAVES) *(uint4 *)(sx[n] + 16 * i) = src[i];
-                    for (int i = tid; i < kn; i += 64 * MXV_WAVES) ss[n][i] = s.x.xs[r + i];
+                    const uint4 *src = (const uint4 *)(s.x + (int64_t)(kdiv > 1 ? p / kdiv : p) * mx_row(nb) + mx_row(k0));
+                    for (int i = tid; i < nst * (MX_XG / 16); i += 64 * MXV_WAVES) *(uint4 *)(sx[n] + 16 * i) = src[i];
                 }
                 __syncthreads();
 #pragma unroll
@@ -337,12 +336,12 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) k_mxv(MxArgs g) {
                         i32x8 B = {0, 0, 0, 0, 0, 0, 0, 0};
                         int sb = (int)MX_ONE;
                         if (on && in) {
-                            const uint8_t *x = sx[n] + MX_XB * b;
+                            const uint8_t *x = sx[n] + MX_XG * (s0 + u) + MX_XB * grp + 8 * (grp & 2);   // (b = 4 (s0 + u) + grp)
                             const uint4 lo = *(const uint4 *)(x + 16 * dig);
                             const uint2 hi = *(const uint2 *)(x + 64 + 8 * dig);
                             B[0] = (int)lo.x; B[1] = (int)lo.y; B[2] = (int)lo.z; B[3] = (int)lo.w;
                             B[4] = (int)hi.x; B[5] = (int)hi.y;
-                            sb = (int)((ss[n][b] >> (8 * dig)) & 0xffu);
+                            sb = sx[n][MX_XG * (s0 + u) + 2 * MX_XB + 4 * grp + dig];
                         }
                         float4_t z = {0.f, 0.f, 0.f, 0.f};
                         z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, z, 4, 2, 0, sa, 0, sb);
@@ -387,8 +386,8 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) k_mxv(MxArgs g) {
                     const int m = tid / (COLS / 8), blk = (tid >> 2) % (COLS / 32);
                     float v[8];
                     mx_load8<false>(s_v[m] + 32 * blk, tid & 3, v);
-                    const int64_t ob = (int64_t)(m < nt ? s_p[n0 + m] : 0) * (s.ncols / 32) + (int64_t)cb * (COLS / 32) + blk;
-                    mx_store_block(v, s.o.xb + ob * MX_XB, s.o.xs + ob, tid & 3, m < nt && (int64_t)cb * COLS + 32 * blk < s.ncols);
+                    mx_store_block(v, s.o + (int64_t)(m < nt ? s_p[n0 + m] : 0) * mx_row(s.ncols / 32), (int64_t)cb * (COLS / 32) + blk, tid & 3,
+                                   m < nt && (int64_t)cb * COLS + 32 * blk < s.ncols);
                 }
             }
             // (s_sum and s_v are written again after the barriers in front of the next rows' products)

@@ -354,12 +354,8 @@ int launch_gb(const GBArgs &g, hipStream_t st);
 int launch_quantize_mx(const float *src, void *dst, int64_t nblocks, hipStream_t st);
 // rows of 32-value blocks (F16: 32 values per "block") of types 1, 2, 6, 8, 39 as fp32
 int launch_dequantize(int type, const void *src, float *dst, int64_t nblocks, hipStream_t st);
-// operand rows: [rows][K/32] blocks of MX_XB = 96 bytes and [rows][K/32] scale words
-struct MxRows {
-    uint8_t *xb = nullptr;   // 16-byte aligned
-    uint32_t *xs = nullptr;
-};
-int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, hipStream_t st);
+// operand rows of K values (mx.hpp; 16-byte aligned), their last granule filled up
+int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, uint8_t *rows, hipStream_t st);
 // Grouped products.  MX_STORE: fp32 rows y; MX_GLU / MX_RELU_SQR: the
 // activation rows leave as the next product's operand o (rows of ncols
 // values, ncols % 32 == 0).  A shared expert (sh_rows > 0) rides in the same
@@ -371,8 +367,9 @@ struct MxSide {
     ExpertMat a, b;            // b: up table (separate gate/up GLU), else unused
     int fused;
     int64_t I;
-    MxRows x;                  // operand rows of a.K values
-    MxRows o;
+    const uint8_t *x;          // operand rows of a.K values
+    int64_t xrows;             // launch_mxg: how many (at most MXG_MAX_X bytes)
+    uint8_t *o;                // (launch_mxv leaves a last granule's blocks past ncols as they are)
     float *y;                  // rows p, stride ldy
     int64_t ldy, ncols;
 };
@@ -401,6 +398,7 @@ struct MxArgs : MxSide {
 };
 constexpr int MXV_IDS = 512;
 constexpr int MXG_BM = 64, MXG_BM_SMALL = 32;
+constexpr int64_t MXG_MAX_X = 0xF0000000ll;            // (32-bit buffer offsets)
 constexpr int64_t MXG_MAX_ROW_BYTES = 1ll << 22;   // of launch_mxg (64 rows within 32-bit offsets)
 int launch_mxv(const MxArgs &g, hipStream_t st);
 int launch_mxg(const MxArgs &g, hipStream_t st);
