@@ -766,30 +766,42 @@ int run_experts_b32(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_
 // block-sum and fp16 arrays: those are one run of 1 + 1/64 + 1/8 + 2 bytes per
 // value of rows filled up to 256 values (carve_workspace), the operand takes 3 +
 // 1/8 per value of rows filled up to 128.
-uint8_t *mx_rows(const ActBuf &a) { return (uint8_t *)a.q8; }
+MxRows mx_rows(void *base, int64_t rows, int64_t K) {
+    MxRows m;
+    m.d = (uint8_t *)base;
+    m.s = (uint32_t *)(m.d + rows * mx_drow(K / 32));
+    return m;
+}
 // tokens per pass of its grouped GEMM, which reads the rows through 32-bit
 // offsets; row_bytes: a token's operand bytes
 int64_t mx_max_tokens(int64_t row_bytes) { return MXG_MAX_X / row_bytes; }
 int64_t mx_layer_tokens(const mi_moe_layer *L) {
-    return mx_max_tokens(std::max(mx_row(L->n_embd / 32), L->n_expert_used * mx_row(L->n_ff / 32)));
+    return mx_max_tokens(std::max(mx_drow(L->n_embd / 32), L->n_expert_used * mx_drow(L->n_ff / 32)));
 }
 
-// MXFP4: the grouped GEMM above two dispatched rows per expert (rows further
-// apart than it addresses keep the other kernel)
-bool use_gemm_mx(const mi_moe_ctx *c, int64_t T, int K, int E, size_t row_bytes) {
+// MXFP4: the grouped GEMM for a product of more dispatched rows than half the
+// experts (K 2048, 2048 rows of 64 experts: 40 rows 33 against 32 us, 64 rows
+// 41 against 38, 512 rows 137 against 49; 16 rows 23 against 31), for a layer
+// above two per expert: its few-row form takes few launches and its sums are
+// exact (64 experts: 80 rows 86 against 90 us, 128 rows 113 against 94).
+// (Rows further apart than it addresses keep the other kernel.)
+bool use_gemm_mx(const mi_moe_ctx *c, int64_t T, int K, int E, size_t row_bytes, bool layer) {
     if ((int64_t)row_bytes > MXG_MAX_ROW_BYTES) return false;   // (then a token's operand row is far below MXG_MAX_X)
     if (c->gemm_threshold > 0) return T >= c->gemm_threshold;
-    return T * K > 2 * (int64_t)E;
+    return layer ? T * K > 2 * (int64_t)E : 2 * T * K > (int64_t)E;
 }
 bool mx_layer_gemm(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
     size_t rb = std::max(L->gate.nb[1], L->down.nb[1]);
     if (act_gated(L->act) && !L->fused_gate_up) rb = std::max(rb, L->up.nb[1]);
-    return use_gemm_mx(c, T, L->n_expert_used, L->n_expert, rb);
+    return use_gemm_mx(c, T, L->n_expert_used, L->n_expert, rb, true);
 }
-// Row tiles of its GEMM: 64 rows above 32 dispatched rows per expert, else 32
+// Row tiles of its GEMM: 64 rows above 24 dispatched rows per expert, else 32
+// (K 2048, 2048 rows of 64 experts, 32 / 64: 16 rows per expert 52 / 54 us, 32
+// rows 84 / 63, 256 rows 314 / 246; 128-row tiles in 1 work-group per CU 250 at
+// 256 rows, 55 / 62 / 77 at 32: no count where they win by more than 10%)
 int mx_bm(const mi_moe_ctx *c, int64_t rows, int E) {
     if (c->gemm_tiles == 1 || c->gemm_tiles == 2) return c->gemm_tiles == 1 ? MXG_BM : MXG_BM_SMALL;
-    return rows > 32 * (int64_t)E ? MXG_BM : MXG_BM_SMALL;
+    return rows > 24 * (int64_t)E ? MXG_BM : MXG_BM_SMALL;
 }
 // The shared expert in the routed experts' launches of few rows: the same
 // table type and activation.
@@ -798,6 +810,64 @@ bool mx_shared_ok(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
     if (mx_row(L->sh_n_ff / 32) > 4 * (int64_t)L->n_expert_used * std::max(L->n_embd, 2 * L->n_ff)) return false;
     return is_mx(L->gate.type) && is_mx(L->sh_gate.type) && is_mx(L->sh_down.type) && L->sh_act == L->act &&
            !(mx_layer_gemm(c, L, T) && mx_layer_tokens(L) > 0) && T <= GV_SHARED_T;
+}
+
+// A few tokens through an MXFP4 layer in three launches: norm, router logits
+// and operand rows (k_mx_front); the experts' ranking, gate/up products and
+// activation rows (k_mxv); down products, weighted sum and residual (k_mxd).
+// Up to MX_FEW_T tokens (and MXV_FRONT_T for the first launch: more run the
+// norm, the router and the operand pass by themselves), the routed part on the
+// few-row product, no dispatch outputs asked for.
+constexpr int64_t MX_FEW_T = 16;
+bool mx_few(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T, const mi_moe_routing *routing) {
+    if (!is_mx(L->gate.type) || !c->fused_decode || T > MX_FEW_T || T * L->n_expert_used > MXV_IDS) return false;
+    if (L->n_embd % 16 || mx_layer_gemm(c, L, T)) return false;
+    if (L->sh_n_ff > 0 && !mx_shared_ok(c, L, T)) return false;
+    return !(routing && (routing->counts || routing->offsets || routing->perm));
+}
+bool mx_few_front(const mi_moe_layer *L, const float *x, const float *xr, int64_t T, const NormParams &np, MxFrontArgs &f) {
+    f = MxFrontArgs{};
+    f.W = L->router_w; f.b = L->router_b; f.x = x; f.xr = xr ? xr : x; f.norm = np;
+    f.T = (int)T; f.D = L->n_embd; f.E = L->n_expert;
+    return T <= MXV_FRONT_T && mx_front_ok(f) && !(xr && np.kind != NORM_NONE);
+}
+// the launches after the logits: rank them here (front: the operand rows are
+// there too), else sel and w are there already
+int run_mx_few(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T, bool front, const Gating &gt, const float *res,
+               float *out, const float *sh_w, hipStream_t st) {
+    const int D = L->n_embd, E = L->n_expert, K = L->n_expert_used, I = L->n_ff;
+    const int64_t rows = T * K, S = L->sh_n_ff;
+    const bool gated = act_gated(L->act);
+    const MxRows mx = mx_rows(c->ax.q8, T, D), ma = mx_rows(c->aact.q8, rows, I);
+    if (!front) {
+        TRY(launch_prep_mx(x, D, T, D, mx, st));
+        stage_end(c, "q8_x", st);
+    }
+    MxArgs a = {};
+    a.a = as_mat(L->gate);
+    if (gated && !L->fused_gate_up) a.b = as_mat(L->up);
+    a.epi = gated ? MX_GLU : MX_RELU_SQR; a.act = L->act; a.fused = L->fused_gate_up; a.I = I;
+    a.x = mx; a.xrows = T; a.o = ma; a.ncols = I; a.ne11 = 1; a.K = K;
+    a.max_active = (int)std::min<int64_t>(E, rows); a.rows = rows; a.n_expert = E; a.bad_total = c->bad_total;
+    if (front) { a.logits = c->logits; a.gating = gt; a.sel = c->sel; a.w = c->w; }
+    else a.ids = c->sel;
+    MxDownArgs d = {};
+    d.a = as_mat(L->down); d.x = ma; d.sel = c->sel; d.w = c->w; d.res = res; d.out = out;
+    d.T = (int)T; d.K = K; d.E = E; d.D = D; d.n_cu = c->n_cu;
+    if (S > 0) {
+        a.sh_rows = T;
+        a.sh.a = as_mat(L->sh_gate);
+        if (gated) a.sh.b = as_mat(L->sh_up);
+        a.sh.I = a.sh.ncols = S;
+        a.sh.x = mx;
+        a.sh.o = mx_rows(c->f1, T, S);
+        d.sh_a = as_mat(L->sh_down); d.sh_x = a.sh.o; d.sh_w = sh_w;
+    }
+    TRY(launch_mxv(a, st));
+    stage_end(c, "gate_up", st);
+    TRY(launch_mxd(d, st));
+    stage_end(c, "down", st);
+    return MI_MOE_OK;
 }
 
 // routed FFN body of a layer with MXFP4 tables: Q8_0 operand rows (mx.hpp),
@@ -836,7 +906,7 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
     const DispBuf &dg = c->disp[0];
     const DispBuf &dd = same_ids ? c->disp[0] : c->disp[1];
     stage_end(c, "dispatch", st);
-    uint8_t *mx = mx_rows(c->ax), *ma = mx_rows(c->aact);
+    const MxRows mx = mx_rows(c->ax.q8, T, D), ma = mx_rows(c->aact.q8, rows, I);
     TRY(launch_prep_mx(x, D, T, D, mx, st));
     stage_end(c, "q8_x", st);
     auto args_for = [&](const ExpertMat &t, const DispBuf &d, int ne11) {
@@ -863,7 +933,7 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
         if (gated) a.sh.b = as_mat(L->sh_up);
         a.sh.I = a.sh.ncols = S;
         a.sh.x = mx;
-        a.sh.o = (uint8_t *)c->f1;   // (free on this path)
+        a.sh.o = mx_rows(c->f1, T, S);   // (free on this path)
         d.sh.x = a.sh.o;
         d.sh.a = as_mat(L->sh_down);
         d.sh.y = c->sh_out; d.sh.ldy = d.sh.ncols = D;
@@ -1419,6 +1489,16 @@ int mi_moe_ctx_stage_times(mi_moe_ctx *c, int max_stages, const char **names, fl
 
 namespace {
 
+Gating layer_gating(const mi_moe_layer *L) {
+    Gating gt;
+    gt.kind = L->gating;
+    gt.sel_bias = L->sel_bias;
+    gt.expert_scale = L->expert_scale;
+    gt.scaling = L->routed_scaling != 0.f ? L->routed_scaling : 1.f;
+    gt.eps = L->gate_eps;
+    return gt;
+}
+
 // the forward with an optional norm of its input (np.kind != NORM_NONE).  A
 // single token on the fused kernel normalizes x inside it (every work-group
 // computes the statistics in k_norm_rows' order while its router row loads
@@ -1450,7 +1530,13 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
     // re-reads x, possibly after other work-groups wrote their out columns.
     const uintptr_t xb = (uintptr_t)x, ob = (uintptr_t)out, row = sizeof(float) * (uintptr_t)D;
     const bool fuse_norm = dec1 && np.kind != NORM_NONE && (ob + row <= xb || xb + row <= ob);
-    if (np.kind != NORM_NONE && !fuse_norm) {
+    // a few tokens of an MXFP4 layer: the norm in the router's launch, unless
+    // another launch reads the normalized rows too (the shared expert's gate
+    // row) or out overlaps the rows in part
+    const bool few = mx_few(c, L, T, routing);
+    MxFrontArgs ff;
+    const bool few_front = few && mx_few_front(L, x, xr, T, np, ff) && !(np.kind != NORM_NONE && L->sh_n_ff > 0 && L->sh_gate_inp);
+    if (np.kind != NORM_NONE && !fuse_norm && !few_front) {
         TRY(launch_norm(np, x, T, D, c->xn, st));
         stage_end(c, "norm", st);
         x = c->xn;
@@ -1466,7 +1552,14 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
         add = c->sh_out;
     }
     int cc = 0;
-    if (dec1) {
+    if (few_front) {
+        ff.x = x; ff.xr = xr ? xr : x;
+        ff.logits = c->logits;
+        ff.o = mx_rows(c->ax.q8, T, D);
+        TRY(launch_mx_front(ff, st));
+        stage_end(c, "router", st);
+        TRY(run_mx_few(c, L, x, T, true, layer_gating(L), res, out, L->sh_gate_inp ? c->sh_w : nullptr, st));
+    } else if (dec1) {
         TRY(run_decode1(c, L, x, res, out, P, C, fuse_norm ? np : NormParams{}, st));
     } else if (!xr && plan_decodeb(c, L, x, T, cc)) {
         TRY(run_decodeb(c, L, x, T, res, out, cc, st));
@@ -1484,12 +1577,7 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
             qx.b_ld = D;
             xq = true;
         }
-        Gating gt;
-        gt.kind = L->gating;
-        gt.sel_bias = L->sel_bias;
-        gt.expert_scale = L->expert_scale;
-        gt.scaling = L->routed_scaling != 0.f ? L->routed_scaling : 1.f;
-        gt.eps = L->gate_eps;
+        const Gating gt = layer_gating(L);
         const int cps = front_split_cps(c, T, D, E);
         bool x_done = false;   // the Q8_K of x came with the router
         if (cps > 0) {
@@ -1505,7 +1593,8 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
             TRY(launch_topk_softmax(c->logits, E, T, E, K, c->sel, K, c->w, st, gt));
         }
         stage_end(c, "topk_softmax", st);
-        TRY(run_experts(c, L, x, T, c->sel, c->sel, c->w, res, out, st, x_done, false, add,
+        if (few) TRY(run_mx_few(c, L, x, T, false, gt, res, out, L->sh_gate_inp ? c->sh_w : nullptr, st));
+        else TRY(run_experts(c, L, x, T, c->sel, c->sel, c->w, res, out, st, x_done, false, add,
                         routing && (routing->counts || routing->offsets || routing->perm), sh_here,
                         L->sh_gate_inp ? c->sh_w : nullptr));
     }
@@ -1718,8 +1807,8 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
     // the grouped GEMM of the 32-value types and F16, in passes past its 32-bit
     // offsets (a single token's rows past them: the GEMV)
     const bool mx = is_mx(as->type);
-    const int64_t ldx = round_up(Kin, 64), tmax = mx ? mx_max_tokens(ne11 * mx_row(Kin / 32)) : gb_max_tokens(ne11 * ldx);
-    const bool mxg = mx && use_gemm_mx(c, T, (int)n_used, (int)E, as->nb[1]) && tmax > 0;
+    const int64_t ldx = round_up(Kin, 64), tmax = mx ? mx_max_tokens(ne11 * mx_drow(Kin / 32)) : gb_max_tokens(ne11 * ldx);
+    const bool mxg = mx && use_gemm_mx(c, T, (int)n_used, (int)E, as->nb[1], false) && tmax > 0;
     const bool gb = is_b32f(as->type) && use_gemm_wide(c, T, (int)n_used, (int)E) && gb_strides_ok(*as) && tmax > 0;
     if ((gb || mxg) && T > tmax) {
         for (int64_t t0 = 0; t0 < T; t0 += tmax) {
@@ -1731,6 +1820,24 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
             TRY(mi_mul_mat_id(c, as, &bt, &it, &dt, stream));
         }
         return MI_MOE_OK;
+    }
+    if (mx && !mxg && rows <= MXV_IDS && (uintptr_t)b->data % 16 == 0) {
+        // few rows in one launch, whose work-groups find their rows and make
+        // their operands themselves (unless dst overlaps what they read)
+        auto apart = [&](const void *p, int64_t n) {
+            const uintptr_t q = (uintptr_t)p, o = (uintptr_t)dst->data;
+            return q + (uintptr_t)(4 * n) <= o || o + (uintptr_t)(4 * rows * N) <= q;
+        };
+        if (apart(b->data, T * ne11 * Kin) && apart(ids->data, rows)) {
+            MxArgs a = {};
+            a.a = as_mat(*as); a.epi = MX_STORE; a.ne11 = (int)ne11; a.K = (int)n_used;
+            a.xf = (const float *)b->data;
+            a.ids = (const int32_t *)ids->data; a.rows = rows; a.n_expert = (int)E;
+            a.bad_total = c->bad_total; a.zero_rows = 1;
+            a.max_active = (int)std::min<int64_t>(E, rows);
+            a.y = (float *)dst->data; a.ldy = N; a.ncols = N;
+            return launch_mxv(a, st);
+        }
     }
     const int max_active = (int)std::min<int64_t>(E, rows);
     const int bm = mx ? mx_bm(c, rows, (int)E) : !gb ? G4_BM : gf_tiles(c, as->type, rows, (int)E, Kin, N) ? GF_BM : gb_bm(c, rows, (int)E, N);
@@ -1746,8 +1853,8 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
     if (mx) {
         MxArgs a = {};
         a.a = M; a.epi = MX_STORE; a.ne11 = (int)ne11; a.K = (int)n_used;
-        a.x = mx_rows(c->ax); a.xrows = T * ne11;
-        TRY(launch_prep_mx(bp, Kin, T * ne11, Kin, mx_rows(c->ax), st));
+        a.x = mx_rows(c->ax.q8, T * ne11, Kin); a.xrows = T * ne11;
+        TRY(launch_prep_mx(bp, Kin, T * ne11, Kin, a.x, st));
         a.perm = dsp.perm; a.counts = dsp.counts; a.offsets = dsp.offsets; a.active_e = dsp.active_e;
         a.n_active = dsp.n_active; a.max_active = max_active;
         a.tile_e = dsp.tile_e; a.tile_start = dsp.tile_start; a.tile_rows = dsp.tile_rows; a.n_tiles = dsp.n_tiles;

@@ -162,72 +162,146 @@ int launch_dequantize(int type, const void *src, float *dst, int64_t nblocks, hi
 // Rows of K values (K % 32 == 0, row r at src + r * ld) into the operand
 // (mx.hpp): four threads per block.  Memory-bound.
 template <bool VEC>
-__global__ void __launch_bounds__(256) k_prep_mx(const float *__restrict__ src, int64_t ld, int64_t nrows, int nb,
-                                                 uint8_t *__restrict__ rows) {
+__global__ void __launch_bounds__(256) k_prep_mx(const float *__restrict__ src, int64_t ld, int64_t nrows, int nb, MxRows o) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, blk = i >> 2;
     const bool live = blk < nrows * nb;
     const int64_t r = live ? blk / nb : 0, b = live ? blk - r * nb : 0;
     float v[8];
     mx_load8<VEC>(src + r * ld + 32 * b, (int)(i & 3), v);
-    uint8_t *row = rows + r * mx_row(nb);
-    mx_store_block(v, row, b, (int)(i & 3), live);
-    if (live && b == nb - 1) mx_store_pad(row, nb, (int)(i & 3));
+    mx_store_block(v, o, r, b, nb, (int)(i & 3), live);
+    if (live && b == nb - 1) mx_store_pad(o, r, nb, (int)(i & 3));
 }
 
-int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, uint8_t *rows, hipStream_t st) {
+int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, hipStream_t st) {
     if (nrows <= 0) return 0;
     if (K % 32 || K > 0x7fffffff) return -6;
     const int64_t wgs = (nrows * (K / 8) + 255) / 256;
     if (wgs > 0x7fffffff) return -6;
     if (ld % 4 == 0 && (uintptr_t)src % 16 == 0)
-        hipLaunchKernelGGL(k_prep_mx<true>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), rows);
-    else hipLaunchKernelGGL(k_prep_mx<false>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), rows);
+        hipLaunchKernelGGL(k_prep_mx<true>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), o);
+    else hipLaunchKernelGGL(k_prep_mx<false>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), o);
     return hip_check_launch();
 }
 
 // ------------------------------------------------------------------ few rows
 // act_pair (act.hpp) in fp64, rounded once: a value that differs in its last
-// bits would move an 8-bit code of the operand that it becomes
-__device__ inline float mx_act(int act, double a, double b) {
+// bits would move an 8-bit code of the operand that it becomes.  (A call: inlined,
+// the constants of exp and erf are kept in registers through the products'
+// loops and do not fit.)
+template <int ACT>
+__device__ __attribute__((noinline)) float mx_act(double a, double b) {
     const double SQRT_2_INV = 0.70710678118654752440, SQRT_2_OVER_PI = 0.79788456080286535588;
-    switch (act) {
-    case 0: return (float)(a / (1.0 + exp(-a)) * b);
-    case 1: return (float)(0.5 * a * (1.0 + erf(a * SQRT_2_INV)) * (b + 1.0));
-    case 2: return (float)(0.5 * a * (1.0 + tanh(SQRT_2_OVER_PI * a * (1.0 + 0.044715 * a * a))) * b);
-    case 3: return (float)(0.5 * a * (1.0 + erf(a * SQRT_2_INV)) * b);
-    default: {
+    if constexpr (ACT == 0) return (float)(a / (1.0 + exp(-a)) * b);
+    else if constexpr (ACT == 1) return (float)(0.5 * a * (1.0 + erf(a * SQRT_2_INV)) * (b + 1.0));
+    // (1 + tanh(u)) / 2 = 1 / (1 + exp(-2 u))
+    else if constexpr (ACT == 2) return (float)(a / (1.0 + exp(-2.0 * SQRT_2_OVER_PI * a * (1.0 + 0.044715 * a * a))) * b);
+    else if constexpr (ACT == 3) return (float)(0.5 * a * (1.0 + erf(a * SQRT_2_INV)) * b);
+    else {
         const double r = a > 0.0 ? a : a != a ? a : 0.0;
         return (float)(r * r);
     }
+}
+
+// A 16-row weight tile times a row, by one wave: the lane's blocks of its
+// weight row (row lane % 16; step u's block 4 (s0 + u) + lane / 16) in
+// registers, the row of activations in LDS.
+//
+// A step is v_mfma_scale_f32_16x16x128_f8f6f4 on four blocks of the 16 rows
+// (the 16 bytes of codes as they are) against one row of activations: column c
+// = 4 b + i holds digit i of the step's block b and zeros in the other three,
+// so each of the 16 x 16 results is one digit's sum over one block, an integer
+// of at most 13 bits times a power of two: exact in fp32 whatever the scales.
+// They are added in fp64, so the result is the exact sum rounded at 2^-53, and
+// what follows (the GLU's values, in fp64 and rounded once, and their codes)
+// does not depend on an order of sums.
+//
+// Loads: two per step and lane (the five dwords of its block, at dword
+// aligned addresses), 68 bytes of a row together; the load path takes such a
+// step in about 50 cycles (22 B per cycle and CU, twice the HBM's share).
+template <int U>
+struct MxTile {
+    MxRaw w[U];
+    const uint8_t *row;   // the lane's weight row
+    // steps s0 .. s0 + sn - 1 of the row's blocks, of which there are nb
+    __device__ __forceinline__ void load(int s0, int sn, int nb, int lane) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int b = 4 * (s0 + u) + (lane >> 4);
+            if (u < sn) mx_load(row + MX_BYTES * (int64_t)(b < nb ? b : 0), w[u]);   // (past the row: block 0, not used)
+        }
     }
+    // acc[n] += steps s0 .. times the N rows whose operands from step sx on are at x[n]
+    template <int N>
+    __device__ __forceinline__ void products(int s0, int sn, int nb, int lane, const uint8_t *const (&xd)[N], const uint32_t *const (&xs)[N], int sx,
+                                             int n, double (&acc)[N][4]) const {
+        const int r16 = lane & 15, grp = lane >> 4, dig = r16 & 3;
+        const bool on = (r16 >> 2) == grp;   // the lane's column holds a digit of the lane's block
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= sn) continue;
+            const int b = 4 * (s0 + u) + grp;
+            const bool in = b < nb;
+            const uint32_t mis = (uint32_t)((uintptr_t)row + (uint32_t)(MX_BYTES * (in ? b : 0))) & 3u;
+            uint32_t c[4];
+            mx_codes(w[u], mis, c);
+            const int sa = in ? (int)mx_scale(w[u], mis) : (int)MX_ONE;
+            i32x8 A = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) A[i] = in ? (int)c[i] : 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (j >= n) continue;
+                i32x8 B = {0, 0, 0, 0, 0, 0, 0, 0};
+                int sb = (int)MX_ONE;
+                if (on && in) {
+                    const uint8_t *x = xd[j] + MX_XB * (b - 4 * sx);
+                    const uint4 lo = *(const uint4 *)(x + 16 * dig);
+                    const uint2 hi = *(const uint2 *)(x + 64 + 8 * dig);
+                    B[0] = (int)lo.x; B[1] = (int)lo.y; B[2] = (int)lo.z; B[3] = (int)lo.w;
+                    B[4] = (int)hi.x; B[5] = (int)hi.y;
+                    sb = (int)((xs[j][b - 4 * sx] >> (8 * dig)) & 0xffu);
+                }
+                float4_t z = {0.f, 0.f, 0.f, 0.f};
+                z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, z, 4, 2, 0, sa, 0, sb);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[j][i] += (double)z[i];
+            }
+        }
+    }
+};
+
+// rows 4 (lane / 16) + i, a partial per column: the sum over the 16 columns
+__device__ __forceinline__ double mx_columns(double a) {
+    a = dpp_add<0xB1>(a);
+    a = dpp_add<0x4E>(a);
+    a = dpp_add<0x141>(a);
+    return dpp_add<0x140>(a);
 }
 
 // Grouped product of few rows per expert.  A work-group (8 waves) owns 64
 // weight rows of one active expert (GLU: 32 gate rows and the matching up
 // rows) as four 16-row tiles, two waves to a tile, each half of the blocks.
-//
-// A wave's step is v_mfma_scale_f32_16x16x128_f8f6f4 on four blocks of its 16
-// rows (lane l: row l % 16, block l / 16 of the step, the 16 bytes of codes as
-// they are) against one row of activations: column c = 4 b + i holds digit i
-// of the step's block b and zeros in the other three, so each of the 16 x 16
-// results is one digit's sum over one block, an integer of at most 13 bits
-// times a power of two: exact in fp32 whatever the scales.  They are added in
-// fp64, so the result is the exact sum rounded at 2^-53, and the GLU's values
-// (in fp64, rounded once) and their codes do not depend on an order of sums.
-//
 // The expert's rows run MXV_NT at a time through LDS, the lanes' weight blocks
-// staying in registers for them.
-constexpr int MXV_NT = 4, MXV_WAVES = 8, MXV_U = 8;   // U: steps of a wave in registers at a time
-constexpr int MXV_KB = 4 * 2 * MXV_U;                 // blocks of a pass over K (both wave halves)
+// staying in registers for all of them (rows of at most MXV_KB blocks; longer
+// ones are loaded again).
+//
+// With g.logits the work-group ranks the tokens' experts itself (a wave per
+// token) and finds its rows among them, with g.ids it finds them among the
+// ids: work-group row j belongs to slot j, and leaves unless the slot is its
+// expert's first.
+constexpr int MXV_NT = 2, MXV_WAVES = 8, MXV_U = 8;   // U: steps of a wave in registers at a time
+constexpr int MXV_KB = 4 * 2 * MXV_U;                  // blocks of a pass over K (both wave halves)
 
-template <int EPI, bool SH>
-__global__ void __launch_bounds__(64 * MXV_WAVES) k_mxv(MxArgs g) {
-    __shared__ __attribute__((aligned(16))) uint8_t sx[MXV_NT][MXV_KB / 4 * MX_XG];
+// ACT: the activation, or -1 for the plain product
+template <int ACT, bool SH>
+__global__ void __launch_bounds__(64 * MXV_WAVES) __attribute__((amdgpu_waves_per_eu(4))) k_mxv(MxArgs g) {
+    __shared__ __attribute__((aligned(16))) uint8_t sx[MXV_NT][MXV_KB * MX_XB];
+    __shared__ uint32_t ss[MXV_NT][MXV_KB];
     __shared__ double s_sum[MXV_NT][128];
-    __shared__ float s_v[MXV_NT][64];
+    __shared__ __attribute__((aligned(16))) float s_v[MXV_NT][64];
     __shared__ int s_p[MXV_IDS];
     __shared__ int s_cnt[MXV_WAVES];
-    constexpr bool GLU = EPI == MX_GLU;
+    constexpr bool STORE = ACT < 0, GLU = !STORE && ACT != ACT_RELU_SQR;
     constexpr int COLS = GLU ? 32 : 64;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const bool shared = SH && (int)blockIdx.x < g.sh_wgs;
@@ -240,12 +314,34 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) k_mxv(MxArgs g) {
     } else {
         const unsigned lin = blockIdx.x - (SH ? g.sh_wgs : 0), j = lin / (unsigned)g.ncb;
         cb = (int)(lin - j * (unsigned)g.ncb);
-        if (g.ids) {
-            // work-group row j belongs to slot j, and leaves unless the slot is its expert's first
-            const int id = tid < g.rows ? g.ids[tid] : -1;
-            e = g.ids[j];
+        if (g.ids || (!STORE && g.logits)) {
+            int id;
+            if (!STORE && g.logits) {
+                // (s_p holds the ids until the rows are found: at most MXV_FRONT_T tokens)
+                const int T = (int)(g.rows / g.K);
+                if (wave < T) {
+                    int mysel;
+                    float myw;
+                    topk_softmax_wave(g.logits + wave * g.n_expert, g.n_expert, g.K, lane, mysel, myw, lin == 0, g.gating);
+                    if (lane < g.K) {
+                        s_p[wave * g.K + lane] = mysel;
+                        if (lin == 0) {
+                            g.sel[wave * g.K + lane] = mysel;
+                            g.w[wave * g.K + lane] = myw;
+                        }
+                    }
+                }
+                __syncthreads();
+                id = tid < g.rows ? s_p[tid] : -1;
+                e = s_p[j];
+                __syncthreads();
+            } else {
+                id = tid < g.rows ? g.ids[tid] : -1;
+                e = g.ids[j];
+            }
             if ((unsigned)e >= (unsigned)g.n_expert) {
                 if (g.bad_total && cb == 0 && tid == 0) atomicAdd(g.bad_total, 1);
+                if (STORE && g.zero_rows && tid < COLS && (int64_t)cb * COLS + tid < s.ncols) s.y[j * s.ldy + (int64_t)cb * COLS + tid] = 0.f;
                 return;
             }
             const uint64_t m = __ballot(id == e);
@@ -271,23 +367,12 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) k_mxv(MxArgs g) {
     const int tile = wave >> 1, half = wave & 1, r16 = lane & 15, grp = lane >> 4;
     // the lane's weight row (past the matrix: row 0, not stored)
     const int64_t col = (int64_t)cb * COLS + 16 * (GLU ? tile & 1 : tile) + r16;
-    const bool col_ok = col < s.ncols;
-    int64_t wrow = col_ok ? col : 0;
-    const uint8_t *rowp = s.a.data + (int64_t)e * s.a.mat_bytes;
-    int64_t rb = s.a.row_bytes;
-    if (GLU && tile >= 2) {
-        if (s.fused) {
-            wrow += s.I;
-        } else {
-            rowp = s.b.data + (int64_t)e * s.b.mat_bytes;
-            rb = s.b.row_bytes;
-        }
-    }
-    rowp += wrow * rb;
+    const int64_t wrow = (col < s.ncols ? col : 0) + (GLU && tile >= 2 && s.fused ? s.I : 0);
+    const ExpertMat &wm = GLU && tile >= 2 && !s.fused ? s.b : s.a;
+    MxTile<MXV_U> w;
+    w.row = wm.data + (int64_t)e * wm.mat_bytes + wrow * wm.row_bytes;
     const int nb = (int)(s.a.K / 32);
     const int kdiv = g.ne11 == 1 && !shared ? g.K : 1;
-    const bool on = (r16 >> 2) == grp;   // the lane's column holds a digit of the lane's block
-    const int dig = r16 & 3;
     for (int q0 = 0; q0 < cnt; q0 += MXV_IDS) {   // (rows that fit s_p)
         const int qn = cnt - q0 < MXV_IDS ? cnt - q0 : MXV_IDS;
         if (shared || perm) {
@@ -304,68 +389,65 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) k_mxv(MxArgs g) {
                 for (int i = 0; i < 4; ++i) acc[n][i] = 0.0;
             for (int k0 = 0; k0 < nb; k0 += MXV_KB) {
                 const int kn = nb - k0 < MXV_KB ? nb - k0 : MXV_KB, nst = (kn + 3) / 4, h0 = (nst + 1) / 2;
-                const int s0 = half ? h0 : 0, sn = half ? nst - h0 : h0;   // the wave's steps
-                MxRaw w[MXV_U];
-#pragma unroll
-                for (int u = 0; u < MXV_U; ++u) {
-                    const int b = 4 * (s0 + u) + grp;
-                    if (u < sn) mx_load(rowp + MX_BYTES * (int64_t)(k0 + (b < kn ? b : 0)), w[u]);   // (past the row: block 0, not used)
-                }
-                if (k0 || n0 || q0) __syncthreads();   // (the activations before are read)
-                for (int n = 0; n < nt; ++n) {
-                    const int p = s_p[n0 + n];
-                    const uint4 *src = (const uint4 *)(s.x + (int64_t)(kdiv > 1 ? p / kdiv : p) * mx_row(nb) + mx_row(k0));
-                    for (int i = tid; i < nst * (MX_XG / 16); i += 64 * MXV_WAVES) *(uint4 *)(sx[n] + 16 * i) = src[i];
-                }
-                __syncthreads();
-#pragma unroll
-                for (int u = 0; u < MXV_U; ++u) {
-                    if (u >= sn) break;
-                    const int b = 4 * (s0 + u) + grp;
-                    const bool in = b < kn;
-                    const uint32_t mis = (uint32_t)(uintptr_t)(rowp + MX_BYTES * (int64_t)(k0 + (in ? b : 0))) & 3u;
-                    uint32_t c[4];
-                    mx_codes(w[u], mis, c);
-                    const int sa = in ? (int)mx_scale(w[u], mis) : (int)MX_ONE;
-                    i32x8 A = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) A[i] = in ? (int)c[i] : 0;
+                const int s0 = k0 / 4 + (half ? h0 : 0), sn = half ? nst - h0 : h0;   // the wave's steps
+                // the rows' operands (in front of the weights' loads: they are
+                // stored to LDS while those are on their way)
+                const bool fx = STORE && !shared && g.xf;
+                static_assert(MXV_KB * MX_XB / 16 <= 64 * MXV_WAVES && 4 * MXV_NT * MXV_KB <= 64 * MXV_WAVES, "a piece of each row, or a quarter block, per thread");
+                // (fx: this thread's quarter of block fb of row fn; two rows, in turn)
+                const int fn = nt > 1 && (tid >> 2) >= kn ? 1 : 0, fb = (tid >> 2) - (fn ? kn : 0);
+                const bool flive = fx && fb < kn;
+                u32x4 xv[2];
+                uint32_t xs1[MXV_NT];
+                static_assert(MXV_NT == 2, "xv");
+                if (fx) {
+                    if (flive) {
+                        const int p = s_p[n0 + fn];
+                        const u32x4 *src = (const u32x4 *)(g.xf + (int64_t)(kdiv > 1 ? p / kdiv : p) * s.a.K + 32 * (k0 + fb)) + (tid & 3);
+                        xv[0] = src[0];
+                        xv[1] = src[4];
+                    }
+                } else {
 #pragma unroll
                     for (int n = 0; n < MXV_NT; ++n) {
-                        if (n >= nt) break;
-                        i32x8 B = {0, 0, 0, 0, 0, 0, 0, 0};
-                        int sb = (int)MX_ONE;
-                        if (on && in) {
-                            const uint8_t *x = sx[n] + MX_XG * (s0 + u) + MX_XB * grp + 8 * (grp & 2);   // (b = 4 (s0 + u) + grp)
-                            const uint4 lo = *(const uint4 *)(x + 16 * dig);
-                            const uint2 hi = *(const uint2 *)(x + 64 + 8 * dig);
-                            B[0] = (int)lo.x; B[1] = (int)lo.y; B[2] = (int)lo.z; B[3] = (int)lo.w;
-                            B[4] = (int)hi.x; B[5] = (int)hi.y;
-                            sb = sx[n][MX_XG * (s0 + u) + 2 * MX_XB + 4 * grp + dig];
-                        }
-                        float4_t z = {0.f, 0.f, 0.f, 0.f};
-                        z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, z, 4, 2, 0, sa, 0, sb);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[n][i] += (double)z[i];
+                        const int p = s_p[n0 + imin(n, nt - 1)];
+                        const int64_t r = kdiv > 1 ? p / kdiv : p;
+                        if (tid < kn * (MX_XB / 16)) xv[n] = ((const u32x4 *)(s.x.d + r * mx_drow(nb) + (int64_t)MX_XB * k0))[tid];
+                        if (tid < kn) xs1[n] = s.x.s[r * mx_srow(nb) + k0 + tid];
                     }
                 }
+                asm volatile("" ::: "memory");
+                if (nb > MXV_KB || (n0 == 0 && q0 == 0)) w.load(s0, sn, nb, lane);
+                if (k0 || n0 || q0) __syncthreads();   // (the activations before are read)
+                if (fx) {
+                    const MxRows o = {sx[fn], ss[fn]};
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(float, (uint32_t)xv[i >> 2][i & 3]);
+                    mx_store_block(v, o, 0, fb, 0, tid & 3, flive);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < MXV_NT; ++n) {
+                        if (tid < kn * (MX_XB / 16)) *(u32x4 *)(sx[n] + 16 * tid) = xv[n];
+                        if (tid < kn) ss[n][tid] = xs1[n];
+                    }
+                }
+                __syncthreads();
+                const uint8_t *const xd[MXV_NT] = {sx[0], sx[1]};
+                const uint32_t *const xs[MXV_NT] = {ss[0], ss[1]};
+                w.template products<MXV_NT>(s0, sn, nb, lane, xd, xs, k0 / 4, nt, acc);
             }
-            // rows 4 (lane / 16) + i, a partial per column: the 16 columns, then the other half's
 #pragma unroll
             for (int n = 0; n < MXV_NT; ++n) {
                 if (n >= nt) break;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    double a = acc[n][i];
-                    a = dpp_add<0xB1>(a);
-                    a = dpp_add<0x4E>(a);
-                    a = dpp_add<0x141>(a);
-                    a = dpp_add<0x140>(a);
+                    const double a = mx_columns(acc[n][i]);
                     if (r16 == 0) s_sum[n][64 * half + 16 * tile + 4 * grp + i] = a;
                 }
             }
             __syncthreads();
-            if (EPI == MX_STORE) {
+            if constexpr (STORE) {
                 const int c = tid & 63, n = tid >> 6;
                 const int64_t cc = (int64_t)cb * COLS + c;
                 if (n < nt && cc < s.ncols) {
@@ -379,15 +461,15 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) k_mxv(MxArgs g) {
                 if (n < nt) {
                     const double a = s_sum[n][c] + s_sum[n][64 + c];
                     const double b = GLU ? s_sum[n][32 + c] + s_sum[n][96 + c] : 0.0;
-                    s_v[n][c] = mx_act(GLU ? g.act : ACT_RELU_SQR, a, b);
+                    s_v[n][c] = mx_act<ACT>(a, b);
                 }
                 __syncthreads();
                 if (tid < MXV_NT * COLS / 8) {
-                    const int m = tid / (COLS / 8), blk = (tid >> 2) % (COLS / 32);
+                    const int m = tid / (COLS / 8), blk = (tid >> 2) % (COLS / 32), onb = (int)(s.ncols / 32);
                     float v[8];
-                    mx_load8<false>(s_v[m] + 32 * blk, tid & 3, v);
-                    mx_store_block(v, s.o + (int64_t)(m < nt ? s_p[n0 + m] : 0) * mx_row(s.ncols / 32), (int64_t)cb * (COLS / 32) + blk, tid & 3,
-                                   m < nt && (int64_t)cb * COLS + 32 * blk < s.ncols);
+                    mx_load8<true>(s_v[m] + 32 * blk, tid & 3, v);
+                    const int64_t r = m < nt ? s_p[n0 + m] : 0, b = (int64_t)cb * (COLS / 32) + blk;
+                    mx_store_block(v, s.o, r, b, onb, tid & 3, m < nt && b < onb);
                 }
             }
             // (s_sum and s_v are written again after the barriers in front of the next rows' products)
@@ -395,17 +477,17 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) k_mxv(MxArgs g) {
     }
 }
 
-template <int EPI>
+template <int ACT>
 static int mxv_launch(const MxArgs &a, hipStream_t st) {
     MxArgs g = a;
-    constexpr int COLS = EPI == MX_GLU ? 32 : 64;
+    constexpr int COLS = ACT >= 0 && ACT != ACT_RELU_SQR ? 32 : 64;
     g.ncb = (int)((g.ncols + COLS - 1) / COLS);
     g.sh_wgs = g.sh_rows > 0 ? (int)((g.sh.ncols + COLS - 1) / COLS) : 0;
-    const int64_t wgs = g.sh_wgs + (int64_t)g.ncb * (g.ids ? g.rows : g.max_active);
+    const int64_t wgs = g.sh_wgs + (int64_t)g.ncb * (g.ids || g.logits ? g.rows : g.max_active);
     if (wgs > 0x7fffffff) return -6;
     const dim3 grid((unsigned)wgs), block(64 * MXV_WAVES);
-    if (g.sh_wgs) hipLaunchKernelGGL((k_mxv<EPI, true>), grid, block, 0, st, g);
-    else hipLaunchKernelGGL((k_mxv<EPI, false>), grid, block, 0, st, g);
+    if (g.sh_wgs) hipLaunchKernelGGL((k_mxv<ACT, true>), grid, block, 0, st, g);
+    else hipLaunchKernelGGL((k_mxv<ACT, false>), grid, block, 0, st, g);
     return hip_check_launch();
 }
 
@@ -416,13 +498,268 @@ static bool mx_side_ok(const MxArgs &g, const MxSide &s) {
 int launch_mxv(const MxArgs &g, hipStream_t st) {
     if (g.max_active <= 0) return 0;
     if (!mx_side_ok(g, g) || (g.sh_rows > 0 && !mx_side_ok(g, g.sh))) return -6;
-    if (g.ids && (g.rows > MXV_IDS || g.n_expert <= 0)) return -6;
-    switch (g.epi) {
-    case MX_STORE: return mxv_launch<MX_STORE>(g, st);
-    case MX_GLU: return mxv_launch<MX_GLU>(g, st);
-    case MX_RELU_SQR: return mxv_launch<MX_RELU_SQR>(g, st);
+    if ((g.ids || g.logits) && (g.rows > MXV_IDS || g.n_expert <= 0)) return -6;
+    if (g.logits && (g.epi == MX_STORE || g.rows > (int64_t)MXV_FRONT_T * g.K || g.rows % g.K || g.K > 64 || g.n_expert > 64 * TOPK_MAX_PER_LANE)) return -6;
+    if (g.xf && (g.epi != MX_STORE || (uintptr_t)g.xf % 16)) return -6;
+    if (g.epi == MX_STORE) return mxv_launch<-1>(g, st);
+    if (g.epi == MX_RELU_SQR) return mxv_launch<ACT_RELU_SQR>(g, st);
+    switch (g.act) {
+    case 0: return mxv_launch<0>(g, st);
+    case 1: return mxv_launch<1>(g, st);
+    case 2: return mxv_launch<2>(g, st);
+    case 3: return mxv_launch<3>(g, st);
     default: return -6;
     }
+}
+
+// ------------------------------------------------------------------ a few tokens' layer: front
+// The norm, the router's logits and the operand rows of up to MXV_FRONT_T
+// tokens in one launch: a wave per expert, lane c the row's 64-value chunk c
+// in the router's fixed fp64 order (k_route.hip: s outer, g inner; chunk
+// partials in chunk order, those of token t by lane t).  The router's rows are
+// read in address order and go through LDS like the tokens' rows (chunk c's
+// float4 q at slot 16 c + (q + c) % 16: 16 lanes that read chunks c .. c + 15
+// hit 16 different slots); reading its chunk by itself each lane of a load is
+// on a line of its own, and a launch of 64 experts (D 2048) takes 7.6 us
+// instead of 5.8.  Every work-group normalizes the tokens' rows itself, a wave per
+// token in k_norm_rows' order (the bits of mi_norm), while its router rows are
+// on their way; the operand blocks are dealt to the work-groups.
+constexpr int MXF_WAVES = 4;
+static_assert(MXV_FRONT_T <= MXF_WAVES, "a wave per token");
+
+__device__ __forceinline__ int mxf_slot(int c, int q) { return 16 * c + ((q + c) & 15); }
+
+// k_norm_rows' sum of the NORM_T threads' partials, thread t = lane + 64 m at p[m]
+__device__ __forceinline__ double mxf_norm_sum(double (&p)[4]) {
+    double r = (p[0] + p[2]) + (p[1] + p[3]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, r);
+        const uint64_t n = ((uint64_t)(uint32_t)__shfl_down((int)(b >> 32), o, 64) << 32) | (uint32_t)__shfl_down((int)(uint32_t)b, o, 64);
+        r = r + __builtin_bit_cast(double, n);
+    }
+    const uint64_t b = __builtin_bit_cast(uint64_t, r);
+    return __builtin_bit_cast(double, ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) |
+                                          (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b));
+}
+
+template <int DM>   // D <= 1024 DM
+__global__ void __launch_bounds__(64 * MXF_WAVES) k_mx_front(MxFrontArgs g) {
+    __shared__ __attribute__((aligned(16))) float4 sx[MXV_FRONT_T][256 * DM];
+    __shared__ __attribute__((aligned(16))) float4 sw[MXF_WAVES][256 * DM];
+    __shared__ double sp[MXF_WAVES][MXV_FRONT_T][65];
+    static_assert(16 * DM <= 64, "a chunk per lane");
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int D = g.D, nch = D >> 6, e = blockIdx.x * MXF_WAVES + wave;
+    // (a row past the experts: row 0, not stored)
+    float4_t w[4 * DM];
+    const float *wr = g.W + (int64_t)(e < g.E ? e : 0) * D;
+#pragma unroll
+    for (int m = 0; m < 4 * DM; ++m) w[m] = 256 * m + 4 * lane < D ? *(const float4_t *)(wr + 256 * m + 4 * lane) : float4_t{0.f, 0.f, 0.f, 0.f};
+    if (wave < g.T) {
+        const float *x = g.xr + (int64_t)wave * D;
+        float v[DM][4][4];   // piece k, m: elements 1024 k + 4 (lane + 64 m) + j
+#pragma unroll
+        for (int k = 0; k < DM; ++k)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int i = 1024 * k + 4 * (lane + 64 * m);
+                const float4_t a = i < D ? *(const float4_t *)(x + i) : float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[k][m][j] = a[j];
+            }
+        float mean = 0.f, sc = 1.f;
+        if (g.norm.kind != NORM_NONE) {
+            double p[4];
+            if (g.norm.kind == NORM_LAYER) {
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    p[m] = 0.0;
+#pragma unroll
+                    for (int k = 0; k < DM; ++k)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) p[m] = p[m] + (double)v[k][m][j];
+                }
+                mean = (float)(mxf_norm_sum(p) / (double)D);
+            }
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                p[m] = 0.0;
+#pragma unroll
+                for (int k = 0; k < DM; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (1024 * k + 4 * (lane + 64 * m) + j < D) {
+                            const float d = g.norm.kind == NORM_LAYER ? v[k][m][j] - mean : v[k][m][j];
+                            p[m] = p[m] + (double)(d * d);
+                        }
+            }
+            sc = 1.0f / sqrtf((float)(mxf_norm_sum(p) / (double)D) + g.norm.eps);
+        }
+#pragma unroll
+        for (int k = 0; k < DM; ++k)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int i = 1024 * k + 4 * (lane + 64 * m);
+                if (i >= D) continue;
+                float o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = g.norm.kind == NORM_NONE ? v[k][m][j] : norm_apply(g.norm, v[k][m][j], i + j, mean, sc);
+                sx[wave][mxf_slot(i >> 6, (i & 63) >> 2)] = make_float4(o[0], o[1], o[2], o[3]);
+            }
+    }
+#pragma unroll
+    for (int m = 0; m < 4 * DM; ++m) {
+        const int i = 256 * m + 4 * lane;
+        if (i < D) sw[wave][mxf_slot(i >> 6, (i & 63) >> 2)] = make_float4(w[m][0], w[m][1], w[m][2], w[m][3]);
+    }
+    __syncthreads();
+    // operand blocks: four threads each, from the rows in LDS or (another router input) from x
+    const int nb = D >> 5;
+    for (int i = blockIdx.x * (64 * MXF_WAVES) + tid; i < 4 * nb * g.T; i += gridDim.x * (64 * MXF_WAVES)) {
+        const int t = (i >> 2) / nb, b = (i >> 2) - t * nb, s = i & 3;
+        float v[8];
+        if (g.x == g.xr) {
+            const float4 lo = sx[t][mxf_slot(b >> 1, 8 * (b & 1) + s)], hi = sx[t][mxf_slot(b >> 1, 8 * (b & 1) + 4 + s)];
+            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+        } else {
+            mx_load8<true>(g.x + (int64_t)t * D + 32 * b, s, v);
+        }
+        mx_store_block(v, g.o, t, b, nb, s, true);
+    }
+    // (a lane past the chunks: chunk 0, not added; tokens past g.T: the last one's row again)
+    const int c = lane < nch ? lane : 0;
+    double part[MXV_FRONT_T];
+    const float4 *xt[MXV_FRONT_T];
+#pragma unroll
+    for (int t = 0; t < MXV_FRONT_T; ++t) {
+        part[t] = 0.0;
+        xt[t] = sx[imin(t, g.T - 1)];
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        float wv[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(float4 *)wv[q] = sw[wave][mxf_slot(c, 4 * q + s)];
+#pragma unroll
+        for (int t = 0; t < MXV_FRONT_T; ++t) {
+            if (t >= g.T) continue;
+            float xv[4][4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *(float4 *)xv[q] = xt[t][mxf_slot(c, 4 * q + s)];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) part[t] = fma((double)wv[q][j], (double)xv[q][j], part[t]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MXV_FRONT_T; ++t) sp[wave][t][lane] = part[t];
+    wave_lds_sync();
+    if (lane < g.T && e < g.E) {
+        double acc = 0.0;
+        for (int k = 0; k < nch; ++k) acc = acc + sp[wave][lane][k];
+        float v = (float)acc;
+        if (g.b) v = v + g.b[e];
+        g.logits[(int64_t)lane * g.E + e] = v;
+    }
+}
+
+bool mx_front_ok(const MxFrontArgs &g) {
+    return g.T >= 1 && g.T <= MXV_FRONT_T && g.D % 64 == 0 && g.D <= 4096 && (uintptr_t)g.W % 16 == 0 && (uintptr_t)g.x % 16 == 0 &&
+           (uintptr_t)g.xr % 16 == 0;
+}
+
+int launch_mx_front(const MxFrontArgs &g, hipStream_t st) {
+    if (!mx_front_ok(g) || (g.norm.kind != NORM_NONE && g.x != g.xr)) return -6;
+    const dim3 grid((unsigned)((g.E + MXF_WAVES - 1) / MXF_WAVES)), block(64 * MXF_WAVES);
+    if (g.D <= 2048) hipLaunchKernelGGL(k_mx_front<2>, grid, block, 0, st, g);
+    else hipLaunchKernelGGL(k_mx_front<4>, grid, block, 0, st, g);
+    return hip_check_launch();
+}
+
+// ------------------------------------------------------------------ a few tokens' layer: down
+// The down product of all slots of a token, the shared expert's with them, the
+// weighted sum and the residual in one launch: a work-group owns COLS columns
+// of one token, wave k (k + 8, ..) a 16-row tile of slot k's expert.  With
+// COLS = 8 the tile's upper eight rows are the lower ones again (no traffic):
+// twice the work-groups for a call of one token.  The sums have the bits of
+// launch_combine on the slots' rounded rows.  Work-group 8 q + x on XCD x: the
+// tokens of a column group one after another on one XCD, whose L2 then holds
+// the experts' rows that they share.
+constexpr int MXD_WAVES = 8, MXD_U = 8, MXD_KMAX = 64;
+
+template <int COLS>
+__global__ void __launch_bounds__(64 * MXD_WAVES) __attribute__((amdgpu_waves_per_eu(4))) k_mxd(MxDownArgs g) {
+    __shared__ __attribute__((aligned(16))) uint8_t sx[MXD_WAVES][4 * MXD_U * MX_XB];
+    __shared__ __attribute__((aligned(16))) uint32_t ss[MXD_WAVES][4 * MXD_U];
+    __shared__ float s_z[MXD_KMAX + 1][16];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int q = blockIdx.x >> 3, grp = q / g.T, t = q - grp * g.T;
+    const int64_t n0 = (int64_t)COLS * (8 * grp + ((int)blockIdx.x & 7));
+    if (n0 >= g.D) return;
+    const int slots = g.K + (g.sh_a.data ? 1 : 0);
+    for (int k = wave; k < slots; k += MXD_WAVES) {
+        const bool shared = k == g.K;
+        const ExpertMat &m = shared ? g.sh_a : g.a;
+        const MxRows &x = shared ? g.sh_x : g.x;
+        const int p = t * g.K + k, e = shared ? 0 : g.sel[p];
+        const int64_t r = shared ? t : p;
+        const int nb = (int)(m.K / 32);
+        if ((unsigned)e >= (unsigned)(shared ? 1 : g.E)) continue;   // (the router's ids: not expected)
+        MxTile<MXD_U> w;
+        w.row = m.data + (int64_t)e * m.mat_bytes + (n0 + (lane & (COLS - 1))) * m.row_bytes;
+        double acc[1][4] = {{0.0, 0.0, 0.0, 0.0}};
+        for (int k0 = 0; k0 < nb; k0 += 4 * MXD_U) {
+            const int kn = imin(nb - k0, 4 * MXD_U), sn = (kn + 3) / 4;
+            // (the operands in front of the weights: they are stored to LDS while those are on their way)
+            const u32x4 *src = (const u32x4 *)(x.d + r * mx_drow(nb) + (int64_t)MX_XB * k0);
+            constexpr int NX = 4 * MXD_U * MX_XB / 1024;
+            u32x4 xv[NX];
+            uint32_t xs1 = 0;
+#pragma unroll
+            for (int i = 0; i < NX; ++i)
+                if (64 * i + lane < kn * (MX_XB / 16)) xv[i] = src[64 * i + lane];
+            if (lane < kn) xs1 = x.s[r * mx_srow(nb) + k0 + lane];
+            asm volatile("" ::: "memory");
+            w.load(k0 / 4, sn, nb, lane);
+            wave_lds_sync();   // (the activations before are read)
+#pragma unroll
+            for (int i = 0; i < NX; ++i)
+                if (64 * i + lane < kn * (MX_XB / 16)) *(u32x4 *)(sx[wave] + 16 * (64 * i + lane)) = xv[i];
+            if (lane < kn) ss[wave][lane] = xs1;
+            wave_lds_sync();
+            const uint8_t *const xd[1] = {sx[wave]};
+            const uint32_t *const xs[1] = {ss[wave]};
+            w.template products<1>(k0 / 4, sn, nb, lane, xd, xs, k0 / 4, 1, acc);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const double a = mx_columns(acc[0][i]);
+            if ((lane & 15) == 0) s_z[k][4 * (lane >> 4) + i] = (float)a;
+        }
+    }
+    __syncthreads();
+    const int64_t n = n0 + tid;
+    if (tid < COLS && n < g.D) {
+        double s = 0.0;
+        for (int k = 0; k < g.K; ++k) s = s + (double)(s_z[k][tid] * g.w[t * g.K + k]);
+        float moe = (float)s;
+        if (g.sh_a.data) moe = moe + (g.sh_w ? s_z[g.K][tid] * g.sh_w[t] : s_z[g.K][tid]);
+        const int64_t o = (int64_t)t * g.D + n;
+        g.out[o] = g.res ? g.res[o] + moe : moe;
+    }
+}
+
+int launch_mxd(const MxDownArgs &g, hipStream_t st) {
+    if (g.T < 1 || g.K < 1 || g.K > MXD_KMAX || g.D % 16 || g.a.type != 39 || g.a.K % 32 || (g.sh_a.data && (g.sh_a.type != 39 || g.sh_a.K % 32))) return -6;
+    // eight columns a work-group where sixteen would leave half of the CUs idle
+    const bool narrow = (int64_t)g.T * (g.D / 16) < g.n_cu;
+    const int64_t groups = (g.D / (narrow ? 8 : 16) + 7) / 8;
+    const dim3 grid((unsigned)(8 * groups * g.T)), block(64 * MXD_WAVES);
+    if (narrow) hipLaunchKernelGGL(k_mxd<8>, grid, block, 0, st, g);
+    else hipLaunchKernelGGL(k_mxd<16>, grid, block, 0, st, g);
+    return hip_check_launch();
 }
 
 }  // namespace mimoe

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include "norm.hpp"
+#include "wave_ops.hpp"
 
 namespace mimoe {
 
@@ -75,7 +76,6 @@ int launch_front(const float *W, const float *b, const float *x, int64_t ldx, in
                  float *logits, const Q8Out *qx, hipStream_t st);
 // top-k (descending, ties -> lower id) and softmax over the selected logits;
 // w may be NULL (op-level top_k)
-struct Gating;
 int launch_topk_softmax(const float *logits, int64_t ld_logits, int64_t T, int E, int K, int32_t *sel,
                         int64_t ld_sel, float *w, hipStream_t st, const Gating &gt);
 // small batches: the router's chunk partials parts[D / 64][T][E] (fp64) by
@@ -354,8 +354,13 @@ int launch_gb(const GBArgs &g, hipStream_t st);
 int launch_quantize_mx(const float *src, void *dst, int64_t nblocks, hipStream_t st);
 // rows of 32-value blocks (F16: 32 values per "block") of types 1, 2, 6, 8, 39 as fp32
 int launch_dequantize(int type, const void *src, float *dst, int64_t nblocks, hipStream_t st);
-// operand rows of K values (mx.hpp; 16-byte aligned), their last granule filled up
-int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, uint8_t *rows, hipStream_t st);
+// operand rows (mx.hpp): digits (64-byte aligned) and scale words (16-byte aligned)
+struct MxRows {
+    uint8_t *d = nullptr;
+    uint32_t *s = nullptr;
+};
+// operand rows of K values, filled up
+int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, hipStream_t st);
 // Grouped products.  MX_STORE: fp32 rows y; MX_GLU / MX_RELU_SQR: the
 // activation rows leave as the next product's operand o (rows of ncols
 // values, ncols % 32 == 0).  A shared expert (sh_rows > 0) rides in the same
@@ -367,9 +372,9 @@ struct MxSide {
     ExpertMat a, b;            // b: up table (separate gate/up GLU), else unused
     int fused;
     int64_t I;
-    const uint8_t *x;          // operand rows of a.K values
-    int64_t xrows;             // launch_mxg: how many (at most MXG_MAX_X bytes)
-    uint8_t *o;                // (launch_mxv leaves a last granule's blocks past ncols as they are)
+    MxRows x;                  // operand rows of a.K values
+    int64_t xrows;             // launch_mxg: how many (at most MXG_MAX_X bytes of digits)
+    MxRows o;                  // (launch_mxv does not fill up the rows)
     float *y;                  // rows p, stride ldy
     int64_t ldy, ncols;
 };
@@ -379,14 +384,25 @@ struct MxArgs : MxSide {
     const int32_t *perm;
     // few rows (launch_mxv): the dispatch's lists, or the rows' expert ids, at
     // most MXV_IDS of them; a row whose id lies outside [0, n_expert) is not
-    // computed, its output row is not written, and it is counted in bad_total
-    // (NULL: not counted), as by the dispatch
+    // computed, its output row is not written (zero_rows, MX_STORE: zeros), and
+    // it is counted in bad_total (NULL: not counted), as by the dispatch
     const int32_t *counts, *offsets, *active_e, *n_active;
     int max_active;
     const int32_t *ids;
     int64_t rows;
-    int n_expert;              // with ids
+    int n_expert;              // with ids or logits
     int32_t *bad_total;
+    int zero_rows;
+    // launch_mxv, MX_STORE: the rows themselves, of a.K floats (16-byte
+    // aligned), made into operands by the work-groups (x is not read)
+    const float *xf;
+    // or (MX_GLU, MX_RELU_SQR; at most MXV_FRONT_T tokens): the router's logits
+    // [T][n_expert], ranked by the work-groups themselves (rows = T K); sel and
+    // w [T][K] are written for the launches that follow
+    const float *logits;
+    Gating gating;
+    int32_t *sel;
+    float *w;
     // launch_mxg: balanced tiles of at most bm rows (MXG_BM or MXG_BM_SMALL)
     int bm;
     const int32_t *tile_e, *tile_start, *tile_rows, *n_tiles;
@@ -397,10 +413,34 @@ struct MxArgs : MxSide {
     int ncb, sh_wgs;           // (set by the launchers)
 };
 constexpr int MXV_IDS = 512;
+constexpr int MXV_FRONT_T = 4;
 constexpr int MXG_BM = 64, MXG_BM_SMALL = 32;
 constexpr int64_t MXG_MAX_X = 0xF0000000ll;            // (32-bit buffer offsets)
 constexpr int64_t MXG_MAX_ROW_BYTES = 1ll << 22;   // of launch_mxg (64 rows within 32-bit offsets)
 int launch_mxv(const MxArgs &g, hipStream_t st);
+// A few tokens' layer: norm, router logits and operand rows (T <= MXV_FRONT_T)
+struct MxFrontArgs {
+    const float *W, *b;        // router [E][D] and bias [E] or NULL
+    const float *x, *xr;       // rows [T][D] of the experts and of the router (the same, or no norm)
+    NormParams norm;           // of x
+    int T, D, E;
+    float *logits;             // [T][E]
+    MxRows o;                  // operand rows (not filled up)
+};
+bool mx_front_ok(const MxFrontArgs &g);
+int launch_mx_front(const MxFrontArgs &g, hipStream_t st);
+// ... and the slots' down products, their weighted sum, the shared expert (sh_a
+// .data not NULL) and the residual: out[t] = res[t] + (sum_k w[t][k] a_{sel[t][k]} x[t][k] + sh_w[t] sh_a sh_x[t])
+struct MxDownArgs {
+    ExpertMat a, sh_a;
+    MxRows x, sh_x;            // operand rows [T K] of a.K values, [T] of sh_a.K
+    const int32_t *sel;        // [T][K], in [0, E)
+    const float *w, *sh_w;     // [T][K]; [T] or NULL (1)
+    const float *res;          // [T][D] or NULL
+    float *out;
+    int T, K, E, D, n_cu;
+};
+int launch_mxd(const MxDownArgs &g, hipStream_t st);
 int launch_mxg(const MxArgs &g, hipStream_t st);
 
 // Single-token MoE block in one kernel (k_decode.hip).

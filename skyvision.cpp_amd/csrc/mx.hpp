@@ -15,34 +15,30 @@
 // without any unpacking of the weights and without a rounding before the
 // sums: four times the work of one MFMA at four times the rate of fp16's.
 //
-// Operand layout: a row is a run of granules of four blocks, 400 bytes each:
-// the digits of blocks 0 and 1, the four blocks' scale words, the digits of
-// blocks 2 and 3 (so each pair of blocks and the scale words are 208 bytes
-// together).  A block's digits are 96 bytes: digits 0..3's first 16 bytes, then
-// digits 0..3's last 8 bytes; 32 codes of 6 bits in the weights' nibble order
-// (code 2 j is value j, code 2 j + 1 value 16 + j).  Byte i of a scale word is
-// digit i's scale byte, 255 where the row's block holds a NaN or leaves the
-// fp16 range of d.  Blocks that fill up the last granule hold zeros.
+// Operand layout (MxRows): the rows' digits, 96 bytes per block (digits 0..3's
+// first 16 bytes, then digits 0..3's last 8 bytes; 32 codes of 6 bits in the
+// weights' nibble order: code 2 j is value j, code 2 j + 1 value 16 + j), rows
+// of an even number of blocks (a pair of blocks is 192 bytes at a multiple of
+// 64); apart from them the rows' scale words, one per block (byte i: digit i's
+// scale byte; 255 where the row's block holds a NaN or leaves the fp16 range
+// of d), rows of a multiple of four words.  The blocks that fill up a row hold
+// zeros.
 #pragma once
 
 #include "common.hpp"
+#include "launch.hpp"
 #include "wave_ops.hpp"
 
 namespace mimoe {
 
 constexpr int MX_BYTES = 17;        // a block of weights
 constexpr int MX_XB = 96;           // a block's digits in the operand
-constexpr int MX_XG = 4 * MX_XB + 16;   // a granule of the operand
 constexpr uint32_t MX_ONE = 127;    // scale byte of 1
 
-// bytes of an operand row of nb blocks; a block's digits and scale word in a row
-__device__ __host__ constexpr int64_t mx_row(int64_t nb) { return (nb + 3) / 4 * MX_XG; }
-__device__ __forceinline__ uint8_t *mx_at(uint8_t *row, int64_t b) {
-    return row + (b >> 2) * MX_XG + (b & 3) * MX_XB + (b & 2) * 8;
-}
-__device__ __forceinline__ uint32_t *mx_scale_at(uint8_t *row, int64_t b) {
-    return (uint32_t *)(row + (b >> 2) * MX_XG + 2 * MX_XB + 4 * (b & 3));
-}
+// bytes of the digits and words of the scales of an operand row of nb blocks, and the bytes of both
+__device__ __host__ constexpr int64_t mx_drow(int64_t nb) { return (nb + 1) / 2 * (2 * MX_XB); }
+__device__ __host__ constexpr int64_t mx_srow(int64_t nb) { return (nb + 3) / 4 * 4; }
+__device__ __host__ constexpr int64_t mx_row(int64_t nb) { return mx_drow(nb) + 4 * mx_srow(nb); }
 
 // a + the value of the lane that CTRL pairs this one with (wave_ops.hpp)
 template <int CTRL>
@@ -67,11 +63,11 @@ __device__ __forceinline__ uint2 mx_digit(const uint32_t (&u)[8], int i) {
     return r;
 }
 
-// Block b of an operand row by the four lanes 4 k .. 4 k + 3: lane s (= lane
-// & 3) holds values 4 s .. 4 s + 3 in v[0..3] and 16 + 4 s .. in v[4..7];
-// writes digit s, lane 0 the scale word.  live: the lane writes (all four lanes
-// of a block take part).
-__device__ __forceinline__ void mx_store_block(const float (&v)[8], uint8_t *row, int64_t b, int s, bool live) {
+// Block b of operand row r (of nb blocks) by the four lanes 4 k .. 4 k + 3:
+// lane s (= lane & 3) holds values 4 s .. 4 s + 3 in v[0..3] and 16 + 4 s .. in
+// v[4..7]; writes digit s, lane 0 the scale word.  live: the lane writes (all
+// four lanes of a block take part).
+__device__ __forceinline__ void mx_store_block(const float (&v)[8], const MxRows &o, int64_t r, int64_t b, int nb, int s, bool live) {
     uint32_t m = 0;   // largest |x| by its bits: a NaN is above every number
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -112,19 +108,20 @@ __device__ __forceinline__ void mx_store_block(const float (&v)[8], uint8_t *row
         else p[i + 2] = t;
     }
     if (!live) return;
-    uint8_t *xb = mx_at(row, b);
+    uint8_t *xb = o.d + r * mx_drow(nb) + MX_XB * b;
     *(uint4 *)(xb + 16 * s) = make_uint4(p[0].x, p[0].y | p[1].x << 16, p[1].x >> 16 | p[1].y << 16, p[2].x);
     *(uint2 *)(xb + 64 + 8 * s) = make_uint2(p[2].y | p[3].x << 16, p[3].x >> 16 | p[3].y << 16);
-    if (s == 0) *mx_scale_at(row, b) = bad ? 0xffffffffu : k * 0x01010101u + 0x0f0a0500u;
+    if (s == 0) o.s[r * mx_srow(nb) + b] = bad ? 0xffffffffu : k * 0x01010101u + 0x0f0a0500u;
 }
-// the blocks nb .. of the row's last granule, by the same lanes
-__device__ __forceinline__ void mx_store_pad(uint8_t *row, int64_t nb, int s) {
-    for (int64_t b = nb; b & 3; ++b) {
-        uint8_t *xb = mx_at(row, b);
+// the blocks that fill up the row, by the same lanes
+__device__ __forceinline__ void mx_store_pad(const MxRows &o, int64_t r, int nb, int s) {
+    if (nb & 1) {
+        uint8_t *xb = o.d + r * mx_drow(nb) + MX_XB * (int64_t)nb;
         *(uint4 *)(xb + 16 * s) = make_uint4(0, 0, 0, 0);
         *(uint2 *)(xb + 64 + 8 * s) = make_uint2(0, 0);
-        if (s == 0) *mx_scale_at(row, b) = MX_ONE * 0x01010101u;
     }
+    for (int64_t b = nb; b & 3; ++b)
+        if (s == 0) o.s[r * mx_srow(nb) + b] = MX_ONE * 0x01010101u;
 }
 
 // lane s's 8 values of the block at x

@@ -151,6 +151,24 @@ def test_product_shapes(ctx, path, n, N, own_rows):
         ctx.set_gemm_threshold(0)
 
 
+@pytest.mark.parametrize("kind", [1, 2, 5])
+@pytest.mark.parametrize("n,N", SHAPES)
+def test_product_row_tiles(ctx, kind, n, N):
+    """every row tile of the GEMM, at row counts below, at and past it"""
+    rng = np.random.default_rng(n + N + kind)
+    raw = table(rng, 3, N, n)
+    ctx.set_gemm_threshold(1)
+    ctx.set_gemm_tiles(kind)
+    try:
+        for counts in ((1, 0, 31), (32, 33, 64), (65, 128, 129), (127, 260, 2)):
+            ids = rng.permutation(np.repeat(np.arange(3), counts))[:, None]
+            b = rows(rng, len(ids), 1, n)
+            check_product(run_product(ctx, raw, b, ids), raw, b, ids, False)
+    finally:
+        ctx.set_gemm_threshold(0)
+        ctx.set_gemm_tiles(0)
+
+
 @pytest.mark.parametrize("path", ["few", "gemm"])
 @pytest.mark.parametrize("pad,offset", [(0, 1), (1, 0), (2, 3), (7, 2), (15, 5)])
 def test_product_any_alignment(ctx, path, pad, offset):
