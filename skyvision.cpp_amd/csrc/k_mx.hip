@@ -543,6 +543,13 @@ __device__ __forceinline__ double mxf_norm_sum(double (&p)[4]) {
                                           (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b));
 }
 
+// four floats at p, aligned to one
+__device__ __forceinline__ float4_t mxf_load4(const float *p) {
+    float4_t v;
+    __builtin_memcpy(&v, __builtin_assume_aligned(p, 4), 16);
+    return v;
+}
+
 template <int DM>   // D <= 1024 DM
 __global__ void __launch_bounds__(64 * MXF_WAVES) k_mx_front(MxFrontArgs g) {
     __shared__ __attribute__((aligned(16))) float4 sx[MXV_FRONT_T][256 * DM];
@@ -569,7 +576,16 @@ __global__ void __launch_bounds__(64 * MXF_WAVES) k_mx_front(MxFrontArgs g) {
                 for (int j = 0; j < 4; ++j) v[k][m][j] = a[j];
             }
         float mean = 0.f, sc = 1.f;
+        float4_t nw[DM][4], nbias[DM][4];   // (norm_apply's, read beside the rows)
         if (g.norm.kind != NORM_NONE) {
+#pragma unroll
+            for (int k = 0; k < DM; ++k)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const int i = 1024 * k + 4 * (lane + 64 * m);
+                    nw[k][m] = g.norm.w && i < D ? mxf_load4(g.norm.w + i) : float4_t{0.f, 0.f, 0.f, 0.f};
+                    nbias[k][m] = g.norm.kind == NORM_LAYER && g.norm.b && i < D ? mxf_load4(g.norm.b + i) : float4_t{0.f, 0.f, 0.f, 0.f};
+                }
             double p[4];
             if (g.norm.kind == NORM_LAYER) {
 #pragma unroll
@@ -604,7 +620,13 @@ __global__ void __launch_bounds__(64 * MXF_WAVES) k_mx_front(MxFrontArgs g) {
                 if (i >= D) continue;
                 float o[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] = g.norm.kind == NORM_NONE ? v[k][m][j] : norm_apply(g.norm, v[k][m][j], i + j, mean, sc);
+                for (int j = 0; j < 4; ++j) {
+                    // norm_apply
+                    o[j] = v[k][m][j];
+                    if (g.norm.kind != NORM_NONE) o[j] = (g.norm.kind == NORM_RMS ? o[j] : o[j] - mean) * sc;
+                    if (g.norm.kind != NORM_NONE && g.norm.w) o[j] = o[j] * nw[k][m][j];
+                    if (g.norm.kind == NORM_LAYER && g.norm.b) o[j] = o[j] + nbias[k][m][j];
+                }
                 sx[wave][mxf_slot(i >> 6, (i & 63) >> 2)] = make_float4(o[0], o[1], o[2], o[3]);
             }
     }
@@ -654,11 +676,13 @@ __global__ void __launch_bounds__(64 * MXF_WAVES) k_mx_front(MxFrontArgs g) {
         }
     }
 #pragma unroll
-    for (int t = 0; t < MXV_FRONT_T; ++t) sp[wave][t][lane] = part[t];
+    for (int t = 0; t < MXV_FRONT_T; ++t) sp[wave][t][lane] = lane < nch ? part[t] : 0.0;
     wave_lds_sync();
     if (lane < g.T && e < g.E) {
+        // (zeros past the chunks: a sum from 0.0 on keeps its bits)
         double acc = 0.0;
-        for (int k = 0; k < nch; ++k) acc = acc + sp[wave][lane][k];
+#pragma unroll
+        for (int k = 0; k < 16 * DM; ++k) acc = acc + sp[wave][lane][k];
         float v = (float)acc;
         if (g.b) v = v + g.b[e];
         g.logits[(int64_t)lane * g.E + e] = v;
