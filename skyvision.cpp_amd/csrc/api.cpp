@@ -899,16 +899,16 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
     // few rows: the work-groups find their rows from the router's ids
     // themselves, unless the caller wants the dispatch's outputs
     const bool self_disp = !gemm && same_ids && !check_ids && !disp_out && rows <= MXV_IDS;
-    if (!self_disp) {
-        TRY(launch_dispatch(ids_gu, T, K, E, bm, 1, c->disp[0].view(), st));
+    const MxRows mx = mx_rows(c->ax.q8, T, D), ma = mx_rows(c->aact.q8, rows, I);
+    if (self_disp) {
+        TRY(launch_prep_mx(x, D, T, D, mx, st));
+    } else {
+        TRY(launch_dispatch_mx(ids_gu, T, K, E, bm, c->disp[0].view(), x, D, T, D, mx, st));
         if (!same_ids) TRY(launch_dispatch(ids_dn, T, K, E, bm, 1, c->disp[1].view(), st));
     }
     const DispBuf &dg = c->disp[0];
     const DispBuf &dd = same_ids ? c->disp[0] : c->disp[1];
-    stage_end(c, "dispatch", st);
-    const MxRows mx = mx_rows(c->ax.q8, T, D), ma = mx_rows(c->aact.q8, rows, I);
-    TRY(launch_prep_mx(x, D, T, D, mx, st));
-    stage_end(c, "q8_x", st);
+    stage_end(c, self_disp ? "q8_x" : "dispatch", st);
     auto args_for = [&](const ExpertMat &t, const DispBuf &d, int ne11) {
         MxArgs g = {};
         g.a = t; g.ne11 = ne11; g.K = K; g.act = L->act;
@@ -1847,14 +1847,15 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
     dv.zero_rows = (float *)dst->data;   // the rows of ids outside [0, E): zeros
     dv.zero_ld = N;
     dv.zero_n = N;
-    TRY(launch_dispatch((const int32_t *)ids->data, T, (int)n_used, (int)E, bm, 1, dv, st));
     const ExpertMat M = as_mat(*as);
     const float *bp = (const float *)b->data;
+    const MxRows xo = mx_rows(c->ax.q8, T * ne11, Kin);
+    if (mx) TRY(launch_dispatch_mx((const int32_t *)ids->data, T, (int)n_used, (int)E, bm, dv, bp, Kin, T * ne11, Kin, xo, st));
+    else TRY(launch_dispatch((const int32_t *)ids->data, T, (int)n_used, (int)E, bm, 1, dv, st));
     if (mx) {
         MxArgs a = {};
         a.a = M; a.epi = MX_STORE; a.ne11 = (int)ne11; a.K = (int)n_used;
-        a.x = mx_rows(c->ax.q8, T * ne11, Kin); a.xrows = T * ne11;
-        TRY(launch_prep_mx(bp, Kin, T * ne11, Kin, a.x, st));
+        a.x = xo; a.xrows = T * ne11;
         a.perm = dsp.perm; a.counts = dsp.counts; a.offsets = dsp.offsets; a.active_e = dsp.active_e;
         a.n_active = dsp.n_active; a.max_active = max_active;
         a.tile_e = dsp.tile_e; a.tile_start = dsp.tile_start; a.tile_rows = dsp.tile_rows; a.n_tiles = dsp.n_tiles;

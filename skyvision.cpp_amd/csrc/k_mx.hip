@@ -163,13 +163,7 @@ int launch_dequantize(int type, const void *src, float *dst, int64_t nblocks, hi
 // (mx.hpp): four threads per block.  Memory-bound.
 template <bool VEC>
 __global__ void __launch_bounds__(256) k_prep_mx(const float *__restrict__ src, int64_t ld, int64_t nrows, int nb, MxRows o) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, blk = i >> 2;
-    const bool live = blk < nrows * nb;
-    const int64_t r = live ? blk / nb : 0, b = live ? blk - r * nb : 0;
-    float v[8];
-    mx_load8<VEC>(src + r * ld + 32 * b, (int)(i & 3), v);
-    mx_store_block(v, o, r, b, nb, (int)(i & 3), live);
-    if (live && b == nb - 1) mx_store_pad(o, r, nb, (int)(i & 3));
+    mx_prep_thread<VEC>(src, ld, nrows, nb, o, (int64_t)blockIdx.x * 256 + threadIdx.x);
 }
 
 int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, hipStream_t st) {
@@ -177,7 +171,7 @@ int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const
     if (K % 32 || K > 0x7fffffff) return -6;
     const int64_t wgs = (nrows * (K / 8) + 255) / 256;
     if (wgs > 0x7fffffff) return -6;
-    if (ld % 4 == 0 && (uintptr_t)src % 16 == 0)
+    if (mx_prep_vec(src, ld))
         hipLaunchKernelGGL(k_prep_mx<true>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), o);
     else hipLaunchKernelGGL(k_prep_mx<false>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), o);
     return hip_check_launch();

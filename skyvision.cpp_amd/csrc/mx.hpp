@@ -139,6 +139,20 @@ __device__ __forceinline__ void mx_load8(const float *x, int s, float (&v)[8]) {
     }
 }
 
+// Rows of 32 nb values (row r at src + r ld) into operand rows: four threads
+// per block, thread i (of nrows nb 4, filled up to whole waves)
+template <bool VEC>
+__device__ __forceinline__ void mx_prep_thread(const float *__restrict__ src, int64_t ld, int64_t nrows, int nb, const MxRows &o, int64_t i) {
+    const int64_t blk = i >> 2;
+    const bool live = blk < nrows * nb;
+    const int64_t r = live ? blk / nb : 0, b = live ? blk - r * nb : 0;
+    float v[8];
+    mx_load8<VEC>(src + r * ld + 32 * b, (int)(i & 3), v);
+    mx_store_block(v, o, r, b, nb, (int)(i & 3), live);
+    if (live && b == nb - 1) mx_store_pad(o, r, nb, (int)(i & 3));
+}
+inline bool mx_prep_vec(const float *src, int64_t ld) { return ld % 4 == 0 && (uintptr_t)src % 16 == 0; }
+
 // A weight block in registers: the five dwords from the one at or below its
 // first byte (each holds a byte of the block: no read leaves the table's
 // dwords), and its codes and scale byte; mis: its first byte's place there
