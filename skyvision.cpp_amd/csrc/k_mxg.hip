@@ -38,7 +38,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void_t;
 
 constexpr int MXG_ROW = 2 * MX_XB;              // LDS bytes of an activation row's step
-constexpr int MXG_WROWS = 256;                  // weight rows of a work-group
 constexpr uint32_t MXG_FAR = 0xF8000000u;       // an offset past the rows (at most MXG_MAX_X bytes), far from wrapping
 
 template <int N> struct Const { static constexpr int value = N; };
@@ -103,16 +102,17 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 #ifdef __HIP_DEVICE_COMPILE__   // (the host pass needs the stub alone)
     constexpr int BM = 32 * WM, NW = WM * WN;
     constexpr bool GLU = EPI == MX_GLU;
-    static_assert(32 * C * WN == MXG_WROWS && BM <= 64 * NW, "256 weight rows, a row per thread");
+    constexpr int WROWS = 32 * C * WN;   // weight rows of a work-group
+    static_assert(WROWS % 128 == 0 && BM <= 64 * NW, "groups of 64 weight rows, a row per thread");
     constexpr bool SPREAD = C == 2;   // a step's loads between its MFMAs
     // loads of 64 pieces, dealt to the waves (where they do not go up evenly, the last one to several)
     constexpr int AI = BM * 12 / 64, NAL = (AI + NW - 1) / NW;
-    constexpr int KG = 4, WPC = 5, WROW = 16 * WPC, WI = 4 * WPC, NWL = (WI + NW - 1) / NW, KS = KG / 2;
+    constexpr int KG = 4, WPC = 5, WROW = 16 * WPC, WI = WROWS / 64 * WPC, NWL = (WI + NW - 1) / NW, KS = KG / 2;
     __shared__ __attribute__((aligned(16))) uint8_t sa0[BM * MXG_ROW];
     __shared__ __attribute__((aligned(16))) uint8_t sa1[BM * MXG_ROW];
     __shared__ __attribute__((aligned(16))) uint8_t sa2[BM * MXG_ROW];
-    __shared__ __attribute__((aligned(16))) uint8_t sw0[MXG_WROWS * WROW];
-    __shared__ __attribute__((aligned(16))) uint8_t sw1[MXG_WROWS * WROW];
+    __shared__ __attribute__((aligned(16))) uint8_t sw0[WROWS * WROW];
+    __shared__ __attribute__((aligned(16))) uint8_t sw1[WROWS * WROW];
     __shared__ int s_p[BM];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31, h = lane >> 5;
     const MxSide s = g;
@@ -129,17 +129,17 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     // Columns of y (of the activation rows) of a work-group and a wave.  The
     // 256 weight rows in LDS: those of the columns in order (GLU: 128 gate
     // rows, then the 128 matching up rows), loaded by groups of 64.
-    constexpr int CB = GLU ? MXG_WROWS / 2 : MXG_WROWS, CW = CB / WN;
+    constexpr int CB = GLU ? WROWS / 2 : WROWS, CW = CB / WN;
     const int64_t c0 = (int64_t)cb * CB, n0 = c0 + CW * wc;
     __amdgpu_buffer_rsrc_t wrsrc[NWL];
     uint32_t woff[NWL];
 #pragma unroll
     for (int i = 0; i < NWL; ++i) {
         const int j = imin(wave + NW * i, WI - 1), grp = j / WPC;
-        const bool up = GLU && grp >= 2;
+        const bool up = GLU && grp >= WROWS / 128;
         const ExpertMat &m = up && !s.fused ? s.b : s.a;
         // (rows past the matrix: its last row again, not stored)
-        const int64_t r0 = c0 + 64 * (GLU ? grp & 1 : grp), first = r0 < s.ncols ? r0 : s.ncols - 1, left = s.ncols - first;
+        const int64_t r0 = c0 + 64 * (GLU ? grp % (WROWS / 128) : grp), first = r0 < s.ncols ? r0 : s.ncols - 1, left = s.ncols - first;
         const uint8_t *p = m.data + (int64_t)e * m.mat_bytes + (first + (up && s.fused ? s.I : 0)) * m.row_bytes;
         const uint32_t mis = (uint32_t)(uintptr_t)p & 3u, rb = (uint32_t)m.row_bytes, last = (left < 64 ? (uint32_t)left : 64u) - 1;
         // (a dword past the last row's bytes reads as zero)
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     // the operands of step T of a stage out of LDS
 #define MXG_TAKE(o, T, sa, sw)                                                                                     \
     {                                                                                                              \
-        _Pragma("unroll") for (int ct = 0; ct < C; ++ct) mxg_read<T>((sw) + wat + WROW * (GLU ? 128 * (ct & 1) + 32 * (ct / 2) : 32 * ct), (o).w[ct]); \
+        _Pragma("unroll") for (int ct = 0; ct < C; ++ct) mxg_read<T>((sw) + wat + WROW * (GLU ? WROWS / 2 * (ct & 1) + 32 * (ct / 2) : 32 * ct), (o).w[ct]); \
         _Pragma("unroll") for (int i = 0; i < 4; ++i) {                                                            \
             (o).lo[i] = *(const u32x4 *)((sa) + xo[i]);                                                            \
             (o).hi[i] = *(const uint2 *)((sa) + xo[4 + (i >> 1)] + 8 * (i & 1));                                   \
@@ -339,16 +339,20 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 #endif
 }
 
-template <int EPI>
+template <int EPI, int C, int WM, int WN>
 static int mxg_launch(const MxArgs &a, hipStream_t st) {
     MxArgs g = a;
-    constexpr int COLS = EPI == MX_GLU ? MXG_WROWS / 2 : MXG_WROWS;   // per work-group
+    constexpr int COLS = 32 * C * WN / (EPI == MX_GLU ? 2 : 1);   // per work-group
     g.ncb = (int)((g.ncols + COLS - 1) / COLS);
     const int64_t wgs = 8 * (int64_t)g.ncb * ((g.max_tiles + 7) / 8);
     if (wgs > 0x7fffffff) return -6;
-    if (g.bm == MXG_BM) hipLaunchKernelGGL((k_mxg<EPI, 4, 2, 2>), dim3((unsigned)wgs), dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_mxg<EPI, 2, 1, 4>), dim3((unsigned)wgs), dim3(256), 0, st, g);
+    hipLaunchKernelGGL((k_mxg<EPI, C, WM, WN>), dim3((unsigned)wgs), dim3(64 * WM * WN), 0, st, g);
     return hip_check_launch();
+}
+
+template <int EPI>
+static int mxg_tiles(const MxArgs &g, hipStream_t st) {
+    return g.bm == MXG_BM ? mxg_launch<EPI, 4, 2, 2>(g, st) : mxg_launch<EPI, 2, 1, 2>(g, st);
 }
 
 int launch_mxg(const MxArgs &g, hipStream_t st) {
@@ -358,9 +362,9 @@ int launch_mxg(const MxArgs &g, hipStream_t st) {
     if (g.a.type != 39 || g.a.K % 32 || g.a.K > 0x7fffffff || (g.epi != MX_STORE && g.ncols % 32)) return -6;
     if (g.xrows <= 0 || g.xrows * mx_drow(g.a.K / 32) > MXG_MAX_X || (uintptr_t)g.x.d % 16 || (uintptr_t)g.x.s % 16) return -6;
     switch (g.epi) {
-    case MX_STORE: return mxg_launch<MX_STORE>(g, st);
-    case MX_GLU: return mxg_launch<MX_GLU>(g, st);
-    case MX_RELU_SQR: return mxg_launch<MX_RELU_SQR>(g, st);
+    case MX_STORE: return mxg_tiles<MX_STORE>(g, st);
+    case MX_GLU: return mxg_tiles<MX_GLU>(g, st);
+    case MX_RELU_SQR: return mxg_tiles<MX_RELU_SQR>(g, st);
     default: return -6;
     }
 }
