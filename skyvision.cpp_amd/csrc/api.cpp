@@ -840,7 +840,7 @@ int run_mx_few(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T, 
     const bool gated = act_gated(L->act);
     const MxRows mx = mx_rows(c->ax.q8, T, D), ma = mx_rows(c->aact.q8, rows, I);
     if (!front) {
-        TRY(launch_prep_mx(x, D, T, D, mx, st));
+        TRY(launch_prep_mx(x, D, T, D, mx, true, st));
         stage_end(c, "q8_x", st);
     }
     MxArgs a = {};
@@ -901,9 +901,9 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
     const bool self_disp = !gemm && same_ids && !check_ids && !disp_out && rows <= MXV_IDS;
     const MxRows mx = mx_rows(c->ax.q8, T, D), ma = mx_rows(c->aact.q8, rows, I);
     if (self_disp) {
-        TRY(launch_prep_mx(x, D, T, D, mx, st));
+        TRY(launch_prep_mx(x, D, T, D, mx, !gemm, st));
     } else {
-        TRY(launch_dispatch_mx(ids_gu, T, K, E, bm, c->disp[0].view(), x, D, T, D, mx, st));
+        TRY(launch_dispatch_mx(ids_gu, T, K, E, bm, c->disp[0].view(), x, D, T, D, mx, !gemm, st));
         if (!same_ids) TRY(launch_dispatch(ids_dn, T, K, E, bm, 1, c->disp[1].view(), st));
     }
     const DispBuf &dg = c->disp[0];
@@ -1850,7 +1850,7 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
     const ExpertMat M = as_mat(*as);
     const float *bp = (const float *)b->data;
     const MxRows xo = mx_rows(c->ax.q8, T * ne11, Kin);
-    if (mx) TRY(launch_dispatch_mx((const int32_t *)ids->data, T, (int)n_used, (int)E, bm, dv, bp, Kin, T * ne11, Kin, xo, st));
+    if (mx) TRY(launch_dispatch_mx((const int32_t *)ids->data, T, (int)n_used, (int)E, bm, dv, bp, Kin, T * ne11, Kin, xo, !mxg, st));
     else TRY(launch_dispatch((const int32_t *)ids->data, T, (int)n_used, (int)E, bm, 1, dv, st));
     if (mx) {
         MxArgs a = {};

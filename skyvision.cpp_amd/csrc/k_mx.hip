@@ -162,18 +162,18 @@ int launch_dequantize(int type, const void *src, float *dst, int64_t nblocks, hi
 // Rows of K values (K % 32 == 0, row r at src + r * ld) into the operand
 // (mx.hpp): four threads per block.  Memory-bound.
 template <bool VEC>
-__global__ void __launch_bounds__(256) k_prep_mx(const float *__restrict__ src, int64_t ld, int64_t nrows, int nb, MxRows o) {
-    mx_prep_thread<VEC>(src, ld, nrows, nb, o, (int64_t)blockIdx.x * 256 + threadIdx.x);
+__global__ void __launch_bounds__(256) k_prep_mx(const float *__restrict__ src, int64_t ld, int64_t nrows, int nb, MxRows o, bool few) {
+    mx_prep_thread<VEC>(src, ld, nrows, nb, o, few, (int64_t)blockIdx.x * 256 + threadIdx.x);
 }
 
-int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, hipStream_t st) {
+int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, bool few, hipStream_t st) {
     if (nrows <= 0) return 0;
     if (K % 32 || K > 0x7fffffff) return -6;
     const int64_t wgs = (nrows * (K / 8) + 255) / 256;
     if (wgs > 0x7fffffff) return -6;
     if (mx_prep_vec(src, ld))
-        hipLaunchKernelGGL(k_prep_mx<true>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), o);
-    else hipLaunchKernelGGL(k_prep_mx<false>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), o);
+        hipLaunchKernelGGL(k_prep_mx<true>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), o, few);
+    else hipLaunchKernelGGL(k_prep_mx<false>, dim3((unsigned)wgs), dim3(256), 0, st, src, ld, nrows, (int)(K / 32), o, few);
     return hip_check_launch();
 }
 
@@ -196,18 +196,23 @@ __device__ __attribute__((noinline)) float mx_act(double a, double b) {
     }
 }
 
-// A 16-row weight tile times a row, by one wave: the lane's blocks of its
-// weight row (row lane % 16; step u's block 4 (s0 + u) + lane / 16) in
-// registers, the row of activations in LDS.
+// A 16-row weight tile times rows of activations, by one wave: the lane's
+// blocks of its weight row (row lane % 16; step u's block 4 (s0 + u) + lane /
+// 16) in registers, the activations in LDS.
 //
 // A step is v_mfma_scale_f32_16x16x128_f8f6f4 on four blocks of the 16 rows
-// (the 16 bytes of codes as they are) against one row of activations: column c
-// = 4 b + i holds digit i of the step's block b and zeros in the other three,
-// so each of the 16 x 16 results is one digit's sum over one block, an integer
-// of at most 13 bits times a power of two: exact in fp32 whatever the scales.
-// They are added in fp64, so the result is the exact sum rounded at 2^-53, and
-// what follows (the GLU's values, in fp64 and rounded once, and their codes)
-// does not depend on an order of sums.
+// (the 16 bytes of codes as they are) against two rows of activations: column
+// c = 8 j + 2 b + i holds digit i of row j's block b of the step and zeros in
+// the other three blocks, so each of the 16 x 16 results is one digit's sum
+// over one block, an integer of at most 13 bits times a power of two: exact in
+// fp32 whatever the scales.  Times the block's significand they are added in
+// fp64, so the result is the exact sum rounded at 2^-53, and what follows (the
+// GLU's values, in fp64 and rounded once, and their codes) does not depend on
+// an order of sums.  What bounds it beside the weights' bytes is the vector
+// work of a step (unpacking 17-byte blocks, four conversions and fp64
+// multiply-adds): two rows share it all; with the significand in the digits
+// (four, a column of each) a row had it alone, and 120 rows of 64 experts
+// (K 2048, 2048 rows) took FIGURE.
 //
 // Loads: two per step and lane (the five dwords of its block, at dword
 // aligned addresses), 68 bytes of a row together; the load path takes such a
@@ -221,55 +226,50 @@ struct MxTile {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int b = 4 * (s0 + u) + (lane >> 4);
-            if (u < sn) mx_load(row + MX_BYTES * (int64_t)(b < nb ? b : 0), w[u]);   // (past the row: block 0, not used)
+            if (u < sn) mx_load(row + MX_BYTES * (int64_t)(b < nb ? b : 0), w[u]);   // (past the row: block 0; the operand is zero there)
         }
     }
-    // acc[n] += steps s0 .. times the N rows whose operands from step sx on are at x[n]
-    template <int N>
-    __device__ __forceinline__ void products(int s0, int sn, int nb, int lane, const uint8_t *const (&xd)[N], const uint32_t *const (&xs)[N], int sx,
-                                             int n, double (&acc)[N][4]) const {
-        const int r16 = lane & 15, grp = lane >> 4, dig = r16 & 3;
-        const bool on = (r16 >> 2) == grp;   // the lane's column holds a digit of the lane's block
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (u >= sn) continue;
-            const int b = 4 * (s0 + u) + grp;
-            const bool in = b < nb;
-            const uint32_t mis = (uint32_t)((uintptr_t)row + (uint32_t)(MX_BYTES * (in ? b : 0))) & 3u;
+    // acc += steps s0 .. times the n (1 or 2) rows whose digits (blocks filled
+    // up to whole steps with zeros) from step sx on are at x + xo[j] and words
+    // at xs[j]; 16 zeros at x + zo.  All in LDS.
+    __device__ __forceinline__ void products(int s0, int sn, int nb, int lane, const uint8_t *x, const int (&xo)[2], int zo, const uint32_t *const (&xs)[2],
+                                             int sx, int n, double (&acc)[4]) const {
+        const int r16 = lane & 15, grp = lane >> 4, j = r16 >> 3, b = (r16 >> 1) & 3, dig = r16 & 1;
+        const bool on = b == grp && j < n;   // the lane's column holds a digit of the lane's block
+        const int at = (j ? xo[1] : xo[0]) + MX_FB * (4 * (s0 - sx) + grp), stride = on ? 4 * MX_FB : 0;
+        const uint8_t *lo = x + (on ? at + 16 * dig : zo), *hi = x + (on ? at + 32 + 8 * dig : zo);
+        const uint32_t *word = (j && n > 1 ? xs[1] : xs[0]) + 4 * (s0 - sx) + b;
+        // (four blocks are 68 bytes: the lane's blocks are all misaligned alike)
+        const uint32_t mis = (uint32_t)((uintptr_t)row + (uint32_t)(MX_BYTES * grp)) & 3u;
+        const auto step = [&](int u) __attribute__((always_inline)) {
             uint32_t c[4];
             mx_codes(w[u], mis, c);
-            const int sa = in ? (int)mx_scale(w[u], mis) : (int)MX_ONE;
-            i32x8 A = {0, 0, 0, 0, 0, 0, 0, 0};
+            int sa = (int)mx_scale(w[u], mis);
+            // (past the row's last block: any codes, times zeros)
+            if (4 * (s0 + u) + 4 > nb) sa = 4 * (s0 + u) + grp < nb ? sa : (int)MX_ONE;
+            const i32x8 A = {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+            const uint4 xl = *(const uint4 *)(lo + stride * u);
+            const uint2 xh = *(const uint2 *)(hi + stride * u);
+            const uint32_t wd = word[4 * u];
+            const i32x8 B = {(int)xl.x, (int)xl.y, (int)xl.z, (int)xl.w, (int)xh.x, (int)xh.y, 0, 0};
+            float4_t z = {0.f, 0.f, 0.f, 0.f};
+            z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, z, 4, 2, 0, sa, 0, (int)(wd + 5u * (uint32_t)dig));
+            const double f = (double)__builtin_bit_cast(float, wd & 0xffffff00u);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) A[i] = in ? (int)c[i] : 0;
+            for (int i = 0; i < 4; ++i) acc[i] = fma((double)z[i], f, acc[i]);
+        };
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                if (j >= n) continue;
-                i32x8 B = {0, 0, 0, 0, 0, 0, 0, 0};
-                int sb = (int)MX_ONE;
-                if (on && in) {
-                    const uint8_t *x = xd[j] + MX_XB * (b - 4 * sx);
-                    const uint4 lo = *(const uint4 *)(x + 16 * dig);
-                    const uint2 hi = *(const uint2 *)(x + 64 + 8 * dig);
-                    B[0] = (int)lo.x; B[1] = (int)lo.y; B[2] = (int)lo.z; B[3] = (int)lo.w;
-                    B[4] = (int)hi.x; B[5] = (int)hi.y;
-                    sb = (int)((xs[j][b - 4 * sx] >> (8 * dig)) & 0xffu);
-                }
-                float4_t z = {0.f, 0.f, 0.f, 0.f};
-                z = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, z, 4, 2, 0, sa, 0, sb);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[j][i] += (double)z[i];
-            }
-        }
+        for (int u = 0; u < U; ++u)
+            if (u < sn) step(u);
     }
 };
 
-// rows 4 (lane / 16) + i, a partial per column: the sum over the 16 columns
+// rows 4 (lane / 16) + i, a partial per column: the sum over a row of
+// activations' 8 columns
 __device__ __forceinline__ double mx_columns(double a) {
     a = dpp_add<0xB1>(a);
     a = dpp_add<0x4E>(a);
-    a = dpp_add<0x141>(a);
-    return dpp_add<0x140>(a);
+    return dpp_add<0x141>(a);
 }
 
 // Grouped product of few rows per expert.  A work-group (8 waves) owns 64
@@ -289,7 +289,8 @@ constexpr int MXV_KB = 4 * 2 * MXV_U;                  // blocks of a pass over 
 // ACT: the activation, or -1 for the plain product
 template <int ACT, bool SH>
 __global__ void __launch_bounds__(64 * MXV_WAVES) __attribute__((amdgpu_waves_per_eu(4))) k_mxv(MxArgs g) {
-    __shared__ __attribute__((aligned(16))) uint8_t sx[MXV_NT][MXV_KB * MX_XB];
+    constexpr int XROW = MXV_KB * MX_FB, ZERO = MXV_NT * XROW;
+    __shared__ __attribute__((aligned(16))) uint8_t sx[ZERO + 16];   // (16 zeros last)
     __shared__ uint32_t ss[MXV_NT][MXV_KB];
     __shared__ double s_sum[MXV_NT][128];
     __shared__ __attribute__((aligned(16))) float s_v[MXV_NT][64];
@@ -358,6 +359,7 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) __attribute__((amdgpu_waves_pe
             perm = g.perm + g.offsets[e];
         }
     }
+    if (tid < 4) ((uint32_t *)(sx + ZERO))[tid] = 0;
     const int tile = wave >> 1, half = wave & 1, r16 = lane & 15, grp = lane >> 4;
     // the lane's weight row (past the matrix: row 0, not stored)
     const int64_t col = (int64_t)cb * COLS + 16 * (GLU ? tile & 1 : tile) + r16;
@@ -376,9 +378,9 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) __attribute__((amdgpu_waves_pe
         }
         for (int n0 = 0; n0 < qn; n0 += MXV_NT) {
             const int nt = qn - n0 < MXV_NT ? qn - n0 : MXV_NT;
-            double acc[MXV_NT][4];
+            double acc[MXV_NT / 2][4];
 #pragma unroll
-            for (int n = 0; n < MXV_NT; ++n)
+            for (int n = 0; n < MXV_NT / 2; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[n][i] = 0.0;
             for (int k0 = 0; k0 < nb; k0 += MXV_KB) {
@@ -387,57 +389,67 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) __attribute__((amdgpu_waves_pe
                 // the rows' operands (in front of the weights' loads: they are
                 // stored to LDS while those are on their way)
                 const bool fx = STORE && !shared && g.xf;
-                static_assert(MXV_KB * MX_XB / 16 <= 64 * MXV_WAVES && 4 * MXV_NT * MXV_KB <= 64 * MXV_WAVES, "a piece of each row, or a quarter block, per thread");
-                // (fx: this thread's quarter of block fb of row fn; two rows, in turn)
-                const int fn = nt > 1 && (tid >> 2) >= kn ? 1 : 0, fb = (tid >> 2) - (fn ? kn : 0);
-                const bool flive = fx && fb < kn;
-                u32x4 xv[2];
-                uint32_t xs1[MXV_NT];
-                static_assert(MXV_NT == 2, "xv");
-                if (fx) {
-                    if (flive) {
-                        const int p = s_p[n0 + fn];
-                        const u32x4 *src = (const u32x4 *)(g.xf + (int64_t)(kdiv > 1 ? p / kdiv : p) * s.a.K + 32 * (k0 + fb)) + (tid & 3);
-                        xv[0] = src[0];
-                        xv[1] = src[4];
-                    }
-                } else {
+                static_assert(2 * MXV_KB * MX_FB / 16 <= 64 * MXV_WAVES && 8 * MXV_KB <= 64 * MXV_WAVES && MXV_NT % 2 == 0, "a piece, or a quarter block, of two rows per thread");
+                // this thread's piece xi (fx: quarter of block xi / 4) of rows xn, xn + 2, ..; rows are filled up to whole steps
+                const int per = fx ? 4 * kn : 3 * 4 * nst, xn = tid >= per ? 1 : 0, xi = tid - (xn ? per : 0);
+                u32x4 xv[MXV_NT / 2][2];
+                uint32_t xs1[MXV_NT / 2];
 #pragma unroll
-                    for (int n = 0; n < MXV_NT; ++n) {
-                        const int p = s_p[n0 + imin(n, nt - 1)];
-                        const int64_t r = kdiv > 1 ? p / kdiv : p;
-                        if (tid < kn * (MX_XB / 16)) xv[n] = ((const u32x4 *)(s.x.d + r * mx_drow(nb) + (int64_t)MX_XB * k0))[tid];
-                        if (tid < kn) xs1[n] = s.x.s[r * mx_srow(nb) + k0 + tid];
+                for (int n = 0; n < MXV_NT / 2; ++n) {
+                    xv[n][0] = xv[n][1] = u32x4{0, 0, 0, 0};
+                    xs1[n] = MX_ONE;
+                    if (2 * n + xn >= nt || xi >= per) continue;
+                    const int p = s_p[n0 + 2 * n + xn];
+                    const int64_t r = kdiv > 1 ? p / kdiv : p;
+                    if (fx) {
+                        const u32x4 *src = (const u32x4 *)(g.xf + r * s.a.K + 32 * (k0 + (xi >> 2))) + (xi & 3);
+                        xv[n][0] = src[0];
+                        xv[n][1] = src[4];
+                    } else {
+                        if (xi < 3 * kn) xv[n][0] = ((const u32x4 *)(s.x.d + r * (int64_t)(nb * MX_FB) + (int64_t)MX_FB * k0))[xi];
+                        if (xi < kn) xs1[n] = s.x.s[r * nb + k0 + xi];
                     }
                 }
                 asm volatile("" ::: "memory");
                 if (nb > MXV_KB || (n0 == 0 && q0 == 0)) w.load(s0, sn, nb, lane);
                 if (k0 || n0 || q0) __syncthreads();   // (the activations before are read)
-                if (fx) {
-                    const MxRows o = {sx[fn], ss[fn]};
-                    float v[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(float, (uint32_t)xv[i >> 2][i & 3]);
-                    mx_store_block(v, o, 0, fb, 0, tid & 3, flive);
-                } else {
+                for (int n = 0; n < MXV_NT / 2; ++n) {
+                    if (2 * n >= nt) continue;
+                    const int m = 2 * n + xn;
+                    if (fx) {
+                        const MxRows o = {sx + XROW * m, ss[m]};
+                        float v[8];
 #pragma unroll
-                    for (int n = 0; n < MXV_NT; ++n) {
-                        if (tid < kn * (MX_XB / 16)) *(u32x4 *)(sx[n] + 16 * tid) = xv[n];
-                        if (tid < kn) ss[n][tid] = xs1[n];
+                        for (int i = 0; i < 8; ++i) v[i] = __builtin_bit_cast(float, (uint32_t)xv[n][i >> 2][i & 3]);
+                        mx_store_few(v, o, 0, xi >> 2, 0, xi & 3, xi < per);
+                        // (the blocks that fill up the last step)
+                        if (tid < 3 * (4 * nst - kn)) {
+                            *(u32x4 *)(sx + XROW * 2 * n + MX_FB * kn + 16 * tid) = u32x4{0, 0, 0, 0};
+                            *(u32x4 *)(sx + XROW * (2 * n + 1) + MX_FB * kn + 16 * tid) = u32x4{0, 0, 0, 0};
+                        }
+                        if (tid < 4 * nst - kn) ss[2 * n][kn + tid] = ss[2 * n + 1][kn + tid] = MX_ONE;
+                    } else if (xi < per) {
+                        *(u32x4 *)(sx + XROW * m + 16 * xi) = xv[n][0];
+                        if (xi < 4 * nst) ss[m][xi] = xs1[n];
                     }
                 }
                 __syncthreads();
-                const uint8_t *const xd[MXV_NT] = {sx[0], sx[1]};
-                const uint32_t *const xs[MXV_NT] = {ss[0], ss[1]};
-                w.template products<MXV_NT>(s0, sn, nb, lane, xd, xs, k0 / 4, nt, acc);
+#pragma unroll
+                for (int n = 0; n < MXV_NT / 2; ++n) {
+                    if (2 * n >= nt) continue;
+                    const int xo[2] = {XROW * 2 * n, XROW * (2 * n + 1)};
+                    const uint32_t *const xs[2] = {ss[2 * n], ss[2 * n + 1]};
+                    w.products(s0, sn, nb, lane, sx, xo, ZERO, xs, k0 / 4, nt - 2 * n, acc[n]);
+                }
             }
 #pragma unroll
-            for (int n = 0; n < MXV_NT; ++n) {
-                if (n >= nt) break;
+            for (int n = 0; n < MXV_NT / 2; ++n) {
+                if (2 * n >= nt) continue;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const double a = mx_columns(acc[n][i]);
-                    if (r16 == 0) s_sum[n][64 * half + 16 * tile + 4 * grp + i] = a;
+                    if ((r16 & 7) == 0) s_sum[2 * n + (r16 >> 3)][64 * half + 16 * tile + 4 * grp + i] = a;
                 }
             }
             __syncthreads();
@@ -463,7 +475,7 @@ __global__ void __launch_bounds__(64 * MXV_WAVES) __attribute__((amdgpu_waves_pe
                     float v[8];
                     mx_load8<true>(s_v[m] + 32 * blk, tid & 3, v);
                     const int64_t r = m < nt ? s_p[n0 + m] : 0, b = (int64_t)cb * (COLS / 32) + blk;
-                    mx_store_block(v, s.o, r, b, onb, tid & 3, m < nt && b < onb);
+                    mx_store_few(v, s.o, r, b, onb, tid & 3, m < nt && b < onb);
                 }
             }
             // (s_sum and s_v are written again after the barriers in front of the next rows' products)
@@ -641,7 +653,7 @@ __global__ void __launch_bounds__(64 * MXF_WAVES) k_mx_front(MxFrontArgs g) {
         } else {
             mx_load8<true>(g.x + (int64_t)t * D + 32 * b, s, v);
         }
-        mx_store_block(v, g.o, t, b, nb, s, true);
+        mx_store_few(v, g.o, t, b, nb, s, true);
     }
     // (a lane past the chunks: chunk 0, not added; tokens past g.T: the last one's row again)
     const int c = lane < nch ? lane : 0;
@@ -709,13 +721,16 @@ constexpr int MXD_WAVES = 8, MXD_U = 8, MXD_KMAX = 64;
 
 template <int COLS>
 __global__ void __launch_bounds__(64 * MXD_WAVES) __attribute__((amdgpu_waves_per_eu(4))) k_mxd(MxDownArgs g) {
-    __shared__ __attribute__((aligned(16))) uint8_t sx[MXD_WAVES][4 * MXD_U * MX_XB];
+    constexpr int XROW = 4 * MXD_U * MX_FB;
+    __shared__ __attribute__((aligned(16))) uint8_t sx[MXD_WAVES * XROW + 16];   // (16 zeros last)
     __shared__ __attribute__((aligned(16))) uint32_t ss[MXD_WAVES][4 * MXD_U];
     __shared__ float s_z[MXD_KMAX + 1][16];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int q = blockIdx.x >> 3, grp = q / g.T, t = q - grp * g.T;
     const int64_t n0 = (int64_t)COLS * (8 * grp + ((int)blockIdx.x & 7));
     if (n0 >= g.D) return;
+    if (tid < 4) ((uint32_t *)(sx + MXD_WAVES * XROW))[tid] = 0;
+    __syncthreads();
     const int slots = g.K + (g.sh_a.data ? 1 : 0);
     for (int k = wave; k < slots; k += MXD_WAVES) {
         const bool shared = k == g.K;
@@ -727,33 +742,32 @@ __global__ void __launch_bounds__(64 * MXD_WAVES) __attribute__((amdgpu_waves_pe
         if ((unsigned)e >= (unsigned)(shared ? 1 : g.E)) continue;   // (the router's ids: not expected)
         MxTile<MXD_U> w;
         w.row = m.data + (int64_t)e * m.mat_bytes + (n0 + (lane & (COLS - 1))) * m.row_bytes;
-        double acc[1][4] = {{0.0, 0.0, 0.0, 0.0}};
+        double acc[4] = {0.0, 0.0, 0.0, 0.0};
         for (int k0 = 0; k0 < nb; k0 += 4 * MXD_U) {
             const int kn = imin(nb - k0, 4 * MXD_U), sn = (kn + 3) / 4;
             // (the operands in front of the weights: they are stored to LDS while those are on their way)
-            const u32x4 *src = (const u32x4 *)(x.d + r * mx_drow(nb) + (int64_t)MX_XB * k0);
-            constexpr int NX = 4 * MXD_U * MX_XB / 1024;
+            const u32x4 *src = (const u32x4 *)(x.d + r * (int64_t)(nb * MX_FB) + (int64_t)MX_FB * k0);
+            constexpr int NX = (4 * MXD_U * MX_FB + 1023) / 1024;
             u32x4 xv[NX];
-            uint32_t xs1 = 0;
+            uint32_t xs1 = MX_ONE;
 #pragma unroll
-            for (int i = 0; i < NX; ++i)
-                if (64 * i + lane < kn * (MX_XB / 16)) xv[i] = src[64 * i + lane];
-            if (lane < kn) xs1 = x.s[r * mx_srow(nb) + k0 + lane];
+            for (int i = 0; i < NX; ++i) xv[i] = 64 * i + lane < kn * (MX_FB / 16) ? src[64 * i + lane] : u32x4{0, 0, 0, 0};
+            if (lane < kn) xs1 = x.s[r * nb + k0 + lane];
             asm volatile("" ::: "memory");
             w.load(k0 / 4, sn, nb, lane);
             wave_lds_sync();   // (the activations before are read)
 #pragma unroll
             for (int i = 0; i < NX; ++i)
-                if (64 * i + lane < kn * (MX_XB / 16)) *(u32x4 *)(sx[wave] + 16 * (64 * i + lane)) = xv[i];
-            if (lane < kn) ss[wave][lane] = xs1;
+                if (64 * i + lane < 4 * MXD_U * MX_FB / 16) *(u32x4 *)(sx + XROW * wave + 16 * (64 * i + lane)) = xv[i];
+            if (lane < 4 * MXD_U) ss[wave][lane] = xs1;
             wave_lds_sync();
-            const uint8_t *const xd[1] = {sx[wave]};
-            const uint32_t *const xs[1] = {ss[wave]};
-            w.template products<1>(k0 / 4, sn, nb, lane, xd, xs, k0 / 4, 1, acc);
+            const int xo[2] = {XROW * wave, XROW * wave};
+            const uint32_t *const xs[2] = {ss[wave], ss[wave]};
+            w.products(k0 / 4, sn, nb, lane, sx, xo, MXD_WAVES * XROW, xs, k0 / 4, 1, acc);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const double a = mx_columns(acc[0][i]);
+            const double a = mx_columns(acc[i]);
             if ((lane & 15) == 0) s_z[k][4 * (lane >> 4) + i] = (float)a;
         }
     }

@@ -895,9 +895,9 @@ __global__ void __launch_bounds__(DISPATCH_THREADS) k_dispatch(const int32_t *__
 // latencies (104 rows of 768 values, 128 experts: 5.5 us, by themselves 5.6 and 4.3).
 template <bool VEC>
 __global__ void __launch_bounds__(DISPATCH_THREADS) k_dispatch_mx(const int32_t *__restrict__ ids, int64_t n, int E, int BM, Dispatch d,
-                                                                  const float *__restrict__ src, int64_t ld, int64_t nrows, int nb, MxRows o) {
+                                                                  const float *__restrict__ src, int64_t ld, int64_t nrows, int nb, MxRows o, bool few) {
     if ((int)blockIdx.x < E) dispatch_expert(ids, n, E, BM, 1, d, blockIdx.x);
-    else mx_prep_thread<VEC>(src, ld, nrows, nb, o, (int64_t)(blockIdx.x - E) * DISPATCH_THREADS + threadIdx.x);
+    else mx_prep_thread<VEC>(src, ld, nrows, nb, o, few, (int64_t)(blockIdx.x - E) * DISPATCH_THREADS + threadIdx.x);
 }
 
 int launch_dispatch(const int32_t *ids, int64_t T, int K, int E, int BM, int balanced, const Dispatch &d,
@@ -909,16 +909,16 @@ int launch_dispatch(const int32_t *ids, int64_t T, int K, int E, int BM, int bal
 }
 
 int launch_dispatch_mx(const int32_t *ids, int64_t T, int K, int E, int BM, const Dispatch &d, const float *src, int64_t ld, int64_t nrows,
-                       int64_t Kx, const MxRows &o, hipStream_t st) {
+                       int64_t Kx, const MxRows &o, bool few, hipStream_t st) {
     if (E <= 0 || E > DISPATCH_MAX_E || K <= 0 || BM <= 0 || nrows <= 0 || Kx % 32 || Kx > 0x7fffffff) return -6;
     const int64_t wgs = E + (nrows * (Kx / 8) + DISPATCH_THREADS - 1) / DISPATCH_THREADS;
     if (wgs > 0x7fffffff) return -6;
     if (mx_prep_vec(src, ld))
         hipLaunchKernelGGL(k_dispatch_mx<true>, dim3((unsigned)wgs), dim3(DISPATCH_THREADS), 0, st, ids, T * (int64_t)K, E, BM, d, src, ld,
-                           nrows, (int)(Kx / 32), o);
+                           nrows, (int)(Kx / 32), o, few);
     else
         hipLaunchKernelGGL(k_dispatch_mx<false>, dim3((unsigned)wgs), dim3(DISPATCH_THREADS), 0, st, ids, T * (int64_t)K, E, BM, d, src, ld,
-                           nrows, (int)(Kx / 32), o);
+                           nrows, (int)(Kx / 32), o, few);
     return hip_check_launch();
 }
 

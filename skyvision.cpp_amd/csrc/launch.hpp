@@ -359,11 +359,11 @@ struct MxRows {
     uint8_t *d = nullptr;
     uint32_t *s = nullptr;
 };
-// operand rows of K values, filled up
-int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, hipStream_t st);
+// operand rows of K values, filled up; few: the operand of launch_mxv and launch_mxd
+int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, bool few, hipStream_t st);
 // launch_dispatch (balanced tiles) and launch_prep_mx (rows of Kx values) in one launch
 int launch_dispatch_mx(const int32_t *ids, int64_t T, int K, int E, int BM, const Dispatch &d, const float *src, int64_t ld, int64_t nrows,
-                       int64_t Kx, const MxRows &o, hipStream_t st);
+                       int64_t Kx, const MxRows &o, bool few, hipStream_t st);
 // Grouped products.  MX_STORE: fp32 rows y; MX_GLU / MX_RELU_SQR: the
 // activation rows leave as the next product's operand o (rows of ncols
 // values, ncols % 32 == 0).  A shared expert (sh_rows > 0) rides in the same

@@ -23,6 +23,12 @@
 // scale byte; 255 where the row's block holds a NaN or leaves the fp16 range
 // of d), rows of a multiple of four words.  The blocks that fill up a row hold
 // zeros.
+//
+// The products of few rows add the blocks' sums in fp64, where the significand
+// costs nothing: their operand (the same MxRows, rows of nb blocks) holds the
+// two digits of q alone, 48 bytes per block (digit 0's and 1's first 16 bytes,
+// then their last 8), and a word per block: the float M / 1024 in its upper 24
+// bits (NaN where x^ is none), digit 0's scale byte 2^(k + 10 + 3) in the low 8.
 #pragma once
 
 #include "common.hpp"
@@ -34,6 +40,8 @@ namespace mimoe {
 constexpr int MX_BYTES = 17;        // a block of weights
 constexpr int MX_XB = 96;           // a block's digits in the operand
 constexpr uint32_t MX_ONE = 127;    // scale byte of 1
+
+constexpr int MX_FB = 48;           // a block's digits in the operand of few rows
 
 // bytes of the digits and words of the scales of an operand row of nb blocks, and the bytes of both
 __device__ __host__ constexpr int64_t mx_drow(int64_t nb) { return (nb + 1) / 2 * (2 * MX_XB); }
@@ -63,11 +71,15 @@ __device__ __forceinline__ uint2 mx_digit(const uint32_t (&u)[8], int i) {
     return r;
 }
 
-// Block b of operand row r (of nb blocks) by the four lanes 4 k .. 4 k + 3:
-// lane s (= lane & 3) holds values 4 s .. 4 s + 3 in v[0..3] and 16 + 4 s .. in
-// v[4..7]; writes digit s, lane 0 the scale word.  live: the lane writes (all
-// four lanes of a block take part).
-__device__ __forceinline__ void mx_store_block(const float (&v)[8], const MxRows &o, int64_t r, int64_t b, int nb, int s, bool live) {
+// A block by the four lanes 4 k .. 4 k + 3: lane s (= lane & 3) holds values 4
+// s .. 4 s + 3 in v[0..3] and 16 + 4 s .. in v[4..7].  Its codes q, and d = M
+// 2^(ex - 25) (ex at least 1); bad: d is no number.
+struct MxBlock {
+    int q[8], M;
+    uint32_t ex;
+    bool bad;
+};
+__device__ __forceinline__ MxBlock mx_block(const float (&v)[8]) {
     uint32_t m = 0;   // largest |x| by its bits: a NaN is above every number
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -81,12 +93,23 @@ __device__ __forceinline__ void mx_store_block(const float (&v)[8], const MxRows
     const float d = __builtin_bit_cast(float, m) / 127.0f;
     const float id = d != 0.0f ? 1.0f / d : 0.0f;
     const uint32_t dh = f32_to_fp16_bits(d), ex = dh >> 10, man = dh & 0x3ffu;   // (d >= 0 or NaN)
-    const bool bad = (ex & 31u) == 31u;
-    const int M = bad ? 0 : (int)(ex ? man + 1024u : man);
-    const uint32_t k = MX_ONE + 3 - 25 + (ex ? ex : 1u);
+    MxBlock k;
+    k.bad = (ex & 31u) == 31u;
+    k.M = k.bad ? 0 : (int)(ex ? man + 1024u : man);
+    k.ex = ex ? ex : 1u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) k.q[j] = (int)roundf(v[j] * id);
+    return k;
+}
+
+// Block b of operand row r (of nb blocks): the lane writes digit s, lane 0 the
+// scale word.  live: the lane writes (all four lanes of a block take part).
+__device__ __forceinline__ void mx_store_block(const float (&v)[8], const MxRows &o, int64_t r, int64_t b, int nb, int s, bool live) {
+    const MxBlock blk = mx_block(v);
+    const uint32_t k = MX_ONE + 3 - 25 + blk.ex;
     uint32_t u[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = (uint32_t)(M * (int)roundf(v[j] * id) + 16 * (1 + 32 + 32 * 32 + 32 * 32 * 32));
+    for (int j = 0; j < 8; ++j) u[j] = (uint32_t)(blk.M * blk.q[j] + 16 * (1 + 32 + 32 * 32 + 32 * 32 * 32));
     uint2 p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) p[i] = mx_digit(u, i);
@@ -111,9 +134,34 @@ __device__ __forceinline__ void mx_store_block(const float (&v)[8], const MxRows
     uint8_t *xb = o.d + r * mx_drow(nb) + MX_XB * b;
     *(uint4 *)(xb + 16 * s) = make_uint4(p[0].x, p[0].y | p[1].x << 16, p[1].x >> 16 | p[1].y << 16, p[2].x);
     *(uint2 *)(xb + 64 + 8 * s) = make_uint2(p[2].y | p[3].x << 16, p[3].x >> 16 | p[3].y << 16);
-    if (s == 0) o.s[r * mx_srow(nb) + b] = bad ? 0xffffffffu : k * 0x01010101u + 0x0f0a0500u;
+    if (s == 0) o.s[r * mx_srow(nb) + b] = blk.bad ? 0xffffffffu : k * 0x01010101u + 0x0f0a0500u;
 }
-// the blocks that fill up the row, by the same lanes
+// The same for few rows: lane s writes half s / 2 of digit s & 1
+__device__ __forceinline__ void mx_store_few(const float (&v)[8], const MxRows &o, int64_t r, int64_t b, int nb, int s, bool live) {
+    const MxBlock blk = mx_block(v);
+    uint32_t u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = (uint32_t)(blk.q[j] + 16 * (1 + 32));
+    const uint2 p0 = mx_digit(u, 0), p1 = mx_digit(u, 1);
+    uint2 t = (s & 1) ? p0 : p1;
+    t.x = (uint32_t)dpp_i<0xB1>((int)t.x);
+    t.y = (uint32_t)dpp_i<0xB1>((int)t.y);
+    const uint2 lo = (s & 1) ? t : p0, hi = (s & 1) ? p1 : t;   // 6 bytes each
+    if (!live) return;
+    const uint32_t w0 = lo.x, w1 = lo.y | hi.x << 16, w2 = hi.x >> 16 | hi.y << 16;
+    uint8_t *xb = o.d + r * (int64_t)(nb * MX_FB) + MX_FB * b;
+    uint32_t *x16 = (uint32_t *)(xb + 16 * (s & 1)), *x8 = (uint32_t *)(xb + 32 + 8 * (s & 1));
+    if (s < 2) {
+        *(uint2 *)x16 = make_uint2(w0, w1);
+        x16[2] = w2;
+    } else {
+        x16[3] = w0;
+        *(uint2 *)x8 = make_uint2(w1, w2);
+    }
+    const uint32_t f = blk.bad ? 0x7fc00000u : __builtin_bit_cast(uint32_t, (float)blk.M * 0x1p-10f);
+    if (s == 0) o.s[r * nb + b] = f | (blk.bad ? MX_ONE : MX_ONE + 3 + 10 - 25 + blk.ex);
+}
+// the blocks that fill up the row (mx_store_block), by the same lanes
 __device__ __forceinline__ void mx_store_pad(const MxRows &o, int64_t r, int nb, int s) {
     if (nb & 1) {
         uint8_t *xb = o.d + r * mx_drow(nb) + MX_XB * (int64_t)nb;
@@ -140,14 +188,19 @@ __device__ __forceinline__ void mx_load8(const float *x, int s, float (&v)[8]) {
 }
 
 // Rows of 32 nb values (row r at src + r ld) into operand rows: four threads
-// per block, thread i (of nrows nb 4, filled up to whole waves)
+// per block, thread i (of nrows nb 4, filled up to whole waves); few: the
+// operand of few rows
 template <bool VEC>
-__device__ __forceinline__ void mx_prep_thread(const float *__restrict__ src, int64_t ld, int64_t nrows, int nb, const MxRows &o, int64_t i) {
+__device__ __forceinline__ void mx_prep_thread(const float *__restrict__ src, int64_t ld, int64_t nrows, int nb, const MxRows &o, bool few, int64_t i) {
     const int64_t blk = i >> 2;
     const bool live = blk < nrows * nb;
     const int64_t r = live ? blk / nb : 0, b = live ? blk - r * nb : 0;
     float v[8];
     mx_load8<VEC>(src + r * ld + 32 * b, (int)(i & 3), v);
+    if (few) {
+        mx_store_few(v, o, r, b, nb, (int)(i & 3), live);
+        return;
+    }
     mx_store_block(v, o, r, b, nb, (int)(i & 3), live);
     if (live && b == nb - 1) mx_store_pad(o, r, nb, (int)(i & 3));
 }
