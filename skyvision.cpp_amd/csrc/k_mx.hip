@@ -212,7 +212,7 @@ __device__ __attribute__((noinline)) float mx_act(double a, double b) {
 // work of a step (unpacking 17-byte blocks, four conversions and fp64
 // multiply-adds): two rows share it all; with the significand in the digits
 // (four, a column of each) a row had it alone, and 120 rows of 64 experts
-// (K 2048, 2048 rows) took FIGURE.
+// (K 2048, 2048 rows) took 60 us instead of 52.
 //
 // Loads: two per step and lane (the five dwords of its block, at dword
 // aligned addresses), 68 bytes of a row together; the load path takes such a
