@@ -1531,8 +1531,7 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
     const uintptr_t xb = (uintptr_t)x, ob = (uintptr_t)out, row = sizeof(float) * (uintptr_t)D;
     const bool fuse_norm = dec1 && np.kind != NORM_NONE && (ob + row <= xb || xb + row <= ob);
     // a few tokens of an MXFP4 layer: the norm in the router's launch, unless
-    // another launch reads the normalized rows too (the shared expert's gate
-    // row) or out overlaps the rows in part
+    // another launch reads the normalized rows too (the shared expert's gate row)
     const bool few = mx_few(c, L, T, routing);
     MxFrontArgs ff;
     const bool few_front = few && mx_few_front(L, x, xr, T, np, ff) && !(np.kind != NORM_NONE && L->sh_n_ff > 0 && L->sh_gate_inp);

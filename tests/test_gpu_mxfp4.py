@@ -464,3 +464,141 @@ def test_quantize_then_layer_run_together(ctx):
         got = out.download(np.float32, (T, D))
         assert np.linalg.norm(got - ref) <= (1e-3 if T * K > 2 * E else 1e-6) * np.linalg.norm(ref)
     st.destroy()
+
+
+# ------------------------------------------------------------------ a few tokens' launches
+# (the launches take norm and router up to 4 tokens and rows of 64-value chunks up to 4096, the rest up to 16 tokens)
+FEW = {
+    "eleven_chunks": dict(D=704, E=5, K=2, I=32, fused=True, act=0),
+    "no_chunks": dict(D=96, E=7, K=3, I=96, fused=False, act=1),
+    "widest": dict(D=4096, E=6, K=2, I=64, fused=False, act=2, gating=2),
+    "past_widest": dict(D=4160, E=6, K=2, I=64, fused=True, act=3),
+    "many_experts": dict(D=64, E=256, K=10, I=32, fused=False, act=4, gating=1),
+    "every_expert": dict(D=128, E=32, K=32, I=32, fused=False, act=0),
+    "long_down": dict(D=128, E=16, K=6, I=2080, fused=False, act=4, gating=1, shared=4128),
+    "gated_shared": dict(D=320, E=12, K=3, I=1056, fused=False, act=0, shared=96, sh_gate_inp=True),
+}
+
+
+def check_few(got, ref, size, K):
+    """the tolerance of layers of few rows (above) for K slots and a shared expert"""
+    assert (np.abs(got - ref) <= ((K + 4) * 2.0 ** -24 + 2.0 ** -21) * size + 2.0 ** -23 * np.abs(ref)).all()
+
+
+@pytest.fixture(scope="module")
+def few_ctx():
+    c = M.Context(0)
+    c.reserve(24, 4160, 2080, 256, 32)
+    yield c
+    c.set_fused_decode(M.DECODE_FUSED)
+    c.close()
+
+
+@pytest.mark.parametrize("name", FEW)
+def test_few_tokens(few_ctx, name):
+    """the few launches and the separate ones against the float64 form, at and past the sizes where they change"""
+    lay = Layer(seed=40 + len(name), **FEW[name])
+    rng = np.random.default_rng(len(name))
+    few_ctx.set_gemm_threshold(1 << 40)
+    for T in (1, 2, 3, 4, 5, 15, 16, 17):
+        x, res = rows(rng, T, lay.D), rows(rng, T, lay.D)
+        ref, size = lay.reference(x, res), sizes(lay, x)
+        xd, rd = M.to_device(x), M.to_device(res)
+        for mode in (M.DECODE_FUSED, M.DECODE_CHAIN):
+            few_ctx.set_fused_decode(mode)
+            out = M.to_device(np.full((T + 1, lay.D), 7.0, np.float32))
+            M.check("forward", few_ctx.forward(lay.L, xd, T, rd, out))
+            M.synchronize()
+            got = out.download(np.float32, (T + 1, lay.D))
+            assert (got[T] == 7.0).all()
+            check_few(got[:T], ref, size, lay.K)
+
+
+@pytest.mark.parametrize("kind", [M.NORM_RMS, M.NORM_LAYER])
+@pytest.mark.parametrize("name", ["eleven_chunks", "no_chunks", "widest", "gated_shared"])
+def test_few_tokens_norm(few_ctx, name, kind):
+    """the norm inside equals the norm in front bit for bit; weights and bias at any 4 bytes, out over the rows"""
+    lay = Layer(seed=50 + len(name), **FEW[name])
+    rng = np.random.default_rng(len(name) + kind)
+    few_ctx.set_gemm_threshold(1 << 40)
+    few_ctx.set_fused_decode(M.DECODE_FUSED)
+    w, b = M.to_device(rows(rng, lay.D + 1)), M.to_device(rows(rng, lay.D + 3))
+    for norm in (M.make_norm(kind, 1e-5, w.addr + 4, b.addr + 12 if kind == M.NORM_LAYER else None), M.make_norm(kind, 1e-5, None, None)):
+        for T in (1, 3, 4, 5):
+            h = M.to_device(rows(rng, T, lay.D))
+            hn, a = M.DeviceBuffer(4 * T * lay.D), M.DeviceBuffer(4 * T * lay.D)
+            M.check("norm", few_ctx.norm(norm, h, T, lay.D, hn))
+            M.check("forward", few_ctx.forward(lay.L, hn, T, h, a))
+            M.check("forward_norm", few_ctx.forward_norm(lay.L, norm, h, T, h, h))
+            M.synchronize()
+            assert np.array_equal(a.download(np.uint8, (4 * T * lay.D,)), h.download(np.uint8, (4 * T * lay.D,)))
+
+
+def test_few_tokens_not_a_number(few_ctx):
+    """a token with a NaN, an infinity, or values past the range of an fp16 scale: itself alone"""
+    lay = Layer(seed=60, **FEW["eleven_chunks"])
+    rng = np.random.default_rng(61)
+    few_ctx.set_gemm_threshold(1 << 40)
+    x = rows(rng, 4, 704)
+    clean = x.copy()
+    x[0, 5], x[1, 700], x[2, 64] = np.nan, np.inf, 1e9
+    for mode in (M.DECODE_FUSED, M.DECODE_CHAIN):
+        few_ctx.set_fused_decode(mode)
+        got = []
+        for v in (x, clean):
+            out = M.DeviceBuffer(4 * 4 * 704)
+            M.check("forward", few_ctx.forward(lay.L, M.to_device(v), 4, None, out))
+            M.synchronize()
+            got.append(out.download(np.float32, (4, 704)))
+        assert np.isnan(got[0][:3]).all()
+        assert np.array_equal(got[0][3], got[1][3]) and np.isfinite(got[1]).all()
+
+
+def test_few_tokens_norm_graph(few_ctx):
+    lay = Layer(seed=62, **FEW["gated_shared"])
+    rng = np.random.default_rng(63)
+    few_ctx.set_gemm_threshold(0)
+    few_ctx.set_fused_decode(M.DECODE_FUSED)
+    norm = M.make_norm(M.NORM_RMS, 1e-6, M.to_device(rows(rng, 320)), None)
+    st = M.Stream()
+    for T in (1, 4, 7):
+        x, out, eager = (M.DeviceBuffer(4 * T * 320) for _ in range(3))
+        x.upload(rows(rng, T, 320))
+        g = M.Graph(st, lambda s: M.check("forward_norm", few_ctx.forward_norm(lay.L, norm, x, T, x, out, None, s.addr)))
+        for _ in range(3):
+            x.upload(rows(rng, T, 320))
+            M.synchronize()
+            g.launch(st)
+            st.synchronize()
+            M.check("forward_norm", few_ctx.forward_norm(lay.L, norm, x, T, x, eager))
+            M.synchronize()
+            assert np.array_equal(out.download(np.uint8, (4 * T * 320,)), eager.download(np.uint8, (4 * T * 320,)))
+        g.destroy()
+    st.destroy()
+
+
+@pytest.mark.parametrize("T,K,shift", [(1, 1, 0), (3, 4, 4), (8, 8, 0), (8, 8, 8), (70, 8, 0), (90, 6, 12)])
+def test_product_of_few_rows_by_ids(ctx, T, K, shift):
+    """rows that the work-groups make operands of themselves, and (rows off 16 bytes, more than 512 rows) that another
+    launch does; ids outside, each expert's rows odd in number"""
+    n, N, E = 2080, 96, 64
+    rng = np.random.default_rng(T + K)
+    raw = table(rng, E, N, n)
+    ctx.set_gemm_threshold(1 << 40)
+    try:
+        for own in (False, True):
+            b = rows(rng, T, K if own else 1, n)
+            ids = rng.integers(-1, 6, (T, K)) if T > 1 else np.array([[E - 1]])
+            bd = M.DeviceBuffer(b.nbytes + 16).upload(b, shift)
+            out = M.to_device(np.full((T * K + 1, N), 7.0, np.float32))
+            ctx.take_errors()
+            wd, idd = M.to_device(raw), M.to_device(ids.astype(np.int32))
+            M.check("mul_mat_id", ctx.mul_mat_id(M.tensor(wd, MX, [n, N, E]), M.tensor(bd.addr + shift, M.TYPE_F32, [n, b.shape[1], T]),
+                                                 M.tensor(idd, M.TYPE_I32, [K, T]), M.tensor(out, M.TYPE_F32, [N, K, T])))
+            M.synchronize()
+            assert ctx.take_errors()[0] == (ids < 0).sum()
+            got = out.download(np.float32, (T * K + 1, N))
+            assert (got[-1] == 7.0).all() and not got[:-1].reshape(T, K, N)[ids < 0].any()
+            check_product(got[:-1].reshape(T, K, N), raw, b, ids, True)
+    finally:
+        ctx.set_gemm_threshold(0)
