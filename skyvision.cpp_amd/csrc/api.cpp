@@ -783,7 +783,7 @@ int64_t mx_layer_tokens(const mi_moe_layer *L) {
 // experts (K 2048, 2048 rows of 64 experts: 40 rows 33 against 32 us, 64 rows
 // 41 against 38, 512 rows 137 against 49; 16 rows 23 against 31), for a layer
 // above two per expert: its few-row form takes few launches and its sums are
-// exact (64 experts: 80 rows 86 against 90 us, 128 rows 113 against 94).
+// exact (64 experts: 80 rows 80 against 84 us, 128 rows 100 against 93).
 // (Rows further apart than it addresses keep the other kernel.)
 bool use_gemm_mx(const mi_moe_ctx *c, int64_t T, int K, int E, size_t row_bytes, bool layer) {
     if ((int64_t)row_bytes > MXG_MAX_ROW_BYTES) return false;   // (then a token's operand row is far below MXG_MAX_X)
@@ -816,7 +816,7 @@ bool mx_shared_ok(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
 // and operand rows (k_mx_front); the experts' ranking, gate/up products and
 // activation rows (k_mxv); down products, weighted sum and residual (k_mxd).
 // Up to MX_FEW_T tokens (and MXV_FRONT_T for the first launch: more run the
-// norm, the router and the operand pass by themselves), the routed part on the
+// norm by itself and the operand rows with the router), the routed part on the
 // few-row product, no dispatch outputs asked for.
 constexpr int64_t MX_FEW_T = 16;
 bool mx_few(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T, const mi_moe_routing *routing) {
@@ -833,13 +833,13 @@ bool mx_few_front(const mi_moe_layer *L, const float *x, const float *xr, int64_
 }
 // the launches after the logits: rank them here (front: the operand rows are
 // there too), else sel and w are there already
-int run_mx_few(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T, bool front, const Gating &gt, const float *res,
+int run_mx_few(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T, bool front, bool x_done, const Gating &gt, const float *res,
                float *out, const float *sh_w, hipStream_t st) {
     const int D = L->n_embd, E = L->n_expert, K = L->n_expert_used, I = L->n_ff;
     const int64_t rows = T * K, S = L->sh_n_ff;
     const bool gated = act_gated(L->act);
     const MxRows mx = mx_rows(c->ax.q8, T, D), ma = mx_rows(c->aact.q8, rows, I);
-    if (!front) {
+    if (!front && !x_done) {
         TRY(launch_prep_mx(x, D, T, D, mx, true, st));
         stage_end(c, "q8_x", st);
     }
@@ -875,7 +875,7 @@ int run_mx_few(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T, 
 // grouped GEMM (k_mxg.hip); the gate/up launch of either writes the down
 // product's operand rows itself.  Arguments as run_experts_b32.
 int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T, const int32_t *ids_gu,
-                   const int32_t *ids_dn, const float *w, const float *res, float *out, hipStream_t st, bool check_ids,
+                   const int32_t *ids_dn, const float *w, const float *res, float *out, hipStream_t st, bool x_done, bool check_ids,
                    const float *add, bool disp_out, bool sh_here, const float *sh_w) {
     const int D = L->n_embd, E = L->n_expert, K = L->n_expert_used, I = L->n_ff;
     const int64_t rows = T * K;
@@ -890,7 +890,7 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
         for (int64_t t0 = 0; t0 < T; t0 += tmax) {
             const int64_t n = std::min(tmax, T - t0);
             TRY(run_experts_mx(c, L, x + t0 * D, n, ids_gu + t0 * K, ids_dn + t0 * K, w + t0 * K, res ? res + t0 * D : nullptr,
-                               out + t0 * D, st, check_ids, add ? add + t0 * D : nullptr, disp_out, false, nullptr));
+                               out + t0 * D, st, false, check_ids, add ? add + t0 * D : nullptr, disp_out, false, nullptr));
         }
         DispBuf whole = c->disp[0];
         whole.bad_total = nullptr;   // (counted by the passes)
@@ -901,9 +901,10 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
     const bool self_disp = !gemm && same_ids && !check_ids && !disp_out && rows <= MXV_IDS;
     const MxRows mx = mx_rows(c->ax.q8, T, D), ma = mx_rows(c->aact.q8, rows, I);
     if (self_disp) {
-        TRY(launch_prep_mx(x, D, T, D, mx, !gemm, st));
+        if (!x_done) TRY(launch_prep_mx(x, D, T, D, mx, !gemm, st));
     } else {
-        TRY(launch_dispatch_mx(ids_gu, T, K, E, bm, c->disp[0].view(), x, D, T, D, mx, !gemm, st));
+        if (x_done) TRY(launch_dispatch(ids_gu, T, K, E, bm, 1, c->disp[0].view(), st));
+        else TRY(launch_dispatch_mx(ids_gu, T, K, E, bm, c->disp[0].view(), x, D, T, D, mx, !gemm, st));
         if (!same_ids) TRY(launch_dispatch(ids_dn, T, K, E, bm, 1, c->disp[1].view(), st));
     }
     const DispBuf &dg = c->disp[0];
@@ -963,7 +964,7 @@ int run_experts(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T,
     if (is_b32f(L->gate.type))
         return run_experts_b32(c, L, x, T, ids_gu, ids_dn, w, res, out, st, x_done, check_ids, add, disp_out, sh_here, sh_w);
     if (is_mx(L->gate.type))
-        return run_experts_mx(c, L, x, T, ids_gu, ids_dn, w, res, out, st, check_ids, add, disp_out, sh_here, sh_w);
+        return run_experts_mx(c, L, x, T, ids_gu, ids_dn, w, res, out, st, x_done, check_ids, add, disp_out, sh_here, sh_w);
     const int D = L->n_embd, E = L->n_expert, K = L->n_expert_used, I = L->n_ff;
     const int64_t rows = T * K;
     const int max_active = (int)std::min<int64_t>(E, rows);
@@ -1557,7 +1558,7 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
         ff.o = mx_rows(c->ax.q8, T, D);
         TRY(launch_mx_front(ff, st));
         stage_end(c, "router", st);
-        TRY(run_mx_few(c, L, x, T, true, layer_gating(L), res, out, L->sh_gate_inp ? c->sh_w : nullptr, st));
+        TRY(run_mx_few(c, L, x, T, true, true, layer_gating(L), res, out, L->sh_gate_inp ? c->sh_w : nullptr, st));
     } else if (dec1) {
         TRY(run_decode1(c, L, x, res, out, P, C, fuse_norm ? np : NormParams{}, st));
     } else if (!xr && plan_decodeb(c, L, x, T, cc)) {
@@ -1572,6 +1573,15 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
             (!gb_path(c, L, T) || T <= gb_layer_tokens(L))) {
             qx = Q8Out{};
             qx.b32 = b32_x_prep(c, L, T);
+            qx.b_src = x;
+            qx.b_ld = D;
+            xq = true;
+        }
+        const bool mx_gemm = is_mx(L->gate.type) && mx_layer_gemm(c, L, T) && mx_layer_tokens(L) > 0;
+        if (is_mx(L->gate.type) && front_takes_b32(L->router_w, xrow, D, D, x, D) && !(mx_gemm && T > mx_layer_tokens(L))) {
+            qx = Q8Out{};
+            qx.mx = mx_rows(c->ax.q8, T, D);
+            qx.mx_few = !mx_gemm;
             qx.b_src = x;
             qx.b_ld = D;
             xq = true;
@@ -1592,7 +1602,7 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
             TRY(launch_topk_softmax(c->logits, E, T, E, K, c->sel, K, c->w, st, gt));
         }
         stage_end(c, "topk_softmax", st);
-        if (few) TRY(run_mx_few(c, L, x, T, false, gt, res, out, L->sh_gate_inp ? c->sh_w : nullptr, st));
+        if (few) TRY(run_mx_few(c, L, x, T, false, x_done, gt, res, out, L->sh_gate_inp ? c->sh_w : nullptr, st));
         else TRY(run_experts(c, L, x, T, c->sel, c->sel, c->w, res, out, st, x_done, false, add,
                         routing && (routing->counts || routing->offsets || routing->perm), sh_here,
                         L->sh_gate_inp ? c->sh_w : nullptr));

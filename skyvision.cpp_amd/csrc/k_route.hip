@@ -381,6 +381,15 @@ __device__ __forceinline__ void front_b32(const Q8Out &o, int64_t t0, int64_t T,
     }
 }
 
+// the same for MXFP4 operand rows (o.mx): a quarter block per thread
+__device__ __forceinline__ void front_mx(const Q8Out &o, int64_t t0, int64_t T, int D, int wg, int nwg) {
+    const int nch = D / 8, rows = T - t0 < 16 ? (int)(T - t0) : 16, step = nwg * (int)blockDim.x;
+    for (int i = wg * (int)blockDim.x + (int)threadIdx.x; i < rows * nch; i += step) {
+        const int r = i / nch, q = i - r * nch;
+        mx_prep_quarter<true>(o.b_src + (t0 + r) * o.b_ld, o.mx, t0 + r, q >> 2, D / 32, q & 3, o.mx_few, true);
+    }
+}
+
 // The front of a forward: every work-group computes its logit tile, and with
 // a Q8_K output (o.q8 or o.xh set) quantizes its share of the slab's x rows
 // (row group item i = row * ngrp + grp by work-group i % net, wave i / net
@@ -432,6 +441,8 @@ __global__ void __launch_bounds__(1024) k_front(const float *__restrict__ W, con
     }
     if constexpr (XO == XO_B32) {
         front_b32(o, t0, T, D, et, net);
+    } else if constexpr (XO == XO_MX) {
+        front_mx(o, t0, T, D, et, net);
     } else if (o.q8 || o.xh) {
         const int nb = D / QK, ngrp = (nb + 3) >> 2;
         for (int i = et + net * wave; i < 16 * ngrp; i += net * RT_WAVES) {
@@ -508,6 +519,8 @@ __global__ void __launch_bounds__(1024) k_front_parts(const float *__restrict__ 
     }
     if constexpr (XO == XO_B32) {
         front_b32(o, t0, T, D, et * nsp + split, net * nsp);
+    } else if constexpr (XO == XO_MX) {
+        front_mx(o, t0, T, D, et * nsp + split, net * nsp);
     } else if (o.q8 || o.xh) {
         const int nb = D / QK, ngrp = (nb + 3) >> 2;
         const int nwg = net * nsp, wg = et * nsp + split, nw = (int)(blockDim.x >> 6);
@@ -540,7 +553,10 @@ int launch_front(const float *W, const float *b, const float *x, int64_t ldx, in
     const int64_t blocks = 8 * net * ((nslab + 7) / 8);
     if (blocks > 0x7fffffff) return -6;
     const Q8Out o = qx ? *qx : Q8Out{};
-    if (b32)
+    if (b32 && o.mx.d)
+        hipLaunchKernelGGL((k_front<true, XO_MX>), dim3((unsigned)blocks), dim3(64 * RT_WAVES), 0, st, W, b, x, ldx,
+                           T, D, E, logits, o);
+    else if (b32)
         hipLaunchKernelGGL((k_front<true, XO_B32>), dim3((unsigned)blocks), dim3(64 * RT_WAVES), 0, st, W, b, x, ldx,
                            T, D, E, logits, o);
     else if (vec && q8_xo(o) == XO_Q4)
@@ -570,7 +586,9 @@ int launch_front_parts(const float *W, const float *x, int64_t ldx, int64_t T, i
     if (blocks > 0x7fffffff) return -6;
     const Q8Out o = qx ? *qx : Q8Out{};
     const dim3 grid((unsigned)blocks), block((unsigned)(64 * cps));
-    if (b32)
+    if (b32 && o.mx.d)
+        hipLaunchKernelGGL((k_front_parts<true, XO_MX>), grid, block, 0, st, W, x, ldx, T, D, E, cps, parts, o);
+    else if (b32)
         hipLaunchKernelGGL((k_front_parts<true, XO_B32>), grid, block, 0, st, W, x, ldx, T, D, E, cps, parts, o);
     else if (vec && q8_xo(o) == XO_Q4)
         hipLaunchKernelGGL((k_front_parts<true, XO_Q4>), grid, block, 0, st, W, x, ldx, T, D, E, cps, parts, o);

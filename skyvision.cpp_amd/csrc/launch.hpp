@@ -47,6 +47,12 @@ struct B32Prep {
     int64_t ldo = 0;           // >= K; values K .. ldo - 1 of a row are written as zeros
 };
 
+// MXFP4 operand rows (mx.hpp): digits (64-byte aligned) and scale words (16-byte aligned)
+struct MxRows {
+    uint8_t *d = nullptr;
+    uint32_t *s = nullptr;
+};
+
 // ---- routing (k_route.hip)
 struct Q8Out {
     int8_t *q8 = nullptr;        // [rows][K] natural order (GEMV path)
@@ -60,8 +66,11 @@ struct Q8Out {
     int pre_act = 0;             // 4 (ACT_RELU_SQR): quantize relu(v)^2 instead of v
     int32_t *range_total = nullptr;   // [1] or null: blocks whose xh saturated at the fp16 range
     // the router's launch only, in place of the above: rows b_src (b_ld apart)
-    // as b32 asks (where front_takes_b32)
+    // as b32 asks or, with mx.d, MXFP4 operand rows (mx_few: of few rows)
+    // (where front_takes_b32)
     B32Prep b32;
+    MxRows mx;
+    int mx_few = 0;
     const float *b_src = nullptr;
     int64_t b_ld = 0;
 };
@@ -354,11 +363,6 @@ int launch_gb(const GBArgs &g, hipStream_t st);
 int launch_quantize_mx(const float *src, void *dst, int64_t nblocks, hipStream_t st);
 // rows of 32-value blocks (F16: 32 values per "block") of types 1, 2, 6, 8, 39 as fp32
 int launch_dequantize(int type, const void *src, float *dst, int64_t nblocks, hipStream_t st);
-// operand rows (mx.hpp): digits (64-byte aligned) and scale words (16-byte aligned)
-struct MxRows {
-    uint8_t *d = nullptr;
-    uint32_t *s = nullptr;
-};
 // operand rows of K values, filled up; few: the operand of launch_mxv and launch_mxd
 int launch_prep_mx(const float *src, int64_t ld, int64_t nrows, int64_t K, const MxRows &o, bool few, hipStream_t st);
 // launch_dispatch (balanced tiles) and launch_prep_mx (rows of Kx values) in one launch

@@ -187,22 +187,27 @@ __device__ __forceinline__ void mx_load8(const float *x, int s, float (&v)[8]) {
     }
 }
 
+// lane s's quarter of block b (of nb) of the row at src into operand row r;
+// few: the operand of few rows
+template <bool VEC>
+__device__ __forceinline__ void mx_prep_quarter(const float *__restrict__ src, const MxRows &o, int64_t r, int64_t b, int nb, int s, bool few, bool live) {
+    float v[8];
+    mx_load8<VEC>(src + 32 * b, s, v);
+    if (few) {
+        mx_store_few(v, o, r, b, nb, s, live);
+        return;
+    }
+    mx_store_block(v, o, r, b, nb, s, live);
+    if (live && b == nb - 1) mx_store_pad(o, r, nb, s);
+}
 // Rows of 32 nb values (row r at src + r ld) into operand rows: four threads
-// per block, thread i (of nrows nb 4, filled up to whole waves); few: the
-// operand of few rows
+// per block, thread i (of nrows nb 4, filled up to whole waves)
 template <bool VEC>
 __device__ __forceinline__ void mx_prep_thread(const float *__restrict__ src, int64_t ld, int64_t nrows, int nb, const MxRows &o, bool few, int64_t i) {
     const int64_t blk = i >> 2;
     const bool live = blk < nrows * nb;
     const int64_t r = live ? blk / nb : 0, b = live ? blk - r * nb : 0;
-    float v[8];
-    mx_load8<VEC>(src + r * ld + 32 * b, (int)(i & 3), v);
-    if (few) {
-        mx_store_few(v, o, r, b, nb, (int)(i & 3), live);
-        return;
-    }
-    mx_store_block(v, o, r, b, nb, (int)(i & 3), live);
-    if (live && b == nb - 1) mx_store_pad(o, r, nb, (int)(i & 3));
+    mx_prep_quarter<VEC>(src + r * ld, o, r, b, nb, (int)(i & 3), few, live);
 }
 inline bool mx_prep_vec(const float *src, int64_t ld) { return ld % 4 == 0 && (uintptr_t)src % 16 == 0; }
 
