@@ -415,7 +415,8 @@ int mi_moe_ctx_stage_clock(mi_moe_ctx *ctx, const char *stage, double *ghz, int 
  * k-quant layers the GEMM when 2 * T * K >= E (from half a dispatched row
  * per expert); for Q4_0 / Q5_0 layers and mi_mul_mat_id when 4 * T * K > 5 * E
  * (more than 1.25 rows per expert), for Q8_0 / F16 layers when 2 * T * K >
- * 3 * E (more than 1.5), for MXFP4 when T * K > 2 * E. */
+ * 3 * E (more than 1.5), for MXFP4 layers when T * K > 2 * E and for
+ * mi_mul_mat_id of such tables when 2 * T * K > E. */
 int mi_moe_ctx_set_gemm_threshold(mi_moe_ctx *ctx, int64_t min_tokens_for_gemm);
 /* Row tiles of the grouped GEMMs.  Of Q4_K gate/up layers: 0 (the default) by
  * shape, 32-row tiles when the call dispatches at most 8 rows per expert on
@@ -434,7 +435,9 @@ int mi_moe_ctx_set_gemm_threshold(mi_moe_ctx *ctx, int64_t min_tokens_for_gemm);
  * and 192-row tiles (kinds 2 and 4: 32-row; 1 and 5: 192-row).  Q4_0 / Q5_0 / Q8_0
  * / F16 layers and mi_mul_mat_id of such tables have 32- and 128-row tiles
  * (kind 2: 32-row, 1: 128-row; others: by shape), mi_mul_mat_id of F16 tables
- * also 192-row tiles (kind 5; by shape above 32 rows per expert).  Kinds 0-2, 4 and 5 give the
+ * also 192-row tiles (kind 5; by shape above 32 rows per expert).  MXFP4: 32-
+ * and 64-row tiles (kind 2: 32-row, 1: 64-row; others: 64-row above 24 rows per
+ * expert).  Kinds 0-2, 4 and 5 give the
  * same bits (the same per-row arithmetic); the skinny products sum each
  * output's products in another order (fp32; the rows agree to ~2e-4 rel-L2
  * after the activations' fp16 and Q8_K roundings). */
@@ -450,6 +453,11 @@ int mi_moe_ctx_set_gemm_tiles(mi_moe_ctx *ctx, int kind);
  * a work-group that does not see a result after a bounded number of polls
  * computes it itself (the same bits), so the kernel needs no co-residency
  * guarantee and cannot deadlock on a GPU shared with other work.
+ * MXFP4 layers of up to 16 tokens, on the products of few rows and without
+ * dispatch outputs, take three launches in the fused mode (router with the
+ * norm; ranking, gate/up and activations; down, weighted sum, shared expert
+ * and residual), above 4 tokens with norm, router, top-k and operand rows in
+ * launches of their own.
  *   MI_DECODE_CHAIN              separate kernels
  *   MI_DECODE_FUSED              fused, plain launch (default)
  *   MI_DECODE_FUSED_COOPERATIVE  retired (MI_MOE_ERR_UNSUPPORTED): the fused
