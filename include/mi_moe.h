@@ -453,7 +453,7 @@ int mi_moe_ctx_set_gemm_tiles(mi_moe_ctx *ctx, int kind);
  * a work-group that does not see a result after a bounded number of polls
  * computes it itself (the same bits), so the kernel needs no co-residency
  * guarantee and cannot deadlock on a GPU shared with other work.
- * MXFP4 layers of up to 16 tokens, on the products of few rows and without
+ * MXFP4 layers of up to 32 tokens, on the products of few rows and without
  * dispatch outputs, take three launches in the fused mode (router with the
  * norm; ranking, gate/up and activations; down, weighted sum, shared expert
  * and residual), above 4 tokens with norm, router, top-k and operand rows in

@@ -817,8 +817,11 @@ bool mx_shared_ok(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
 // activation rows (k_mxv); down products, weighted sum and residual (k_mxd).
 // Up to MX_FEW_T tokens (and MXV_FRONT_T for the first launch: more run the
 // norm by itself and the operand rows with the router), the routed part on the
-// few-row product, no dispatch outputs asked for.
-constexpr int64_t MX_FEW_T = 16;
+// few-row product, no dispatch outputs asked for.  (128 experts, 8 slots: 24
+// tokens 115 us, in separate launches 123, 32 tokens 136 and 142; 6 slots, 40
+// tokens: both 314.  The first launch against norm and router apart: one token
+// 25.4 and 29.5 us, four 44.9 and 47.0.)
+constexpr int64_t MX_FEW_T = 32;
 bool mx_few(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T, const mi_moe_routing *routing) {
     if (!is_mx(L->gate.type) || !c->fused_decode || T > MX_FEW_T || T * L->n_expert_used > MXV_IDS) return false;
     if (L->n_embd % 16 || mx_layer_gemm(c, L, T)) return false;

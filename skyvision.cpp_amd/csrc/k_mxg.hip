@@ -3,10 +3,10 @@
 // the plain product.  Format and operand: mx.hpp.
 //
 // A work-group of WM x WN waves owns a balanced tile of at most BM = 32 WM
-// dispatched rows of one expert and 256 weight rows (GLU: 128 gate rows and the
-// matching 128 up rows); a wave 32 rows and C column tiles of 32 on
-// v_mfma_scale_f32_32x32x64_f8f6f4: four MFMAs per (column tile, two blocks),
-// one per digit.  Lane half h of the MFMA takes block 2 step + h.
+// dispatched rows of one expert and WROWS = 32 C WN weight rows (GLU: half of
+// them gate rows, half the matching up rows); a wave 32 rows and C column tiles
+// of 32 on v_mfma_scale_f32_32x32x64_f8f6f4: four MFMAs per (column tile, two
+// blocks), one per digit.  Lane half h of the MFMA takes block 2 step + h.
 //
 // The K loop runs over steps of two blocks.  While step s's MFMAs run, step s +
 // 1's operands are read from LDS into registers and step s + 3's loads go out,
@@ -16,16 +16,29 @@
 //    4 % 4): the rows of 16 lanes on different banks); rows past the tile read
 //    out of range (no memory traffic).  Each lane's own scale words go to
 //    registers, four steps ahead.
-//  * weights: stages of KG blocks in two buffers, each of the 256 rows' runs of
-//    68 (KG = 4) or 136 (8) bytes as 5 or 9 pieces from the dword at or below
-//    its first byte (blocks start at any byte, and rows may be misaligned).
+//  * weights: stages of four blocks in two buffers, each row's run of 68 bytes
+//    as 5 pieces from the dword at or below its first byte (blocks start at any
+//    byte, and rows may be misaligned).
 // One barrier per step; the loads of the step stay in flight across it, those
 // that the next steps need have come (all loads are made, past the last step its
 // own again: the counted waits rely on it).
 //
-// What the load path takes decides the shapes (measured, L2-resident data: 60 B
-// per cycle and CU for contiguous runs, 33 for rows of 13 pieces, 22 for rows
-// of 5): the larger the tile and the runs, the fewer of its cycles per MFMA.
+// Two tiles.  64 rows x 256 weight rows, four waves, 78 KB of LDS, two
+// work-groups to a CU: many rows per expert.  32 x 128, two waves, 39 KB, four
+// to a CU: few, where the tables' stream counts and more work-groups that wait
+// apart carry it (128 rows of 128 experts, K 2048: 32 x 256 in four waves 37 us,
+// 32 x 128 29; 301 tokens of 8 slots, K 704, N 2816: both 65).  A step's loads go
+// out in front of its LDS reads, in the small tile between its MFMAs (64 rows of
+// 64 experts 50 -> 47 us; the large tile 240 -> 246).
+//
+// What bounds the large tile (16384 rows of 64 experts, K 2048, N 2048: 225 us,
+// 610 TFLOP/s of the contract's products, four times that on the MFMA): a wave's
+// step is 57 vector instructions (most of them unpack weights), 12 LDS reads and
+// 16 MFMAs, and two waves to a SIMD overlap them in part: without the loop's
+// loads it takes 175 us, without the MFMAs 185, the stores are 22 of it.  Of the
+// load path it takes 59%: that takes 60 B per cycle and CU of contiguous runs and
+// 22 of runs of 5 pieces.  128-row tiles with runs of 9 pieces (8 waves, or 4 of
+// 64 x 128 in 512 registers) were slower: 250 and 270 against 246.
 #include "act.hpp"
 #include "common.hpp"
 #include "launch.hpp"
@@ -265,8 +278,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     // st / 2 % 3, registers by st % 2: 6 KS steps to a turn.  The loads of step
     // st: scale words of step st + 4 (even steps), activations of step st + 3
     // over step st's, and after a stage's last step the stage after next over
-    // it.  At its end at most its own loads are out (KG = 8: and the step's
-    // before's weights, which are needed two steps later).
+    // it.  At its end at most its own loads are out.
 #define MXG_A(k) ((k) % 3 == 0 ? sa0 : (k) % 3 == 1 ? sa1 : sa2)
 #define MXG_W(k) ((k) / KS % 2 == 0 ? sw0 : sw1)
     // step st's loads, part k of n
@@ -306,7 +318,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
         for (int i = 0; i < 16; ++i) {
             const int m = 32 * wr + 8 * (i >> 2) + 4 * h + (i & 3);
             if (m >= mrows) continue;
-            // (nontemporal: 2048 tokens, 2048 columns 249 -> 240 us, the tables stay in L2)
+            // (nontemporal: 16384 rows of 2048 columns 245 -> 241 us)
             float *y = s.y + (int64_t)s_p[m] * s.ldy;
 #pragma unroll
             for (int ct = 0; ct < C; ++ct) {

@@ -602,3 +602,37 @@ def test_product_of_few_rows_by_ids(ctx, T, K, shift):
             check_product(got[:-1].reshape(T, K, N), raw, b, ids, True)
     finally:
         ctx.set_gemm_threshold(0)
+
+
+def test_few_tokens_at_their_largest(ctx):
+    """31, 32 (the last that the few launches take) and 33 tokens"""
+    lay = Layer(seed=70, **FEW["gated_shared"])
+    rng = np.random.default_rng(71)
+    ctx.set_gemm_threshold(1 << 40)
+    try:
+        for T in (31, 32, 33):
+            x, res = rows(rng, T, 320), rows(rng, T, 320)
+            out = M.DeviceBuffer(4 * T * 320)
+            xd, rd = M.to_device(x), M.to_device(res)
+            M.check("forward", ctx.forward(lay.L, xd, T, rd, out))
+            M.synchronize()
+            check_few(out.download(np.float32, (T, 320)), lay.reference(x, res), sizes(lay, x), lay.K)
+    finally:
+        ctx.set_gemm_threshold(0)
+
+
+def test_product_tiles_same_bits(ctx):
+    """a row's sums do not depend on the tile that it is in"""
+    rng = np.random.default_rng(72)
+    raw, b = table(rng, 4, 300, 704), rows(rng, 333, 1, 704)
+    ids = rng.integers(0, 4, (333, 2))
+    ctx.set_gemm_threshold(1)
+    try:
+        got = []
+        for kind in (1, 2):
+            ctx.set_gemm_tiles(kind)
+            got.append(run_product(ctx, raw, b, ids))
+        assert np.array_equal(got[0], got[1])
+    finally:
+        ctx.set_gemm_threshold(0)
+        ctx.set_gemm_tiles(0)
