@@ -636,3 +636,48 @@ def test_product_tiles_same_bits(ctx):
     finally:
         ctx.set_gemm_threshold(0)
         ctx.set_gemm_tiles(0)
+
+
+@pytest.mark.parametrize("T", [1, 3, 20, 80])
+def test_layer_rows_off_16_bytes(ctx, T):
+    lay = Layer(seed=73, **LAYERS["qwen_like"])
+    rng = np.random.default_rng(74)
+    x, res = rows(rng, T, 512), rows(rng, T, 512)
+    got = []
+    for off in (0, 4):
+        xd, rd = M.DeviceBuffer(x.nbytes + 16).upload(x, off), M.DeviceBuffer(x.nbytes + 16).upload(res, off)
+        out = M.DeviceBuffer(x.nbytes + 16)
+        M.check("forward", ctx.forward(lay.L, xd.addr + off, T, rd.addr + off, out.addr + off))
+        M.synchronize()
+        got.append(out.download(np.float32, (T, 512), off))
+        check_layer(got[-1], lay.reference(x, res), sizes(lay, x), T * lay.K <= 2 * lay.E)
+
+
+def test_two_contexts_on_two_streams(ctx):
+    """calls that run side by side, each context's workspace its own"""
+    lay = Layer(seed=75, **LAYERS["nemotron_like"])
+    rng = np.random.default_rng(76)
+    other = M.Context(0)
+    other.reserve(64, 672, 448, 12, 6)
+    streams = (M.Stream(), M.Stream())
+    try:
+        for T in (1, 4, 12, 60):
+            x = [M.to_device(rows(rng, T, 672)) for _ in range(2)]
+            alone = []
+            for c, v in zip((ctx, other), x):
+                o = M.DeviceBuffer(4 * T * 672)
+                M.check("forward", c.forward(lay.L, v, T, v, o))
+                M.synchronize()
+                alone.append(o.download(np.uint8, (4 * T * 672,)))
+            outs = [M.DeviceBuffer(4 * T * 672) for _ in range(2)]
+            for _ in range(8):
+                for c, v, o, st in zip((ctx, other), x, outs, streams):
+                    M.check("forward", c.forward(lay.L, v, T, v, o, None, st.addr))
+            for st in streams:
+                st.synchronize()
+            for a, o in zip(alone, outs):
+                assert np.array_equal(a, o.download(np.uint8, (4 * T * 672,)))
+    finally:
+        for st in streams:
+            st.destroy()
+        other.close()
