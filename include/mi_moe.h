@@ -64,7 +64,8 @@ typedef enum {                     /* activation between the two expert products
     MI_ACT_RELU_SQR      = 4,      /* relu(u)^2 of ONE product, non-gated experts: ggml_sqr(ggml_relu(
                                       mul_mat_id(up_exps, x))), nemotronomni_model.cpp:366-367; the
                                       layer's gate tensor holds ffn_up_exps ne=[D, I, E],
-                                      fused_gate_up must be 0 and up is ignored                     */
+                                      fused_gate_up must be 0 and up is ignored.  u = NaN: 0, as
+                                      ggml's relu; MXFP4 tables: NaN, as the gated acts             */
 } mi_act;
 
 typedef enum {

@@ -191,10 +191,7 @@ __device__ __attribute__((noinline)) float mx_act(double a, double b) {
     // (1 + tanh(u)) / 2 = 1 / (1 + exp(-2 u))
     else if constexpr (ACT == 2) return (float)(a / (1.0 + exp(-2.0 * SQRT_2_OVER_PI * a * (1.0 + 0.044715 * a * a))) * b);
     else if constexpr (ACT == 3) return (float)(0.5 * a * (1.0 + erf(a * SQRT_2_INV)) * b);
-    else {
-        const double r = a > 0.0 ? a : a != a ? a : 0.0;
-        return (float)(r * r);
-    }
+    else return (float)mx_relu_sqr(a);
 }
 
 // A 16-row weight tile times rows of activations, by one wave: the lane's

@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
             const int64_t n = n0 + 32 * ct;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                v[(8 * (i >> 2) + 4 * h + (i & 3)) * 32 + l32] = GLU ? act_pair(g.act, acc[2 * ct][i], acc[2 * ct + 1][i]) : relu_sqr(acc[ct][i]);
+                v[(8 * (i >> 2) + 4 * h + (i & 3)) * 32 + l32] = GLU ? act_pair(g.act, acc[2 * ct][i], acc[2 * ct + 1][i]) : mx_relu_sqr(acc[ct][i]);
             wave_lds_sync();
 #pragma unroll
             for (int q = 0; q < 2; ++q) {

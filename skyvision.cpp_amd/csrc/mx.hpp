@@ -172,6 +172,14 @@ __device__ __forceinline__ void mx_store_pad(const MxRows &o, int64_t r, int nb,
         if (s == 0) o.s[r * mx_srow(nb) + b] = MX_ONE * 0x01010101u;
 }
 
+// relu^2 between the two products, on either path: a NaN stays one (as in the
+// gated forms), so an operand row that is no number shows in the layer's output
+template <typename F>
+__device__ __forceinline__ F mx_relu_sqr(F a) {
+    const F r = a <= F(0) ? F(0) : a;
+    return r * r;
+}
+
 // lane s's 8 values of the block at x
 template <bool VEC>
 __device__ __forceinline__ void mx_load8(const float *x, int s, float (&v)[8]) {
