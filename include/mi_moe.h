@@ -443,6 +443,13 @@ int mi_moe_ctx_set_gemm_threshold(mi_moe_ctx *ctx, int64_t min_tokens_for_gemm);
  * output's products in another order (fp32; the rows agree to ~2e-4 rel-L2
  * after the activations' fp16 and Q8_K roundings). */
 int mi_moe_ctx_set_gemm_tiles(mi_moe_ctx *ctx, int kind);
+/* Bytes of operand rows (6 per value of a row, in whole pairs of 32) that a
+ * pass of the MXFP4 GEMM addresses, at most 0xF0000000; 0: that many, the
+ * default.  A call of more tokens than fit runs in passes with the same bits
+ * (a pass that falls below the GEMM threshold takes the products of few rows);
+ * one whose single token does not fit takes the products of few rows.  Smaller
+ * values let small calls take that route. */
+int mi_moe_ctx_set_mx_pass_bytes(mi_moe_ctx *ctx, int64_t bytes);
 /* Schedule of decode calls of mi_moe_forward (1 token, and batches of 2..16
  * tokens; for experts of more than 2 MiB, batches that dispatch at most one
  * row per expert on average, T * K <= E).  The fused mode runs the whole block in one kernel of one work-group per

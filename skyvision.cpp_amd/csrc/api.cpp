@@ -115,6 +115,7 @@ struct mi_moe_ctx {
     // k-quant GEMM row tiles: 0 by shape, 1 G4_BM, 2 G4_BM_SMALL, 3 GS_BM (k_gs), 4 G4_BM_TINY, 5 G4_BM_MID;
     // 32-value types and F16: 1 GB_BM_LARGE, 2 GB_BM_SMALL, else by shape (5: GF_BM for mul_mat_id of F16)
     int gemm_tiles = 0;
+    int64_t mx_pass_bytes = MXG_MAX_X;   // operand digits of a pass of the MXFP4 GEMM
     int n_cu = 0;                 // compute units of the device
     // single-token fused kernel (k_decode.hip)
     int fused_decode = MI_DECODE_FUSED;
@@ -773,10 +774,10 @@ MxRows mx_rows(void *base, int64_t rows, int64_t K) {
     return m;
 }
 // tokens per pass of its grouped GEMM, which reads the rows through 32-bit
-// offsets; row_bytes: a token's operand bytes
-int64_t mx_max_tokens(int64_t row_bytes) { return MXG_MAX_X / row_bytes; }
-int64_t mx_layer_tokens(const mi_moe_layer *L) {
-    return mx_max_tokens(std::max(mx_drow(L->n_embd / 32), L->n_expert_used * mx_drow(L->n_ff / 32)));
+// offsets (0: not even one); row_bytes: a token's operand bytes
+int64_t mx_max_tokens(const mi_moe_ctx *c, int64_t row_bytes) { return c->mx_pass_bytes / row_bytes; }
+int64_t mx_layer_tokens(const mi_moe_ctx *c, const mi_moe_layer *L) {
+    return mx_max_tokens(c, std::max(mx_drow(L->n_embd / 32), L->n_expert_used * mx_drow(L->n_ff / 32)));
 }
 
 // MXFP4: the grouped GEMM for a product of more dispatched rows than half the
@@ -809,7 +810,7 @@ bool mx_shared_ok(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
     // (its activation rows go to f1, which holds cap_kmax and 2 cap_I floats per slot)
     if (mx_row(L->sh_n_ff / 32) > 4 * (int64_t)L->n_expert_used * std::max(L->n_embd, 2 * L->n_ff)) return false;
     return is_mx(L->gate.type) && is_mx(L->sh_gate.type) && is_mx(L->sh_down.type) && L->sh_act == L->act &&
-           !(mx_layer_gemm(c, L, T) && mx_layer_tokens(L) > 0) && T <= GV_SHARED_T;
+           !(mx_layer_gemm(c, L, T) && mx_layer_tokens(c, L) > 0) && T <= GV_SHARED_T;
 }
 
 // A few tokens through an MXFP4 layer in three launches: norm, router logits
@@ -885,9 +886,9 @@ int run_experts_mx(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t
     const int max_active = (int)std::min<int64_t>(E, rows);
     const bool same_ids = ids_gu == ids_dn;
     const bool gated = act_gated(L->act);
-    const bool gemm = mx_layer_gemm(c, L, T) && mx_layer_tokens(L) > 0;
+    const bool gemm = mx_layer_gemm(c, L, T) && mx_layer_tokens(c, L) > 0;
     const int bm = mx_bm(c, rows, E);
-    const int64_t tmax = mx_layer_tokens(L);
+    const int64_t tmax = mx_layer_tokens(c, L);
     if (gemm && T > tmax) {
         // in passes; then the dispatch of the whole call, whose counts, offsets and lists the caller may read
         for (int64_t t0 = 0; t0 < T; t0 += tmax) {
@@ -1416,6 +1417,13 @@ int mi_moe_ctx_set_gemm_tiles(mi_moe_ctx *c, int kind) {
     return MI_MOE_OK;
 }
 
+int mi_moe_ctx_set_mx_pass_bytes(mi_moe_ctx *c, int64_t bytes) {
+    if (!c) return MI_MOE_ERR_NULL;
+    if (bytes < 0 || bytes > MXG_MAX_X) return MI_MOE_ERR_ARG;
+    c->mx_pass_bytes = bytes ? bytes : MXG_MAX_X;
+    return MI_MOE_OK;
+}
+
 int mi_moe_ctx_set_fused_decode(mi_moe_ctx *c, int on) {
     if (!c) return MI_MOE_ERR_NULL;
     if (on < MI_DECODE_CHAIN || on > MI_DECODE_FUSED) return MI_MOE_ERR_ARG;
@@ -1580,8 +1588,8 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
             qx.b_ld = D;
             xq = true;
         }
-        const bool mx_gemm = is_mx(L->gate.type) && mx_layer_gemm(c, L, T) && mx_layer_tokens(L) > 0;
-        if (is_mx(L->gate.type) && front_takes_b32(L->router_w, xrow, D, D, x, D) && !(mx_gemm && T > mx_layer_tokens(L))) {
+        const bool mx_gemm = is_mx(L->gate.type) && mx_layer_gemm(c, L, T) && mx_layer_tokens(c, L) > 0;
+        if (is_mx(L->gate.type) && front_takes_b32(L->router_w, xrow, D, D, x, D) && !(mx_gemm && T > mx_layer_tokens(c, L))) {
             qx = Q8Out{};
             qx.mx = mx_rows(c->ax.q8, T, D);
             qx.mx_few = !mx_gemm;
@@ -1819,7 +1827,7 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
     // the grouped GEMM of the 32-value types and F16, in passes past its 32-bit
     // offsets (a single token's rows past them: the GEMV)
     const bool mx = is_mx(as->type);
-    const int64_t ldx = round_up(Kin, 64), tmax = mx ? mx_max_tokens(ne11 * mx_drow(Kin / 32)) : gb_max_tokens(ne11 * ldx);
+    const int64_t ldx = round_up(Kin, 64), tmax = mx ? mx_max_tokens(c, ne11 * mx_drow(Kin / 32)) : gb_max_tokens(ne11 * ldx);
     const bool mxg = mx && use_gemm_mx(c, T, (int)n_used, (int)E, as->nb[1], false) && tmax > 0;
     const bool gb = is_b32f(as->type) && use_gemm_wide(c, T, (int)n_used, (int)E) && gb_strides_ok(*as) && tmax > 0;
     if ((gb || mxg) && T > tmax) {

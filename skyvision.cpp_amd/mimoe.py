@@ -110,6 +110,7 @@ SYMBOLS = {
                                 C.POINTER(C.c_int)], C.c_int),
     "mi_moe_ctx_set_gemm_threshold": ([P, i64], C.c_int),
     "mi_moe_ctx_set_gemm_tiles": ([P, C.c_int], C.c_int),
+    "mi_moe_ctx_set_mx_pass_bytes": ([P, i64], C.c_int),
     "mi_moe_ctx_set_fused_decode": ([P, C.c_int], C.c_int),
     "mi_moe_ctx_set_decode_rescue": ([P, C.c_int], C.c_int),
     "mi_row_size": ([i32, i64], C.c_size_t),
@@ -284,6 +285,10 @@ class Context:
         skinny 16-row products (all-Q4_K layers), 4 8-row where they apply,
         5 64-row; 32-value types and F16: 1 128-row, 2 32-row, else by shape"""
         call("mi_moe_ctx_set_gemm_tiles", self.h, int(kind))
+
+    def set_mx_pass_bytes(self, nbytes: int) -> None:
+        """bytes of operand rows in a pass of the MXFP4 GEMM (0: as many as it addresses)"""
+        call("mi_moe_ctx_set_mx_pass_bytes", self.h, int(nbytes))
 
     def set_fused_decode(self, mode) -> None:
         """False / DECODE_CHAIN, True / DECODE_FUSED (DECODE_FUSED_COOPERATIVE is

@@ -2,8 +2,9 @@
 import numpy as np
 import pytest
 
+import _mxfp4 as X
 import mimoe as M
-from test_gpu_mxfp4 import LAYERS, Layer, rows
+from test_gpu_mxfp4 import LAYERS, Layer, check_layer, check_product, rows, run_product, sizes, table
 
 gpu = pytest.mark.gpu
 
@@ -59,3 +60,116 @@ def test_relu_sqr_keeps_nan(ctx, where, T, threshold):
     assert np.isfinite(want).all()
     assert np.array_equal(np.isnan(got), np.repeat(hit[:, None], lay.D, 1)), (np.isnan(got).any(1) != hit).nonzero()
     assert np.array_equal(got[~hit].view(np.uint32), want[~hit].view(np.uint32))
+
+
+# ------------------------------------------------------------------ operands past a pass
+def digit_bytes(n):
+    """of an operand row of n values: 96 a block, whole pairs of blocks"""
+    return (n // 32 + 1) // 2 * 192
+
+
+def layer_bytes(lay, tokens):
+    return tokens * max(digit_bytes(lay.D), lay.K * digit_bytes(lay.I))
+
+
+@pytest.fixture
+def passes(ctx):
+    ctx.set_gemm_threshold(1)
+    ctx.take_errors()
+    yield ctx
+    ctx.set_mx_pass_bytes(0)
+    ctx.set_gemm_threshold(0)
+    ctx.take_errors()
+
+
+def test_pass_bytes_refusals_without_device():
+    assert M.load().mi_moe_ctx_set_mx_pass_bytes(None, 0) == M.ERR_NULL
+
+
+@gpu
+def test_pass_bytes_refusals(passes):
+    lib = M.load()
+    assert [lib.mi_moe_ctx_set_mx_pass_bytes(passes.h, n) for n in (-1, 0xF0000001, 0xF0000000, 1, 0)] == [M.ERR_ARG, M.ERR_ARG, 0, 0, 0]
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [1, 16, 33])
+@pytest.mark.parametrize("name", ["moondream_like", "nemotron_like", "talker_like"])
+def test_layer_in_passes(passes, name, tokens):
+    """outputs and dispatch lists of the undivided call to the bit; the last pass is a short one"""
+    lay = Layer(seed=83, **LAYERS[name])
+    T = 70
+    rng = np.random.default_rng(84)
+    x, res = rows(rng, T, lay.D), rows(rng, T, lay.D)
+    got = []
+    for nbytes in (0, layer_bytes(lay, tokens) + 100):
+        passes.set_mx_pass_bytes(nbytes)
+        lists = {"counts": lay.E, "offsets": lay.E + 1, "perm": T * lay.K, "sel": T * lay.K}
+        bufs = {k: M.DeviceBuffer(4 * n) for k, n in lists.items()}
+        r = M.Routing()
+        for k, b in bufs.items():
+            setattr(r, k, b.addr)
+        got.append([forward(passes, lay, x, res, r).view(np.int32).ravel()] + [bufs[k].download(np.int32, (n,)) for k, n in lists.items()])
+    for a, b in zip(*got):
+        assert np.array_equal(a, b)
+    check_layer(got[1][0].view(np.float32).reshape(T, lay.D), lay.reference(x, res), sizes(lay, x), False)
+
+
+@gpu
+@pytest.mark.parametrize("two_ids", [False, True])
+def test_expert_ffn_in_passes(passes, two_ids):
+    """the caller's ids, one or two buffers of them, some outside: the same rows and the same count"""
+    lay = Layer(seed=85, **LAYERS["qwen_like"])
+    T, E, K = 61, lay.E, lay.K
+    rng = np.random.default_rng(86)
+    x, w = rows(rng, T, lay.D), rng.random((T, K)).astype(np.float32)
+    gu = rng.integers(-1, E + 1, (T, K)).astype(np.int32)
+    dn = rng.integers(-1, E + 1, (T, K)).astype(np.int32) if two_ids else gu
+    xd, wd, gd = M.to_device(x), M.to_device(w), M.to_device(gu)
+    dd = M.to_device(dn) if two_ids else gd
+    got = []
+    for nbytes in (0, layer_bytes(lay, 20)):
+        passes.set_mx_pass_bytes(nbytes)
+        out = M.DeviceBuffer(4 * T * lay.D)
+        M.check("expert_ffn", passes.expert_ffn(lay.L, xd, T, xd, gd, dd, wd, out))
+        M.synchronize()
+        got.append((out.download(np.float32, (T, lay.D)), passes.take_errors()[0]))
+    assert np.array_equal(got[0][0].view(np.uint32), got[1][0].view(np.uint32))
+    outside = sum(int(((i < 0) | (i >= E)).sum()) for i in ((gu, dn) if two_ids else (gu,)))
+    assert got[0][1] == got[1][1] == outside
+    ref = X.ffn(lay.host, x, gu, dn, w)
+    assert np.linalg.norm(got[1][0] - x - ref) <= 1e-3 * np.linalg.norm(ref)
+
+
+@gpu
+@pytest.mark.parametrize("own_rows", [False, True])
+def test_product_in_passes(passes, own_rows):
+    rng = np.random.default_rng(87)
+    raw = table(rng, 6, 40, 96)
+    b = rows(rng, 50, 3 if own_rows else 1, 96)
+    ids = rng.integers(-1, 7, (50, 3))
+    whole = run_product(passes, raw, b, ids)
+    assert passes.take_errors()[0] == int(((ids < 0) | (ids >= 6)).sum())
+    for tokens in (1, 7, 25):
+        passes.set_mx_pass_bytes(tokens * b.shape[1] * digit_bytes(96) + 50)
+        got = run_product(passes, raw, b, ids)
+        assert np.array_equal(got.view(np.uint32), whole.view(np.uint32)), tokens
+        assert passes.take_errors()[0] == int(((ids < 0) | (ids >= 6)).sum())
+    check_product(whole, raw, b, ids, False)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["qwen_like", "nemotron_like"])
+def test_a_token_past_a_pass(passes, name):
+    """takes the products of few rows, at any count of tokens"""
+    lay = Layer(seed=88, **LAYERS[name])
+    rng = np.random.default_rng(89)
+    passes.set_mx_pass_bytes(layer_bytes(lay, 1) - 1)
+    for T in (1, 5, 70):
+        x = rows(rng, T, lay.D)
+        got = forward(passes, lay, x, x)
+        check_layer(got, lay.reference(x, x), sizes(lay, x), not lay.shared or T <= 32)
+    raw, ids = table(rng, 6, 40, 96), rng.integers(0, 6, (50, 3))
+    b = rows(rng, 50, 3, 96)
+    passes.set_mx_pass_bytes(3 * digit_bytes(96) - 1)
+    check_product(run_product(passes, raw, b, ids), raw, b, ids, True)
