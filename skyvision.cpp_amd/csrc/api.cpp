@@ -765,8 +765,8 @@ int run_experts_b32(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_
 
 // The operand rows (mx.hpp) of an activation set lie over its code, scale,
 // block-sum and fp16 arrays: those are one run of 1 + 1/64 + 1/8 + 2 bytes per
-// value of rows filled up to 256 values (carve_workspace), the operand takes 3 +
-// 1/8 per value of rows filled up to 128.
+// value of rows filled up to 256 values, the operand takes 3 + 1/8 per value of
+// rows filled up to 128 (checked where the workspace is laid out: mx_rows_fit).
 MxRows mx_rows(void *base, int64_t rows, int64_t K) {
     MxRows m;
     m.d = (uint8_t *)base;
@@ -1237,8 +1237,20 @@ constexpr size_t ws_bytes(int64_t max_tokens, int64_t D, int64_t I, int64_t E, i
     return need;
 }
 
+// Whether an activation set's codes, scales, block sums and fp16 values of n
+// values (n % 256 == 0) are one run, up to end, that holds the MXFP4 operand
+// rows of as many (mx_rows).  A shorter row filled up to whole pairs of blocks,
+// or one of several rows' values (the shared expert's), takes no more.
+bool mx_rows_fit(const ActBuf &a, const void *end, int64_t n) {
+    const size_t run = carve_size<int8_t>(n) + carve_size<float>(n / QK) + carve_size<int16_t>(n / 16) + carve_size<_Float16>(n);
+    const char *q = (const char *)a.q8;
+    return q < (const char *)a.d8 && a.d8 < (const void *)a.bs && a.bs < (const void *)a.h && q + run == (const char *)end &&
+           (size_t)mx_row(n / 32) <= run;
+}
+
 // Lays the workspace of ws_bytes(...) bytes at base out into c's pointers and
-// records the capacities; false if the layout and ws_bytes disagree.
+// records the capacities; false if the layout and ws_bytes disagree, or the
+// MXFP4 operand rows do not fit it.
 bool carve_workspace(mi_moe_ctx *c, char *base, int64_t max_tokens, int32_t D, int32_t I, int32_t E, int32_t K) {
     const int64_t rows = max_tokens * K;
     const int64_t kmax = std::max<int64_t>(D, I);
@@ -1299,7 +1311,8 @@ bool carve_workspace(mi_moe_ctx *c, char *base, int64_t max_tokens, int32_t D, i
     c->cap_kmax = kmax_q;
     c->cap_tiles = tiles;
     c->cap_z = rows * wide;
-    return (size_t)(q - base) == ws_bytes(max_tokens, D, I, E, K);
+    return (size_t)(q - base) == ws_bytes(max_tokens, D, I, E, K) && mx_rows_fit(c->ax, c->ax.bsh, rows * kmax_q) &&
+           mx_rows_fit(c->aact, c->f1, rows * iq);
 }
 
 }  // namespace

@@ -173,3 +173,38 @@ def test_a_token_past_a_pass(passes, name):
     b = rows(rng, 50, 3, 96)
     passes.set_mx_pass_bytes(3 * digit_bytes(96) - 1)
     check_product(run_product(passes, raw, b, ids), raw, b, ids, True)
+
+
+# ------------------------------------------------------------------ the exact workspace
+EXACT = {
+    "one_block": dict(D=32, E=3, K=2, I=32, fused=True, act=0),
+    "odd_blocks": dict(D=96, E=5, K=3, I=288, fused=False, act=1),
+    "wide_shared": dict(D=160, E=4, K=4, I=96, fused=False, act=4, gating=1, shared=384),   # n_ff * n_expert_used
+    "whole": dict(D=256, E=4, K=1, I=256, fused=False, act=2, shared=256, sh_gate_inp=True),
+}
+
+
+@gpu
+@pytest.mark.parametrize("name", EXACT)
+@pytest.mark.parametrize("threshold", [1, 1 << 40])
+def test_exact_workspace(ctx, name, threshold):
+    """a context reserved for the call alone gives the bits of a roomy one"""
+    lay = Layer(seed=90, **EXACT[name])
+    rng = np.random.default_rng(91)
+    for T in (1, 37):
+        tight = M.Context(0)
+        tight.reserve(T, lay.D, lay.I, lay.E, lay.K)
+        x, res = rows(rng, T, lay.D), rows(rng, T, lay.D)
+        raw, ids = table(rng, lay.E, 48, lay.D), rng.integers(0, lay.E, (T, lay.K))
+        b = rows(rng, T, lay.K, lay.D)
+        got = []
+        try:
+            for c in (ctx, tight):
+                c.set_gemm_threshold(threshold)
+                got.append((forward(c, lay, x, res), run_product(c, raw, b, ids)))
+        finally:
+            ctx.set_gemm_threshold(0)
+            tight.close()
+        assert all(np.array_equal(p.view(np.uint32), q.view(np.uint32)) for p, q in zip(*got))
+        check_layer(got[0][0], lay.reference(x, res), sizes(lay, x), threshold > 1)
+        check_product(got[0][1], raw, b, ids, threshold > 1)
