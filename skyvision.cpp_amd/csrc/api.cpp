@@ -825,7 +825,7 @@ bool mx_shared_ok(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T) {
 constexpr int64_t MX_FEW_T = 32;
 bool mx_few(const mi_moe_ctx *c, const mi_moe_layer *L, int64_t T, const mi_moe_routing *routing) {
     if (!is_mx(L->gate.type) || !c->fused_decode || T > MX_FEW_T || T * L->n_expert_used > MXV_IDS) return false;
-    if (L->n_embd % 16 || mx_layer_gemm(c, L, T)) return false;
+    if (mx_layer_gemm(c, L, T)) return false;
     if (L->sh_n_ff > 0 && !mx_shared_ok(c, L, T)) return false;
     return !(routing && (routing->counts || routing->offsets || routing->perm));
 }

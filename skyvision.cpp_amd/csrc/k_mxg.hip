@@ -68,31 +68,22 @@ __device__ __forceinline__ f32x16 mxg_mfma(const i32x8 &a, const i32x8 &b, const
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 2, 4, DIG, sa, 0, sb);
 }
 
-// The lane's block 2 T + h of a stage out of its row's LDS pieces: with m = 0
-// .. 3 the row's misalignment, its first byte is byte o = m + 2 T + h past 32 T
-// + 16 h, so 24 bytes from there (T >= 2: 28) hold it.  (Wide reads: dword by
-// dword the reads of 32 rows 20 dwords apart take 8 cycles each, these 5.)
-typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+// The lane's block 2 T + h (T = 0, 1) of a stage out of its row's LDS pieces:
+// with m = 0 .. 3 the row's misalignment, its first byte is byte o = m + 2 T + h
+// past 32 T + 16 h, so 24 bytes from there hold it.  (Wide reads: dword by dword
+// the reads of 32 rows 20 dwords apart take 8 cycles each, these 5.)
 struct MxgRaw {
     u32x4 a;
-    u32x3 b;
+    uint2 b;
 };
 template <int T>
 __device__ __forceinline__ void mxg_read(const uint8_t *p, MxgRaw &r) {   // p: the row's pieces + 16 h
     r.a = *(const u32x4 *)(p + 32 * T);
-    if constexpr (T < 2) {
-        const uint2 b = *(const uint2 *)(p + 32 * T + 16);
-        r.b[0] = b.x;
-        r.b[1] = b.y;
-    } else {
-        r.b = *(const u32x3 *)(p + 32 * T + 16);
-    }
+    r.b = *(const uint2 *)(p + 32 * T + 16);
 }
 template <int T>
 __device__ __forceinline__ void mxg_unpack(const MxgRaw &r, uint32_t mh, i32x8 &c, int &scale) {   // mh: m + h
-    constexpr int S = T < 2 ? 0 : 1;
-    const uint32_t o = mh + 2 * T - 4 * S, v[7] = {r.a[0], r.a[1], r.a[2], r.a[3], r.b[0], r.b[1], r.b[2]};
-    const uint32_t *w = v + S;
+    const uint32_t o = mh + 2 * T, w[6] = {r.a[0], r.a[1], r.a[2], r.a[3], r.b.x, r.b.y};
     const bool up = o >= 3u;   // the codes, from byte o + 1 <= 7, start in dword 1
     uint32_t x[5];
 #pragma unroll
@@ -140,8 +131,8 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     const int nb = (int)(s.a.K / 32), ns = (nb + 1) / 2;
     const int wr = wave / WN, wc = wave - wr * WN;
     // Columns of y (of the activation rows) of a work-group and a wave.  The
-    // 256 weight rows in LDS: those of the columns in order (GLU: 128 gate
-    // rows, then the 128 matching up rows), loaded by groups of 64.
+    // WROWS weight rows in LDS: those of the columns in order (GLU: half of them
+    // gate rows, then the matching up rows), loaded by groups of 64.
     constexpr int CB = GLU ? WROWS / 2 : WROWS, CW = CB / WN;
     const int64_t c0 = (int64_t)cb * CB, n0 = c0 + CW * wc;
     __amdgpu_buffer_rsrc_t wrsrc[NWL];
@@ -288,8 +279,9 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
         if constexpr (I.value % KS == KS - 1) load_w(st / KS + 2, MXG_W(I.value), NWL * k / n, NWL * (k + 1) / n);
         __builtin_amdgcn_sched_barrier(0);
     };
+    static_assert(6 * KS == 12, "steps of a turn");
 #define MXG_STEP(I)                                                                       \
-    if constexpr ((I) < 6 * KS) {                                                         \
+    {                                                                                     \
         if (st0 + (I) >= ns) break;                                                       \
         const u32x4 w4 = sc[(I) / 2 % 3];                                                 \
         const int sa = (int)((I) % 2 == 0 ? (h ? w4[1] : w4[0]) : (h ? w4[3] : w4[2]));   \
