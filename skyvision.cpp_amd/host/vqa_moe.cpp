@@ -465,6 +465,20 @@ int main(int argc, char **argv) {
         CHECK(std::fabs(o2[0] - want[0]) < 1e-5f && std::fabs(o2[1] - want[1]) < 1e-5f, "table values");
         std::fprintf(stderr, "table out = [%.7f, %.7f]\n", o2[0], o2[1]);
     }
+    // ggml's strides of every tensor type: nb[0] the bytes of a block (one value of the plain types)
+    {
+        const struct { int type, n; size_t block, row; } kinds[] = {
+            {MI_TYPE_F32, 3, 4, 12}, {MI_TYPE_I32, 3, 4, 12}, {MI_TYPE_F16, 96, 2, 192}, {MI_TYPE_Q4_K, 512, 144, 288},
+            {MI_TYPE_Q6_K, 512, 210, 420}, {MI_TYPE_Q4_0, 96, 18, 54}, {MI_TYPE_Q5_0, 96, 22, 66}, {MI_TYPE_Q8_0, 96, 34, 102},
+            {MI_TYPE_MXFP4, 96, 17, 51}};
+        int bad = 0;
+        for (const auto &k : kinds) {
+            const Tensor *t = s.new_tensor(k.type, k.n, 5, 2);
+            if (!t || t->nb[0] != k.block || t->nb[1] != k.row || t->nb[2] != 5 * k.row || t->nb[3] != 10 * k.row) bad++;
+        }
+        CHECK(!bad, "tensor strides");
+        if (!bad) std::fprintf(stderr, "tensor strides of %d types\n", (int)(sizeof(kinds) / sizeof(kinds[0])));
+    }
     // residual split: res = [10, 20] -> out = res + (want - x)
     const float rv[2] = {10.0f, 20.0f};
     Tensor *res = mk(rv, 2, 1);

@@ -1,4 +1,7 @@
 """Calls of MXFP4 layers and products beside those of test_gpu_mxfp4.py.  Tolerances as there."""
+import pathlib
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -208,3 +211,34 @@ def test_exact_workspace(ctx, name, threshold):
         assert all(np.array_equal(p.view(np.uint32), q.view(np.uint32)) for p, q in zip(*got))
         check_layer(got[0][0], lay.reference(x, res), sizes(lay, x), threshold > 1)
         check_product(got[0][1], raw, b, ids, threshold > 1)
+
+
+# ------------------------------------------------------------------ the C++ host mirror
+SELFTEST = pathlib.Path(M.__file__).parent / "host" / "vqa_moe_selftest"
+
+
+@gpu
+def test_host_tensor_strides():
+    r = subprocess.run([str(SELFTEST)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "tensor strides of 9 types" in r.stderr, r.stderr
+
+
+@gpu
+@pytest.mark.parametrize("same", [True, False])
+@pytest.mark.parametrize("threshold", [1 << 30, 1])
+def test_host_table_form(tmp_path, same, threshold):
+    """vqa::moe::build_expert_ffn_table_res on MXFP4 tables"""
+    rng = np.random.default_rng(92)
+    D, I, E, K, T = 160, 96, 6, 3, 12
+    L = dict(E=E, I=I, act=0, fused=False, gate=table(rng, E, I, D), up=table(rng, E, I, D), down=table(rng, E, D, I))
+    x, res, w = rows(rng, T, D), rows(rng, T, D), rng.random((T, K)).astype(np.float32)
+    gu = rng.integers(0, E, (T, K)).astype(np.int32)
+    dn = gu if same else rng.integers(0, E, (T, K)).astype(np.int32)
+    (tmp_path / "meta.txt").write_text(f"{T} {D} {I} {E} {K} {M.TYPE_MXFP4} {M.TYPE_MXFP4} 0 {int(same)} {threshold}\n")
+    for name, a in (("x", x), ("res", res), ("gate", L["gate"]), ("up", L["up"]), ("down", L["down"]), ("ids_gu", gu), ("ids_dn", dn), ("w", w)):
+        (tmp_path / f"{name}.bin").write_bytes(np.ascontiguousarray(a).tobytes())
+    r = subprocess.run([str(SELFTEST), "--table", str(tmp_path)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    got = np.fromfile(tmp_path / "out.bin", np.float32).reshape(T, D)
+    y = np.abs(X.ffn_slots(L, x, gu, dn) * w[..., None]).sum(1)
+    check_layer(got, res + X.ffn(L, x, gu, dn, w), y, threshold > 1)
