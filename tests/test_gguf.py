@@ -212,3 +212,28 @@ def test_gguf_layer_forward(tmp_path, style, qtype):
     M.check("free", M.load().mi_dev_free(buf))
     g.close()
     ctx.close()
+
+
+def test_gguf_mxfp4_tensor_info(tmp_path):
+    p = tmp_path / "mx.gguf"
+    _, t = qwen_file(p, qtype=O.TYPE_MXFP4)
+    g = M.Gguf(p)
+    for name, ne, nbytes in (("ffn_up_exps", [D, I, E, 1], E * I * (D // 32) * 17), ("ffn_down_exps", [I, D, E, 1], E * D * (I // 32) * 17)):
+        assert g.tensor_info(f"blk.0.{name}.weight") == (M.TYPE_MXFP4, ne, nbytes)
+    assert len(t["up"]) == E * I * (D // 32) * 17
+    g.close()
+
+
+def test_gguf_mxfp4_past_the_file(tmp_path):
+    """a table whose 17-byte blocks run past the file's end is refused when the file is opened"""
+    p = tmp_path / "mx.gguf"
+    qwen_file(p, qtype=O.TYPE_MXFP4)
+    p.write_bytes(p.read_bytes()[:-33])   # (the last table is whole multiples of the alignment: its last bytes)
+    h = M.P()
+    assert M.load().mi_gguf_open(M.C.byref(h), str(p).encode()) == M.ERR_FORMAT
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("style", ["moondream", "qwen3omni"])
+def test_gguf_mxfp4_layer_forward(tmp_path, style):
+    test_gguf_layer_forward(tmp_path, style, O.TYPE_MXFP4)
