@@ -7,6 +7,7 @@ import pytest
 
 import _mxfp4 as X
 import mimoe as M
+import pyoracle as O
 from test_gpu_mxfp4 import LAYERS, Layer, check_layer, check_product, rows, run_product, sizes, table
 
 gpu = pytest.mark.gpu
@@ -242,3 +243,64 @@ def test_host_table_form(tmp_path, same, threshold):
     got = np.fromfile(tmp_path / "out.bin", np.float32).reshape(T, D)
     y = np.abs(X.ffn_slots(L, x, gu, dn) * w[..., None]).sum(1)
     check_layer(got, res + X.ffn(L, x, gu, dn, w), y, threshold > 1)
+
+
+# ------------------------------------------------------------------ shared experts of another type or activation
+MIXED = {   # routed type, its act, the shared expert's type and act
+    "mx_q8_0": (O.TYPE_MXFP4, 0, O.TYPE_Q8_0, 0),
+    "mx_q4_k": (O.TYPE_MXFP4, 1, O.TYPE_Q4_K, 1),
+    "mx_f32": (O.TYPE_MXFP4, 4, O.TYPE_F32, 4),
+    "mx_other_act": (O.TYPE_MXFP4, 0, O.TYPE_MXFP4, 4),
+    "mx_ungated": (O.TYPE_MXFP4, 4, O.TYPE_MXFP4, 0),
+    "q8_0_mx": (O.TYPE_Q8_0, 0, O.TYPE_MXFP4, 0),
+    "q4_k_mx": (O.TYPE_Q4_K, 2, O.TYPE_MXFP4, 3),
+    "f32_mx": (O.TYPE_F32, 0, O.TYPE_MXFP4, 4),
+}
+
+
+@gpu
+@pytest.mark.parametrize("gated_row", [False, True])
+@pytest.mark.parametrize("name", MIXED)
+def test_mixed_shared_expert(ctx, name, gated_row):
+    """MXFP4 experts beside a shared expert of another type or activation, and an MXFP4 shared expert beside other tables:
+    against the oracle, the norm inside against the norm apart, with lists asked for against without"""
+    rt, act, st, sh_act = MIXED[name]
+    D, E, K, I, S = 512, 10, 3, 256, 256
+    rng = np.random.default_rng(93)
+    w = lambda t, *shape: (lambda a: a if t == O.TYPE_F32 else O.quantize(t, a))((rng.standard_normal(shape) * 0.05).astype(np.float32))
+    host = dict(D=D, E=E, K=K, I=I, act=act, fused=False, gate_type=rt, down_type=rt, router_w=(rng.standard_normal((E, D)) * 0.05).astype(np.float32),
+                router_b=None, gate=w(rt, E, I, D), up=None if act == 4 else w(rt, E, I, D), down=w(rt, E, D, I),
+                sh_I=S, sh_act=sh_act, sh_type=st, sh_down_type=st, sh_gate=w(st, S, D), sh_up=None if sh_act == 4 else w(st, S, D),
+                sh_down=w(st, D, S), sh_gate_inp=(rng.standard_normal(D) * 0.05).astype(np.float32) if gated_row else None)
+    dev = {k: M.to_device(v) for k, v in host.items() if isinstance(v, np.ndarray)}
+    L = M.make_layer(D, E, K, I, dev["router_w"], None, M.tensor(dev["gate"], rt, [D, I, E]), None if act == 4 else M.tensor(dev["up"], rt, [D, I, E]),
+                     M.tensor(dev["down"], rt, [I, D, E]), False, act)
+    L.sh_n_ff, L.sh_act = S, sh_act
+    L.sh_gate, L.sh_down = M.tensor(dev["sh_gate"], st, [D, S]), M.tensor(dev["sh_down"], st, [S, D])
+    if sh_act != 4:
+        L.sh_up = M.tensor(dev["sh_up"], st, [D, S])
+    if gated_row:
+        L.sh_gate_inp = dev["sh_gate_inp"].addr
+    norm = M.make_norm(M.NORM_RMS, 1e-6)
+    for T in (1, 3, 8, 70):
+        x, res = rows(rng, T, D), rows(rng, T, D)
+        xd, rd = M.to_device(x), M.to_device(res)
+        outs = [M.DeviceBuffer(4 * T * D) for _ in range(4)]
+        M.check("forward", ctx.forward(L, xd, T, rd, outs[0]))
+        counts = M.DeviceBuffer(4 * E)
+        r = M.Routing()
+        r.counts = counts.addr
+        M.check("forward", ctx.forward(L, xd, T, rd, outs[1], r))
+        xn = M.DeviceBuffer(4 * T * D)
+        M.check("norm", ctx.norm(norm, xd, T, D, xn))
+        M.check("forward", ctx.forward(L, xn, T, rd, outs[2]))
+        M.check("forward_norm", ctx.forward_norm(L, norm, xd, T, rd, outs[3]))
+        M.synchronize()
+        got = [o.download(np.float32, (T, D)) for o in outs]
+        ref, dbg = O.moe_forward(host, x, res)
+        e = float(np.linalg.norm(got[0] - ref) / np.linalg.norm(ref - res))
+        print(f"{name} gated row {gated_row} T={T}: rel-L2 {e:.2e}", flush=True)
+        assert e <= 1e-2
+        assert np.array_equal(counts.download(np.int32, (E,)), dbg["counts"])
+        assert np.array_equal(got[0].view(np.uint32), got[1].view(np.uint32))
+        assert np.array_equal(got[2].view(np.uint32), got[3].view(np.uint32))
