@@ -304,3 +304,56 @@ def test_mixed_shared_expert(ctx, name, gated_row):
         assert np.array_equal(counts.download(np.int32, (E,)), dbg["counts"])
         assert np.array_equal(got[0].view(np.uint32), got[1].view(np.uint32))
         assert np.array_equal(got[2].view(np.uint32), got[3].view(np.uint32))
+
+
+# ------------------------------------------------------------------ addresses, graphs
+@gpu
+@pytest.mark.parametrize("T", [1, 3, 20, 80])
+def test_layer_rows_off_16_bytes_same_bits(ctx, T):
+    """the loads of rows off 16 bytes give the bits of aligned ones (another first launch up to 4 tokens)"""
+    lay = Layer(seed=94, **LAYERS["qwen_like"])
+    rng = np.random.default_rng(95)
+    x, res = rows(rng, T, 512), rows(rng, T, 512)
+    got = []
+    for off in (0, 4):
+        xd, rd = M.DeviceBuffer(x.nbytes + 16).upload(x, off), M.DeviceBuffer(x.nbytes + 16).upload(res, off)
+        out = M.DeviceBuffer(x.nbytes + 16)
+        M.check("forward", ctx.forward(lay.L, xd.addr + off, T, rd.addr + off, out.addr + off))
+        M.synchronize()
+        got.append(out.download(np.uint32, (T, 512), off))
+    assert np.array_equal(*got)
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 6, 70])
+def test_expert_ffn_graph(ctx, T):
+    """captured and replayed with other rows and ids in the same buffers, eager calls between the replays"""
+    lay = Layer(seed=96, **LAYERS["moondream_like"])
+    rng = np.random.default_rng(97)
+    D, E, K = lay.D, lay.E, lay.K
+    xd, idd, wd, out, eager = M.DeviceBuffer(4 * T * D), M.DeviceBuffer(4 * T * K), M.DeviceBuffer(4 * T * K), M.DeviceBuffer(4 * T * D), M.DeviceBuffer(4 * T * D)
+
+    def fill():
+        x, ids, w = rows(rng, T, D), rng.integers(0, E, (T, K)).astype(np.int32), rng.random((T, K)).astype(np.float32)
+        for b, v in ((xd, x), (idd, ids), (wd, w)):
+            b.upload(v)
+        M.synchronize()
+        return x, ids, w
+
+    st = M.Stream()
+    fill()
+    g = M.Graph(st, lambda s: M.check("expert_ffn", ctx.expert_ffn(lay.L, xd, T, xd, idd, idd, wd, out, s.addr)))
+    try:
+        for _ in range(4):
+            x, ids, w = fill()
+            M.check("expert_ffn", ctx.expert_ffn(lay.L, xd, T, xd, idd, idd, wd, eager))
+            M.synchronize()
+            g.launch(st)
+            st.synchronize()
+            a, b = out.download(np.float32, (T, D)), eager.download(np.float32, (T, D))
+            assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+            ref = X.ffn(lay.host, x, ids, ids, w)
+            assert np.linalg.norm(a - x - ref) <= 1e-3 * np.linalg.norm(ref)
+    finally:
+        g.destroy()
+        st.destroy()
