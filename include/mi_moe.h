@@ -141,7 +141,9 @@ typedef struct {
  * NULL).  Layouts are row-major with tokens outermost.  Asking for counts,
  * offsets or perm makes small calls (at most 1024 ids on the 32-row GEMM
  * tiles) launch the dispatch kernel that writes them, which the products
- * otherwise do without; the results are bit-identical either way. */
+ * otherwise do without; the results are bit-identical either way (MXFP4 layers
+ * of up to 32 tokens then add in fp64 in another order: the same float32 unless
+ * a sum lies within those roundings, 2^-53, of a border between two). */
 typedef struct {
     float   *logits;               /* [T][E]   router logits                      */
     int32_t *sel;                  /* [T][K]   expert ids, descending logit (in
@@ -298,9 +300,11 @@ int mi_top_k(mi_moe_ctx *ctx, const mi_tensor *a, int32_t k, mi_tensor *dst, mi_
  * ggml vec_dot_type, like ggml-cpu: Q8_K for k-quants, Q8_0 for the 32-value
  * formats and MXFP4, fp16 for F16 (F32 tables take b as given).  MXFP4: the
  * products of the codes are exact and summed in fp64 (few rows per expert) or
- * fp32; a dst value is NaN where its table row holds a NaN block or its b row
- * a NaN, an infinity or a block whose Q8_0 scale leaves the fp16 range (|x|
- * above 8.3e6).
+ * fp32, within fp32's normal range: where the terms' sizes add up past 2^127
+ * dst may be infinite or NaN, and a block's part of the sum (32 terms) below
+ * 2^-126 may count as zero.  A dst value is NaN where its table row holds a NaN
+ * block or its b row a NaN, an infinity or a block whose Q8_0 scale leaves the
+ * fp16 range (|x| above 8.3e6).
  * Ids must lie in [0, E): the dst row of an id outside is written as zeros
  * and the id is counted for mi_moe_ctx_take_errors. */
 int mi_mul_mat_id(mi_moe_ctx *ctx, const mi_tensor *as, const mi_tensor *b, const mi_tensor *ids,
@@ -322,8 +326,9 @@ int mi_mul_mat_id(mi_moe_ctx *ctx, const mi_tensor *as, const mi_tensor *b, cons
 int mi_quantize(mi_moe_ctx *ctx, int32_t type, const float *src, void *dst, int64_t nrows,
                 int64_t n_per_row, mi_stream_t stream);
 
-/* The values that rows of a table stand for (ggml's to_float of the type):
- * src: nrows rows of row_size bytes device, dst: F32 [nrows][n_per_row] device,
+/* The values that rows of a table stand for (ggml's to_float of the type; an
+ * MXFP4 block of scale byte 255 is NaN, which ggml's form does not know, and a
+ * value past fp32's range an infinity): src: nrows rows of row_size bytes device, dst: F32 [nrows][n_per_row] device,
  * not overlapping src.  Types MXFP4, Q4_0, Q5_0, Q8_0 and F16 (n_per_row a
  * multiple of 32); others MI_MOE_ERR_TYPE. */
 int mi_dequantize(mi_moe_ctx *ctx, int32_t type, const void *src, float *dst, int64_t nrows,

@@ -203,10 +203,12 @@ __device__ __attribute__((noinline)) float mx_act(double a, double b) {
 // c = 8 j + 2 b + i holds digit i of row j's block b of the step and zeros in
 // the other three blocks, so each of the 16 x 16 results is one digit's sum
 // over one block, an integer of at most 13 bits times a power of two: exact in
-// fp32 whatever the scales.  Times the block's significand they are added in
-// fp64, so the result is the exact sum rounded at 2^-53, and what follows (the
-// GLU's values, in fp64 and rounded once, and their codes) does not depend on
-// an order of sums.  What bounds it beside the weights' bytes is the vector
+// fp32 as long as that lies in its normal range (both scales are in it: a sum
+// past 2^128 is infinite, one below 2^-126 may be zero).  Times the block's
+// significand they are added in fp64, so the result is the exact sum but for
+// roundings at 2^-53, and what follows (the GLU's values, in fp64 and rounded
+// once, and their codes) does not depend on an order of sums unless a value
+// lies that near to a border.  What bounds it beside the weights' bytes is the vector
 // work of a step (unpacking 17-byte blocks, four conversions and fp64
 // multiply-adds): two rows share it all; with the significand in the digits
 // (four, a column of each) a row had it alone, and 120 rows of 64 experts

@@ -357,3 +357,30 @@ def test_expert_ffn_graph(ctx, T):
     finally:
         g.destroy()
         st.destroy()
+
+
+# ------------------------------------------------------------------ sums at the end of float32's range
+@gpu
+@pytest.mark.parametrize("threshold", [1, 1 << 40])
+def test_product_past_the_range(ctx, threshold):
+    """sums of positive terms: within the products' tolerance where they stay below 2^126, no numbers above 2^129 (digits
+    of both signs past 2^128: infinite or NaN), one row not disturbing the next"""
+    rng = np.random.default_rng(99)
+    raw = np.abs(X.values(table(rng, 2, 48, 96)))
+    raw = O.quantize(O.TYPE_MXFP4, raw.astype(np.float32))
+    raw[:, 0::3, 0::17] = 247    # 2^120
+    raw[:, 1::3, 0::17] = 254    # 2^127
+    b = np.abs(rows(rng, 40, 2, 96)) * np.float32(0.01)
+    b[0::2] *= np.float32(1e4)
+    ids = rng.integers(0, 2, (40, 2))
+    ctx.set_gemm_threshold(threshold)
+    try:
+        got = run_product(ctx, raw, b, ids)
+    finally:
+        ctx.set_gemm_threshold(0)
+    ref = X.product(raw, b, ids)
+    small, large = ref <= 2.0 ** 126, ref >= 2.0 ** 129
+    assert small.any() and large.any() and (small & (ref > 2.0 ** 118)).any()
+    tol = 2.0 ** -24 * ref + (2.0 ** -50 if threshold > 1 else 2 * 96 / 16 * 2.0 ** -23) * ref
+    assert (np.abs(got - ref) <= tol)[small].all()
+    assert not np.isfinite(got[large]).any()
