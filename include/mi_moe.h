@@ -422,7 +422,9 @@ int mi_moe_ctx_stage_clock(mi_moe_ctx *ctx, const char *stage, double *ghz, int 
  * per expert); for Q4_0 / Q5_0 layers and mi_mul_mat_id when 4 * T * K > 5 * E
  * (more than 1.25 rows per expert), for Q8_0 / F16 layers when 2 * T * K >
  * 3 * E (more than 1.5), for MXFP4 layers when T * K > 2 * E and for
- * mi_mul_mat_id of such tables when 2 * T * K > E. */
+ * mi_mul_mat_id of such tables when 2 * T * K > E.  (MXFP4 layers meet there
+ * when the tokens spread over the experts; a batch whose tokens all choose the
+ * same few is faster on the GEMM from about 12 tokens on.) */
 int mi_moe_ctx_set_gemm_threshold(mi_moe_ctx *ctx, int64_t min_tokens_for_gemm);
 /* Row tiles of the grouped GEMMs.  Of Q4_K gate/up layers: 0 (the default) by
  * shape, 32-row tiles when the call dispatches at most 8 rows per expert on
@@ -469,7 +471,7 @@ int mi_moe_ctx_set_mx_pass_bytes(mi_moe_ctx *ctx, int64_t bytes);
  * MXFP4 layers of up to 32 tokens, on the products of few rows and without
  * dispatch outputs, take three launches in the fused mode (router with the
  * norm; ranking, gate/up and activations; down, weighted sum, shared expert
- * and residual), above 4 tokens with norm, router, top-k and operand rows in
+ * and residual), above 4 tokens with the norm, the router and the top-k in
  * launches of their own.
  *   MI_DECODE_CHAIN              separate kernels
  *   MI_DECODE_FUSED              fused, plain launch (default)

@@ -783,8 +783,13 @@ int64_t mx_layer_tokens(const mi_moe_ctx *c, const mi_moe_layer *L) {
 // MXFP4: the grouped GEMM for a product of more dispatched rows than half the
 // experts (K 2048, 2048 rows of 64 experts: 40 rows 33 against 32 us, 64 rows
 // 41 against 38, 512 rows 137 against 49; 16 rows 23 against 31), for a layer
-// above two per expert: its few-row form takes few launches and its sums are
-// exact (64 experts: 80 rows 80 against 84 us, 128 rows 100 against 93).
+// above two per expert, where the two meet when the router spreads its tokens
+// (few rows / GEMM: 64 experts of 1024, 1.5 rows each 79 / 88 us, 2 93 / 93, 3
+// 116 / 93; 128 of 768, 1.5 111 / 123, 2 131 / 136, 3 173 / 144; 128 of 1856,
+// relu^2, 1.5 206 / 214, 2 227 / 228, 3 292 / 242).  Tokens that all choose the
+// same 6 or 8 experts would change over earlier, at about 12 rows on each (16
+// tokens 68 / 54, 32 tokens 99 / 54, 43 tokens of 1856 192 / 72), which the
+// host cannot see from the call.
 // (Rows further apart than it addresses keep the other kernel.)
 bool use_gemm_mx(const mi_moe_ctx *c, int64_t T, int K, int E, size_t row_bytes, bool layer) {
     if ((int64_t)row_bytes > MXG_MAX_ROW_BYTES) return false;   // (then a token's operand row is far below MXG_MAX_X)

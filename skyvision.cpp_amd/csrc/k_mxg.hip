@@ -31,8 +31,9 @@
 // out in front of its LDS reads, in the small tile between its MFMAs (64 rows of
 // 64 experts 50 -> 47 us; the large tile 240 -> 246).
 //
-// What bounds the large tile (16384 rows of 64 experts, K 2048, N 2048: 225 us,
-// 610 TFLOP/s of the contract's products, four times that on the MFMA): a wave's
+// What bounds the large tile (16384 rows of 64 experts, K 2048, N 2048: 223 us
+// of a call of 239, 241 - 248 under a profiler; 610 TFLOP/s of the contract's
+// products, four times that on the MFMA): a wave's
 // step is 57 vector instructions (most of them unpack weights), 12 LDS reads and
 // 16 MFMAs, and two waves to a SIMD overlap them in part: without the loop's
 // loads it takes 175 us, without the MFMAs 185, the stores are 22 of it.  Of the

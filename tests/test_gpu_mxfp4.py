@@ -467,7 +467,7 @@ def test_quantize_then_layer_run_together(ctx):
 
 
 # ------------------------------------------------------------------ a few tokens' launches
-# (the launches take norm and router up to 4 tokens and rows of 64-value chunks up to 4096, the rest up to 16 tokens)
+# (the launches take norm and router up to 4 tokens and rows of 64-value chunks up to 4096, the rest up to 32 tokens)
 FEW = {
     "eleven_chunks": dict(D=704, E=5, K=2, I=32, fused=True, act=0),
     "no_chunks": dict(D=96, E=7, K=3, I=96, fused=False, act=1),
