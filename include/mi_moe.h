@@ -49,6 +49,8 @@ typedef enum {                     /* ggml_type ids */
     MI_TYPE_Q8_0 = 8,              /*  34 B / 32 values: d f16 | qs[32] i8;       x = d q        */
     MI_TYPE_Q4_K = 12,             /* 144 B / 256 values, convert/q4k.py:9-10  */
     MI_TYPE_Q6_K = 14,             /* 210 B / 256 values, convert/q6k.py:10-11 */
+    MI_TYPE_Q8_K = 15,             /* rows in 8 bits (ggml's vec_dot_type of the k-quants), 292 B / 256 values:
+                                       d f32 | qs[256] i8 | bsums[16] i16 (sums of 16 codes); x = d q */
     MI_TYPE_I32  = 26,
     MI_TYPE_MXFP4 = 39,            /*  17 B / 32 values: e E8M0 | qs[16] E2M1 codes (value j: low nibble of
                                        qs[j], 16 + j: high); x = 2^(e - 127) +-{0, .5, 1, 1.5, 2, 3, 4, 6};
@@ -174,6 +176,42 @@ typedef struct {
     const float *bias;
 } mi_moe_norm;
 
+/* A router over logits (mi_moe_route, mi_moe_forward_router): scores, a bias
+ * for the choice, groups of experts of which the best are kept, top-k, weights.
+ *   s[e] = sigmoid(l[e]), or the softmax over all E (ggml_soft_max)
+ *   c[e] = s[e] + sel_bias[e]
+ *   n_group > 1: expert e is of group e / (E / n_group); a group's value is the
+ *     sum of its group_top largest c; the n_group_used groups of the largest
+ *     values are kept
+ *   ids: the K largest c of the kept groups' experts, largest first
+ *   w[k] = s[ids[k]] [/ (sum_K s + eps)] * scaling [* expert_scale[ids[k]]]
+ * Equal values: the lower id (group) first.  Every exp and sigmoid is evaluated
+ * in fp64 and rounded to float32 once, and what is ranked are float32 numbers
+ * (as the layer's gatings rank; without groups MI_SCORE_SIGMOID chooses as
+ * MI_GATING_SIGMOID_BIAS, MI_SCORE_SOFTMAX as MI_GATING_SOFTMAX_ALL).  A c that
+ * is NaN comes behind every number (a group's value is of its numbers; a group
+ * of fewer than group_top of them comes behind the others); slots that no number
+ * fills take the lowest ids not taken and the weight NaN.  -inf as a logit or
+ * bias is a number (a mask); a softmax of nothing but -inf is NaN. */
+typedef enum {
+    MI_SCORE_SOFTMAX = 0,
+    MI_SCORE_SIGMOID = 1,
+} mi_score;
+
+typedef struct {
+    int32_t n_expert;              /* E, at most 1024 */
+    int32_t n_expert_used;         /* K, at most 64 and the experts of the kept groups */
+    int32_t score;                 /* mi_score */
+    int32_t n_group;               /* divides E, at most 64; 0 or 1: no groups */
+    int32_t n_group_used;          /* 1 .. n_group (not read without groups) */
+    int32_t group_top;             /* 1 or 2, at most E / n_group (not read without groups) */
+    int32_t renorm;                /* 1: weights divided by their sum + eps */
+    float   eps;
+    float   scaling;               /* 0 is read as 1 */
+    const float *sel_bias;         /* F32 [E] or NULL */
+    const float *expert_scale;     /* F32 [E] or NULL */
+} mi_moe_router;
+
 typedef struct mi_moe_ctx mi_moe_ctx;
 
 /* ---- context -------------------------------------------------------------
@@ -264,11 +302,40 @@ int mi_moe_forward_norm(mi_moe_ctx *ctx, const mi_moe_layer *layer, const mi_moe
                         int64_t n_tokens, const float *res, float *out, const mi_moe_routing *routing,
                         mi_stream_t stream);
 
+/* The block with its experts chosen by `router` in place of the layer's gating
+ * (whose fields gating, sel_bias, expert_scale, routed_scaling and gate_eps are
+ * then not read): mi_moe_forward_norm and mi_moe_forward_router_input otherwise
+ * (norm and x_router may be NULL).  router's n_expert and n_expert_used are the
+ * layer's.  Runs the kernel chain at every token count; ids and weights are
+ * those of mi_moe_route on the logits. */
+int mi_moe_forward_router(mi_moe_ctx *ctx, const mi_moe_layer *layer, const mi_moe_router *router,
+                          const mi_moe_norm *norm, const float *x, const float *x_router, int64_t n_tokens,
+                          const float *res, float *out, const mi_moe_routing *routing, mi_stream_t stream);
+
+/* ids and weights of rows of logits (mi_moe_router): logits F32 ne=[E, T], any
+ * row stride; sel I32 [T][K], weights F32 [T][K] device, not overlapping the
+ * logits or each other.  The routing that mi_moe_expert_ffn takes; no workspace. */
+int mi_moe_route(mi_moe_ctx *ctx, const mi_moe_router *router, const mi_tensor *logits, int32_t *sel, float *weights,
+                 mi_stream_t stream);
+
 /* y = norm(x) over each row of n_cols <= 4096 (F32 [n_rows][n_cols] device;
  * y may equal x): the norms of mi_moe_forward_norm as an op (ggml_norm /
  * ggml_rms_norm followed by ggml_mul / ggml_add with the weight and bias). */
 int mi_norm(mi_moe_ctx *ctx, const mi_moe_norm *norm, const float *x, int64_t n_rows, int32_t n_cols,
             float *y, mi_stream_t stream);
+
+/* The norm with the residual's addition in front and rows in 8 bits behind:
+ * h = x + add, y = norm(h), per row of D = x.ne[0] <= 16384 values, ggml_add
+ * followed by mi_norm's norm (sums in fp64, every other step rounded to
+ * float32).  x, add, sum, y: F32 ne=[D, T] of any row stride; add NULL: h = x;
+ * sum (NULL: not wanted) receives h, y (NULL: not wanted) the norm; either may
+ * be x or add (data and strides alike), otherwise the outputs overlap nothing.
+ * q (NULL: not wanted): y in Q8_0 (D % 32 == 0) or Q8_K (D % 256 == 0), byte for byte ggml's quantize_row of the float32 y, at any
+ * row stride of whole 2 (Q8_0) or 4 (Q8_K) bytes, a block with a NaN or an
+ * infinity being one of scale NaN and codes 0 - what mi_mul_mat takes.  y or q is
+ * required.  No workspace. */
+int mi_add_norm(mi_moe_ctx *ctx, const mi_moe_norm *norm, const mi_tensor *x, const mi_tensor *add, mi_tensor *sum,
+                mi_tensor *y, mi_tensor *q, mi_stream_t stream);
 
 /* ---- routed FFN with caller-supplied routing ------------------------------
  * Replaces vqa::moe::build_expert_ffn_table_res (src/core/engine/moe_compute.hpp:66-71,
@@ -310,6 +377,20 @@ int mi_top_k(mi_moe_ctx *ctx, const mi_tensor *a, int32_t k, mi_tensor *dst, mi_
 int mi_mul_mat_id(mi_moe_ctx *ctx, const mi_tensor *as, const mi_tensor *b, const mi_tensor *ids,
                   mi_tensor *dst, mi_stream_t stream);
 
+/* ggml_mul_mat(ctx, a ne=[K, N], b ne=[K, T]) -> F32 ne=[N, T]: dst[n, t] =
+ * a[:, n] . b[:, t] for a matrix in 4 bits with group scales, Q4_0 or Q4_K (the
+ * dense products around the experts: attention's matrices, dense blocks, the
+ * head).  b: F32 rows, which go to a's vec_dot_type first (Q8_0, Q8_K) like
+ * ggml-cpu's, or rows that are in that type already (mi_add_norm, mi_quantize to
+ * Q8_0): the same bits of dst.  Each block's products are summed exactly in
+ * integers, the blocks in fp32.  Any row strides (b F32 and dst whole floats, Q8_0
+ * 2 bytes, Q8_K 4); dst overlaps neither.  A row of b with a NaN, an infinity or a
+ * block whose Q8_0 scale leaves the fp16 range (|x| above 8.3e6) makes its dst
+ * row NaN, a row of a with a scale that is not finite makes its column NaN or
+ * infinite.  F32 rows use the context's workspace (mi_moe_ctx_reserve: T within
+ * max_tokens * n_expert_used, K within the wider of n_embd and n_ff). */
+int mi_mul_mat(mi_moe_ctx *ctx, const mi_tensor *a, const mi_tensor *b, mi_tensor *dst, mi_stream_t stream);
+
 /* ---- weight preparation ----------------------------------------------------
  * quantize_row_q4_K_ref / quantize_row_q6_K_ref (ggml; ported in
  * convert/q4k.py:27-127 and convert/q6k.py:103-193; called through
@@ -330,7 +411,7 @@ int mi_quantize(mi_moe_ctx *ctx, int32_t type, const float *src, void *dst, int6
  * MXFP4 block of scale byte 255 is NaN, which ggml's form does not know, and a
  * value past fp32's range an infinity): src: nrows rows of row_size bytes device, dst: F32 [nrows][n_per_row] device,
  * not overlapping src.  Types MXFP4, Q4_0, Q5_0, Q8_0 and F16 (n_per_row a
- * multiple of 32); others MI_MOE_ERR_TYPE. */
+ * multiple of 32) and Q8_K (of 256; rows 4-byte aligned); others MI_MOE_ERR_TYPE. */
 int mi_dequantize(mi_moe_ctx *ctx, int32_t type, const void *src, float *dst, int64_t nrows,
                   int64_t n_per_row, mi_stream_t stream);
 

@@ -178,12 +178,33 @@ size_t type_row_size(int32_t type, int64_t n) {
     case MI_TYPE_F16: return (size_t)n * 2;
     case MI_TYPE_Q4_K: return n % QK ? 0 : (size_t)(n / QK) * Q4K_BYTES;
     case MI_TYPE_Q6_K: return n % QK ? 0 : (size_t)(n / QK) * Q6K_BYTES;
+    case MI_TYPE_Q8_K: return n % QK ? 0 : (size_t)(n / QK) * Q8K_BYTES;
     case MI_TYPE_Q4_0: return n % 32 ? 0 : (size_t)(n / 32) * 18;
     case MI_TYPE_Q5_0: return n % 32 ? 0 : (size_t)(n / 32) * 22;
     case MI_TYPE_Q8_0: return n % 32 ? 0 : (size_t)(n / 32) * 34;
     case MI_TYPE_MXFP4: return n % 32 ? 0 : (size_t)(n / 32) * MX_BYTES;
     default: return 0;
     }
+}
+
+// rows ne=[n, T] (F32, Q8_0 or Q8_K) of any stride that the kernels address
+int check_rows(const mi_tensor &t, int64_t n, int64_t T) {
+    if (t.ne[0] != n || t.ne[1] != T || t.ne[2] != 1 || t.ne[3] != 1) return MI_MOE_ERR_SHAPE;
+    const size_t rs = type_row_size(t.type, n), unit = t.type == MI_TYPE_Q8_0 ? 2 : 4;
+    if (rs == 0 || (t.type == MI_TYPE_F32 && t.nb[0] != 4) || (T > 1 && t.nb[1] < rs)) return MI_MOE_ERR_SHAPE;
+    if ((uintptr_t)t.data % unit || t.nb[1] % unit) return MI_MOE_ERR_UNSUPPORTED;
+    return MI_MOE_OK;
+}
+struct Span {
+    const void *p;
+    size_t n;
+};
+Span rows_span(const mi_tensor &t) {
+    return {t.data, t.ne[1] > 0 ? t.nb[1] * (size_t)(t.ne[1] - 1) + type_row_size(t.type, t.ne[0]) : 0};
+}
+bool overlap(const Span &a, const Span &b) {
+    const uintptr_t p = (uintptr_t)a.p, q = (uintptr_t)b.p;
+    return p < q + b.n && q < p + a.n;
 }
 
 // an expert table ne=[K, N, E] with ggml strides
@@ -1539,8 +1560,11 @@ Gating layer_gating(const mi_moe_layer *L) {
 // statistics before its chunk loop, config-4 prefill 9.96 vs 9.57 ms.)
 // xr: the rows the router reads when they differ from the experts' input
 // (null: x; the norm, if any, applies to x only).
+// rt: the router in place of the layer's gating (null: the gating), on the
+// logits of a launch of their own: none of the fused kernels ranks for it.
 int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T, const float *res, float *out,
-                 const mi_moe_routing *routing, const NormParams &np, hipStream_t st, const float *xr = nullptr) {
+                 const mi_moe_routing *routing, const NormParams &np, hipStream_t st, const float *xr = nullptr,
+                 const RouterParams *rt = nullptr) {
     if (!c) return MI_MOE_ERR_NULL;
     if (T < 0) return MI_MOE_ERR_SHAPE;
     TRY(validate_layer(c, L, true, true));
@@ -1554,7 +1578,7 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
     if (xr == x) xr = nullptr;
     int P = 0, C = 0;
     // the fused decode kernels route on the rows they quantize for the experts
-    const bool dec1 = T == 1 && !xr && plan_decode1(c, L, x, P, C);
+    const bool dec1 = T == 1 && !xr && !rt && plan_decode1(c, L, x, P, C);
     // The single-token kernel normalizes x itself only when out does not
     // overlap x: a work-group that computes a late router row or Q8_K block
     // re-reads x, possibly after other work-groups wrote their out columns.
@@ -1562,7 +1586,7 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
     const bool fuse_norm = dec1 && np.kind != NORM_NONE && (ob + row <= xb || xb + row <= ob);
     // a few tokens of an MXFP4 layer: the norm in the router's launch, unless
     // another launch reads the normalized rows too (the shared expert's gate row)
-    const bool few = mx_few(c, L, T, routing);
+    const bool few = !rt && mx_few(c, L, T, routing);
     MxFrontArgs ff;
     const bool few_front = few && mx_few_front(L, x, xr, T, np, ff) && !(np.kind != NORM_NONE && L->sh_n_ff > 0 && L->sh_gate_inp);
     if (np.kind != NORM_NONE && !fuse_norm && !few_front) {
@@ -1590,7 +1614,7 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
         TRY(run_mx_few(c, L, x, T, true, true, layer_gating(L), res, out, L->sh_gate_inp ? c->sh_w : nullptr, st));
     } else if (dec1) {
         TRY(run_decode1(c, L, x, res, out, P, C, fuse_norm ? np : NormParams{}, st));
-    } else if (!xr && plan_decodeb(c, L, x, T, cc)) {
+    } else if (!xr && !rt && plan_decodeb(c, L, x, T, cc)) {
         TRY(run_decodeb(c, L, x, T, res, out, cc, st));
     } else {
         // router + Q8_K(x) in one launch where the shape fits (the router's
@@ -1616,7 +1640,7 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
             xq = true;
         }
         const Gating gt = layer_gating(L);
-        const int cps = front_split_cps(c, T, D, E);
+        const int cps = rt ? 0 : front_split_cps(c, T, D, E);
         bool x_done = false;   // the Q8_K of x came with the router
         if (cps > 0) {
             double *parts = (double *)c->z;   // free until the down product
@@ -1628,7 +1652,8 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
             TRY(launch_front(L->router_w, L->router_b, xrow, D, T, D, E, c->logits, xq ? &qx : nullptr, st));
             x_done = xq;
             stage_end(c, "router", st);
-            TRY(launch_topk_softmax(c->logits, E, T, E, K, c->sel, K, c->w, st, gt));
+            if (rt) TRY(launch_route(c->logits, E, T, E, K, *rt, c->sel, c->w, st));
+            else TRY(launch_topk_softmax(c->logits, E, T, E, K, c->sel, K, c->w, st, gt));
         }
         stage_end(c, "topk_softmax", st);
         if (few) TRY(run_mx_few(c, L, x, T, false, x_done, gt, res, out, L->sh_gate_inp ? c->sh_w : nullptr, st));
@@ -1652,6 +1677,38 @@ int forward_impl(mi_moe_ctx *c, const mi_moe_layer *L, const float *x, int64_t T
         if (routing->perm)
             HIP_TRY(hipMemcpyAsync(routing->perm, d.perm, sizeof(int32_t) * T * K, hipMemcpyDeviceToDevice, st));
     }
+    return MI_MOE_OK;
+}
+
+// checks of a router; E and K of the call
+int router_params(const mi_moe_router *r, RouterParams &p) {
+    if (!r) return MI_MOE_ERR_NULL;
+    const int64_t E = r->n_expert, K = r->n_expert_used;
+    if (E <= 0 || K <= 0 || K > E) return MI_MOE_ERR_SHAPE;
+    if (r->score != MI_SCORE_SOFTMAX && r->score != MI_SCORE_SIGMOID) return MI_MOE_ERR_ARG;
+    if (E > ROUTER_MAX_E || K > ROUTER_MAX_K) return MI_MOE_ERR_UNSUPPORTED;
+    p = RouterParams{};
+    if (r->n_group < 0) return MI_MOE_ERR_SHAPE;
+    if (r->n_group > 1) {
+        if (E % r->n_group || r->n_group_used <= 0 || r->n_group_used > r->n_group) return MI_MOE_ERR_SHAPE;
+        const int64_t gs = E / r->n_group;
+        if (K > r->n_group_used * gs) return MI_MOE_ERR_SHAPE;
+        if (r->group_top < 1 || r->group_top > 2) return MI_MOE_ERR_ARG;
+        if (r->group_top > gs) return MI_MOE_ERR_SHAPE;
+        if (r->n_group > ROUTER_MAX_GROUPS) return MI_MOE_ERR_UNSUPPORTED;
+        // every group kept: the choice is over all
+        if (r->n_group_used < r->n_group) {
+            p.n_group = r->n_group;
+            p.n_kept = r->n_group_used;
+            p.group_top = r->group_top;
+        }
+    }
+    p.score = r->score;
+    p.renorm = r->renorm != 0;
+    p.eps = r->eps;
+    p.scaling = r->scaling != 0.f ? r->scaling : 1.f;
+    p.sel_bias = r->sel_bias;
+    p.expert_scale = r->expert_scale;
     return MI_MOE_OK;
 }
 
@@ -1754,6 +1811,82 @@ int mi_moe_forward_norm(mi_moe_ctx *c, const mi_moe_layer *L, const mi_moe_norm 
     NormParams np;
     TRY(norm_params(norm, np));
     return forward_impl(c, L, h, T, res, out, routing, np, (hipStream_t)stream);
+}
+
+int mi_moe_forward_router(mi_moe_ctx *c, const mi_moe_layer *L, const mi_moe_router *router, const mi_moe_norm *norm,
+                          const float *x, const float *x_router, int64_t T, const float *res, float *out,
+                          const mi_moe_routing *routing, mi_stream_t stream) {
+    if (!c || !L) return MI_MOE_ERR_NULL;
+    RouterParams rt;
+    TRY(router_params(router, rt));
+    if (router->n_expert != L->n_expert || router->n_expert_used != L->n_expert_used) return MI_MOE_ERR_SHAPE;
+    NormParams np;
+    TRY(norm_params(norm, np));
+    mi_moe_layer l = *L;   // the gating's fields are not read
+    l.gating = MI_GATING_SOFTMAX_TOPK;
+    l.sel_bias = l.expert_scale = nullptr;
+    return forward_impl(c, &l, x, T, res, out, routing, np, (hipStream_t)stream, x_router, &rt);
+}
+
+int mi_moe_route(mi_moe_ctx *c, const mi_moe_router *router, const mi_tensor *logits, int32_t *sel, float *weights,
+                 mi_stream_t stream) {
+    if (!c || !logits || !logits->data || !sel || !weights) return MI_MOE_ERR_NULL;
+    RouterParams p;
+    TRY(router_params(router, p));
+    if (logits->type != MI_TYPE_F32) return MI_MOE_ERR_TYPE;
+    const int64_t E = router->n_expert, K = router->n_expert_used, T = logits->ne[1];
+    if (T < 0) return MI_MOE_ERR_SHAPE;
+    TRY(check_rows(*logits, E, T));
+    if (T == 0) return MI_MOE_OK;
+    const Span in = rows_span(*logits), s = {sel, (size_t)(T * K) * 4}, w = {weights, (size_t)(T * K) * 4};
+    if (overlap(in, s) || overlap(in, w) || overlap(s, w)) return MI_MOE_ERR_ARG;
+    HIP_TRY(hipSetDevice(c->device));
+    return launch_route((const float *)logits->data, (int64_t)(logits->nb[1] / 4), T, (int)E, (int)K, p, sel, weights,
+                        (hipStream_t)stream);
+}
+
+int mi_add_norm(mi_moe_ctx *c, const mi_moe_norm *norm, const mi_tensor *x, const mi_tensor *add, mi_tensor *sum,
+                mi_tensor *y, mi_tensor *q, mi_stream_t stream) {
+    if (!c || !norm || !x || (!y && !q)) return MI_MOE_ERR_NULL;
+    NormParams np;
+    TRY(norm_params(norm, np));
+    if (np.kind == NORM_NONE) return MI_MOE_ERR_ARG;
+    const int64_t D = x->ne[0], T = x->ne[1];
+    if (D <= 0 || T < 0) return MI_MOE_ERR_SHAPE;
+    const mi_tensor *f[4] = {x, add, sum, y};
+    for (const mi_tensor *t : f) {
+        if (!t) continue;
+        if (!t->data) return MI_MOE_ERR_NULL;
+        if (t->type != MI_TYPE_F32) return MI_MOE_ERR_TYPE;
+        TRY(check_rows(*t, D, T));
+    }
+    if (q) {
+        if (!q->data) return MI_MOE_ERR_NULL;
+        if (q->type != MI_TYPE_Q8_0 && q->type != MI_TYPE_Q8_K) return MI_MOE_ERR_TYPE;
+        TRY(check_rows(*q, D, T));
+    }
+    if (D > ADD_NORM_MAX_D || T > 0x7fffffff) return MI_MOE_ERR_UNSUPPORTED;
+    if (T == 0) return MI_MOE_OK;
+    // an output is apart from everything, or sum / y is x or add itself
+    const mi_tensor *outs[3] = {sum, y, q}, *ins[2] = {x, add};
+    for (int i = 0; i < 3; ++i) {
+        if (!outs[i]) continue;
+        for (int j = i + 1; j < 3; ++j)
+            if (outs[j] && overlap(rows_span(*outs[i]), rows_span(*outs[j]))) return MI_MOE_ERR_ARG;
+        for (const mi_tensor *in : ins) {
+            if (!in || !overlap(rows_span(*outs[i]), rows_span(*in))) continue;
+            if (i == 2 || outs[i]->data != in->data || (T > 1 && outs[i]->nb[1] != in->nb[1])) return MI_MOE_ERR_ARG;
+        }
+    }
+    HIP_TRY(hipSetDevice(c->device));
+    AddNormArgs a = {};
+    a.norm = np;
+    a.x = (const float *)x->data; a.ldx = (int64_t)(x->nb[1] / 4);
+    if (add) { a.add = (const float *)add->data; a.lda = (int64_t)(add->nb[1] / 4); }
+    if (sum) { a.sum = (float *)sum->data; a.lds = (int64_t)(sum->nb[1] / 4); }
+    if (y) { a.y = (float *)y->data; a.ldy = (int64_t)(y->nb[1] / 4); }
+    if (q) { a.q = (uint8_t *)q->data; a.ldq = (int64_t)q->nb[1]; a.qtype = q->type; }
+    return launch_add_norm(a, T, (int)D, (hipStream_t)stream);
 }
 
 int mi_norm(mi_moe_ctx *c, const mi_moe_norm *norm, const float *x, int64_t n_rows, int32_t n_cols, float *y,
@@ -1958,6 +2091,35 @@ int mi_mul_mat_id(mi_moe_ctx *c, const mi_tensor *as, const mi_tensor *b, const 
     return launch_gemm4(a, st);
 }
 
+int mi_mul_mat(mi_moe_ctx *c, const mi_tensor *a, const mi_tensor *b, mi_tensor *dst, mi_stream_t stream) {
+    if (!c || !a || !b || !dst || !a->data || !b->data || !dst->data) return MI_MOE_ERR_NULL;
+    if (a->type != MI_TYPE_Q4_0 && a->type != MI_TYPE_Q4_K) return MI_MOE_ERR_TYPE;
+    const int32_t t8 = a->type == MI_TYPE_Q4_0 ? MI_TYPE_Q8_0 : MI_TYPE_Q8_K;
+    if ((b->type != MI_TYPE_F32 && b->type != t8) || dst->type != MI_TYPE_F32) return MI_MOE_ERR_TYPE;
+    const int64_t K = a->ne[0], N = a->ne[1], T = b->ne[1];
+    if (K <= 0 || N <= 0 || T < 0 || a->ne[2] != 1 || a->ne[3] != 1) return MI_MOE_ERR_SHAPE;
+    const size_t rs = type_row_size(a->type, K);
+    if (rs == 0 || a->nb[1] < rs) return MI_MOE_ERR_SHAPE;
+    if (a->type == MI_TYPE_Q4_K && ((uintptr_t)a->data % 16 || a->nb[1] % 16)) return MI_MOE_ERR_UNSUPPORTED;
+    if (a->type == MI_TYPE_Q4_0 && ((uintptr_t)a->data % 2 || a->nb[1] % 2)) return MI_MOE_ERR_UNSUPPORTED;
+    TRY(check_rows(*b, K, T));
+    TRY(check_rows(*dst, N, T));
+    if (N > 0x7fffffff || K > 0x7fffffff) return MI_MOE_ERR_UNSUPPORTED;
+    if (b->type == MI_TYPE_F32) {
+        if (!c->reserved || T > c->cap_rows || K > c->cap_kmax) return MI_MOE_ERR_CAPACITY;
+    }
+    if (T == 0) return MI_MOE_OK;
+    const Span sa = {a->data, a->nb[1] * (size_t)(N - 1) + rs}, out = rows_span(*dst);
+    if (overlap(out, sa) || overlap(out, rows_span(*b))) return MI_MOE_ERR_ARG;
+    HIP_TRY(hipSetDevice(c->device));
+    MmArgs g = {};
+    g.a = (const uint8_t *)a->data; g.type = a->type; g.row_bytes = (int64_t)a->nb[1]; g.K = K; g.N = N;
+    g.b = b->data; g.btype = b->type; g.ldb = (int64_t)b->nb[1]; g.T = T;
+    g.y = (float *)dst->data; g.ldy = (int64_t)(dst->nb[1] / 4);
+    g.ws = c->ax.q8;
+    return launch_mm(g, (hipStream_t)stream);
+}
+
 int mi_quantize(mi_moe_ctx *c, int32_t type, const float *src, void *dst, int64_t nrows, int64_t n_per_row,
                 mi_stream_t stream) {
     if (!c || !src || !dst) return MI_MOE_ERR_NULL;
@@ -1984,6 +2146,12 @@ int mi_quantize(mi_moe_ctx *c, int32_t type, const float *src, void *dst, int64_
 int mi_dequantize(mi_moe_ctx *c, int32_t type, const void *src, float *dst, int64_t nrows, int64_t n_per_row,
                   mi_stream_t stream) {
     if (!c || !src || !dst) return MI_MOE_ERR_NULL;
+    if (type == MI_TYPE_Q8_K) {
+        if (nrows < 0 || n_per_row <= 0 || n_per_row % QK) return MI_MOE_ERR_SHAPE;
+        if ((uintptr_t)dst % 4 || (uintptr_t)src % 4) return MI_MOE_ERR_UNSUPPORTED;
+        HIP_TRY(hipSetDevice(c->device));
+        return launch_dequantize_q8k(src, dst, nrows * (n_per_row / QK), (hipStream_t)stream);
+    }
     if (!is_b32f(type) && !is_mx(type)) return MI_MOE_ERR_TYPE;
     if (nrows < 0 || n_per_row <= 0 || n_per_row % 32) return MI_MOE_ERR_SHAPE;
     if ((uintptr_t)dst % 4) return MI_MOE_ERR_UNSUPPORTED;

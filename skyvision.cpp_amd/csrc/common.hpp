@@ -20,6 +20,7 @@ namespace mimoe {
 constexpr int QK = 256;
 constexpr int Q4K_BYTES = 144;
 constexpr int Q6K_BYTES = 210;
+constexpr int Q8K_BYTES = 292;
 constexpr int WAVE = 64;
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));

@@ -36,6 +36,22 @@ int launch_rmsnorm(const float *x, int64_t T, int D, float eps, float *y, hipStr
 // y = norm(x) per row of D <= 4096 (norm.hpp; x may equal y)
 int launch_norm(const NormParams &p, const float *x, int64_t T, int D, float *y, hipStream_t st);
 
+// h = x + add, y = norm(h), q = y in 8 bits, per row of D <= ADD_NORM_MAX_D
+// values (k_addnorm.hip); row strides in floats, of q in bytes; add, sum, y, q
+// may be null (not y and q both)
+struct AddNormArgs {
+    const float *x, *add;
+    float *sum, *y;
+    uint8_t *q;
+    int qtype;           // 8 Q8_0, 15 Q8_K
+    int64_t ldx, lda, lds, ldy, ldq;
+    NormParams norm;
+};
+constexpr int ADD_NORM_MAX_D = 16384;
+int launch_add_norm(const AddNormArgs &a, int64_t T, int D, hipStream_t st);
+// values of Q8_K rows (rows of nblocks / nrows blocks one after another)
+int launch_dequantize_q8k(const void *src, float *dst, int64_t nblocks, hipStream_t st);
+
 // the activation operands of one consumer weight type of the 32-value types and F16 (k_b32.hip)
 enum { B32_PREP_NONE = -1, B32_PREP_CODES = 0, B32_PREP_DQ = 1, B32_PREP_F16 = 2 };
 struct B32Prep {
@@ -95,6 +111,19 @@ int launch_front_parts(const float *W, const float *x, int64_t ldx, int64_t T, i
                        double *parts, const Q8Out *qx, hipStream_t st);
 int launch_topk_parts(const double *parts, int D, const float *bias, float *logits, int64_t T, int E, int K,
                       int32_t *sel, int64_t ld_sel, float *w, hipStream_t st, const Gating &gt);
+
+// a router's parameters (mi_moe_router; k_router.hip)
+struct RouterParams {
+    int score = 0;       // 0 softmax over all, 1 sigmoid
+    int n_group = 1, n_kept = 1, group_top = 1;
+    int renorm = 0;
+    float eps = 0.f, scaling = 1.f;
+    const float *sel_bias = nullptr, *expert_scale = nullptr;   // [E] or null
+};
+constexpr int ROUTER_MAX_E = 1024, ROUTER_MAX_K = 64, ROUTER_MAX_GROUPS = 64;
+// ids and weights [T][K] of rows of logits (row t at logits + t * ldl)
+int launch_route(const float *logits, int64_t ldl, int64_t T, int E, int K, const RouterParams &p, int32_t *sel,
+                 float *w, hipStream_t st);
 
 struct Dispatch {
     int32_t *counts;     // [E]
@@ -504,5 +533,23 @@ int launch_decodeb(const DecArgs &g, int grid, hipStream_t st);
 int launch_decode1(const DecArgs &g, int grid, hipStream_t st);
 // work-groups of the decode grid (one per CU), 0 if one per CU cannot be resident
 int decode1_max_grid(int device, int *grid);
+
+// ---- dense products of 4-bit matrices (k_mm.hip)
+// y[t][n] = a[n] . b[t]: a Q4_0 (2) or Q4_K (12) rows, b rows as fp32 (0) or in
+// a's 8-bit form (Q8_0 = 8 / Q8_K = 15).  ws: mm_ws_bytes of workspace, 16-byte aligned.
+struct MmArgs {
+    const uint8_t *a;
+    int type;
+    int64_t row_bytes, K, N;
+    const void *b;
+    int btype;
+    int64_t ldb;          // bytes
+    int64_t T;
+    float *y;
+    int64_t ldy;          // floats
+    void *ws;
+};
+size_t mm_ws_bytes(int type, int btype, int64_t T, int64_t K);
+int launch_mm(const MmArgs &g, hipStream_t st);
 
 }  // namespace mimoe

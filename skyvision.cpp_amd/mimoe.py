@@ -19,16 +19,18 @@ DECODE_FUSED_EXCLUSIVE = DECODE_FUSED   # former name
 
 TYPE_F32, TYPE_F16, TYPE_Q4_K, TYPE_Q6_K, TYPE_I32 = 0, 1, 12, 14, 26
 TYPE_Q4_0, TYPE_Q5_0, TYPE_Q8_0, TYPE_MXFP4 = 2, 6, 8, 39
+TYPE_Q8_K = 15
 ACT_SILU, ACT_GELU_ERF_GP1, ACT_GELU_TANH, ACT_GELU_ERF, ACT_RELU_SQR = 0, 1, 2, 3, 4
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 GATING_SOFTMAX_TOPK, GATING_SIGMOID_BIAS, GATING_SOFTMAX_ALL = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 ABI_VERSION = 3
 # mi_moe_status
 OK, ERR_NULL, ERR_SHAPE, ERR_TYPE, ERR_CAPACITY, ERR_HIP = 0, -1, -2, -3, -4, -5
 ERR_UNSUPPORTED, ERR_DEVICE, ERR_ARG, ERR_FORMAT = -6, -7, -8, -9
 QK_K = 256
 BLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q6_K: 210, TYPE_Q4_0: 18, TYPE_Q5_0: 22, TYPE_Q8_0: 34,
-               TYPE_MXFP4: 17}
+               TYPE_MXFP4: 17, TYPE_Q8_K: 292}
 STATUS = {0: "ok", -1: "null", -2: "shape", -3: "type", -4: "capacity", -5: "hip",
           -6: "unsupported", -7: "device", -8: "arg"}
 
@@ -77,6 +79,23 @@ def make_norm(kind: int, eps: float, weight=None, bias=None) -> Norm:
     return n
 
 
+class Router(C.Structure):
+    _fields_ = [("n_expert", i32), ("n_expert_used", i32), ("score", i32), ("n_group", i32), ("n_group_used", i32),
+                ("group_top", i32), ("renorm", i32), ("eps", C.c_float), ("scaling", C.c_float),
+                ("sel_bias", P), ("expert_scale", P)]
+
+
+def make_router(E: int, K: int, score: int, n_group: int = 1, n_group_used: int = 1, group_top: int = 1,
+                renorm: bool = True, eps: float = 0.0, scaling: float = 1.0, sel_bias=None, expert_scale=None) -> Router:
+    """sel_bias / expert_scale: DeviceBuffer (kept alive by the returned Router)
+    or a device address."""
+    r = Router(E, K, score, n_group, n_group_used, group_top, int(renorm), eps, scaling)
+    r.sel_bias = sel_bias.addr if isinstance(sel_bias, DeviceBuffer) else sel_bias
+    r.expert_scale = expert_scale.addr if isinstance(expert_scale, DeviceBuffer) else expert_scale
+    r._buffers = (sel_bias, expert_scale)
+    return r
+
+
 class Routing(C.Structure):
     _fields_ = [("logits", P), ("sel", P), ("weights", P), ("counts", P), ("offsets", P),
                 ("perm", P)]
@@ -92,6 +111,11 @@ SYMBOLS = {
     "mi_moe_forward_noalloc": ([C.POINTER(Layer), P, i64, P, P, C.POINTER(Routing), P], C.c_int),
     "mi_moe_forward_router_input": ([P, C.POINTER(Layer), P, P, i64, P, P, C.POINTER(Routing), P], C.c_int),
     "mi_moe_expert_ffn": ([P, C.POINTER(Layer), P, i64, P, P, P, P, P, P], C.c_int),
+    "mi_moe_forward_router": ([P, C.POINTER(Layer), C.POINTER(Router), C.POINTER(Norm), P, P, i64, P, P,
+                               C.POINTER(Routing), P], C.c_int),
+    "mi_moe_route": ([P, C.POINTER(Router), C.POINTER(Tensor), P, P, P], C.c_int),
+    "mi_add_norm": ([P, C.POINTER(Norm)] + [C.POINTER(Tensor)] * 5 + [P], C.c_int),
+    "mi_mul_mat": ([P, C.POINTER(Tensor), C.POINTER(Tensor), C.POINTER(Tensor), P], C.c_int),
     "mi_top_k": ([P, C.POINTER(Tensor), i32, C.POINTER(Tensor), P], C.c_int),
     "mi_mul_mat_id": ([P, C.POINTER(Tensor), C.POINTER(Tensor), C.POINTER(Tensor),
                        C.POINTER(Tensor), P], C.c_int),
@@ -251,7 +275,7 @@ def tensor(buf, type_: int, ne, nb=None, offset: int = 0) -> Tensor:
     """ggml-style descriptor; default strides are ggml's contiguous ones."""
     ne = list(ne) + [1] * (4 - len(ne))
     if nb is None:
-        if type_ in (TYPE_Q4_K, TYPE_Q6_K, TYPE_Q4_0, TYPE_Q5_0, TYPE_Q8_0, TYPE_MXFP4):
+        if type_ in BLOCK_BYTES:
             nb0 = BLOCK_BYTES[type_]
             nb1 = row_size(type_, ne[0])
         else:
@@ -346,6 +370,28 @@ class Context:
                                                   _addr(out), C.byref(routing) if routing is not None else None,
                                                   _addr(stream))
 
+    def forward_router(self, layer: Layer, router: Router, norm: Norm | None, x, x_router, T: int, res, out,
+                       routing: Routing | None = None, stream=None) -> int:
+        """mi_moe_forward_router: the experts chosen by router in place of the layer's gating"""
+        return load().mi_moe_forward_router(self.h, C.byref(layer), C.byref(router),
+                                            C.byref(norm) if norm is not None else None, _addr(x), _addr(x_router), T,
+                                            _addr(res), _addr(out), C.byref(routing) if routing is not None else None,
+                                            _addr(stream))
+
+    def route(self, router: Router, logits: Tensor, sel, weights, stream=None) -> int:
+        """sel, weights [T][K] = router's choice on rows of logits"""
+        return load().mi_moe_route(self.h, C.byref(router), C.byref(logits), _addr(sel), _addr(weights), _addr(stream))
+
+    def add_norm(self, norm: Norm, x: Tensor, add: Tensor | None, sum: Tensor | None, y: Tensor | None,
+                 q: Tensor | None = None, stream=None) -> int:
+        """sum = x + add, y = norm(sum) in float32, q = y in Q8_0 or Q8_K"""
+        t = [C.byref(v) if v is not None else None for v in (x, add, sum, y, q)]
+        return load().mi_add_norm(self.h, C.byref(norm), *t, _addr(stream))
+
+    def mul_mat(self, a: Tensor, b: Tensor, dst: Tensor, stream=None) -> int:
+        """dst[:, t] = a . b[:, t]: a in Q4_0 or Q4_K, b float32 rows or rows in Q8_0 / Q8_K"""
+        return load().mi_mul_mat(self.h, C.byref(a), C.byref(b), C.byref(dst), _addr(stream))
+
     def expert_ffn(self, layer: Layer, x, T: int, res, ids_gu, ids_dn, w, out, stream=None) -> int:
         return load().mi_moe_expert_ffn(self.h, C.byref(layer), _addr(x), T, _addr(res),
                                         _addr(ids_gu), _addr(ids_dn), _addr(w), _addr(out),
@@ -363,7 +409,7 @@ class Context:
                                   _addr(stream))
 
     def dequantize(self, type_: int, src, dst, nrows: int, n_per_row: int, stream=None) -> int:
-        """dst = the float32 values of rows of an MXFP4, Q4_0, Q5_0, Q8_0 or F16 table"""
+        """dst = the float32 values of rows of an MXFP4, Q4_0, Q5_0, Q8_0, Q8_K or F16 table"""
         return load().mi_dequantize(self.h, type_, _addr(src), _addr(dst), nrows, n_per_row, _addr(stream))
 
     def tile(self, src: Tensor, dst, desc: Tensor | None = None, stream=None) -> int:
