@@ -12,6 +12,7 @@
 // the matrix is read once and nothing else is.
 #include "b32.hpp"
 #include "common.hpp"
+#include "lanes.hpp"
 #include "launch.hpp"
 #include "wave_ops.hpp"
 
@@ -22,8 +23,6 @@ typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 typedef uint32_t u32_a2 __attribute__((aligned(2)));
 
-constexpr int MM_W = 8;                // waves of a work-group
-constexpr int MM_THREADS = 64 * MM_W;
 constexpr int MM_LDS = 160 * 1024;
 
 // The operands of 16 tokens for one set of blocks (Q4_0: 4 blocks, 128 values;
@@ -51,6 +50,41 @@ __device__ __forceinline__ uint2 mm_pack8(const int (&q)[8]) {
     return make_uint2(c[0], c[1]);
 }
 
+// the lane's 8 of a block's values as codes, and the block's scale (NaN where a
+// value is not finite or the scale leaves its type): Q8_0, 4 lanes a block
+__device__ __forceinline__ void mm_codes_q8_0(const float (&v)[8], uint2 &c, float &d) {
+    int bad = mm_bad8(v);
+    bad |= dpp_i<0xB1>(bad);
+    bad |= dpp_i<0x4E>(bad);
+    int q[8];
+    uint32_t dh;
+    b32_q8_codes(v, q, dh);
+    c = mm_pack8(q);
+    d = h2f((uint16_t)dh);
+    if (bad || !(d <= 65504.f)) d = __builtin_nanf("");
+}
+// Q8_K, 32 lanes a block.  d and the codes change sign together with the sign
+// that ggml gives them (of the first largest |x|): their products are the same.
+__device__ __forceinline__ void mm_codes_q8_K(const float (&v)[8], uint2 &c, float &d) {
+    const unsigned long long bb = __ballot(mm_bad8(v));
+    const bool bad = (uint32_t)(threadIdx.x & 32 ? bb >> 32 : bb) != 0u;
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t = fmaxf(t, fabsf(v[i]));
+    t = fmaxf(t, dpp_f<0xB1>(t));
+    t = fmaxf(t, dpp_f<0x4E>(t));
+    t = fmaxf(t, dpp_f<0x141>(t));
+    t = fmaxf(t, dpp_f<0x140>(t));
+    t = fmaxf(t, __shfl_xor(t, 16, 64));
+    const bool zero = t == 0.f;
+    const float is = zero ? 0.f : 127.f / t;
+    d = bad ? __builtin_nanf("") : zero ? 0.f : 1 / is;
+    int q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = bad || zero ? 0 : (int)__builtin_rintf(is * v[i]);
+    c = mm_pack8(q);
+}
+
 // piece p (8 values of token row m of the tile) of the tile's operands into its
 // record at o: Q4_0: block p / 4, quarter p % 4; Q4_K: values 8 p ..  The lanes
 // that share a block's largest value (4 or 32, aligned) call it together.
@@ -76,15 +110,7 @@ __device__ __forceinline__ void mm_piece(const uint8_t *row, int p, int m, bool 
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = 0.f;
             }
-            int bad = mm_bad8(v);
-            bad |= dpp_i<0xB1>(bad);
-            bad |= dpp_i<0x4E>(bad);
-            int q[8];
-            uint32_t dh;
-            b32_q8_codes(v, q, dh);
-            c = mm_pack8(q);
-            d = h2f((uint16_t)dh);
-            if (bad || !(d <= 65504.f)) d = __builtin_nanf("");
+            mm_codes_q8_0(v, c, d);
         } else if (live) {
             const uint8_t *b = row + 34 * blk;
             c.x = *(const u32_a2 *)(b + 2 + 4 * g);
@@ -114,26 +140,7 @@ __device__ __forceinline__ void mm_piece(const uint8_t *row, int p, int m, bool 
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = 0.f;
             }
-            const unsigned long long bb = __ballot(mm_bad8(v));
-            const bool bad = (uint32_t)(threadIdx.x & 32 ? bb >> 32 : bb) != 0u;
-            float t = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t = fmaxf(t, fabsf(v[i]));
-            t = fmaxf(t, dpp_f<0xB1>(t));
-            t = fmaxf(t, dpp_f<0x4E>(t));
-            t = fmaxf(t, dpp_f<0x141>(t));
-            t = fmaxf(t, dpp_f<0x140>(t));
-            t = fmaxf(t, __shfl_xor(t, 16, 64));
-            // d and the codes change sign together with the sign ggml gives them
-            // (of the first largest |x|): their products are the same
-            const bool zero = t == 0.f;
-            const float is = zero ? 0.f : 127.f / t;
-            d = zero ? 0.f : 1 / is;
-            int q[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = bad || zero ? 0 : (int)__builtin_rintf(is * v[i]);
-            if (bad) d = __builtin_nanf("");
-            c = mm_pack8(q);
+            mm_codes_q8_K(v, c, d);
         } else if (live) {
             const uint8_t *b = row + 292 * (p >> 5);
             c = make_uint2(*(const uint32_t *)(b + 4 + 8 * e), *(const uint32_t *)(b + 8 + 8 * e));
@@ -155,7 +162,7 @@ __global__ void __launch_bounds__(256) k_mm_rows(const uint8_t *b, int64_t ldb, 
     using R = MmRec<TYPE>;
     const int64_t t = blockIdx.y;
     const int p = blockIdx.x * 256 + threadIdx.x, set = p / (R::VALUES / 8);
-    if (set >= nsets) return;   // whole waves (64 pieces: whole sets)
+    if (set >= nsets) return;   // whole sets of lanes
     mm_piece<TYPE, 1>(b + t * ldb, p, (int)(t & 15), vec, 8 * p < K, ws + ((t >> 4) * nsets + set) * R::BYTES);
 }
 
@@ -164,7 +171,7 @@ struct MmPlan {
     int vec;       // fp32 rows 16-byte aligned
     int nsets;     // sets of a row
     int chunks, cs;  // chunks of cs sets whose operands lie in LDS at a time
-    int wk;        // waves that share a row tile, each taking every wk-th set
+    int wk;        // waves that share a row tile, each taking every wk-th step of sets
     int ntiles;    // row tiles of 16
 };
 
@@ -189,24 +196,15 @@ __device__ __forceinline__ void mm_load(MmRaw<TYPE> &r, const uint8_t *row, int 
 }
 
 __device__ __forceinline__ long mm_u64(uint32_t lo, uint32_t hi) { return (long)(((uint64_t)hi << 32) | lo); }
-__device__ __forceinline__ void swap16(uint32_t &a, uint32_t &b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-    a = r[0];
-    b = r[1];
-}
-__device__ __forceinline__ void swap32(uint32_t &a, uint32_t &b) {
-    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-    a = r[0];
-    b = r[1];
-}
-
 // acc[mt] += the set's part for token tile mt; x: the set's record of tile 0,
-// xs: bytes from a tile's record to the next tile's
-template <int TYPE, int MT>
+// xs: bytes from a tile's record to the next tile's.  NI: rows of a lane group's
+// four that hold tokens.
+template <int TYPE, int MT, int NI>
 __device__ __forceinline__ void mm_set(const MmRaw<TYPE> &r, const uint8_t *x, int xs, int set, int nb, int lane,
-                                       float4_t (&acc)[MT]) {
+                                       float (&acc)[MT][NI]) {
     const int g = lane >> 4;
     const i32x4 z = {0, 0, 0, 0};
+    typedef float fNI __attribute__((ext_vector_type(NI)));
     if constexpr (TYPE == 2) {
         // lane group g holds block g of the set; the products want dword g of
         // block j in group g: a 4 x 4 transpose over the groups
@@ -223,26 +221,27 @@ __device__ __forceinline__ void mm_set(const MmRaw<TYPE> &r, const uint8_t *x, i
         d[3] = d[1];
         swap32(d[0], d[2]);
         swap32(d[1], d[3]);
-        u32x4 xc[MT][2];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            xc[m][0] = *(const u32x4 *)(x + m * xs + 16 * lane);
-            xc[m][1] = *(const u32x4 *)(x + m * xs + 1024 + 16 * lane);
-        }
+        for (int jj = 0; jj < 2; ++jj) {
+            u32x4 xv[MT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float da = h2f((uint16_t)d[j]);
-            // 16 (q - 8) as signed bytes: the nibble on top, its highest bit turned
-            const uint32_t lo = ((w[j] << 4) & 0xF0F0F0F0u) ^ 0x80808080u, hi = (w[j] & 0xF0F0F0F0u) ^ 0x80808080u;
-            const long wb = mm_u64(lo, hi);
+            for (int m = 0; m < MT; ++m) xv[m] = *(const u32x4 *)(x + m * xs + 1024 * jj + 16 * lane);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const u32x4 xv = xc[m][j >> 1];
-                const long xa = j & 1 ? mm_u64(xv.z, xv.w) : mm_u64(xv.x, xv.y);
-                const i32x4 c = __builtin_amdgcn_mfma_i32_16x16x32_i8(xa, wb, z, 0, 0, 0);
-                const float4_t db = *(const float4_t *)(x + m * xs + 2048 + 64 * j + 16 * g);
+            for (int h = 0; h < 2; ++h) {
+                const int j = 2 * jj + h;
+                const float da = h2f((uint16_t)d[j]);
+                // 16 (q - 8) as signed bytes: the nibble on top, its highest bit turned
+                const uint32_t lo = ((w[j] << 4) & 0xF0F0F0F0u) ^ 0x80808080u, hi = (w[j] & 0xF0F0F0F0u) ^ 0x80808080u;
+                const long wb = mm_u64(lo, hi);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[m][i] = fmaf((float)c[i], da * db[i], acc[m][i]);
+                for (int m = 0; m < MT; ++m) {
+                    const long xa = h ? mm_u64(xv[m].z, xv[m].w) : mm_u64(xv[m].x, xv[m].y);
+                    const i32x4 c = __builtin_amdgcn_mfma_i32_16x16x32_i8(xa, wb, z, 0, 0, 0);
+                    const fNI db = *(const fNI *)(x + m * xs + 2048 + 64 * j + 16 * g);
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) acc[m][i] = fmaf((float)c[i], da * db[i], acc[m][i]);
+                }
+                if constexpr (MT > 2) __builtin_amdgcn_sched_barrier(0);   // (keeps the operands of later blocks in LDS)
             }
         }
     } else {
@@ -254,9 +253,11 @@ __device__ __forceinline__ void mm_set(const MmRaw<TYPE> &r, const uint8_t *x, i
         const uint32_t mg = (g & 2 ? mn[1] : mn[0]) >> (16 * (g & 1));
         const _Float16 m0 = (_Float16)(float)(mg & 0xffu), m1 = (_Float16)(float)((mg >> 8) & 0xffu);
         const half4_t mb = {m0, m0, m1, m1};
-        i32x4 s[MT];
+        int s[MT][NI];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) s[m] = z;
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < NI; ++i) s[m][i] = 0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const long lo = mm_u64(r.q[c].x & 0x0F0F0F0Fu, r.q[c].y & 0x0F0F0F0Fu);
@@ -268,33 +269,43 @@ __device__ __forceinline__ void mm_set(const MmRaw<TYPE> &r, const uint8_t *x, i
                 const i32x4 a = __builtin_amdgcn_mfma_i32_16x16x32_i8(mm_u64(xv.x, xv.y), lo, z, 0, 0, 0);
                 const i32x4 b = __builtin_amdgcn_mfma_i32_16x16x32_i8(mm_u64(xv.z, xv.w), hi, z, 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[m][i] += __mul24(a[i], s0) + __mul24(b[i], s1);
+                for (int i = 0; i < NI; ++i) {   // |a| < 2^16, scales below 64
+                    s[m][i] = __mul24(a[i], s0) + s[m][i];
+                    s[m][i] = __mul24(b[i], s1) + s[m][i];
+                }
             }
+            if constexpr (MT > 2) __builtin_amdgcn_sched_barrier(0);   // (keeps the operands of later blocks in LDS)
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const half4_t bs = *(const half4_t *)(x + m * xs + 4096 + 8 * lane);
             const float4_t zf = {0.f, 0.f, 0.f, 0.f};
             const float4_t mm = __builtin_amdgcn_mfma_f32_16x16x16f16(bs, mb, zf, 0, 0, 0);
-            const float4_t db = *(const float4_t *)(x + m * xs + 4608 + 16 * g);
+            const fNI db = *(const fNI *)(x + m * xs + 4608 + 16 * g);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(fmaf(d, (float)s[m][i], -(dm * mm[i])), db[i], acc[m][i]);
+            for (int i = 0; i < NI; ++i) acc[m][i] = fmaf(fmaf(d, (float)s[m][i], -(dm * mm[i])), db[i], acc[m][i]);
         }
     }
 }
 
-// Work-group (x, y): tokens 16 MT y .., row tiles x (W / wk), + gridDim.x (W / wk) ..
-template <int TYPE, int MT>
-__global__ void __launch_bounds__(MM_THREADS) k_mm(MmArgs g, MmPlan p) {
+// sets of a step (their loads go together): 256 values
+template <int TYPE> constexpr int MM_U = TYPE == 2 ? 2 : 1;
+
+// Work-group (x, y) of W waves: tokens 16 MT y .. (NI < 4: 4 NI tokens at most,
+// token t in row 4 (t / NI) + t % NI of the MFMA's), row tiles x (W / wk), +
+// gridDim.x (W / wk) ..
+template <int TYPE, int MT, int NI, int W>
+__global__ void __launch_bounds__(64 * W, 4) k_mm(MmArgs g, MmPlan p) {
     using R = MmRec<TYPE>;
+    constexpr int U = MM_U<TYPE>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wk = p.wk, wn = MM_W / wk, kw = wave % wk, nw = wave / wk;
+    const int wk = p.wk, wn = W / wk, kw = wave % wk, nw = wave / wk;
     const int64_t t0 = (int64_t)blockIdx.y * 16 * MT;
     const int nt = (int)(g.T - t0 < 16 * MT ? g.T - t0 : 16 * MT);   // tokens here
     const int nb = (int)(g.K / 32);
     const int xs = p.cs * R::BYTES;   // a token tile's records in LDS
-    float4_t *red = (float4_t *)(lds + MT * xs);   // [2][W][MT][64]
+    float *red = (float *)(lds + MT * xs);   // [2][W][MT][64][NI]
 
     // the operands of chunk ch
     auto fill = [&](int ch) __attribute__((always_inline)) {
@@ -304,101 +315,357 @@ __global__ void __launch_bounds__(MM_THREADS) k_mm(MmArgs g, MmPlan p) {
             for (int m = 0; m < MT && 16 * m < nt; ++m) {
                 const u32x4 *src = (const u32x4 *)((const uint8_t *)g.ws + ((t0 / 16 + m) * p.nsets + s0) * R::BYTES);
                 u32x4 *dst = (u32x4 *)(lds + m * xs);
-                for (int i = tid; i < per; i += MM_THREADS) dst[i] = src[i];
+                for (int i = tid; i < per; i += 64 * W) dst[i] = src[i];
             }
         } else {
             // pieces of 8 values; a wave's 64 pieces are of one token
-            constexpr int PS = R::VALUES / 8;   // pieces of a set: 16 or 32
+            constexpr int PS = R::VALUES / 8;      // pieces of a set: 16 or 32
             const int pt = (ns * PS + 63) & ~63;   // of a token, rounded up to whole waves
-            for (int i = tid; i < pt * nt; i += MM_THREADS) {
-                const int t = i / pt, q = i - t * pt, set = q / PS, pc = s0 * PS + q;
+            for (int t = 0, i = tid; t < nt; i += 64 * W) {
+                while (i >= pt && t < nt) {
+                    i -= pt;
+                    ++t;
+                }
+                if (t >= nt) break;
+                const int set = i / PS, pc = s0 * PS + i;
                 if (set >= ns) continue;   // (whole groups of lanes that share a block)
                 const uint8_t *row = (const uint8_t *)g.b + (t0 + t) * g.ldb;
-                uint8_t *o = lds + (t >> 4) * xs + set * R::BYTES;
-                if (p.src == 1) mm_piece<TYPE, 1>(row, pc, t & 15, p.vec, 8 * pc < g.K, o);
-                else mm_piece<TYPE, 2>(row, pc, t & 15, false, 8 * pc < g.K, o);
+                const int m = NI == 4 ? t & 15 : 4 * (t / NI) + t % NI;
+                uint8_t *o = lds + (NI == 4 ? t >> 4 : 0) * xs + set * R::BYTES;
+                if (p.src == 1) mm_piece<TYPE, 1>(row, pc, m, p.vec, 8 * pc < g.K, o);
+                else mm_piece<TYPE, 2>(row, pc, m, false, 8 * pc < g.K, o);
             }
         }
     };
 
-    const int spc = (p.cs + wk - 1) / wk;              // steps of a chunk
-    const int spt = spc * p.chunks;                    // of a row tile
-    const int stride = (int)gridDim.x * wn;
-    const int first = (int)blockIdx.x * wn;            // the work-group's first tile
-    const int iters = (p.ntiles - first + stride - 1) / stride;
-    const int total = iters * spt;
-
-    auto step_of = [&](int st, int &tile, int &set) __attribute__((always_inline)) {
-        const int it = st / spt, s = st - it * spt, ch = s / spc;
-        tile = first + nw + it * stride;
-        set = ch * p.cs + (s - ch * spc) * wk + kw;
-        if ((s - ch * spc) * wk + kw >= p.cs || tile >= p.ntiles) set = p.nsets;   // nothing here
+    const int stride = (int)gridDim.x * wn;   // tiles from one round to the next
+    // the step whose loads are issued next: its tile, chunk end and first set
+    int ltile = (int)blockIdx.x * wn + nw, lch = 0, lset = kw * U;
+    MmRaw<TYPE> nxt[U];
+    const uint8_t *lrow = nullptr;
+    auto row_of = [&]() __attribute__((always_inline)) {
+        const int64_t n = 16 * (int64_t)imin(ltile, p.ntiles - 1) + (lane & 15);
+        lrow = g.a + (n < g.N ? n : g.N - 1) * g.row_bytes;
     };
-    auto load = [&](MmRaw<TYPE> &r, int st) __attribute__((always_inline)) {
-        int tile, set;
-        step_of(st, tile, set);
-        // (clamped: a step that holds nothing loads some row's set and drops it)
-        const int64_t n = 16 * (int64_t)imin(tile, p.ntiles - 1) + (lane & 15);
-        mm_load<TYPE>(r, g.a + (n < g.N ? n : g.N - 1) * g.row_bytes, imin(set, p.nsets - 1), nb, lane >> 4);
-    };
-
-    float4_t acc[MT];
+    // (clamped in the rows and in K: what lies past them is loaded again and dropped)
+    auto load = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m] = {0.f, 0.f, 0.f, 0.f};
-    MmRaw<TYPE> cur, nxt;
-    load(cur, 0);
+        for (int u = 0; u < U; ++u) mm_load<TYPE>(nxt[u], lrow, imin(lset + u, p.nsets - 1), nb, lane >> 4);
+    };
+    auto advance = [&]() __attribute__((always_inline)) {
+        lset += wk * U;
+        if (lset >= imin((lch + 1) * p.cs, p.nsets)) {
+            if (++lch == p.chunks) {
+                lch = 0;
+                ltile += stride;
+                row_of();
+            }
+            lset = lch * p.cs + kw * U;
+        }
+    };
+    row_of();
+    load();
     if (p.chunks == 1) {
         fill(0);
         __syncthreads();
     }
-    for (int st = 0; st < total; ++st) {
-        if (st + 1 < total) load(nxt, st + 1);
-        const int it = st / spt, s = st - it * spt, ch = s / spc;
-        if (p.chunks > 1 && s == ch * spc) {
-            __syncthreads();
-            fill(ch);
-            __syncthreads();
-        }
-        int tile, set;
-        step_of(st, tile, set);
-        if (set < p.nsets) mm_set<TYPE, MT>(cur, lds + (set - ch * p.cs) * R::BYTES, xs, set, nb, lane, acc);
-        if (s == spt - 1) {
-            const int n = 16 * tile + (lane & 15);
-            if (wk == 1) {
-                if (tile < p.ntiles && n < g.N) {
+    int par = 0;
+    for (int tb = (int)blockIdx.x * wn; tb < p.ntiles; tb += stride) {   // the work-group's tiles tb .. tb + wn - 1
+        float acc[MT][NI];
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int t = 16 * m + 4 * (lane >> 4) + i;
-                            if (t < nt) g.y[(t0 + t) * g.ldy + n] = acc[m][i];
-                        }
-                }
-            } else {
-                // the tile's parts, one buffer per parity: a wave that is through
-                // with this one is past the barrier after its last use
-                float4_t *rb = red + (it & 1) * MM_W * MT * 64;
-#pragma unroll
-                for (int m = 0; m < MT; ++m) rb[(wave * MT + m) * 64 + lane] = acc[m];
+            for (int i = 0; i < NI; ++i) acc[m][i] = 0.f;
+        for (int ch = 0; ch < p.chunks; ++ch) {
+            if (p.chunks > 1) {
                 __syncthreads();
-                const float *rf = (const float *)rb;
-                for (int e = tid; e < wn * MT * 256; e += MM_THREADS) {
-                    const int i = e & 3, l = (e >> 2) & 63, m = (e >> 8) % MT, w = (e >> 8) / MT;
-                    const int t = 16 * m + 4 * (l >> 4) + i, tl = first + w + it * stride;
-                    const int64_t nn = 16 * (int64_t)tl + (l & 15);
-                    if (t >= nt || tl >= p.ntiles || nn >= g.N) continue;
-                    float v = rf[((w * wk) * MT + m) * 256 + 4 * l + i];
-                    for (int k = 1; k < wk; ++k) v += rf[((w * wk + k) * MT + m) * 256 + 4 * l + i];
-                    g.y[(t0 + t) * g.ldy + nn] = v;
-                }
+                fill(ch);
+                __syncthreads();
             }
+            const int end = imin((ch + 1) * p.cs, p.nsets);
+            int set = ch * p.cs + kw * U;
+            if (set >= end) advance(), load();   // no step here: the cursor moves with the loops
+            for (; set < end; set += wk * U) {
+                MmRaw<TYPE> cur[U];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m] = {0.f, 0.f, 0.f, 0.f};
+                for (int u = 0; u < U; ++u) cur[u] = nxt[u];
+                advance();
+                load();
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (set + u < end)
+                        mm_set<TYPE, MT, NI>(cur[u], lds + (set + u - ch * p.cs) * R::BYTES, xs, set + u, nb, lane, acc);
+            }
         }
-        cur = nxt;
+        if (wk == 1) {
+            const int64_t n = 16 * (int64_t)(tb + nw) + (lane & 15);
+            if (n < g.N) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) {
+                        const int t = 16 * m + NI * (lane >> 4) + i;
+                        if (t < nt) g.y[(t0 + t) * g.ldy + n] = acc[m][i];
+                    }
+            }
+        } else {
+            // the tiles' parts, one buffer per parity: a wave that writes a buffer
+            // again is past the barrier after its last use
+            float *rb = red + par * (W * MT * 64 * NI);
+            par ^= 1;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < NI; ++i) rb[((wave * MT + m) * 64 + lane) * NI + i] = acc[m][i];
+            __syncthreads();
+            for (int e = tid; e < wn * MT * 64 * NI; e += 64 * W) {
+                const int i = e % NI, l = (e / NI) & 63, m = e / (NI * 64) % MT, w = e / (NI * 64 * MT);
+                const int t = 16 * m + NI * (l >> 4) + i;
+                const int64_t n = 16 * (int64_t)(tb + w) + (l & 15);
+                if (t >= nt || n >= g.N) continue;
+                float v = rb[((w * wk) * MT + m) * 64 * NI + l * NI + i];
+                for (int k = 1; k < wk; ++k) v += rb[((w * wk + k) * MT + m) * 64 * NI + l * NI + i];
+                g.y[(t0 + t) * g.ldy + n] = v;
+            }
+        }
     }
 }
 
+// ---------------------------------------------------------------- up to 4 rows
+// One lane per 32 values of a row of the matrix (Q4_0: a block; Q4_K: 16 bytes
+// of codes, 16 values of one sub-block and 16 of the next), 2^lg lanes per
+// row: a wave's loads are runs of whole rows.  The dots run on v_dot4_i32_i8.
+//
+// The tokens' operands per unit of 32 values, in LDS: the codes of the low
+// nibbles (16 bytes), of the high ones (16 bytes), and {scale f32, Q4_0: -8 times
+// the codes' sum; Q4_K: the two sums of 16 codes, as halves of a word}.
+struct MvPlan {
+    int src, vec;      // as MmPlan (src 1 or 2)
+    int nu;            // units of a row
+    int lg, chunks;    // lanes per row (log2), units of a row / lanes, rounded up
+    int64_t batches;   // of R * 64 / lanes rows
+};
+
+template <int TYPE, int SRC>
+__device__ __forceinline__ void mv_piece(const uint8_t *row, int p, bool vec, bool live, uint8_t *lo, uint8_t *hi, uint2 *sc) {
+    uint2 c = make_uint2(0u, 0u);
+    float d = 0.f;
+    if constexpr (SRC == 1) {
+        float v[8];
+        const float *x = (const float *)row + 8 * p;
+        if (live) {
+            if (vec) {
+                const float4 a = *(const float4 *)x, b = *(const float4 *)(x + 4);
+                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = x[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        }
+        if constexpr (TYPE == 2) mm_codes_q8_0(v, c, d);
+        else mm_codes_q8_K(v, c, d);
+    } else if (live) {
+        if constexpr (TYPE == 2) {
+            const uint8_t *b = row + 34 * (p >> 2);
+            c.x = *(const u32_a2 *)(b + 2 + 8 * (p & 3));
+            c.y = *(const u32_a2 *)(b + 6 + 8 * (p & 3));
+            d = h2f(*(const uint16_t *)b);
+            if (!(fabsf(d) <= 65504.f)) d = __builtin_nanf("");
+        } else {
+            const uint8_t *b = row + 292 * (p >> 5);
+            c = make_uint2(*(const uint32_t *)(b + 4 + 8 * (p & 31)), *(const uint32_t *)(b + 8 + 8 * (p & 31)));
+            d = *(const float *)b;
+            if (!(fabsf(d) <= 3.402823466e38f)) d = __builtin_nanf("");
+        }
+    }
+    int s = __builtin_amdgcn_sdot4(0x01010101, (int)c.x, __builtin_amdgcn_sdot4(0x01010101, (int)c.y, 0, false), false);
+    s += dpp_i<0xB1>(s);
+    if constexpr (TYPE == 2) {
+        s += dpp_i<0x4E>(s);
+        if (!live) return;
+        *(uint2 *)((p & 2 ? hi : lo) + 16 * (p >> 2) + 8 * (p & 1)) = c;
+        if ((p & 3) == 0) sc[p >> 2] = make_uint2(__builtin_bit_cast(uint32_t, d), (uint32_t)(-8 * s));
+    } else {
+        if (!live) return;
+        // sub-block j = p / 4 % 8: bits of chunk j / 2, low or high nibbles by j & 1; half p / 2 & 1
+        const int j = (p >> 2) & 7, unit = 8 * (p >> 5) + 2 * (j >> 1) + ((p >> 1) & 1);
+        *(uint2 *)((j & 1 ? hi : lo) + 16 * unit + 8 * (p & 1)) = c;
+        if (!(p & 1)) {
+            ((int16_t *)(sc + unit))[2 + (j & 1)] = (int16_t)s;
+            if (!(j & 1)) *(float *)(sc + unit) = d;
+        }
+    }
+}
+
+template <int TYPE> struct MvRaw;
+template <> struct MvRaw<2> { u32x4 q; uint32_t d; };
+template <> struct MvRaw<12> { u32x4 h, q; };
+
+constexpr int MV_W = 4;
+
+template <int TYPE, int T, int R>
+__global__ void __launch_bounds__(64 * MV_W) k_mv(MmArgs g, MvPlan p) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nl = 1 << p.lg, l = lane & (nl - 1), rw = 64 >> p.lg;   // lanes of a row, rows of a load
+    const int64_t step = (int64_t)gridDim.x * MV_W;
+    int64_t b = (int64_t)blockIdx.x * MV_W + wave, lb = b;
+    int lch = 0;
+    MvRaw<TYPE> nxt[R];
+    // (clamped in the rows and in K: what lies past them is loaded again and dropped)
+    auto load = [&]() __attribute__((always_inline)) {
+        const int u = imin((lch << p.lg) + l, p.nu - 1);
+        const int64_t n0 = (lb < p.batches ? lb : p.batches - 1) * (R * rw) + (lane >> p.lg);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t n = n0 + r * rw;
+            const uint8_t *a = g.a + (n < g.N ? n : g.N - 1) * g.row_bytes;
+            if constexpr (TYPE == 2) {
+                nxt[r].q = *(const u32x4_a2 *)(a + 18 * u + 2);
+                nxt[r].d = *(const uint16_t *)(a + 18 * u);
+            } else {
+                a += 144 * (int64_t)(u >> 3);
+                nxt[r].h = *(const u32x4 *)a;
+                nxt[r].q = *(const u32x4 *)(a + 16 + 16 * (u & 7));
+            }
+        }
+        if (++lch == p.chunks) {
+            lch = 0;
+            lb += step;
+        }
+    };
+    load();
+    const int pieces = 4 * p.nu, pt = (pieces + 63) & ~63;
+    const int xb = 40 * p.nu;   // a token's operands
+    // pieces of 8 values; a wave's 64 pieces are of one token
+    for (int t = 0, i = tid; t < T; i += 64 * MV_W) {
+        while (i >= pt && t < T) {
+            i -= pt;
+            ++t;
+        }
+        if (t >= T) break;
+        const uint8_t *row = (const uint8_t *)g.b + t * g.ldb;
+        uint8_t *o = lds + t * xb;
+        if (p.src == 1) mv_piece<TYPE, 1>(row, i, p.vec, i < pieces, o, o + 16 * p.nu, (uint2 *)(o + 32 * p.nu));
+        else mv_piece<TYPE, 2>(row, i, false, i < pieces, o, o + 16 * p.nu, (uint2 *)(o + 32 * p.nu));
+    }
+    __syncthreads();
+    for (; b < p.batches; b += step) {
+        float acc[R][T];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < T; ++t) acc[r][t] = 0.f;
+        for (int ch = 0; ch < p.chunks; ++ch) {
+            MvRaw<TYPE> cur[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) cur[r] = nxt[r];
+            load();
+            const int u0 = (ch << p.lg) + l, u = imin(u0, p.nu - 1);
+            const bool live = u0 < p.nu;
+            u32x4 xl[T], xh[T];
+            uint2 xs[T];
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const uint8_t *o = lds + t * xb;
+                xl[t] = *(const u32x4 *)(o + 16 * u);
+                xh[t] = *(const u32x4 *)(o + 16 * p.nu + 16 * u);
+                xs[t] = *(const uint2 *)(o + 32 * p.nu + 8 * u);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if constexpr (TYPE == 2) {
+                    const float da = live ? h2f((uint16_t)cur[r].d) : 0.f;
+                    int s[T];
+#pragma unroll
+                    for (int t = 0; t < T; ++t) s[t] = (int)xs[t].y;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int lo = (int)(cur[r].q[j] & 0x0F0F0F0Fu), hi = (int)((cur[r].q[j] >> 4) & 0x0F0F0F0Fu);
+#pragma unroll
+                        for (int t = 0; t < T; ++t)
+                            s[t] = __builtin_amdgcn_sdot4(hi, (int)xh[t][j], __builtin_amdgcn_sdot4(lo, (int)xl[t][j], s[t], false), false);
+                    }
+#pragma unroll
+                    for (int t = 0; t < T; ++t)
+                        acc[r][t] = fmaf((float)s[t], da * __builtin_bit_cast(float, xs[t].x), acc[r][t]);
+                } else {
+                    const uint32_t w0 = cur[r].h.y, w1 = cur[r].h.z, w2 = cur[r].h.w;
+                    const float d = live ? h2f((uint16_t)(cur[r].h.x & 0xffff)) : 0.f;
+                    const float dm = live ? h2f((uint16_t)(cur[r].h.x >> 16)) : 0.f;
+                    // scales and minima of sub-blocks 2 c, 2 c + 1, c = u / 2 % 4
+                    const uint32_t sc = (l & 4 ? (w2 & 0x0F0F0F0Fu) | ((w0 >> 2) & 0x30303030u) : w0 & 0x3F3F3F3Fu) >> (8 * (l & 2));
+                    const uint32_t mn = (l & 4 ? ((w2 >> 4) & 0x0F0F0F0Fu) | ((w1 >> 2) & 0x30303030u) : w1 & 0x3F3F3F3Fu) >> (8 * (l & 2));
+                    int s0[T], s1[T];
+#pragma unroll
+                    for (int t = 0; t < T; ++t) s0[t] = s1[t] = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int lo = (int)(cur[r].q[j] & 0x0F0F0F0Fu), hi = (int)((cur[r].q[j] >> 4) & 0x0F0F0F0Fu);
+#pragma unroll
+                        for (int t = 0; t < T; ++t) {
+                            s0[t] = __builtin_amdgcn_sdot4(lo, (int)xl[t][j], s0[t], false);
+                            s1[t] = __builtin_amdgcn_sdot4(hi, (int)xh[t][j], s1[t], false);
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < T; ++t) {
+                        const int s = __mul24(s0[t], (int)(sc & 0xffu)) + __mul24(s1[t], (int)((sc >> 8) & 0xffu));
+                        const int m = __mul24((int)(int16_t)xs[t].y, (int)(mn & 0xffu)) + __mul24((int)xs[t].y >> 16, (int)((mn >> 8) & 0xffu));
+                        acc[r][t] = fmaf(fmaf(d, (float)s, -(dm * (float)m)), __builtin_bit_cast(float, xs[t].x), acc[r][t]);
+                    }
+                }
+            }
+        }
+        const int64_t n0 = b * (R * rw) + (lane >> p.lg);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const float v = group_sum(acc[r][t], nl);
+                const int64_t n = n0 + r * rw;
+                if (l == 0 && n < g.N) g.y[t * g.ldy + n] = v;
+            }
+    }
+}
+
+// lanes of a row: the most whose last round wastes at most an eighth of all
+static int mv_lg(int nu) {
+    for (int lg = 6; lg > 3; --lg)
+        if (8 * ((nu + (1 << lg) - 1) >> lg << lg) <= 9 * nu) return lg;
+    return 3;
+}
+
+template <int TYPE, int T, int R>
+static int mv_go(const MmArgs &g, MvPlan p, hipStream_t st) {
+    const int64_t rows = R * (64 >> p.lg);   // of a wave
+    p.batches = (g.N + rows - 1) / rows;
+    const int64_t most = (p.batches + MV_W - 1) / MV_W;
+    const dim3 grid((unsigned)(most < 2048 ? most : 2048)), block(64 * MV_W);
+    hipLaunchKernelGGL((k_mv<TYPE, T, R>), grid, block, (size_t)T * 40 * p.nu, st, g, p);
+    return hip_check_launch();
+}
+
+template <int TYPE, int T>
+static int mv_launch(const MmArgs &g, hipStream_t st) {
+    MvPlan p = {};
+    p.src = g.btype != 0 ? 2 : 1;
+    p.vec = (uintptr_t)g.b % 16 == 0 && g.ldb % 16 == 0;
+    p.nu = (int)(g.K / 32);
+    p.lg = mv_lg(p.nu);
+    p.chunks = (p.nu + (1 << p.lg) - 1) >> p.lg;
+    // four rows a lane where that leaves every SIMD four waves
+    return g.N >= 4 * 4096 * (64 >> p.lg) ? mv_go<TYPE, T, 4>(g, p, st) : mv_go<TYPE, T, 1>(g, p, st);
+}
+
+constexpr int64_t MV_T = 4;   // rows of b
+template <int TYPE>
+static bool mv_ok(const MmArgs &g) { return g.T <= MV_T && g.T * 40 * (g.K / 32) <= MM_LDS; }
+
+constexpr int64_t MM_PASS_T = 32768;   // rows of one pass (grid dimensions)
 constexpr int64_t MM_PREP_T = 8;   // fp32 rows from so many on: their records in a launch of their own
 
 size_t mm_ws_bytes(int type, int btype, int64_t T, int64_t K) {
@@ -407,9 +674,38 @@ size_t mm_ws_bytes(int type, int btype, int64_t T, int64_t K) {
                      : (size_t)((T + 15) / 16 * (K / 256) * MmRec<12>::BYTES);
 }
 
+template <int TYPE, int MT, int NI, int W>
+static int mm_go(const MmArgs &g, MmPlan p, hipStream_t st) {
+    using R = MmRec<TYPE>;
+    const int64_t slices = (g.T + 16 * MT - 1) / (16 * MT);
+    // waves that share a row tile: the fewest that give every SIMD four waves
+    p.wk = 1;
+    while (p.wk < (MT > 2 ? 1 : 8) && p.ntiles * slices * p.wk < 4096) p.wk *= 2;
+    const int red = p.wk > 1 ? 2 * W * MT * 64 * NI * 4 : 0;
+    const int fit = (MM_LDS - red) / (MT * R::BYTES) / MM_U<TYPE> * MM_U<TYPE>;
+    p.chunks = (p.nsets + fit - 1) / fit;
+    p.cs = (p.nsets + p.chunks - 1) / p.chunks;
+    p.cs = (p.cs + MM_U<TYPE> - 1) / MM_U<TYPE> * MM_U<TYPE>;
+    p.chunks = (p.nsets + p.cs - 1) / p.cs;
+    const int lds = MT * p.cs * R::BYTES + red;
+    const int per_cu = imin(2, imax(1, MM_LDS / lds));
+    const int wn = W / p.wk;
+    const int64_t want = (256 * per_cu + slices - 1) / slices;   // work-groups of a slice
+    const int64_t most = (p.ntiles + wn - 1) / wn;
+    const dim3 grid((unsigned)(want < most ? want : most), (unsigned)slices), block(64 * W);
+    hipLaunchKernelGGL((k_mm<TYPE, MT, NI, W>), grid, block, lds, st, g, p);
+    return hip_check_launch();
+}
+
 template <int TYPE>
 static int mm_launch(const MmArgs &g, hipStream_t st) {
     using R = MmRec<TYPE>;
+    if (mv_ok<TYPE>(g)) {
+        if (g.T == 1) return mv_launch<TYPE, 1>(g, st);
+        if (g.T == 2) return mv_launch<TYPE, 2>(g, st);
+        if (g.T == 3) return mv_launch<TYPE, 3>(g, st);
+        return mv_launch<TYPE, 4>(g, st);
+    }
     MmPlan p = {};
     p.nsets = (int)((g.K + R::VALUES - 1) / R::VALUES);
     p.ntiles = (int)((g.N + 15) / 16);
@@ -422,29 +718,23 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
         if (rc) return rc;
         p.src = 0;
     }
-    const int mt = g.T <= 16 ? 1 : g.T <= 32 ? 2 : 4;
-    const int64_t slices = (g.T + 16 * mt - 1) / (16 * mt);
-    if (slices > 65535) return -6;
-    p.wk = mt == 4 ? 1 : MM_W;
-    const int red = p.wk > 1 ? 2 * MM_W * mt * 1024 : 0;
-    const int fit = (MM_LDS - red) / (mt * R::BYTES);
-    p.chunks = (p.nsets + fit - 1) / fit;
-    p.cs = (p.nsets + p.chunks - 1) / p.chunks;
-    const int lds = mt * p.cs * R::BYTES + red;
-    const int per_cu = imin(4, imax(1, MM_LDS / lds));
-    const int wn = MM_W / p.wk;
-    const int64_t want = (256 * per_cu + slices - 1) / slices;   // work-groups of a slice
-    const int64_t most = (p.ntiles + wn - 1) / wn;
-    const dim3 grid((unsigned)(want < most ? want : most), (unsigned)slices), block(MM_THREADS);
-    if (mt == 1) hipLaunchKernelGGL((k_mm<TYPE, 1>), grid, block, lds, st, g, p);
-    else if (mt == 2) hipLaunchKernelGGL((k_mm<TYPE, 2>), grid, block, lds, st, g, p);
-    else hipLaunchKernelGGL((k_mm<TYPE, 4>), grid, block, lds, st, g, p);
-    return hip_check_launch();
+    if (p.src != 0 && g.T <= 4) return mm_go<TYPE, 1, 1, 8>(g, p, st);
+    if (p.src != 0 && g.T <= 8) return mm_go<TYPE, 1, 2, 8>(g, p, st);
+    if (g.T <= 16) return mm_go<TYPE, 1, 4, 8>(g, p, st);
+    if (g.T <= 32) return mm_go<TYPE, 2, 4, 8>(g, p, st);
+    return mm_go<TYPE, 2, 4, 8>(g, p, st);
 }
 
 int launch_mm(const MmArgs &g, hipStream_t st) {
-    if (g.T <= 0) return 0;
-    return g.type == 2 ? mm_launch<2>(g, st) : mm_launch<12>(g, st);
+    for (int64_t t = 0; t < g.T; t += MM_PASS_T) {
+        MmArgs a = g;
+        a.b = (const uint8_t *)g.b + t * g.ldb;
+        a.y = g.y + t * g.ldy;
+        a.T = g.T - t < MM_PASS_T ? g.T - t : MM_PASS_T;
+        const int rc = g.type == 2 ? mm_launch<2>(a, st) : mm_launch<12>(a, st);
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 }  // namespace mimoe
