@@ -18,7 +18,10 @@
 
 namespace mimoe {
 
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef __attribute__((address_space(1))) void global_void_t;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 typedef uint32_t u32_a2 __attribute__((aligned(2)));
@@ -37,52 +40,67 @@ template <int TYPE> struct MmRec;
 template <> struct MmRec<2> { static constexpr int VALUES = 128, CODES = 2048, BYTES = 2048 + 256; };
 template <> struct MmRec<12> { static constexpr int VALUES = 256, CODES = 4096, BYTES = 4096 + 512 + 64; };
 
-__device__ __forceinline__ bool mm_bad8(const float (&v)[8]) {
-    bool bad = false;
+// the largest |v| as bits (a NaN or an infinity: 0x7f800000 or more)
+__device__ __forceinline__ uint32_t mm_amax8(const float (&v)[8]) {
+    uint32_t m = 0u;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) bad |= !(fabsf(v[j]) <= 3.402823466e38f);
-    return bad;
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu;
+        m = u > m ? u : m;
+    }
+    return m;
 }
-__device__ __forceinline__ uint2 mm_pack8(const int (&q)[8]) {
-    uint32_t c[2] = {0u, 0u};
+template <int CTRL>
+__device__ __forceinline__ uint32_t mm_dpp_max(uint32_t m) {
+    const uint32_t o = (uint32_t)dpp_i<CTRL>((int)m);
+    return o > m ? o : m;
+}
+// the lowest bytes of eight words
+__device__ __forceinline__ uint2 mm_bytes8(const uint32_t (&q)[8]) {
+    uint32_t h[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c[j >> 2] |= (uint32_t)(q[j] & 0xff) << (8 * (j & 3));
-    return make_uint2(c[0], c[1]);
+    for (int j = 0; j < 4; ++j) h[j] = __builtin_amdgcn_perm(q[2 * j + 1], q[2 * j], 0x0C0C0400u);
+    return make_uint2(__builtin_amdgcn_perm(h[1], h[0], 0x05040100u), __builtin_amdgcn_perm(h[3], h[2], 0x05040100u));
 }
-
 // the lane's 8 of a block's values as codes, and the block's scale (NaN where a
-// value is not finite or the scale leaves its type): Q8_0, 4 lanes a block
+// value is not finite or the scale leaves its type): Q8_0, 4 lanes a block.
+// roundf(t): t + the number before 1/2 with t's sign, cut (|t| <= 127.5: the sum
+// of a fraction of 1/2 or more rounds to the next integer, of less stays below).
 __device__ __forceinline__ void mm_codes_q8_0(const float (&v)[8], uint2 &c, float &d) {
-    int bad = mm_bad8(v);
-    bad |= dpp_i<0xB1>(bad);
-    bad |= dpp_i<0x4E>(bad);
-    int q[8];
-    uint32_t dh;
-    b32_q8_codes(v, q, dh);
-    c = mm_pack8(q);
-    d = h2f((uint16_t)dh);
-    if (bad || !(d <= 65504.f)) d = __builtin_nanf("");
+    uint32_t m = mm_amax8(v);
+    m = mm_dpp_max<0xB1>(m);
+    m = mm_dpp_max<0x4E>(m);
+    const float df = __builtin_bit_cast(float, m) / 127.0f;
+    const float id = df != 0.0f ? 1.0f / df : 0.0f;
+    uint32_t q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float t = v[j] * id;
+        q[j] = (uint32_t)(int)(t + __builtin_copysignf(0.49999997f, t));
+    }
+    c = mm_bytes8(q);
+    d = (float)(_Float16)df;
+    if (m >= 0x7f800000u || !(d <= 65504.f)) d = __builtin_nanf("");
 }
 // Q8_K, 32 lanes a block.  d and the codes change sign together with the sign
 // that ggml gives them (of the first largest |x|): their products are the same.
+// rint by the sum with 1.5 * 2^23, whose low bits hold the integer.
 __device__ __forceinline__ void mm_codes_q8_K(const float (&v)[8], uint2 &c, float &d) {
-    const unsigned long long bb = __ballot(mm_bad8(v));
-    const bool bad = (uint32_t)(threadIdx.x & 32 ? bb >> 32 : bb) != 0u;
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t = fmaxf(t, fabsf(v[i]));
-    t = fmaxf(t, dpp_f<0xB1>(t));
-    t = fmaxf(t, dpp_f<0x4E>(t));
-    t = fmaxf(t, dpp_f<0x141>(t));
-    t = fmaxf(t, dpp_f<0x140>(t));
-    t = fmaxf(t, __shfl_xor(t, 16, 64));
-    const bool zero = t == 0.f;
-    const float is = zero ? 0.f : 127.f / t;
+    uint32_t m = mm_amax8(v);
+    m = mm_dpp_max<0xB1>(m);
+    m = mm_dpp_max<0x4E>(m);
+    m = mm_dpp_max<0x141>(m);
+    m = mm_dpp_max<0x140>(m);
+    uint32_t o = m;
+    swap16(m, o);
+    m = o > m ? o : m;
+    const bool zero = m == 0u, bad = m >= 0x7f800000u;
+    const float is = zero || bad ? 0.f : 127.f / __builtin_bit_cast(float, m);
     d = bad ? __builtin_nanf("") : zero ? 0.f : 1 / is;
-    int q[8];
+    uint32_t q[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = bad || zero ? 0 : (int)__builtin_rintf(is * v[i]);
-    c = mm_pack8(q);
+    for (int i = 0; i < 8; ++i) q[i] = __builtin_bit_cast(uint32_t, bad ? 12582912.f : is * v[i] + 12582912.f);
+    c = mm_bytes8(q);
 }
 
 // piece p (8 values of token row m of the tile) of the tile's operands into its
@@ -195,6 +213,13 @@ __device__ __forceinline__ void mm_load(MmRaw<TYPE> &r, const uint8_t *row, int 
     }
 }
 
+// a b + c, |a|, |b| < 2^23, one instruction (the empty statement keeps a chain of
+// them from being regrouped into products and three-operand additions)
+__device__ __forceinline__ int mad24(int a, int b, int c) {
+    int r = __mul24(a, b) + c;
+    asm("" : "+v"(r));
+    return r;
+}
 __device__ __forceinline__ long mm_u64(uint32_t lo, uint32_t hi) { return (long)(((uint64_t)hi << 32) | lo); }
 // acc[mt] += the set's part for token tile mt; x: the set's record of tile 0,
 // xs: bytes from a tile's record to the next tile's.  NI: rows of a lane group's
@@ -254,27 +279,55 @@ __device__ __forceinline__ void mm_set(const MmRaw<TYPE> &r, const uint8_t *x, i
         const _Float16 m0 = (_Float16)(float)(mg & 0xffu), m1 = (_Float16)(float)((mg >> 8) & 0xffu);
         const half4_t mb = {m0, m0, m1, m1};
         int s[MT][NI];
+        if constexpr (MT == 1) {
+            // a sub-block a MFMA, its scale on the sums
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int i = 0; i < NI; ++i) s[0][i] = 0;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) s[m][i] = 0;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const long lo = mm_u64(r.q[c].x & 0x0F0F0F0Fu, r.q[c].y & 0x0F0F0F0Fu);
-            const long hi = mm_u64((r.q[c].x >> 4) & 0x0F0F0F0Fu, (r.q[c].y >> 4) & 0x0F0F0F0Fu);
-            const int s0 = (int)((sc[c >> 1] >> (16 * (c & 1))) & 0xffu), s1 = (int)((sc[c >> 1] >> (16 * (c & 1) + 8)) & 0xffu);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const u32x4 xv = *(const u32x4 *)(x + m * xs + 1024 * c + 16 * lane);
+            for (int c = 0; c < 4; ++c) {
+                const long lo = mm_u64(r.q[c].x & 0x0F0F0F0Fu, r.q[c].y & 0x0F0F0F0Fu);
+                const long hi = mm_u64((r.q[c].x >> 4) & 0x0F0F0F0Fu, (r.q[c].y >> 4) & 0x0F0F0F0Fu);
+                const int s0 = (int)((sc[c >> 1] >> (16 * (c & 1))) & 0xffu), s1 = (int)((sc[c >> 1] >> (16 * (c & 1) + 8)) & 0xffu);
+                const u32x4 xv = *(const u32x4 *)(x + 1024 * c + 16 * lane);
                 const i32x4 a = __builtin_amdgcn_mfma_i32_16x16x32_i8(mm_u64(xv.x, xv.y), lo, z, 0, 0, 0);
                 const i32x4 b = __builtin_amdgcn_mfma_i32_16x16x32_i8(mm_u64(xv.z, xv.w), hi, z, 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < NI; ++i) {   // |a| < 2^16, scales below 64
-                    s[m][i] = __mul24(a[i], s0) + s[m][i];
-                    s[m][i] = __mul24(b[i], s1) + s[m][i];
+                for (int i = 0; i < NI; ++i) s[0][i] = mad24(b[i], s1, mad24(a[i], s0, s[0][i]));   // |a| < 2^16, scales below 64
+            }
+        } else {
+            // scale times code as 8 h + l, both digits in 8 bits (15 * 7 = 105): two sub-blocks
+            // a MFMA, the whole block's sums of either digit with no other instruction between
+            const uint32_t dl[2] = {sc[0] & 0x07070707u, sc[1] & 0x07070707u};
+            const uint32_t dh[2] = {(sc[0] >> 3) & 0x07070707u, (sc[1] >> 3) & 0x07070707u};
+            i32x4 sl[MT], sh[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) sl[m] = sh[m] = z;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint32_t q[4] = {r.q[c].x & 0x0F0F0F0Fu, r.q[c].y & 0x0F0F0F0Fu, (r.q[c].x >> 4) & 0x0F0F0F0Fu,
+                                       (r.q[c].y >> 4) & 0x0F0F0F0Fu};
+                i32x4 wl, wh;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    // the sub-block's digits in both halves of a word; bytes stay below 256 in a product
+                    const uint32_t sel = 0x0C000C00u + 0x00010001u * (2 * (c & 1) + (k >> 1));
+                    const ushort2_t l = __builtin_bit_cast(ushort2_t, __builtin_amdgcn_perm(0u, dl[c >> 1], sel));
+                    const ushort2_t h = __builtin_bit_cast(ushort2_t, __builtin_amdgcn_perm(0u, dh[c >> 1], sel));
+                    const ushort2_t v = __builtin_bit_cast(ushort2_t, q[k]);
+                    wl[k] = __builtin_bit_cast(int, v * l);
+                    wh[k] = __builtin_bit_cast(int, v * h);
+                }
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const i32x4 xv = *(const i32x4 *)(x + m * xs + 1024 * c + 16 * lane);
+                    sl[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv, wl, sl[m], 0, 0, 0);
+                    sh[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv, wh, sh[m], 0, 0, 0);
                 }
             }
-            if constexpr (MT > 2) __builtin_amdgcn_sched_barrier(0);   // (keeps the operands of later blocks in LDS)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < NI; ++i) s[m][i] = sl[m][i] + 8 * sh[m][i];
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -295,7 +348,7 @@ template <int TYPE> constexpr int MM_U = TYPE == 2 ? 2 : 1;
 // token t in row 4 (t / NI) + t % NI of the MFMA's), row tiles x (W / wk), +
 // gridDim.x (W / wk) ..
 template <int TYPE, int MT, int NI, int W>
-__global__ void __launch_bounds__(64 * W, 4) k_mm(MmArgs g, MmPlan p) {
+__global__ void __launch_bounds__(64 * W) k_mm(MmArgs g, MmPlan p) {
     using R = MmRec<TYPE>;
     constexpr int U = MM_U<TYPE>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -313,10 +366,13 @@ __global__ void __launch_bounds__(64 * W, 4) k_mm(MmArgs g, MmPlan p) {
         if (p.src == 0) {
             const int per = ns * (R::BYTES / 16);
             for (int m = 0; m < MT && 16 * m < nt; ++m) {
-                const u32x4 *src = (const u32x4 *)((const uint8_t *)g.ws + ((t0 / 16 + m) * p.nsets + s0) * R::BYTES);
-                u32x4 *dst = (u32x4 *)(lds + m * xs);
-                for (int i = tid; i < per; i += 64 * W) dst[i] = src[i];
+                const uint8_t *src = (const uint8_t *)g.ws + ((t0 / 16 + m) * p.nsets + s0) * R::BYTES;
+                for (int i = 64 * wave; i < per; i += 64 * W)   // 1 KB a wave, straight into LDS
+                    if (i + lane < per)
+                        __builtin_amdgcn_global_load_lds((const global_void_t *)(src + 16 * (i + lane)),
+                                                         (lds_void_t *)(lds + m * xs + 16 * i), 16, 0, 0);
             }
+            vm_drain();
         } else {
             // pieces of 8 values; a wave's 64 pieces are of one token
             constexpr int PS = R::VALUES / 8;      // pieces of a set: 16 or 32
@@ -431,7 +487,7 @@ __global__ void __launch_bounds__(64 * W, 4) k_mm(MmArgs g, MmPlan p) {
     }
 }
 
-// ---------------------------------------------------------------- up to 4 rows
+// ---------------------------------------------------------------- up to 8 rows
 // One lane per 32 values of a row of the matrix (Q4_0: a block; Q4_K: 16 bytes
 // of codes, 16 values of one sub-block and 16 of the next), 2^lg lanes per
 // row: a wave's loads are runs of whole rows.  The dots run on v_dot4_i32_i8.
@@ -500,19 +556,36 @@ __device__ __forceinline__ void mv_piece(const uint8_t *row, int p, bool vec, bo
     }
 }
 
+// sum over aligned groups of 2^lg lanes (8 .. 64)
+__device__ __forceinline__ float mv_sum(float v, int lg) {
+    v += dpp_f<0xB1>(v);
+    v += dpp_f<0x4E>(v);
+    v += dpp_f<0x141>(v);
+    if (lg > 3) v += dpp_f<0x140>(v);
+    if (lg > 4) {
+        uint32_t a = __builtin_bit_cast(uint32_t, v), b = a;
+        swap16(a, b);
+        v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    }
+    if (lg > 5) {
+        uint32_t a = __builtin_bit_cast(uint32_t, v), b = a;
+        swap32(a, b);
+        v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    }
+    return v;
+}
+
 template <int TYPE> struct MvRaw;
 template <> struct MvRaw<2> { u32x4 q; uint32_t d; };
 template <> struct MvRaw<12> { u32x4 h, q; };
 
-constexpr int MV_W = 4;
-
-template <int TYPE, int T, int R>
-__global__ void __launch_bounds__(64 * MV_W) k_mv(MmArgs g, MvPlan p) {
+template <int TYPE, int T, int R, int W>
+__global__ void __launch_bounds__(64 * W) k_mv(MmArgs g, MvPlan p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nl = 1 << p.lg, l = lane & (nl - 1), rw = 64 >> p.lg;   // lanes of a row, rows of a load
-    const int64_t step = (int64_t)gridDim.x * MV_W;
-    int64_t b = (int64_t)blockIdx.x * MV_W + wave, lb = b;
+    const int64_t step = (int64_t)gridDim.x * W;
+    int64_t b = (int64_t)blockIdx.x * W + wave, lb = b;
     int lch = 0;
     MvRaw<TYPE> nxt[R];
     // (clamped in the rows and in K: what lies past them is loaded again and dropped)
@@ -541,7 +614,7 @@ __global__ void __launch_bounds__(64 * MV_W) k_mv(MmArgs g, MvPlan p) {
     const int pieces = 4 * p.nu, pt = (pieces + 63) & ~63;
     const int xb = 40 * p.nu;   // a token's operands
     // pieces of 8 values; a wave's 64 pieces are of one token
-    for (int t = 0, i = tid; t < T; i += 64 * MV_W) {
+    for (int t = 0, i = tid; t < T; i += 64 * W) {
         while (i >= pt && t < T) {
             i -= pt;
             ++t;
@@ -625,48 +698,71 @@ __global__ void __launch_bounds__(64 * MV_W) k_mv(MmArgs g, MvPlan p) {
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                const float v = group_sum(acc[r][t], nl);
+                const float v = mv_sum(acc[r][t], p.lg);
                 const int64_t n = n0 + r * rw;
                 if (l == 0 && n < g.N) g.y[t * g.ldy + n] = v;
             }
     }
 }
 
-// lanes of a row: the most whose last round wastes at most an eighth of all
-static int mv_lg(int nu) {
-    for (int lg = 6; lg > 3; --lg)
-        if (8 * ((nu + (1 << lg) - 1) >> lg << lg) <= 9 * nu) return lg;
-    return 3;
+// Two work-groups of 8 waves a CU (one of 16): every work-group makes the
+// operands for itself, so few walk over many rows (65536 x 2048 Q4_K, one row:
+// 8 work-groups of 4 waves a CU 17.2 us, 2 of 8 16.4).
+constexpr int MV_WAVES = 4096;   // waves of the device at a time
+
+// log2 of the lanes of a row: the fewest rounds of loads, over the chunks of a
+// row and the batches of a wave; the most lanes (the longest runs of a load)
+// among equals
+static int mv_lg(int64_t nu, int64_t N, int R) {
+    int best = 6;
+    int64_t rounds = INT64_MAX;
+    for (int lg = 6; lg >= 3; --lg) {
+        const int64_t chunks = (nu + (1 << lg) - 1) >> lg, rows = R * (64 >> lg), batches = (N + rows - 1) / rows;
+        const int64_t c = chunks * ((batches + MV_WAVES - 1) / MV_WAVES);
+        if (c < rounds) rounds = c, best = lg;
+    }
+    return best;
 }
 
-template <int TYPE, int T, int R>
-static int mv_go(const MmArgs &g, MvPlan p, hipStream_t st) {
-    const int64_t rows = R * (64 >> p.lg);   // of a wave
-    p.batches = (g.N + rows - 1) / rows;
-    const int64_t most = (p.batches + MV_W - 1) / MV_W;
-    const dim3 grid((unsigned)(most < 2048 ? most : 2048)), block(64 * MV_W);
-    hipLaunchKernelGGL((k_mv<TYPE, T, R>), grid, block, (size_t)T * 40 * p.nu, st, g, p);
-    return hip_check_launch();
-}
-
-template <int TYPE, int T>
-static int mv_launch(const MmArgs &g, hipStream_t st) {
+template <int TYPE, int T, int R, int W>
+static int mv_go(const MmArgs &g, hipStream_t st) {
     MvPlan p = {};
     p.src = g.btype != 0 ? 2 : 1;
     p.vec = (uintptr_t)g.b % 16 == 0 && g.ldb % 16 == 0;
     p.nu = (int)(g.K / 32);
-    p.lg = mv_lg(p.nu);
+    p.lg = mv_lg(p.nu, g.N, R);
     p.chunks = (p.nu + (1 << p.lg) - 1) >> p.lg;
-    // four rows a lane where that leaves every SIMD four waves
-    return g.N >= 4 * 4096 * (64 >> p.lg) ? mv_go<TYPE, T, 4>(g, p, st) : mv_go<TYPE, T, 1>(g, p, st);
+    const int64_t rows = R * (64 >> p.lg);   // of a wave
+    p.batches = (g.N + rows - 1) / rows;
+    const int64_t most = (p.batches + W - 1) / W, cap = MV_WAVES / W;
+    const dim3 grid((unsigned)(most < cap ? most : cap)), block(64 * W);
+    hipLaunchKernelGGL((k_mv<TYPE, T, R, W>), grid, block, (size_t)T * 40 * p.nu, st, g, p);
+    return hip_check_launch();
 }
 
-constexpr int64_t MV_T = 4;   // rows of b
+// Many rows: several a lane, more loads in flight (registers allow 4 up to two
+// rows of b, 2 up to four).  Few: one, and work-groups of 16 waves, which share
+// the operands (8192 x 2048 Q4_0, one row: 4 waves 6.2 us, 16 4.4).
+template <int TYPE, int T>
+static int mv_launch(const MmArgs &g, hipStream_t st) {
+    return g.N >= 4 * MV_WAVES ? mv_go<TYPE, T, (T <= 2 ? 4 : T <= 4 ? 2 : 1), 8>(g, st) : mv_go<TYPE, T, 1, 16>(g, st);
+}
+
+// Up to 8 rows of b, while the dots are not what bounds it: the time of these
+// kernels grows with the rows of b, that of k_mm does not, but for its operands'
+// launch or their work in every work-group (8192 x 2048 Q4_0, 8 rows: 9.5 us
+// against 11.6; 65536 x 2048, 4 and 6 rows: Q4_0 25.6 and 36.8 against 31.2 and
+// 31.9, Q4_K 2 and 4 rows: 20.3 and 29.2 against 22.4 and 23.5).
 template <int TYPE>
-static bool mv_ok(const MmArgs &g) { return g.T <= MV_T && g.T * 40 * (g.K / 32) <= MM_LDS; }
+static bool mv_ok(const MmArgs &g) {
+    return g.T <= 8 && g.T * 40 * (g.K / 32) <= MM_LDS && g.T * g.N * g.K <= (int64_t)5 << (TYPE == 2 ? 27 : 26);
+}
 
 constexpr int64_t MM_PASS_T = 32768;   // rows of one pass (grid dimensions)
-constexpr int64_t MM_PREP_T = 8;   // fp32 rows from so many on: their records in a launch of their own
+// fp32 rows from so many on: their records in a launch of their own, else every
+// work-group makes them for itself (8192 x 2048 Q4_0: 5 rows 11.0 us, with the
+// launch 11.6; 13 rows 14.8 and 11.7)
+constexpr int64_t MM_PREP_T = 8;
 
 size_t mm_ws_bytes(int type, int btype, int64_t T, int64_t K) {
     if (btype != 0 || T < MM_PREP_T) return 0;
@@ -704,7 +800,11 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
         if (g.T == 1) return mv_launch<TYPE, 1>(g, st);
         if (g.T == 2) return mv_launch<TYPE, 2>(g, st);
         if (g.T == 3) return mv_launch<TYPE, 3>(g, st);
-        return mv_launch<TYPE, 4>(g, st);
+        if (g.T == 4) return mv_launch<TYPE, 4>(g, st);
+        if (g.T == 5) return mv_launch<TYPE, 5>(g, st);
+        if (g.T == 6) return mv_launch<TYPE, 6>(g, st);
+        if (g.T == 7) return mv_launch<TYPE, 7>(g, st);
+        return mv_launch<TYPE, 8>(g, st);
     }
     MmPlan p = {};
     p.nsets = (int)((g.K + R::VALUES - 1) / R::VALUES);
@@ -721,8 +821,10 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
     if (p.src != 0 && g.T <= 4) return mm_go<TYPE, 1, 1, 8>(g, p, st);
     if (p.src != 0 && g.T <= 8) return mm_go<TYPE, 1, 2, 8>(g, p, st);
     if (g.T <= 16) return mm_go<TYPE, 1, 4, 8>(g, p, st);
-    if (g.T <= 32) return mm_go<TYPE, 2, 4, 8>(g, p, st);
-    return mm_go<TYPE, 2, 4, 8>(g, p, st);
+    // 32 tokens of a work-group until 64 leave three waves for every two SIMDs (8192
+    // x 2048 Q4_K: 128 rows 17.9 us against 18.4 with 64, 200 rows 31.8 against 19.6)
+    if (g.T <= 32 || p.ntiles * ((g.T + 63) / 64) < 1536) return mm_go<TYPE, 2, 4, 8>(g, p, st);
+    return mm_go<TYPE, 4, 4, 8>(g, p, st);
 }
 
 int launch_mm(const MmArgs &g, hipStream_t st) {
