@@ -10,109 +10,238 @@
 // Values that are no numbers never win (NaN; experts of groups that are out and
 // lanes past E are NaN too); slots left take the lowest ids and the weight NaN.
 #include "common.hpp"
+#include "lanes.hpp"
 #include "launch.hpp"
 #include "wave_ops.hpp"
 
 namespace mimoe {
 
-// One wave per token, lane l holding the experts 64 i + l.
+// A float's place among all others as an integer; NaN (and what is out of the
+// race) below every number.  + 0: -0 is 0.
+constexpr int KEY_NONE = (int)0x80000000;
+__device__ __forceinline__ int key_of(float c) {
+    const int b = __builtin_bit_cast(int, c + 0.f);
+    return c == c ? b ^ ((b >> 31) & 0x7fffffff) : KEY_NONE;
+}
+__device__ __forceinline__ float value_of(int k) { return __builtin_bit_cast(float, k ^ ((k >> 31) & 0x7fffffff)); }
+
+// exp(x) for |x| <= 700 in fp64, off by a unit in the last place or so: n = rint(x
+// log2 e), the Taylor series of exp(x - n ln 2) to the 13th power (|.| <= ln 2 / 2:
+// the next term is below 2^-57), times 2^n
+__device__ __forceinline__ double exp_f64(double x) {
+    const double n = __builtin_rint(x * 1.4426950408889634074);
+    const double r = fma(-n, 1.90821492927058770002e-10, fma(-n, 6.93147180369123816490e-01, x));
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, r, 1.0 / 479001600.0);
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return __builtin_amdgcn_ldexp(p, (int)n);
+}
+// 1 / x, x from 1 to 2^1011: the hardware's estimate and two Newton steps
+__device__ __forceinline__ double rcp_f64(double x) {
+    double r = __builtin_amdgcn_rcp(x);
+    r = fma(fma(-x, r, 1.0), r, r);
+    return fma(fma(-x, r, 1.0), r, r);
+}
+// fl32(1 / (1 + exp(-x))): the argument is held to 700, past which the result
+// is 0 or 1 in 32 bits
+__device__ __forceinline__ float sigmoid_f32(float x) {
+    const float c = fminf(fmaxf(x, -700.f), 700.f);
+    return x == x ? (float)rcp_f64(1.0 + exp_f64(-(double)c)) : x;
+}
+// fl32(exp(x)), x <= 0 (or NaN)
+__device__ __forceinline__ float exp_f32(float x) {
+    return x == x ? (float)exp_f64((double)fmaxf(x, -700.f)) : x;
+}
+
+// the wave's largest, uniform
+__device__ __forceinline__ int wave_max_i(int m) {
+    int o = dpp_i<0xB1>(m);
+    m = o > m ? o : m;
+    o = dpp_i<0x4E>(m);
+    m = o > m ? o : m;
+    o = dpp_i<0x141>(m);
+    m = o > m ? o : m;
+    o = dpp_i<0x140>(m);
+    m = o > m ? o : m;
+    o = __builtin_amdgcn_update_dpp(m, m, 0x142, 0xA, 0xF, false);   // rows 0 -> 1, 2 -> 3
+    m = o > m ? o : m;
+    o = __builtin_amdgcn_update_dpp(m, m, 0x143, 0xC, 0xF, false);   // row 1 -> 2, 3
+    m = o > m ? o : m;
+    return __builtin_amdgcn_readlane(m, 63);
+}
+
+struct RoutePlan {
+    int gs;          // experts of a group
+    int magic;       // e / gs = e magic >> 20 for e < 1024
+    int ls;          // log2 of the lanes that find a group's value
+    int vec;         // rows of logits and bias in whole, aligned pieces of NPER
+};
+
+constexpr int RT_W = 4;   // waves (tokens) of a work-group
+
+// One wave per token, lane l holding the experts NPER l .. NPER l + NPER - 1 as
+// sortable integers; a group's value is found by 2^ls lanes from a copy in LDS
+// (groups of any size), the groups' places by counting, the experts by K rounds
+// of the wave's largest, each lane offering its best.
 template <int NPER>
-__global__ void __launch_bounds__(256) k_route(const float *__restrict__ logits, int64_t ldl, int64_t T, int E, int K,
-                                               RouterParams p, int32_t *__restrict__ sel, float *__restrict__ w) {
-    const int lane = threadIdx.x & 63;
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= T) return;   // whole waves
+__global__ void __launch_bounds__(64 * RT_W) k_route(const float *__restrict__ logits, int64_t ldl, int64_t T, int E, int K,
+                                                     RouterParams p, RoutePlan q, int32_t *__restrict__ sel, float *__restrict__ w) {
+    __shared__ float s_score[RT_W][64 * NPER];
+    __shared__ int s_key[RT_W][64 * NPER];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t t = (int64_t)blockIdx.x * RT_W + wave;
+    if (t >= T) return;   // whole waves, each on its own
     const float *l = logits + t * ldl;
-    const float NaN = __builtin_nanf("");
-    float s[NPER], c[NPER];
+    const int e0 = NPER * lane;
+    float s[NPER], bias[NPER];
+    typedef float fN __attribute__((ext_vector_type(NPER)));
 #pragma unroll
-    for (int i = 0; i < NPER; ++i) s[i] = lane + 64 * i < E ? l[lane + 64 * i] : -INFINITY;
+    for (int i = 0; i < NPER; ++i) s[i] = -INFINITY, bias[i] = 0.f;
+    if (q.vec) {
+        if (e0 < E) {
+            const fN v = *(const fN *)(l + e0);
+#pragma unroll
+            for (int i = 0; i < NPER; ++i) s[i] = v[i];
+            if (p.sel_bias) {
+                const fN b = *(const fN *)(p.sel_bias + e0);
+#pragma unroll
+                for (int i = 0; i < NPER; ++i) bias[i] = b[i];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NPER; ++i)
+            if (e0 + i < E) {
+                s[i] = l[e0 + i];
+                if (p.sel_bias) bias[i] = p.sel_bias[e0 + i];
+            }
+    }
     if (p.score == 1) {
 #pragma unroll
-        for (int i = 0; i < NPER; ++i) s[i] = gating_sigmoid(s[i]);
+        for (int i = 0; i < NPER; ++i) s[i] = sigmoid_f32(s[i]);
     } else {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < NPER; ++i) mx = fmaxf(mx, s[i]);
-        mx = wave_max(mx);
+        mx = wave_max_uniform(mx);
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < NPER; ++i) {
-            s[i] = lane + 64 * i < E ? (float)exp((double)(s[i] - mx)) : 0.f;
+            s[i] = e0 + i < E ? exp_f32(s[i] - mx) : 0.f;
             sum += (double)s[i];
         }
-        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        sum = wave_sum_d(sum);
         const float inv = (float)(1.0 / sum);
 #pragma unroll
         for (int i = 0; i < NPER; ++i) s[i] = s[i] * inv;
     }
+    int k[NPER];
 #pragma unroll
     for (int i = 0; i < NPER; ++i) {
-        const int e = lane + 64 * i;
-        c[i] = e >= E ? NaN : p.sel_bias ? s[i] + p.sel_bias[e] : s[i];
+        s_score[wave][e0 + i] = s[i];
+        k[i] = e0 + i >= E ? KEY_NONE : key_of(p.sel_bias ? s[i] + bias[i] : s[i]);
     }
     if (p.n_group > 1) {
-        const int gs = E / p.n_group;
-        float val = NaN;   // lane g: group g's value
-        for (int g = 0; g < p.n_group; ++g) {
-            // the two largest numbers of the group (NaN: none)
-            float a = NaN, b = NaN;
 #pragma unroll
-            for (int i = 0; i < NPER; ++i) {
-                const int e = lane + 64 * i;
-                const float v = e >= g * gs && e < (g + 1) * gs ? c[i] : NaN;
-                b = fmaxf(b, fminf(a, v) == fminf(a, v) && a == a && v == v ? fminf(a, v) : NaN);
-                a = fmaxf(a, v);
+        for (int i = 0; i < NPER; ++i) s_key[wave][e0 + i] = k[i];
+        wave_lds_sync();
+        // the group's two largest, over its 2^ls lanes
+        const int S = 1 << q.ls, g = lane >> q.ls;
+        int a = KEY_NONE, b = KEY_NONE;
+        if (g < p.n_group) {
+            const int *gk = &s_key[wave][g * q.gs];
+            for (int i = lane & (S - 1); i < q.gs; i += S) {
+                const int v = gk[i], lo = v < a ? v : a;
+                b = lo > b ? lo : b;
+                a = v > a ? v : a;
             }
-            for (int o = 32; o > 0; o >>= 1) {
-                const float a2 = __shfl_xor(a, o, 64), b2 = __shfl_xor(b, o, 64);
-                const float lo = a == a && a2 == a2 ? fminf(a, a2) : NaN;
-                b = fmaxf(fmaxf(b, b2), lo);
-                a = fmaxf(a, a2);
-            }
-            const float v = p.group_top == 1 ? a : a == a ? (b == b ? a + b : -INFINITY) : NaN;
-            if (lane == g) val = v;
         }
-        // the best n_kept groups (no numbers: behind, lowest first)
-        unsigned long long kept = 0;
-        for (int r = 0; r < p.n_kept; ++r) {
-            const float m = wave_max_uniform(val);
-            unsigned long long b = __ballot(val == m && !(kept >> lane & 1));
-            if (b == 0) b = __ballot(lane < p.n_group && !(kept >> lane & 1));
-            const int g = (int)__builtin_ctzll(b);
-            kept |= 1ull << g;
-            if (lane == g) val = NaN;
+        for (int o = 1; o < S; o <<= 1) {
+            int a2, b2;
+            if (o == 1) a2 = dpp_i<0xB1>(a), b2 = dpp_i<0xB1>(b);
+            else if (o == 2) a2 = dpp_i<0x4E>(a), b2 = dpp_i<0x4E>(b);
+            else if (o == 4) a2 = dpp_i<0x141>(a), b2 = dpp_i<0x141>(b);
+            else if (o == 8) a2 = dpp_i<0x140>(a), b2 = dpp_i<0x140>(b);
+            else a2 = __shfl_xor(a, o, 64), b2 = __shfl_xor(b, o, 64);
+            const int lo = a < a2 ? a : a2;
+            b = b > b2 ? b : b2;
+            b = lo > b ? lo : b;
+            a = a > a2 ? a : a2;
         }
+        const int val = p.group_top == 1 || a == KEY_NONE ? a
+                        : key_of(b == KEY_NONE ? -INFINITY : value_of(a) + value_of(b));
+        // a group's place: those before it
+        int before = 0;
+        for (int o = 0; o < p.n_group; ++o) {
+            const int v = __builtin_amdgcn_readlane(val, o << q.ls);
+            before += v > val || (v == val && o < g) ? 1 : 0;
+        }
+        const unsigned long long kept = __ballot(g < p.n_group && before < p.n_kept);
 #pragma unroll
-        for (int i = 0; i < NPER; ++i)
-            if (lane + 64 * i < E && !(kept >> ((lane + 64 * i) / gs) & 1)) c[i] = NaN;
+        for (int i = 0; i < NPER; ++i) {
+            const int ge = ((e0 + i) * q.magic) >> 20;
+            if (!((kept >> ((ge << q.ls) & 63)) & 1)) k[i] = KEY_NONE;
+        }
+    }
+    // each lane's experts, best first (neighbours change places only for a larger
+    // one: equal ones stay in order)
+    int id[NPER];
+#pragma unroll
+    for (int i = 0; i < NPER; ++i) id[i] = e0 + i;
+    if constexpr (NPER <= 4) {
+#pragma unroll
+        for (int n = NPER - 1; n > 0; --n)
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const bool sw = k[i + 1] > k[i];
+                const int kh = sw ? k[i + 1] : k[i], kl = sw ? k[i] : k[i + 1];
+                const int ih = sw ? id[i + 1] : id[i], il = sw ? id[i] : id[i + 1];
+                k[i] = kh; k[i + 1] = kl;
+                id[i] = ih; id[i + 1] = il;
+            }
     }
     int mysel = -1;
-    float mys = NaN;   // lane k: the k-th expert's score
     for (int r = 0; r < K; ++r) {
-        float m = c[0];
+        int best = k[0], bid = id[0];
+        if constexpr (NPER > 4) {
 #pragma unroll
-        for (int i = 1; i < NPER; ++i) m = fmaxf(m, c[i]);
-        m = wave_max_uniform(m);
-        int e = -1;
-#pragma unroll
-        for (int i = 0; i < NPER; ++i) {
-            const unsigned long long b = __ballot(c[i] == m);
-            if (e < 0 && b != 0ull) e = 64 * i + (int)__builtin_ctzll(b);
+            for (int i = 1; i < NPER; ++i) {
+                const bool up = k[i] > best;
+                best = up ? k[i] : best;
+                bid = up ? id[i] : bid;
+            }
         }
-        if (e < 0) break;   // (uniform) no number left
-        float sv = 0.f;
+        const int m = wave_max_i(best);
+        if (m == KEY_NONE) break;   // (uniform) no number left
+        const int win = (int)__builtin_ctzll(__ballot(best == m));   // lanes hold ascending ids
+        const int e = __builtin_amdgcn_readlane(bid, win);
+        mysel = lane == r ? e : mysel;
+        if constexpr (NPER <= 4) {
+            const bool mine = lane == win;
 #pragma unroll
-        for (int i = 0; i < NPER; ++i) {
-            if (e == 64 * i + lane) c[i] = NaN;
-            const float x = lane_f(s[i], e & 63);
-            if (i == (e >> 6)) sv = x;
-        }
-        if (lane == r) {
-            mysel = e;
-            mys = sv;
+            for (int i = 0; i + 1 < NPER; ++i) {
+                k[i] = mine ? k[i + 1] : k[i];
+                id[i] = mine ? id[i + 1] : id[i];
+            }
+            k[NPER - 1] = mine ? KEY_NONE : k[NPER - 1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < NPER; ++i) k[i] = id[i] == e ? KEY_NONE : k[i];
         }
     }
+    wave_lds_sync();
+    float v = lane < K ? (mysel < 0 ? __builtin_nanf("") : s_score[wave][mysel]) : 0.f;
     const unsigned long long none = __ballot(lane < K && mysel < 0);
     if (none) {
         for (int r = (int)__builtin_ctzll(none); r < K; ++r) {
@@ -121,10 +250,9 @@ __global__ void __launch_bounds__(256) k_route(const float *__restrict__ logits,
             if (lane == r) mysel = e;
         }
     }
-    float v = lane < K ? mys : 0.f;
     if (p.renorm) {
         double sum = 0.0;
-        for (int k = 0; k < K; ++k) sum = sum + (double)lane_f(v, k);
+        for (int j = 0; j < K; ++j) sum = sum + (double)lane_f(v, j);
         v = v / ((float)sum + p.eps);
     }
     v = v * p.scaling;
@@ -140,13 +268,21 @@ int launch_route(const float *logits, int64_t ldl, int64_t T, int E, int K, cons
     if (T <= 0) return 0;
     if (E <= 0 || E > ROUTER_MAX_E || K <= 0 || K > ROUTER_MAX_K || K > E) return -6;
     if (p.n_group < 1 || p.n_group > ROUTER_MAX_GROUPS || E % p.n_group || p.n_kept < 1 || p.n_kept > p.n_group) return -6;
-    if ((T + 3) / 4 > 0x7fffffff) return -6;
-    const dim3 grid((unsigned)((T + 3) / 4)), block(256);
-#define ROUTE(N) hipLaunchKernelGGL(k_route<N>, grid, block, 0, st, logits, ldl, T, E, K, p, sel, w)
-    if (E <= 64) ROUTE(1);
-    else if (E <= 128) ROUTE(2);
-    else if (E <= 256) ROUTE(4);
-    else if (E <= 512) ROUTE(8);
+    if ((T + RT_W - 1) / RT_W > 0x7fffffff) return -6;
+    const int nper = E <= 64 ? 1 : E <= 128 ? 2 : E <= 256 ? 4 : E <= 512 ? 8 : 16;
+    RoutePlan q;
+    q.gs = E / p.n_group;
+    q.magic = ((1 << 20) + q.gs - 1) / q.gs;   // e (magic gs - 2^20) < 1024 * 512 < 2^20: exact
+    q.ls = 0;
+    while (p.n_group << (q.ls + 1) <= 64) ++q.ls;
+    const uintptr_t unit = 4 * (uintptr_t)nper;
+    q.vec = E % nper == 0 && (uintptr_t)logits % unit == 0 && (uintptr_t)(ldl * 4) % unit == 0 && (uintptr_t)p.sel_bias % unit == 0;
+    const dim3 grid((unsigned)((T + RT_W - 1) / RT_W)), block(64 * RT_W);
+#define ROUTE(N) hipLaunchKernelGGL(k_route<N>, grid, block, 0, st, logits, ldl, T, E, K, p, q, sel, w)
+    if (nper == 1) ROUTE(1);
+    else if (nper == 2) ROUTE(2);
+    else if (nper == 4) ROUTE(4);
+    else if (nper == 8) ROUTE(8);
     else ROUTE(16);
 #undef ROUTE
     return hip_check_launch();
