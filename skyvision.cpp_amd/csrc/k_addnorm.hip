@@ -31,10 +31,16 @@ __device__ __forceinline__ void an_store_q8_0(const float (&v)[4], uint8_t *row,
     const bool bad = m >= 0x7f800000u;
     const float d = __builtin_bit_cast(float, m) / 127.0f;
     const float id = d != 0.0f ? 1.0f / d : 0.0f;
-    const uint32_t dh = bad ? 0x7e00u : f32_to_fp16_bits(d);
-    uint32_t c = 0u;
+    const uint32_t dh = bad ? 0x7e00u : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)d);
+    // roundf(t): t + the number before 1/2 with t's sign, cut (|t| <= 127.5: the
+    // sum of a fraction of 1/2 or more rounds to the next integer, of less stays below)
+    uint32_t q[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c |= ((uint32_t)(int)roundf(v[j] * id) & 0xffu) << (8 * j);
+    for (int j = 0; j < 4; ++j) {
+        const float t = v[j] * id;
+        q[j] = (uint32_t)(int)(t + __builtin_copysignf(0.49999997f, t));
+    }
+    uint32_t c = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[3], q[2], 0x0C0C0400u), __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0400u), 0x05040100u);
     if (bad) c = 0u;
     // words (D % 64 == 0): a pair of blocks is 17 aligned words; words 0 .. 8 hold the even block's scale
     // and codes and the odd one's scale (the codes half a word off), the rest the
@@ -203,12 +209,14 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) k_add_norm(AddNormArgs 
 template <bool VEC>
 static int an_launch(const AddNormArgs &a, int64_t T, int D, hipStream_t st) {
 #define AN(W, P) hipLaunchKernelGGL((k_add_norm<W, P, VEC>), dim3((unsigned)(W == 1 ? (T + 3) / 4 : T)), dim3(W == 1 ? 256 : 64 * W), 0, st, a, T, D)
-    // a wave per row (no barrier) where that fills the device, else the row over
-    // the waves of a work-group
-    if (T >= 1024 && D <= 4096) {
+    // the row over the waves of a work-group (more waves than it needs to hold the
+    // row: one row of 2048, 8 waves 2.65 us, 4 2.9); a wave per row, without barriers,
+    // for thousands of rows that leave as fp32 (4096 rows of 2048: 20.0 us against
+    // 23.0; with codes, whose arithmetic then sits in one wave, 33.3 against 32.0, and
+    // 1024 rows 8.3 against 6.6)
+    if (T >= 2048 && D <= 2048 && !a.q) {
         if (D <= 1024) AN(1, 4);
-        else if (D <= 2048) AN(1, 8);
-        else AN(1, 16);
+        else AN(1, 8);
     } else if (D <= 2048) AN(8, 1);
     else if (D <= 4096) AN(16, 1);
     else if (D <= 8192) AN(16, 2);

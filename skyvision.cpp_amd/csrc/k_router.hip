@@ -53,16 +53,15 @@ __device__ __forceinline__ double rcp_f64(double x) {
     r = fma(fma(-x, r, 1.0), r, r);
     return fma(fma(-x, r, 1.0), r, r);
 }
-// fl32(1 / (1 + exp(-x))): the argument is held to 700, past which the result
-// is 0 or 1 in 32 bits
-__device__ __forceinline__ float sigmoid_f32(float x) {
-    const float c = fminf(fmaxf(x, -700.f), 700.f);
-    return x == x ? (float)rcp_f64(1.0 + exp_f64(-(double)c)) : x;
+// x held to +-700, NaN kept
+__device__ __forceinline__ double held700(float x) {
+    x = x < -700.f ? -700.f : x;
+    return (double)(x > 700.f ? 700.f : x);
 }
+// fl32(1 / (1 + exp(-x))); past +-700 the result is 0 or 1 in 32 bits
+__device__ __forceinline__ float sigmoid_f32(float x) { return (float)rcp_f64(1.0 + exp_f64(-held700(x))); }
 // fl32(exp(x)), x <= 0 (or NaN)
-__device__ __forceinline__ float exp_f32(float x) {
-    return x == x ? (float)exp_f64((double)fmaxf(x, -700.f)) : x;
-}
+__device__ __forceinline__ float exp_f32(float x) { return (float)exp_f64(held700(x)); }
 
 // the wave's largest, uniform
 __device__ __forceinline__ int wave_max_i(int m) {
@@ -195,11 +194,13 @@ __global__ void __launch_bounds__(64 * RT_W) k_route(const float *__restrict__ l
         }
     }
     // each lane's experts, best first (neighbours change places only for a larger
-    // one: equal ones stay in order)
-    int id[NPER];
-#pragma unroll
-    for (int i = 0; i < NPER; ++i) id[i] = e0 + i;
+    // one: equal ones stay in order); up to four: their numbers in the lane as the
+    // bytes of a word
+    uint32_t ord = 0;
     if constexpr (NPER <= 4) {
+        int id[NPER];
+#pragma unroll
+        for (int i = 0; i < NPER; ++i) id[i] = i;
 #pragma unroll
         for (int n = NPER - 1; n > 0; --n)
 #pragma unroll
@@ -210,16 +211,20 @@ __global__ void __launch_bounds__(64 * RT_W) k_route(const float *__restrict__ l
                 k[i] = kh; k[i + 1] = kl;
                 id[i] = ih; id[i + 1] = il;
             }
+#pragma unroll
+        for (int i = 0; i < NPER; ++i) ord |= (uint32_t)id[i] << (8 * i);
     }
     int mysel = -1;
     for (int r = 0; r < K; ++r) {
-        int best = k[0], bid = id[0];
-        if constexpr (NPER > 4) {
+        int best = k[0], bid = e0;
+        if constexpr (NPER <= 4) {
+            bid = e0 + (int)(ord & 0xffu);
+        } else {
 #pragma unroll
             for (int i = 1; i < NPER; ++i) {
                 const bool up = k[i] > best;
                 best = up ? k[i] : best;
-                bid = up ? id[i] : bid;
+                bid = up ? e0 + i : bid;
             }
         }
         const int m = wave_max_i(best);
@@ -229,15 +234,13 @@ __global__ void __launch_bounds__(64 * RT_W) k_route(const float *__restrict__ l
         mysel = lane == r ? e : mysel;
         if constexpr (NPER <= 4) {
             const bool mine = lane == win;
+            ord = mine ? ord >> 8 : ord;
 #pragma unroll
-            for (int i = 0; i + 1 < NPER; ++i) {
-                k[i] = mine ? k[i + 1] : k[i];
-                id[i] = mine ? id[i + 1] : id[i];
-            }
+            for (int i = 0; i + 1 < NPER; ++i) k[i] = mine ? k[i + 1] : k[i];
             k[NPER - 1] = mine ? KEY_NONE : k[NPER - 1];
         } else {
 #pragma unroll
-            for (int i = 0; i < NPER; ++i) k[i] = id[i] == e ? KEY_NONE : k[i];
+            for (int i = 0; i < NPER; ++i) k[i] = e0 + i == e ? KEY_NONE : k[i];
         }
     }
     wave_lds_sync();
