@@ -10,6 +10,8 @@
 // bytes; the tokens' operands lie in LDS in the lanes' order (MM records) for
 // the whole K, written once per work-group, which then walks over row tiles:
 // the matrix is read once and nothing else is.
+#include <type_traits>
+
 #include "b32.hpp"
 #include "common.hpp"
 #include "lanes.hpp"
@@ -103,68 +105,75 @@ __device__ __forceinline__ void mm_codes_q8_K(const float (&v)[8], uint2 &c, flo
     c = mm_bytes8(q);
 }
 
-// piece p (8 values of token row m of the tile) of the tile's operands into its
-// record at o: Q4_0: block p / 4, quarter p % 4; Q4_K: values 8 p ..  The lanes
-// that share a block's largest value (4 or 32, aligned) call it together.
-// SRC 1: row of fp32 values; 2: of 8-bit blocks.  live: the piece is in the row.
-template <int TYPE, int SRC>
-__device__ __forceinline__ void mm_piece(const uint8_t *row, int p, int m, bool vec, bool live, uint8_t *o) {
-    if constexpr (TYPE == 2) {
-        const int blk = p >> 2, g = p & 3;
-        uint2 c = make_uint2(0u, 0u);
-        float d = 0.f;
-        if constexpr (SRC == 1) {
-            float v[8];
-            const float *x = (const float *)row + 32 * blk + 4 * g;
-            if (live) {
-                if (vec) {
-                    const float4 a = *(const float4 *)x, b = *(const float4 *)(x + 16);
-                    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-                } else {
+// A piece: 8 of a row's values, as they are read (SRC 1: fp32; 2: codes and the
+// scale of an 8-bit block, NaN where it is not finite).  fetch only loads, so
+// several go out before the first is used.  Zeros where the piece is not live.
+template <int SRC> struct MmPiece;
+template <> struct MmPiece<1> {
+    float v[8];
+    // values at x, the second four gap values behind the first
+    __device__ __forceinline__ void fetch(const float *x, int gap, bool vec, bool live) {
+        if (live && vec) {
+            const float4 a = *(const float4 *)x, b = *(const float4 *)(x + gap);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = x[(j & 3) + 16 * (j >> 2)];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = 0.f;
-            }
-            mm_codes_q8_0(v, c, d);
-        } else if (live) {
-            const uint8_t *b = row + 34 * blk;
-            c.x = *(const u32_a2 *)(b + 2 + 4 * g);
-            c.y = *(const u32_a2 *)(b + 18 + 4 * g);
-            d = h2f(*(const uint16_t *)b);
-            if (!(fabsf(d) <= 65504.f)) d = __builtin_nanf("");
+            for (int j = 0; j < 8; ++j) v[j] = live ? x[(j & 3) + (j >> 2) * gap] : 0.f;
         }
-        const int j = blk & 3;
+    }
+};
+template <> struct MmPiece<2> {
+    uint2 c;
+    float d;
+};
+// order of a piece in its block: Q4_0 operands of k_mm take values 4 g .. 4 g + 3
+// and 16 + 4 g .. (g = p % 4: what the nibbles of a dword of the table hold), all
+// others 8 in a row
+template <int TYPE, int SRC, bool SPLIT>
+__device__ __forceinline__ void mm_fetch(MmPiece<SRC> &r, const uint8_t *row, int p, bool vec, bool live) {
+    if constexpr (SRC == 1) {
+        if constexpr (SPLIT) r.fetch((const float *)row + 32 * (p >> 2) + 4 * (p & 3), 16, vec, live);
+        else r.fetch((const float *)row + 8 * (int64_t)p, 4, vec, live);
+    } else {
+        r.c = make_uint2(0u, 0u);
+        r.d = 0.f;
+        if (!live) return;
+        if constexpr (TYPE == 2) {
+            const uint8_t *b = row + 34 * (int64_t)(p >> 2);
+            const int o = SPLIT ? 4 * (p & 3) : 8 * (p & 3);
+            r.c = make_uint2(*(const u32_a2 *)(b + 2 + o), *(const u32_a2 *)(b + 2 + o + (SPLIT ? 16 : 4)));
+            r.d = h2f(*(const uint16_t *)b);
+        } else {
+            const uint8_t *b = row + 292 * (int64_t)(p >> 5) + 4;
+            r.c = make_uint2(*(const uint32_t *)(b + 8 * (p & 31)), *(const uint32_t *)(b + 8 * (p & 31) + 4));
+            r.d = *(const float *)(b - 4);
+        }
+    }
+}
+// its codes and scale; the lanes that share a block (4 or 32, aligned) call it together
+template <int TYPE, int SRC>
+__device__ __forceinline__ void mm_codes(const MmPiece<SRC> &r, uint2 &c, float &d) {
+    if constexpr (SRC == 1) {
+        if constexpr (TYPE == 2) mm_codes_q8_0(r.v, c, d);
+        else mm_codes_q8_K(r.v, c, d);
+    } else {
+        c = r.c;
+        d = fabsf(r.d) <= 3.402823466e38f ? r.d : __builtin_nanf("");   // (an fp16 infinity is one here)
+    }
+}
+
+// piece p of token row m of a tile into the tile's record at o
+template <int TYPE, int SRC>
+__device__ __forceinline__ void mm_put(const MmPiece<SRC> &r, int p, int m, uint8_t *o) {
+    uint2 c;
+    float d;
+    mm_codes<TYPE, SRC>(r, c, d);
+    if constexpr (TYPE == 2) {
+        const int j = (p >> 2) & 3, g = p & 3;
         *(uint2 *)(o + 16 * (64 * (j >> 1) + 16 * g + m) + 8 * (j & 1)) = c;
         if (g == 0) *(float *)(o + 2048 + 64 * j + 4 * m) = d * 0.0625f;
     } else {
         const int e = p & 31, j = e >> 2, g = e & 3;   // sub-block and quarter
-        uint2 c = make_uint2(0u, 0u);
-        float d = 0.f;
-        if constexpr (SRC == 1) {
-            float v[8];
-            const float *x = (const float *)row + 8 * p;
-            if (live) {
-                if (vec) {
-                    const float4 a = *(const float4 *)x, b = *(const float4 *)(x + 4);
-                    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = x[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = 0.f;
-            }
-            mm_codes_q8_K(v, c, d);
-        } else if (live) {
-            const uint8_t *b = row + 292 * (p >> 5);
-            c = make_uint2(*(const uint32_t *)(b + 4 + 8 * e), *(const uint32_t *)(b + 8 + 8 * e));
-            d = *(const float *)b;
-            if (!(fabsf(d) <= 3.402823466e38f)) d = __builtin_nanf("");
-        }
         *(uint2 *)(o + 16 * (64 * (j >> 1) + 16 * g + m) + 8 * (j & 1)) = c;
         int s = __builtin_amdgcn_sdot4(0x01010101, (int)c.x, __builtin_amdgcn_sdot4(0x01010101, (int)c.y, 0, false), false);
         s += dpp_i<0xB1>(s);
@@ -181,7 +190,9 @@ __global__ void __launch_bounds__(256) k_mm_rows(const uint8_t *b, int64_t ldb, 
     const int64_t t = blockIdx.y;
     const int p = blockIdx.x * 256 + threadIdx.x, set = p / (R::VALUES / 8);
     if (set >= nsets) return;   // whole sets of lanes
-    mm_piece<TYPE, 1>(b + t * ldb, p, (int)(t & 15), vec, 8 * p < K, ws + ((t >> 4) * nsets + set) * R::BYTES);
+    MmPiece<1> r;
+    mm_fetch<TYPE, 1, TYPE == 2>(r, b + t * ldb, p, vec, 8 * (int64_t)p < K);
+    mm_put<TYPE, 1>(r, p, (int)(t & 15), ws + ((t >> 4) * nsets + set) * R::BYTES);
 }
 
 struct MmPlan {
@@ -374,23 +385,36 @@ __global__ void __launch_bounds__(64 * W) k_mm(MmArgs g, MmPlan p) {
             }
             vm_drain();
         } else {
-            // pieces of 8 values; a wave's 64 pieces are of one token
             constexpr int PS = R::VALUES / 8;      // pieces of a set: 16 or 32
-            const int pt = (ns * PS + 63) & ~63;   // of a token, rounded up to whole waves
-            for (int t = 0, i = tid; t < nt; i += 64 * W) {
-                while (i >= pt && t < nt) {
-                    i -= pt;
-                    ++t;
+            const int pt = (ns * PS + 63) & ~63;   // of a token, rounded up to whole waves: a wave's 64 are of one token
+            auto make = [&](auto src) __attribute__((always_inline)) {
+                constexpr int SRC = decltype(src)::value, NB = 4;   // NB pieces' loads go out together
+                int t = 0, i = tid;
+                while (t < nt) {
+                    MmPiece<SRC> r[NB];
+                    int tt[NB], ii[NB];
+#pragma unroll
+                    for (int n = 0; n < NB; ++n, i += 64 * W) {
+                        while (i >= pt && t < nt) {
+                            i -= pt;
+                            ++t;
+                        }
+                        tt[n] = i < ns * PS ? t : nt;   // (else past the row's sets: whole groups of lanes that share a block)
+                        ii[n] = i;
+                        if (tt[n] < nt)
+                            mm_fetch<TYPE, SRC, TYPE == 2>(r[n], (const uint8_t *)g.b + (t0 + t) * g.ldb, s0 * PS + i, p.vec,
+                                                           8 * (int64_t)(s0 * PS + i) < g.K);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        if (tt[n] >= nt) continue;
+                        const int m = NI == 4 ? tt[n] & 15 : 4 * (tt[n] / NI) + tt[n] % NI;
+                        mm_put<TYPE, SRC>(r[n], ii[n], m, lds + (NI == 4 ? tt[n] >> 4 : 0) * xs + ii[n] / PS * R::BYTES);
+                    }
                 }
-                if (t >= nt) break;
-                const int set = i / PS, pc = s0 * PS + i;
-                if (set >= ns) continue;   // (whole groups of lanes that share a block)
-                const uint8_t *row = (const uint8_t *)g.b + (t0 + t) * g.ldb;
-                const int m = NI == 4 ? t & 15 : 4 * (t / NI) + t % NI;
-                uint8_t *o = lds + (NI == 4 ? t >> 4 : 0) * xs + set * R::BYTES;
-                if (p.src == 1) mm_piece<TYPE, 1>(row, pc, m, p.vec, 8 * pc < g.K, o);
-                else mm_piece<TYPE, 2>(row, pc, m, false, 8 * pc < g.K, o);
-            }
+            };
+            if (p.src == 1) make(std::integral_constant<int, 1>{});
+            else make(std::integral_constant<int, 2>{});
         }
     };
 
@@ -502,41 +526,12 @@ struct MvPlan {
     int64_t batches;   // of R * 64 / lanes rows
 };
 
+// piece p of a token's row into its operands
 template <int TYPE, int SRC>
-__device__ __forceinline__ void mv_piece(const uint8_t *row, int p, bool vec, bool live, uint8_t *lo, uint8_t *hi, uint2 *sc) {
-    uint2 c = make_uint2(0u, 0u);
-    float d = 0.f;
-    if constexpr (SRC == 1) {
-        float v[8];
-        const float *x = (const float *)row + 8 * p;
-        if (live) {
-            if (vec) {
-                const float4 a = *(const float4 *)x, b = *(const float4 *)(x + 4);
-                v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = x[i];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        }
-        if constexpr (TYPE == 2) mm_codes_q8_0(v, c, d);
-        else mm_codes_q8_K(v, c, d);
-    } else if (live) {
-        if constexpr (TYPE == 2) {
-            const uint8_t *b = row + 34 * (p >> 2);
-            c.x = *(const u32_a2 *)(b + 2 + 8 * (p & 3));
-            c.y = *(const u32_a2 *)(b + 6 + 8 * (p & 3));
-            d = h2f(*(const uint16_t *)b);
-            if (!(fabsf(d) <= 65504.f)) d = __builtin_nanf("");
-        } else {
-            const uint8_t *b = row + 292 * (p >> 5);
-            c = make_uint2(*(const uint32_t *)(b + 4 + 8 * (p & 31)), *(const uint32_t *)(b + 8 + 8 * (p & 31)));
-            d = *(const float *)b;
-            if (!(fabsf(d) <= 3.402823466e38f)) d = __builtin_nanf("");
-        }
-    }
+__device__ __forceinline__ void mv_put(const MmPiece<SRC> &r, int p, bool live, uint8_t *lo, uint8_t *hi, uint2 *sc) {
+    uint2 c;
+    float d;
+    mm_codes<TYPE, SRC>(r, c, d);
     int s = __builtin_amdgcn_sdot4(0x01010101, (int)c.x, __builtin_amdgcn_sdot4(0x01010101, (int)c.y, 0, false), false);
     s += dpp_i<0xB1>(s);
     if constexpr (TYPE == 2) {
@@ -613,18 +608,32 @@ __global__ void __launch_bounds__(64 * W) k_mv(MmArgs g, MvPlan p) {
     load();
     const int pieces = 4 * p.nu, pt = (pieces + 63) & ~63;
     const int xb = 40 * p.nu;   // a token's operands
-    // pieces of 8 values; a wave's 64 pieces are of one token
-    for (int t = 0, i = tid; t < T; i += 64 * W) {
-        while (i >= pt && t < T) {
-            i -= pt;
-            ++t;
+    auto make = [&](auto src) __attribute__((always_inline)) {
+        constexpr int SRC = decltype(src)::value, NB = T > 2 ? 2 : 1;   // NB pieces' loads go out together
+        int t = 0, i = tid;
+        while (t < T) {
+            MmPiece<SRC> r[NB];
+            int tt[NB], ii[NB];
+#pragma unroll
+            for (int n = 0; n < NB; ++n, i += 64 * W) {
+                while (i >= pt && t < T) {
+                    i -= pt;
+                    ++t;
+                }
+                tt[n] = t;
+                ii[n] = i;
+                if (t < T) mm_fetch<TYPE, SRC, false>(r[n], (const uint8_t *)g.b + t * g.ldb, i, p.vec, i < pieces);
+            }
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                if (tt[n] >= T) continue;   // (whole waves: a wave's 64 pieces are of one token)
+                uint8_t *o = lds + tt[n] * xb;
+                mv_put<TYPE, SRC>(r[n], ii[n], ii[n] < pieces, o, o + 16 * p.nu, (uint2 *)(o + 32 * p.nu));
+            }
         }
-        if (t >= T) break;
-        const uint8_t *row = (const uint8_t *)g.b + t * g.ldb;
-        uint8_t *o = lds + t * xb;
-        if (p.src == 1) mv_piece<TYPE, 1>(row, i, p.vec, i < pieces, o, o + 16 * p.nu, (uint2 *)(o + 32 * p.nu));
-        else mv_piece<TYPE, 2>(row, i, false, i < pieces, o, o + 16 * p.nu, (uint2 *)(o + 32 * p.nu));
-    }
+    };
+    if (p.src == 1) make(std::integral_constant<int, 1>{});
+    else make(std::integral_constant<int, 2>{});
     __syncthreads();
     for (; b < p.batches; b += step) {
         float acc[R][T];
@@ -760,8 +769,8 @@ static bool mv_ok(const MmArgs &g) {
 
 constexpr int64_t MM_PASS_T = 32768;   // rows of one pass (grid dimensions)
 // fp32 rows from so many on: their records in a launch of their own, else every
-// work-group makes them for itself (8192 x 2048 Q4_0: 5 rows 11.0 us, with the
-// launch 11.6; 13 rows 14.8 and 11.7)
+// work-group makes them for itself (2048 x 2048 and 8192 x 2048 Q4_0: 13 rows 12.0
+// and 12.2 us, with the launch 8.5 and 11.8)
 constexpr int64_t MM_PREP_T = 8;
 
 size_t mm_ws_bytes(int type, int btype, int64_t T, int64_t K) {
@@ -784,7 +793,7 @@ static int mm_go(const MmArgs &g, MmPlan p, hipStream_t st) {
     p.cs = (p.cs + MM_U<TYPE> - 1) / MM_U<TYPE> * MM_U<TYPE>;
     p.chunks = (p.nsets + p.cs - 1) / p.cs;
     const int lds = MT * p.cs * R::BYTES + red;
-    const int per_cu = imin(2, imax(1, MM_LDS / lds));
+    const int per_cu = imin(16 / W, imax(1, MM_LDS / lds));
     const int wn = W / p.wk;
     const int64_t want = (256 * per_cu + slices - 1) / slices;   // work-groups of a slice
     const int64_t most = (p.ntiles + wn - 1) / wn;
@@ -818,8 +827,9 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
         if (rc) return rc;
         p.src = 0;
     }
-    if (p.src != 0 && g.T <= 4) return mm_go<TYPE, 1, 1, 8>(g, p, st);
-    if (p.src != 0 && g.T <= 8) return mm_go<TYPE, 1, 2, 8>(g, p, st);
+    if (p.src != 0 && g.T <= 4) return mm_go<TYPE, 1, 1, 16>(g, p, st);
+    if (p.src != 0 && g.T <= 8) return mm_go<TYPE, 1, 2, 16>(g, p, st);
+    if (p.src != 0 && g.T <= 16) return mm_go<TYPE, 1, 4, 16>(g, p, st);   // (rows in 8 bits)
     if (g.T <= 16) return mm_go<TYPE, 1, 4, 8>(g, p, st);
     // 32 tokens of a work-group until 64 leave three waves for every two SIMDs (8192
     // x 2048 Q4_K: 128 rows 17.9 us against 18.4 with 64, 200 rows 31.8 against 19.6)
