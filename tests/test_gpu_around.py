@@ -441,6 +441,105 @@ def test_forward_router(type_, T):
     ctx.close()
 
 
+@pytest.mark.parametrize("type_", [M.TYPE_Q4_K, M.TYPE_Q8_0], ids=["q4_K", "q8_0"])
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_forward_router_as_the_gating(type_, T):
+    """a router without groups and the layer's own gating of the same kind: the same bits, shared expert and all"""
+    rng = np.random.default_rng(T + 50)
+    D, E, K, I = 512, 32, 4, 256
+    ctx = M.Context(0)
+    ctx.reserve(T, D, I, E, K)
+    keep = []
+    L = _layer(rng, type_, D, E, K, I, keep)
+
+    def tab(n, k):
+        keep.append(M.to_device(O.quantize(type_, (0.08 * rng.standard_normal((n, k))).astype(F32))))
+        return M.tensor(keep[-1], type_, [k, n])
+
+    L.sh_n_ff, L.sh_act, L.sh_gate, L.sh_up, L.sh_down = I, M.ACT_SILU, tab(I, D), tab(I, D), tab(D, I)
+    bias = M.to_device((0.1 * rng.standard_normal(E)).astype(F32))
+    L.gating, L.sel_bias, L.routed_scaling, L.gate_eps = M.GATING_SIGMOID_BIAS, bias.addr, 2.5, 1e-20
+    r = M.make_router(E, K, M.SCORE_SIGMOID, renorm=True, eps=1e-20, scaling=2.5, sel_bias=bias)
+    x, res = Rows(T, D, data=stream_rows(rng, T, D)), Rows(T, D, data=stream_rows(rng, T, D))
+    a, b = Rows(T, D), Rows(T, D)
+    M.check("forward", ctx.forward(L, x.buf, T, res.buf, a.buf))
+    L.gating = 77      # (not read)
+    M.check("forward", ctx.forward_router(L, r, None, x.buf, None, T, res.buf, b.buf))
+    M.synchronize()
+    assert np.array_equal(a.get(), b.get())
+    # captured and replayed on another input
+    st = M.Stream()
+    g = M.Graph(st, lambda s: M.check("forward", ctx.forward_router(L, r, None, x.buf, None, T, res.buf, b.buf, None, s.h)))
+    for i in range(3):
+        x.buf.upload(stream_rows(rng, T, D))
+        M.check("forward", ctx.forward_router(L, r, None, x.buf, None, T, res.buf, a.buf))
+        M.synchronize()
+        b.buf.zero()
+        M.synchronize()
+        g.launch(st)
+        st.synchronize()
+        assert np.array_equal(a.buf.download(F32, (T, D)), b.buf.download(F32, (T, D)))
+    g.destroy()
+    st.destroy()
+    ctx.close()
+
+
+@pytest.mark.parametrize("type_", [M.TYPE_Q4_0, M.TYPE_Q4_K], ids=["q4_0", "q4_K"])
+def test_mul_mat_many_rows(type_):
+    """more rows than one pass takes"""
+    ctx = M.Context(0)
+    T, N, n = 33000, 19, 256
+    ctx.reserve(T, n, 32, 1, 1)
+    rng = np.random.default_rng(1)
+    check_mul_mat(ctx, type_, T, N, n, x=(rng.standard_normal((T, n))).astype(F32))
+    ctx.close()
+
+
+@pytest.mark.parametrize("type_", [M.TYPE_Q4_0, M.TYPE_Q4_K], ids=["q4_0", "q4_K"])
+@pytest.mark.parametrize("T,n", [(1, 65536), (4, 40960), (8, 20480), (17, 12288), (70, 5120), (1, 1 << 17)])
+def test_mul_mat_long_rows(type_, T, n):
+    """rows whose operands do not fit LDS at once, or only for few tokens"""
+    ctx = M.Context(0)
+    ctx.reserve(T, n, 32, 1, 1)
+    check_mul_mat(ctx, type_, T, 37, n)
+    ctx.close()
+
+
+@pytest.mark.parametrize("T", [2, 20])
+def test_mul_mat_subnormal_scales(ctx, T):
+    """Q8_0 scales in fp16's subnormal range, and below it: the codes of the oracle, scales rounded as its"""
+    rng = np.random.default_rng(3)
+    x = stream_rows(rng, T, 256)
+    x[:, :64] *= F32(1e-5)
+    x[:, 64:128] *= F32(3e-7)
+    x[:, 128:160] *= F32(1e-9)
+    raw = O.quantize(M.TYPE_Q4_0, (0.05 * rng.standard_normal((40, 256))).astype(F32)).reshape(40, -1)
+    check_mul_mat(ctx, M.TYPE_Q4_0, T, 40, 256, x, raw)
+    dq, dy = Rows(T, 256, M.TYPE_Q8_0), Rows(T, 256)
+    w = np.exp(-20 * rng.random(256)).astype(F32)
+    M.check("add_norm", ctx.add_norm(M.make_norm(M.NORM_RMS, 0.0, M.to_device(w)), Rows(T, 256, data=x).desc, None, None, dy.desc, dq.desc))
+    assert np.array_equal(dq.get(), A.q8_bytes(dy.get(), M.TYPE_Q8_0))
+
+
+def test_halves(ctx):
+    """values on the border between two codes: away from zero in Q8_0, to even in Q8_K"""
+    q = np.tile(np.concatenate([np.arange(-126.5, 127, 1), [127, 126.5]]), 8)[:2048].astype(F32).reshape(2, 1024)
+    q[:, ::32] = 127      # every block's largest: the scale is 1
+    for kind in (M.TYPE_Q8_0, M.TYPE_Q8_K):
+        w = M.to_device(q[0])
+        ones = np.ones((1, 1024), F32)      # norm: 1 / sqrt(1 + eps), eps = 0
+        dq, dy = Rows(1, 1024, kind), Rows(1, 1024)
+        M.check("add_norm", ctx.add_norm(M.make_norm(M.NORM_RMS, 0.0, w), Rows(1, 1024, data=ones).desc, None, None, dy.desc, dq.desc))
+        assert np.array_equal(dy.get(), q[:1])
+        assert np.array_equal(dq.get(), A.q8_bytes(q[:1], kind))
+    raw = O.quantize(M.TYPE_Q4_0, (0.05 * np.random.default_rng(0).standard_normal((33, 1024))).astype(F32)).reshape(33, -1)
+    rawk = O.quantize(M.TYPE_Q4_K, (0.05 * np.random.default_rng(0).standard_normal((33, 1024))).astype(F32)).reshape(33, -1)
+    for T in (1, 2, 18):
+        x = np.tile(q, (9, 1))[:T]
+        check_mul_mat(ctx, M.TYPE_Q4_0, T, 33, 1024, x, raw)
+        check_mul_mat(ctx, M.TYPE_Q4_K, T, 33, 1024, x, rawk)
+
+
 def test_capacity(ctx):
     small = M.Context(0)
     small.reserve(4, 512, 256, 4, 2)
