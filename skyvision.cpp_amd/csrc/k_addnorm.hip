@@ -10,8 +10,6 @@
 
 namespace mimoe {
 
-constexpr float AN_MAX = 3.402823466e38f;
-
 // codes of 4 values at 4 i of a row (8 lanes hold a 32-value block) to the
 // row's Q8_0 blocks; live: the values are in the row
 __device__ __forceinline__ void an_store_q8_0(const float (&v)[4], uint8_t *row, int i, bool live, bool words) {
@@ -64,28 +62,51 @@ __device__ __forceinline__ void an_store_q8_0(const float (&v)[4], uint8_t *row,
     }
 }
 
-// N blocks of 256 values held by a wave, lane l the values 4 l of each: to the
-// row's Q8_K blocks ib0, ib0 + step, ..
+// N blocks of 256 values held by a wave, lane l the values 4 l of each, to the
+// row's Q8_K blocks ib0, ib0 + step, ..: d = 1 / iscale, iscale = -127 / the first
+// value of the largest |.|, codes rint(iscale v) (|127 v / m| < 127.5: none leaves
+// 8 bits) by the sum with 1.5 * 2^23, whose low bits hold the integer
 template <int N>
 __device__ __forceinline__ void an_store_q8_K(const float (&v)[N][4], uint8_t *row, int ib0, int step, int nblk, int lane) {
-    int q[N][4];
-    float d[N];
-    q8k_wave_n<N>(v, lane, q, d);
+    uint32_t u[N][4], m[N];   // |v| and the largest as bits: a NaN or an infinity shows as 0x7f800000 or more
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        bool bad = false;
+        m[n] = 0u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bad |= !(fabsf(v[n][j]) <= AN_MAX);
-        if (__ballot(bad)) {
-            d[n] = __builtin_nanf("");
-#pragma unroll
-            for (int j = 0; j < 4; ++j) q[n][j] = 0;
+        for (int j = 0; j < 4; ++j) {
+            u[n][j] = __builtin_bit_cast(uint32_t, v[n][j]) & 0x7fffffffu;
+            m[n] = u[n][j] > m[n] ? u[n][j] : m[n];
         }
-        const int s = q8k_bsum16(q[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) m[n] = wave_max_u(m[n]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
         if (ib0 + n * step >= nblk) continue;   // (uniform)
+        // the first holder's sign, on the lanes' masks (a select among v's elements would
+        // put v into memory): element 0's where it holds the largest, else element 1's, ..
+        const uint32_t mu = (uint32_t)__builtin_amdgcn_readfirstlane((int)m[n]);
+        const uint64_t h0 = __ballot(u[n][0] == mu), h1 = __ballot(u[n][1] == mu), h2 = __ballot(u[n][2] == mu),
+                       h3 = __ballot(u[n][3] == mu);
+        const uint64_t n0 = __ballot(v[n][0] < 0.f), n1 = __ballot(v[n][1] < 0.f), n2 = __ballot(v[n][2] < 0.f),
+                       n3 = __ballot(v[n][3] < 0.f);
+        const uint64_t neg = (h0 & n0) | (~h0 & ((h1 & n1) | (~h1 & ((h2 & n2) | (~h2 & n3)))));
+        const int first = (int)__builtin_ctzll(h0 | h1 | h2 | h3);   // (some lane holds it)
+        const float val = __builtin_bit_cast(float, mu | (uint32_t)((neg >> first) & 1) << 31);
+        const bool bad = mu >= 0x7f800000u, zero = mu == 0u;
+        const float iscale = bad || zero ? 0.f : -127.f / val;
+        const float d = bad ? __builtin_nanf("") : zero ? 0.f : 1 / iscale;
+        uint32_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = __builtin_bit_cast(uint32_t, (bad ? 0.f : iscale * v[n][j]) + 12582912.f);
+        const uint32_t c = __builtin_amdgcn_perm(__builtin_amdgcn_perm(q[3], q[2], 0x0C0C0400u),
+                                                 __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0400u), 0x05040100u);
+        int s = __builtin_amdgcn_sdot4(0x01010101, (int)c, 0, false);   // ggml's sums of 16 codes, over 4 lanes
+        s += dpp_i<0xB1>(s);
+        s += dpp_i<0x4E>(s);
         uint8_t *blk = row + (int64_t)(ib0 + n * step) * Q8K_BYTES;
-        *(uint32_t *)(blk + 4 + 4 * lane) = pack_i8x4(q[n]);
-        if (lane == 0) *(float *)blk = d[n];
+        *(uint32_t *)(blk + 4 + 4 * lane) = c;
+        if (lane == 0) *(float *)blk = d;
         if ((lane & 3) == 0) *(int16_t *)(blk + 260 + 2 * (lane >> 2)) = (int16_t)s;
     }
 }
@@ -112,27 +133,32 @@ __device__ __forceinline__ void an_store4(float *x, int i, int D, const float (&
     }
 }
 
-// W waves per row (W = 1: four rows a work-group of four waves), thread i of
-// them holding the values at 256 W k + 4 i, k < P.  VEC: rows of whole float4,
-// 16-byte aligned (D % 4 == 0 where not: the row's tail is read value by value).
+// A work-group of W waves per row, thread i holding the values at 256 W k + 4 i,
+// k < P.  VEC: rows of whole float4, 16-byte aligned.
+// Bound by the memory: 4096 rows of 2048 with the sum and Q8_K codes, 110 MB in
+// 24 us; 4096 rows of 8192 in fp32, 537 MB in 100 us (5.4 TB/s, a large copy 5.1).
 template <int W, int P, bool VEC>
-__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) k_add_norm(AddNormArgs a, int64_t T, int D) {
+__global__ void __launch_bounds__(64 * W) k_add_norm(AddNormArgs a, int D, double rD) {
     __shared__ double red[2][W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t t = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-    if (W == 1 && t >= T) return;   // whole waves
-    const int id = W == 1 ? lane : (int)threadIdx.x;
+    const int64_t t = blockIdx.x;
+    const int id = (int)threadIdx.x;
     constexpr int ROUND = 256 * W;
     // the sum over the row, the same bits in every thread
     auto row_sum = [&](double v, double *r) __attribute__((always_inline)) {
         v = wave_sum_d(v);
-        if constexpr (W == 1) return v;
         if (lane == 0) r[wave] = v;
         __syncthreads();
         double s = r[0];
 #pragma unroll
         for (int i = 1; i < W; ++i) s += r[i];
         return s;
+    };
+    // sum / D, rounded to fp32: the quotient by the reciprocal and one correction (an
+    // infinite sum stays one)
+    auto mean = [&](double v) __attribute__((always_inline)) {
+        const double e = v * rD, r = fma(fma(-e, (double)D, v), rD, e);
+        return (float)(r == r ? r : e);
     };
     float v[P][4], ad[P][4];
     const float *x = a.x + t * a.ldx, *add = a.add + t * a.lda;
@@ -146,16 +172,11 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) k_add_norm(AddNormArgs 
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[k][j] = v[k][j] + ad[k][j];
     }
-    // a row of several waves waits for its sums: the weights come meanwhile (a
-    // wave of its own has others to run, and the registers are the row's)
-    constexpr bool EARLY = W > 1;
-    float w[EARLY ? P : 1][4], b[EARLY ? P : 1][4];
-    if constexpr (EARLY) {
+    float w[P][4], b[P][4];   // (on their way while the sums are formed)
 #pragma unroll
-        for (int k = 0; k < P; ++k) {
-            if (a.norm.w) an_load4<VEC>(a.norm.w, ROUND * k + 4 * id, D, w[k]);
-            if (a.norm.b) an_load4<VEC>(a.norm.b, ROUND * k + 4 * id, D, b[k]);
-        }
+    for (int k = 0; k < P; ++k) {
+        if (a.norm.w) an_load4<VEC>(a.norm.w, ROUND * k + 4 * id, D, w[k]);
+        if (a.norm.b) an_load4<VEC>(a.norm.b, ROUND * k + 4 * id, D, b[k]);
     }
     if (a.sum) {
 #pragma unroll
@@ -171,53 +192,47 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) k_add_norm(AddNormArgs 
             s0 = s0 + (double)v[k][2];
             s1 = s1 + (double)v[k][3];
         }
-        m = (float)(row_sum(s0 + s1, red[0]) / (double)D);
+        m = mean(row_sum(s0 + s1, red[0]));
     }
     double s0 = 0.0, s1 = 0.0;
 #pragma unroll
     for (int k = 0; k < P; ++k)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float d = ROUND * k + 4 * id + j < D ? v[k][j] - m : 0.f;   // (RMS: m = 0, exact)
-            if (j & 1) s1 = s1 + (double)(d * d);
-            else s0 = s0 + (double)(d * d);
+            const float d = v[k][j] - m;   // (RMS: m = 0, exact)
+            const float dd = ROUND * k + 4 * id + (VEC ? 0 : j) < D ? d * d : 0.f;
+            if (j & 1) s1 = s1 + (double)dd;
+            else s0 = s0 + (double)dd;
         }
-    const float var = (float)(row_sum(s0 + s1, red[1]) / (double)D);
+    const float var = mean(row_sum(s0 + s1, red[1]));
     const float sc = 1.0f / sqrtf(var + a.norm.eps);
     const bool words = a.ldq % 4 == 0 && ((uintptr_t)a.q & 3) == 0 && D % 64 == 0;   // Q8_0 in whole words
 #pragma unroll
     for (int k = 0; k < P; ++k) {
         const int i = ROUND * k + 4 * id;
-        const int kw = EARLY ? k : 0;
-        if constexpr (!EARLY) {
-            if (a.norm.w) an_load4<VEC>(a.norm.w, i, D, w[0]);
-            if (a.norm.b) an_load4<VEC>(a.norm.b, i, D, b[0]);
-        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float y = (v[k][j] - m) * sc;   // norm_apply, step for step
-            if (a.norm.w) y = y * w[kw][j];
-            if (a.norm.b) y = y + b[kw][j];
-            v[k][j] = i + j < D ? y : 0.f;
+            if (a.norm.w) y = y * w[k][j];
+            if (a.norm.b) y = y + b[k][j];
+            v[k][j] = i + (VEC ? 0 : j) < D ? y : 0.f;
         }
         if (a.y) an_store4<VEC>(a.y + t * a.ldy, i, D, v[k]);
         if (a.q && a.qtype == 8) an_store_q8_0(v[k], a.q + t * a.ldq, i >> 2, i < D, words);
     }
-    if (a.q && a.qtype == 15) an_store_q8_K<P>(v, a.q + t * a.ldq, W == 1 ? 0 : wave, W, D / QK, lane);
+    if (a.q && a.qtype == 15) an_store_q8_K<P>(v, a.q + t * a.ldq, wave, W, D / QK, lane);
 }
 
 template <bool VEC>
 static int an_launch(const AddNormArgs &a, int64_t T, int D, hipStream_t st) {
-#define AN(W, P) hipLaunchKernelGGL((k_add_norm<W, P, VEC>), dim3((unsigned)(W == 1 ? (T + 3) / 4 : T)), dim3(W == 1 ? 256 : 64 * W), 0, st, a, T, D)
-    // the row over the waves of a work-group (more waves than it needs to hold the
-    // row: one row of 2048, 8 waves 2.65 us, 4 2.9); a wave per row, without barriers,
-    // for thousands of rows that leave as fp32 (4096 rows of 2048: 20.0 us against
-    // 23.0; with codes, whose arithmetic then sits in one wave, 33.3 against 32.0, and
-    // 1024 rows 8.3 against 6.6)
-    if (T >= 2048 && D <= 2048 && !a.q) {
-        if (D <= 1024) AN(1, 4);
-        else AN(1, 8);
-    } else if (D <= 2048) AN(8, 1);
+#define AN(W, P) hipLaunchKernelGGL((k_add_norm<W, P, VEC>), dim3((unsigned)T), dim3(64 * W), 0, st, a, D, 1.0 / (double)D)
+    // few rows: more waves than hold the row (one row of 2048: 8 waves 2.65 us, 4
+    // 2.9); many: fewer, whose sums and scalars cost less (2000 rows of 2048: 8 waves
+    // 12.8 us, 2 11.3; 1024 rows of 4096 to Q8_K 18.9 and with 4 17.7)
+    if (T >= 512 && D <= 1024) AN(2, 2);
+    else if (T >= 512 && D <= 2048) AN(2, 4);
+    else if (T >= 512 && D <= 4096) AN(4, 4);
+    else if (D <= 2048) AN(8, 1);
     else if (D <= 4096) AN(16, 1);
     else if (D <= 8192) AN(16, 2);
     else AN(16, 4);

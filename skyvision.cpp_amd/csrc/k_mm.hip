@@ -52,11 +52,6 @@ __device__ __forceinline__ uint32_t mm_amax8(const float (&v)[8]) {
     }
     return m;
 }
-template <int CTRL>
-__device__ __forceinline__ uint32_t mm_dpp_max(uint32_t m) {
-    const uint32_t o = (uint32_t)dpp_i<CTRL>((int)m);
-    return o > m ? o : m;
-}
 // the lowest bytes of eight words
 __device__ __forceinline__ uint2 mm_bytes8(const uint32_t (&q)[8]) {
     uint32_t h[4];
@@ -70,8 +65,8 @@ __device__ __forceinline__ uint2 mm_bytes8(const uint32_t (&q)[8]) {
 // of a fraction of 1/2 or more rounds to the next integer, of less stays below).
 __device__ __forceinline__ void mm_codes_q8_0(const float (&v)[8], uint2 &c, float &d) {
     uint32_t m = mm_amax8(v);
-    m = mm_dpp_max<0xB1>(m);
-    m = mm_dpp_max<0x4E>(m);
+    m = dpp_max_u<0xB1>(m);
+    m = dpp_max_u<0x4E>(m);
     const float df = __builtin_bit_cast(float, m) / 127.0f;
     const float id = df != 0.0f ? 1.0f / df : 0.0f;
     uint32_t q[8];
@@ -89,10 +84,10 @@ __device__ __forceinline__ void mm_codes_q8_0(const float (&v)[8], uint2 &c, flo
 // rint by the sum with 1.5 * 2^23, whose low bits hold the integer.
 __device__ __forceinline__ void mm_codes_q8_K(const float (&v)[8], uint2 &c, float &d) {
     uint32_t m = mm_amax8(v);
-    m = mm_dpp_max<0xB1>(m);
-    m = mm_dpp_max<0x4E>(m);
-    m = mm_dpp_max<0x141>(m);
-    m = mm_dpp_max<0x140>(m);
+    m = dpp_max_u<0xB1>(m);
+    m = dpp_max_u<0x4E>(m);
+    m = dpp_max_u<0x141>(m);
+    m = dpp_max_u<0x140>(m);
     uint32_t o = m;
     swap16(m, o);
     m = o > m ? o : m;

@@ -73,9 +73,10 @@ __device__ __forceinline__ int wave_max_i(int m) {
     m = o > m ? o : m;
     o = dpp_i<0x140>(m);
     m = o > m ? o : m;
-    o = __builtin_amdgcn_update_dpp(m, m, 0x142, 0xA, 0xF, false);   // rows 0 -> 1, 2 -> 3
+    // (the smallest where no lane reads: the move and the comparison are one instruction)
+    o = __builtin_amdgcn_update_dpp(KEY_NONE, m, 0x142, 0xA, 0xF, false);   // rows 0 -> 1, 2 -> 3
     m = o > m ? o : m;
-    o = __builtin_amdgcn_update_dpp(m, m, 0x143, 0xC, 0xF, false);   // row 1 -> 2, 3
+    o = __builtin_amdgcn_update_dpp(KEY_NONE, m, 0x143, 0xC, 0xF, false);   // row 1 -> 2, 3
     m = o > m ? o : m;
     return __builtin_amdgcn_readlane(m, 63);
 }

@@ -47,6 +47,25 @@ __device__ __forceinline__ void pair32(double v, double &a, double &b) {
     b = __builtin_bit_cast(double, (uint64_t)h1 << 32 | l1);
 }
 
+// the largest over the wave, in every lane
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max_u(uint32_t m) {
+    const uint32_t o = (uint32_t)dpp_i<CTRL>((int)m);
+    return o > m ? o : m;
+}
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t m) {
+    m = dpp_max_u<0xB1>(m);
+    m = dpp_max_u<0x4E>(m);
+    m = dpp_max_u<0x141>(m);
+    m = dpp_max_u<0x140>(m);
+    uint32_t o = m;
+    swap16(m, o);
+    m = o > m ? o : m;
+    o = m;
+    swap32(m, o);
+    return o > m ? o : m;
+}
+
 // sum over the wave, the same bits in every lane
 __device__ __forceinline__ double wave_sum_d(double v) {
     v += dpp_d<0xB1>(v);
