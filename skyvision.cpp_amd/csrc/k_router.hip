@@ -85,6 +85,7 @@ struct RoutePlan {
     int gs;          // experts of a group
     int magic;       // e / gs = e magic >> 20 for e < 1024
     int ls;          // log2 of the lanes that find a group's value
+    int whole;       // a lane's experts are of one group
     int vec;         // rows of logits and bias in whole, aligned pieces of NPER
 };
 
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__(64 * RT_W) k_route(const float *__restrict__ l
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < NPER; ++i) {
-            s[i] = e0 + i < E ? exp_f32(s[i] - mx) : 0.f;
+            s[i] = exp_f32(s[i] - mx);   // (past E: -inf, 0 unless the whole row is NaN)
             sum += (double)s[i];
         }
         sum = wave_sum_d(sum);
@@ -179,19 +180,23 @@ __global__ void __launch_bounds__(64 * RT_W) k_route(const float *__restrict__ l
             b = lo > b ? lo : b;
             a = a > a2 ? a : a2;
         }
-        const int val = p.group_top == 1 || a == KEY_NONE ? a
-                        : key_of(b == KEY_NONE ? -INFINITY : value_of(a) + value_of(b));
-        // a group's place: those before it
+        int val = p.group_top == 1 || a == KEY_NONE ? a
+                  : key_of(b == KEY_NONE ? -INFINITY : value_of(a) + value_of(b));
+        // a group's place: those before it, larger, or equal and lower (larger than
+        // the integer below; no number: still above the smallest integer)
+        val = val > KEY_NONE ? val : KEY_NONE + 1;
         int before = 0;
-        for (int o = 0; o < p.n_group; ++o) {
-            const int v = __builtin_amdgcn_readlane(val, o << q.ls);
-            before += v > val || (v == val && o < g) ? 1 : 0;
-        }
+        for (int o = 0; o < p.n_group; ++o)
+            before += __builtin_amdgcn_readlane(val, o << q.ls) > (o < g ? val - 1 : val) ? 1 : 0;
         const unsigned long long kept = __ballot(g < p.n_group && before < p.n_kept);
+        bool in = true;
 #pragma unroll
         for (int i = 0; i < NPER; ++i) {
-            const int ge = ((e0 + i) * q.magic) >> 20;
-            if (!((kept >> ((ge << q.ls) & 63)) & 1)) k[i] = KEY_NONE;
+            if (i == 0 || !q.whole) {   // (uniform)
+                const uint32_t ge = __umul24((uint32_t)(e0 + i), (uint32_t)q.magic) >> 20;
+                in = (kept >> ((ge << q.ls) & 63)) & 1;
+            }
+            k[i] = in ? k[i] : KEY_NONE;
         }
     }
     // each lane's experts, best first (neighbours change places only for a larger
@@ -217,21 +222,20 @@ __global__ void __launch_bounds__(64 * RT_W) k_route(const float *__restrict__ l
     }
     int mysel = -1;
     for (int r = 0; r < K; ++r) {
-        int best = k[0], bid = e0;
-        if constexpr (NPER <= 4) {
-            bid = e0 + (int)(ord & 0xffu);
-        } else {
+        int best = k[0], at = (int)ord;   // (up to four: the lane's best is the lowest byte)
+        if constexpr (NPER > 4) {
+            at = 0;
 #pragma unroll
             for (int i = 1; i < NPER; ++i) {
                 const bool up = k[i] > best;
                 best = up ? k[i] : best;
-                bid = up ? e0 + i : bid;
+                at = up ? i : at;
             }
         }
         const int m = wave_max_i(best);
         if (m == KEY_NONE) break;   // (uniform) no number left
         const int win = (int)__builtin_ctzll(__ballot(best == m));   // lanes hold ascending ids
-        const int e = __builtin_amdgcn_readlane(bid, win);
+        const int e = NPER * win + (__builtin_amdgcn_readlane(at, win) & 0xff);
         mysel = lane == r ? e : mysel;
         if constexpr (NPER <= 4) {
             const bool mine = lane == win;
@@ -277,6 +281,7 @@ int launch_route(const float *logits, int64_t ldl, int64_t T, int E, int K, cons
     RoutePlan q;
     q.gs = E / p.n_group;
     q.magic = ((1 << 20) + q.gs - 1) / q.gs;   // e (magic gs - 2^20) < 1024 * 512 < 2^20: exact
+    q.whole = q.gs % nper == 0;
     q.ls = 0;
     while (p.n_group << (q.ls + 1) <= 64) ++q.ls;
     const uintptr_t unit = 4 * (uintptr_t)nper;
