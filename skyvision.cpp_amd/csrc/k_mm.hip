@@ -778,9 +778,11 @@ template <int TYPE, int MT, int NI, int W>
 static int mm_go(const MmArgs &g, MmPlan p, hipStream_t st) {
     using R = MmRec<TYPE>;
     const int64_t slices = (g.T + 16 * MT - 1) / (16 * MT);
-    // waves that share a row tile: the fewest that give every SIMD four waves
+    // waves that share a row tile: the fewest that fill the CUs' 16 waves (8 where the
+    // operands of more tokens leave room for one work-group; 128 rows of 8192 x 2048
+    // Q4_K: 16.6 us, for 16 waves 18.1)
     p.wk = 1;
-    while (p.wk < (MT > 2 ? 1 : 8) && p.ntiles * slices * p.wk < 4096) p.wk *= 2;
+    while (p.wk < (MT > 2 ? 1 : 8) && p.ntiles * slices * p.wk < 256 * (MT > 1 ? 8 : 16)) p.wk *= 2;
     const int red = p.wk > 1 ? 2 * W * MT * 64 * NI * 4 : 0;
     const int fit = (MM_LDS - red) / (MT * R::BYTES) / MM_U<TYPE> * MM_U<TYPE>;
     p.chunks = (p.nsets + fit - 1) / fit;
@@ -827,7 +829,7 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
     if (p.src != 0 && g.T <= 16) return mm_go<TYPE, 1, 4, 16>(g, p, st);   // (rows in 8 bits)
     if (g.T <= 16) return mm_go<TYPE, 1, 4, 8>(g, p, st);
     // 32 tokens of a work-group until 64 leave three waves for every two SIMDs (8192
-    // x 2048 Q4_K: 128 rows 17.9 us against 18.4 with 64, 200 rows 31.8 against 19.6)
+    // x 2048 Q4_K: 128 rows 16.6 us against 18.4 with 64, 200 rows 31.8 against 18.9)
     if (g.T <= 32 || p.ntiles * ((g.T + 63) / 64) < 1536) return mm_go<TYPE, 2, 4, 8>(g, p, st);
     return mm_go<TYPE, 4, 4, 8>(g, p, st);
 }
