@@ -27,6 +27,7 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float4_t float4_a4 __attribute__((aligned(4)));   // (global memory: any dword address)
 
 // ---------------------------------------------------------------- fp16 bits
 // IEEE binary16 <-> binary32 by integer arithmetic (round to nearest even),

@@ -111,22 +111,31 @@ __device__ __forceinline__ void an_store_q8_K(const float (&v)[N][4], uint8_t *r
     }
 }
 
-// 4 values at i of a row of D (zeros past it)
-template <bool VEC>
+// 4 values at i of a row of D (zeros past it), at any float's address.  TAIL: D is
+// no multiple of 4, the last piece goes value by value (without it a kernel has
+// no such code: 4096 rows of 2048 to Q8_K 30.3 -> 28.7 us)
+template <bool TAIL>
 __device__ __forceinline__ void an_load4(const float *x, int i, int D, float (&v)[4]) {
-    if constexpr (VEC) {
-        const float4 a = i < D ? *(const float4 *)(x + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    if constexpr (!TAIL) {
+        float4_t a = {0.f, 0.f, 0.f, 0.f};
+        if (i < D) a = *(const float4_a4 *)(x + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = a[j];
+    } else if (i + 4 <= D) {
+        const float4_t a = *(const float4_a4 *)(x + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = a[j];
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = i + j < D ? x[i + j] : 0.f;
     }
 }
-template <bool VEC>
+template <bool TAIL>
 __device__ __forceinline__ void an_store4(float *x, int i, int D, const float (&v)[4]) {
-    if constexpr (VEC) {
-        if (i < D) *(float4 *)(x + i) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
+    if (TAIL ? i + 4 <= D : i < D) {
+        const float4_t a = {v[0], v[1], v[2], v[3]};
+        *(float4_a4 *)(x + i) = a;
+    } else if constexpr (TAIL) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (i + j < D) x[i + j] = v[j];
@@ -134,10 +143,10 @@ __device__ __forceinline__ void an_store4(float *x, int i, int D, const float (&
 }
 
 // A work-group of W waves per row, thread i holding the values at 256 W k + 4 i,
-// k < P.  VEC: rows of whole float4, 16-byte aligned.
+// k < P.
 // Bound by the memory: 4096 rows of 2048 with the sum and Q8_K codes, 110 MB in
 // 24 us; 4096 rows of 8192 in fp32, 537 MB in 100 us (5.4 TB/s, a large copy 5.1).
-template <int W, int P, bool VEC>
+template <int W, int P, bool TAIL>
 __global__ void __launch_bounds__(64 * W) k_add_norm(AddNormArgs a, int D, double rD) {
     __shared__ double red[2][W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -163,10 +172,10 @@ __global__ void __launch_bounds__(64 * W) k_add_norm(AddNormArgs a, int D, doubl
     float v[P][4], ad[P][4];
     const float *x = a.x + t * a.ldx, *add = a.add + t * a.lda;
 #pragma unroll
-    for (int k = 0; k < P; ++k) an_load4<VEC>(x, ROUND * k + 4 * id, D, v[k]);
+    for (int k = 0; k < P; ++k) an_load4<TAIL>(x, ROUND * k + 4 * id, D, v[k]);
     if (a.add) {
 #pragma unroll
-        for (int k = 0; k < P; ++k) an_load4<VEC>(add, ROUND * k + 4 * id, D, ad[k]);
+        for (int k = 0; k < P; ++k) an_load4<TAIL>(add, ROUND * k + 4 * id, D, ad[k]);
 #pragma unroll
         for (int k = 0; k < P; ++k)
 #pragma unroll
@@ -175,12 +184,12 @@ __global__ void __launch_bounds__(64 * W) k_add_norm(AddNormArgs a, int D, doubl
     float w[P][4], b[P][4];   // (on their way while the sums are formed)
 #pragma unroll
     for (int k = 0; k < P; ++k) {
-        if (a.norm.w) an_load4<VEC>(a.norm.w, ROUND * k + 4 * id, D, w[k]);
-        if (a.norm.b) an_load4<VEC>(a.norm.b, ROUND * k + 4 * id, D, b[k]);
+        if (a.norm.w) an_load4<TAIL>(a.norm.w, ROUND * k + 4 * id, D, w[k]);
+        if (a.norm.b) an_load4<TAIL>(a.norm.b, ROUND * k + 4 * id, D, b[k]);
     }
     if (a.sum) {
 #pragma unroll
-        for (int k = 0; k < P; ++k) an_store4<VEC>(a.sum + t * a.lds, ROUND * k + 4 * id, D, v[k]);
+        for (int k = 0; k < P; ++k) an_store4<TAIL>(a.sum + t * a.lds, ROUND * k + 4 * id, D, v[k]);
     }
     float m = 0.f;
     if (a.norm.kind == NORM_LAYER) {
@@ -200,7 +209,7 @@ __global__ void __launch_bounds__(64 * W) k_add_norm(AddNormArgs a, int D, doubl
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float d = v[k][j] - m;   // (RMS: m = 0, exact)
-            const float dd = ROUND * k + 4 * id + (VEC ? 0 : j) < D ? d * d : 0.f;
+            const float dd = ROUND * k + 4 * id + (TAIL ? j : 0) < D ? d * d : 0.f;
             if (j & 1) s1 = s1 + (double)dd;
             else s0 = s0 + (double)dd;
         }
@@ -215,17 +224,17 @@ __global__ void __launch_bounds__(64 * W) k_add_norm(AddNormArgs a, int D, doubl
             float y = (v[k][j] - m) * sc;   // norm_apply, step for step
             if (a.norm.w) y = y * w[k][j];
             if (a.norm.b) y = y + b[k][j];
-            v[k][j] = i + (VEC ? 0 : j) < D ? y : 0.f;
+            v[k][j] = i + (TAIL ? j : 0) < D ? y : 0.f;
         }
-        if (a.y) an_store4<VEC>(a.y + t * a.ldy, i, D, v[k]);
+        if (a.y) an_store4<TAIL>(a.y + t * a.ldy, i, D, v[k]);
         if (a.q && a.qtype == 8) an_store_q8_0(v[k], a.q + t * a.ldq, i >> 2, i < D, words);
     }
     if (a.q && a.qtype == 15) an_store_q8_K<P>(v, a.q + t * a.ldq, wave, W, D / QK, lane);
 }
 
-template <bool VEC>
+template <bool TAIL>
 static int an_launch(const AddNormArgs &a, int64_t T, int D, hipStream_t st) {
-#define AN(W, P) hipLaunchKernelGGL((k_add_norm<W, P, VEC>), dim3((unsigned)T), dim3(64 * W), 0, st, a, D, 1.0 / (double)D)
+#define AN(W, P) hipLaunchKernelGGL((k_add_norm<W, P, TAIL>), dim3((unsigned)T), dim3(64 * W), 0, st, a, D, 1.0 / (double)D)
     // few rows: more waves than hold the row (one row of 2048: 8 waves 2.65 us, 4
     // 2.9); many: fewer, whose sums and scalars cost less (2000 rows of 2048: 8 waves
     // 12.8 us, 2 11.3; 1024 rows of 4096 to Q8_K 18.9 and with 4 17.7)
@@ -245,10 +254,7 @@ int launch_add_norm(const AddNormArgs &a, int64_t T, int D, hipStream_t st) {
     if (D <= 0 || D > ADD_NORM_MAX_D || T > 0x7fffffff || (a.norm.kind != NORM_RMS && a.norm.kind != NORM_LAYER)) return -6;
     if (a.q && a.qtype != 8 && a.qtype != 15) return -3;
     if (a.q && D % (a.qtype == 8 ? 32 : QK)) return -2;
-    auto vec = [](const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 4 == 0; };   // null: fine
-    const bool v = D % 4 == 0 && vec(a.x, a.ldx) && vec(a.add, a.lda) && vec(a.sum, a.lds) && vec(a.y, a.ldy) &&
-                   vec(a.norm.w, 0) && vec(a.norm.b, 0);
-    return v ? an_launch<true>(a, T, D, st) : an_launch<false>(a, T, D, st);
+    return D % 4 ? an_launch<true>(a, T, D, st) : an_launch<false>(a, T, D, st);
 }
 
 // values of Q8_K blocks, one wave per block

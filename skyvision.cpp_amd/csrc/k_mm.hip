@@ -4,12 +4,21 @@
 //   Q4_K . Q8_K: d_b (d sum_j sc_j sum_j q c - dmin sum_j m_j sum_j c)     (256, j: 32 values)
 // The sums over codes are exact integers, the blocks are added in fp32.
 //
-// The codes' products run on v_mfma_i32_16x16x32_i8, whose 32 products are one
-// 32-value block: 16 tokens x 16 rows of the matrix, one group of 16 lanes per
-// quarter of the block.  A lane holds a row's codes straight from the table's
-// bytes; the tokens' operands lie in LDS in the lanes' order (MM records) for
-// the whole K, written once per work-group, which then walks over row tiles:
-// the matrix is read once and nothing else is.
+// Two kernels.  k_mv (up to 8 rows of b): a lane per 32 values of whole rows of
+// the matrix on v_dot4_i32_i8, bound by the stream of the matrix: one row through
+// 65536 x 2048 Q4_K (75 MB) 16.8 us = 4.5 TB/s out of the last-level cache, 18.5 us
+// from memory (a large copy moves 5.1 TB/s); 2048 x 2048 3.6 us, of which the call's
+// latency is most.
+// k_mm (more): the codes' products on the int8 MFMA, whose 32 (16x16x32) or 64
+// (16x16x64) products are one or two 32-value blocks of 16 tokens x 16 rows of
+// the matrix, one group of 16 lanes per quarter of a block.  A lane holds a row's
+// codes straight from the table's bytes; the tokens' operands lie in LDS in the
+// lanes' order (MM records) for the whole K where they fit, written once per
+// work-group, which then walks over row tiles: the matrix is read once per 16 to
+// 64 tokens.  Bound by the vector instructions that unpack codes and apply the
+// scales: 13 rows through 3712 x 2688 Q4_0 7.9 us (2.4 of them k_mm_rows), 200
+// rows through 8192 x 2048 Q4_K 19.7 us (340 TFLOP/s; matrix units busy 28 % of
+// k_mm's time, vector ones 40 %, the operands' way into LDS some 15 %).
 #include <type_traits>
 
 #include "b32.hpp"
@@ -29,6 +38,7 @@ typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 typedef uint32_t u32_a2 __attribute__((aligned(2)));
 
 constexpr int MM_LDS = 160 * 1024;
+constexpr int MM_W = 8;   // waves of a k_mm work-group (16: 16 rows of 8192 x 2048 Q4_0 with the operands made in it 13.3 us, 8: 10.5)
 
 // The operands of 16 tokens for one set of blocks (Q4_0: 4 blocks, 128 values;
 // Q4_K: one of 256): the 8 code bytes of lane (token m, quarter g) per 32-value
@@ -107,14 +117,14 @@ template <int SRC> struct MmPiece;
 template <> struct MmPiece<1> {
     float v[8];
     // values at x, the second four gap values behind the first
-    __device__ __forceinline__ void fetch(const float *x, int gap, bool vec, bool live) {
-        if (live && vec) {
-            const float4 a = *(const float4 *)x, b = *(const float4 *)(x + gap);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = live ? x[(j & 3) + (j >> 2) * gap] : 0.f;
+    __device__ __forceinline__ void fetch(const float *x, int gap, bool live) {
+        float4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;
+        if (live) {
+            a = *(const float4_a4 *)x;
+            b = *(const float4_a4 *)(x + gap);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
     }
 };
 template <> struct MmPiece<2> {
@@ -125,10 +135,10 @@ template <> struct MmPiece<2> {
 // and 16 + 4 g .. (g = p % 4: what the nibbles of a dword of the table hold), all
 // others 8 in a row
 template <int TYPE, int SRC, bool SPLIT>
-__device__ __forceinline__ void mm_fetch(MmPiece<SRC> &r, const uint8_t *row, int p, bool vec, bool live) {
+__device__ __forceinline__ void mm_fetch(MmPiece<SRC> &r, const uint8_t *row, int p, bool live) {
     if constexpr (SRC == 1) {
-        if constexpr (SPLIT) r.fetch((const float *)row + 32 * (p >> 2) + 4 * (p & 3), 16, vec, live);
-        else r.fetch((const float *)row + 8 * (int64_t)p, 4, vec, live);
+        if constexpr (SPLIT) r.fetch((const float *)row + 32 * (p >> 2) + 4 * (p & 3), 16, live);
+        else r.fetch((const float *)row + 8 * (int64_t)p, 4, live);
     } else {
         r.c = make_uint2(0u, 0u);
         r.d = 0.f;
@@ -180,19 +190,18 @@ __device__ __forceinline__ void mm_put(const MmPiece<SRC> &r, int p, int m, uint
 
 // records of a call's rows: ws + ((tile of 16 tokens) * nsets + set) * BYTES
 template <int TYPE>
-__global__ void __launch_bounds__(256) k_mm_rows(const uint8_t *b, int64_t ldb, int64_t T, int K, int nsets, int vec, uint8_t *ws) {
+__global__ void __launch_bounds__(256) k_mm_rows(const uint8_t *b, int64_t ldb, int64_t T, int K, int nsets, uint8_t *ws) {
     using R = MmRec<TYPE>;
     const int64_t t = blockIdx.y;
     const int p = blockIdx.x * 256 + threadIdx.x, set = p / (R::VALUES / 8);
     if (set >= nsets) return;   // whole sets of lanes
     MmPiece<1> r;
-    mm_fetch<TYPE, 1, TYPE == 2>(r, b + t * ldb, p, vec, 8 * (int64_t)p < K);
+    mm_fetch<TYPE, 1, TYPE == 2>(r, b + t * ldb, p, 8 * (int64_t)p < K);
     mm_put<TYPE, 1>(r, p, (int)(t & 15), ws + ((t >> 4) * nsets + set) * R::BYTES);
 }
 
 struct MmPlan {
     int src;       // operands: 0 records at ws, 1 fp32 rows, 2 rows in 8 bits
-    int vec;       // fp32 rows 16-byte aligned
     int nsets;     // sets of a row
     int chunks, cs;  // chunks of cs sets whose operands lie in LDS at a time
     int wk;        // waves that share a row tile, each taking every wk-th step of sets
@@ -353,10 +362,10 @@ template <int TYPE> constexpr int MM_U = TYPE == 2 ? 2 : 1;
 // Work-group (x, y) of W waves: tokens 16 MT y .. (NI < 4: 4 NI tokens at most,
 // token t in row 4 (t / NI) + t % NI of the MFMA's), row tiles x (W / wk), +
 // gridDim.x (W / wk) ..
-template <int TYPE, int MT, int NI, int W>
-__global__ void __launch_bounds__(64 * W) k_mm(MmArgs g, MmPlan p) {
+template <int TYPE, int MT, int NI>
+__global__ void __launch_bounds__(64 * MM_W) k_mm(MmArgs g, MmPlan p) {
     using R = MmRec<TYPE>;
-    constexpr int U = MM_U<TYPE>;
+    constexpr int U = MM_U<TYPE>, W = MM_W;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wk = p.wk, wn = W / wk, kw = wave % wk, nw = wave / wk;
@@ -397,7 +406,7 @@ __global__ void __launch_bounds__(64 * W) k_mm(MmArgs g, MmPlan p) {
                         tt[n] = i < ns * PS ? t : nt;   // (else past the row's sets: whole groups of lanes that share a block)
                         ii[n] = i;
                         if (tt[n] < nt)
-                            mm_fetch<TYPE, SRC, TYPE == 2>(r[n], (const uint8_t *)g.b + (t0 + t) * g.ldb, s0 * PS + i, p.vec,
+                            mm_fetch<TYPE, SRC, TYPE == 2>(r[n], (const uint8_t *)g.b + (t0 + t) * g.ldb, s0 * PS + i,
                                                            8 * (int64_t)(s0 * PS + i) < g.K);
                     }
 #pragma unroll
@@ -515,7 +524,7 @@ __global__ void __launch_bounds__(64 * W) k_mm(MmArgs g, MmPlan p) {
 // nibbles (16 bytes), of the high ones (16 bytes), and {scale f32, Q4_0: -8 times
 // the codes' sum; Q4_K: the two sums of 16 codes, as halves of a word}.
 struct MvPlan {
-    int src, vec;      // as MmPlan (src 1 or 2)
+    int src;           // as MmPlan (1 or 2)
     int nu;            // units of a row
     int lg, chunks;    // lanes per row (log2), units of a row / lanes, rounded up
     int64_t batches;   // of R * 64 / lanes rows
@@ -617,7 +626,7 @@ __global__ void __launch_bounds__(64 * W) k_mv(MmArgs g, MvPlan p) {
                 }
                 tt[n] = t;
                 ii[n] = i;
-                if (t < T) mm_fetch<TYPE, SRC, false>(r[n], (const uint8_t *)g.b + t * g.ldb, i, p.vec, i < pieces);
+                if (t < T) mm_fetch<TYPE, SRC, false>(r[n], (const uint8_t *)g.b + t * g.ldb, i, i < pieces);
             }
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
@@ -732,7 +741,6 @@ template <int TYPE, int T, int R, int W>
 static int mv_go(const MmArgs &g, hipStream_t st) {
     MvPlan p = {};
     p.src = g.btype != 0 ? 2 : 1;
-    p.vec = (uintptr_t)g.b % 16 == 0 && g.ldb % 16 == 0;
     p.nu = (int)(g.K / 32);
     p.lg = mv_lg(p.nu, g.N, R);
     p.chunks = (p.nu + (1 << p.lg) - 1) >> p.lg;
@@ -744,22 +752,27 @@ static int mv_go(const MmArgs &g, hipStream_t st) {
     return hip_check_launch();
 }
 
-// Many rows: several a lane, more loads in flight (registers allow 4 up to two
-// rows of b, 2 up to four).  Few: one, and work-groups of 16 waves, which share
-// the operands (8192 x 2048 Q4_0, one row: 4 waves 6.2 us, 16 4.4).
+// Rows of a lane: one where few, and work-groups of 16 waves, which share the
+// operands (8192 x 2048 Q4_0, one row of b: 4 waves 6.2 us, 16 4.4); more loads in
+// flight where many: two (16384 x 2048 Q4_0: 7.0 -> 6.4 us), four, as far as the
+// registers allow (65536 x 2048 Q4_0: two 23.7 us, four 21.8; 16384: 6.4 and 8.0)
 template <int TYPE, int T>
 static int mv_launch(const MmArgs &g, hipStream_t st) {
-    return g.N >= 4 * MV_WAVES ? mv_go<TYPE, T, (T <= 2 ? 4 : T <= 4 ? 2 : 1), 8>(g, st) : mv_go<TYPE, T, 1, 16>(g, st);
+    if constexpr (T <= 2)
+        if (g.N >= 12 * MV_WAVES) return mv_go<TYPE, T, 4, 8>(g, st);
+    if (g.N >= 4 * MV_WAVES) return mv_go<TYPE, T, (T <= 4 ? 2 : 1), 8>(g, st);
+    return mv_go<TYPE, T, 1, 16>(g, st);
 }
 
 // Up to 8 rows of b, while the dots are not what bounds it: the time of these
-// kernels grows with the rows of b, that of k_mm does not, but for its operands'
-// launch or their work in every work-group (8192 x 2048 Q4_0, 8 rows: 9.5 us
-// against 11.6; 65536 x 2048, 4 and 6 rows: Q4_0 25.6 and 36.8 against 31.2 and
-// 31.9, Q4_K 2 and 4 rows: 20.3 and 29.2 against 22.4 and 23.5).
+// kernels grows with the rows of b, that of k_mm hardly does, but for its operands
+// (columns of 2048, us here and there: Q4_0 6 rows 8192 x 2048 8.5 and 9.8, 16384
+// 13.6 and 12.7, 4 rows 65536 30.7 and 30.9; Q4_K 4 rows 8192 7.4 and 8.0, 16384 11.8
+// and 10.1, 2 rows 65536 22.7 and 24.3).
 template <int TYPE>
 static bool mv_ok(const MmArgs &g) {
-    return g.T <= 8 && g.T * 40 * (g.K / 32) <= MM_LDS && g.T * g.N * g.K <= (int64_t)5 << (TYPE == 2 ? 27 : 26);
+    if (g.T > 8 || g.T * 40 * (g.K / 32) > MM_LDS) return false;
+    return g.T <= (TYPE == 2 ? 4 : 2) || g.T * g.N * g.K <= (int64_t)9 << (TYPE == 2 ? 24 : 23);
 }
 
 constexpr int64_t MM_PASS_T = 32768;   // rows of one pass (grid dimensions)
@@ -774,15 +787,15 @@ size_t mm_ws_bytes(int type, int btype, int64_t T, int64_t K) {
                      : (size_t)((T + 15) / 16 * (K / 256) * MmRec<12>::BYTES);
 }
 
-template <int TYPE, int MT, int NI, int W>
+template <int TYPE, int MT, int NI>
 static int mm_go(const MmArgs &g, MmPlan p, hipStream_t st) {
     using R = MmRec<TYPE>;
+    constexpr int W = MM_W;
     const int64_t slices = (g.T + 16 * MT - 1) / (16 * MT);
-    // waves that share a row tile: the fewest that fill the CUs' 16 waves (8 where the
-    // operands of more tokens leave room for one work-group; 128 rows of 8192 x 2048
-    // Q4_K: 16.6 us, for 16 waves 18.1)
+    // waves that share a row tile: the fewest that give every CU eight (8192 x 2048
+    // Q4_0, 16 rows: 9.9 us, for 16 waves 11.8; 128 rows Q4_K: 16.6 and 18.1)
     p.wk = 1;
-    while (p.wk < (MT > 2 ? 1 : 8) && p.ntiles * slices * p.wk < 256 * (MT > 1 ? 8 : 16)) p.wk *= 2;
+    while (p.wk < (MT > 2 ? 1 : 8) && p.ntiles * slices * p.wk < 256 * 8) p.wk *= 2;
     const int red = p.wk > 1 ? 2 * W * MT * 64 * NI * 4 : 0;
     const int fit = (MM_LDS - red) / (MT * R::BYTES) / MM_U<TYPE> * MM_U<TYPE>;
     p.chunks = (p.nsets + fit - 1) / fit;
@@ -790,12 +803,11 @@ static int mm_go(const MmArgs &g, MmPlan p, hipStream_t st) {
     p.cs = (p.cs + MM_U<TYPE> - 1) / MM_U<TYPE> * MM_U<TYPE>;
     p.chunks = (p.nsets + p.cs - 1) / p.cs;
     const int lds = MT * p.cs * R::BYTES + red;
-    const int per_cu = imin(16 / W, imax(1, MM_LDS / lds));
     const int wn = W / p.wk;
-    const int64_t want = (256 * per_cu + slices - 1) / slices;   // work-groups of a slice
+    const int64_t want = (256 + slices - 1) / slices;   // work-groups of a slice: one a CU, which then makes or copies the operands once
     const int64_t most = (p.ntiles + wn - 1) / wn;
     const dim3 grid((unsigned)(want < most ? want : most), (unsigned)slices), block(64 * W);
-    hipLaunchKernelGGL((k_mm<TYPE, MT, NI, W>), grid, block, lds, st, g, p);
+    hipLaunchKernelGGL((k_mm<TYPE, MT, NI>), grid, block, lds, st, g, p);
     return hip_check_launch();
 }
 
@@ -815,23 +827,21 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
     MmPlan p = {};
     p.nsets = (int)((g.K + R::VALUES - 1) / R::VALUES);
     p.ntiles = (int)((g.N + 15) / 16);
-    p.vec = (uintptr_t)g.b % 16 == 0 && g.ldb % 16 == 0;
     p.src = g.btype != 0 ? 2 : 1;
     if (g.btype == 0 && g.T >= MM_PREP_T) {
         const dim3 grid((unsigned)((p.nsets * (R::VALUES / 8) + 255) / 256), (unsigned)g.T);
-        hipLaunchKernelGGL(k_mm_rows<TYPE>, grid, dim3(256), 0, st, (const uint8_t *)g.b, g.ldb, g.T, (int)g.K, p.nsets, p.vec, (uint8_t *)g.ws);
+        hipLaunchKernelGGL(k_mm_rows<TYPE>, grid, dim3(256), 0, st, (const uint8_t *)g.b, g.ldb, g.T, (int)g.K, p.nsets, (uint8_t *)g.ws);
         const int rc = hip_check_launch();
         if (rc) return rc;
         p.src = 0;
     }
-    if (p.src != 0 && g.T <= 4) return mm_go<TYPE, 1, 1, 16>(g, p, st);
-    if (p.src != 0 && g.T <= 8) return mm_go<TYPE, 1, 2, 16>(g, p, st);
-    if (p.src != 0 && g.T <= 16) return mm_go<TYPE, 1, 4, 16>(g, p, st);   // (rows in 8 bits)
-    if (g.T <= 16) return mm_go<TYPE, 1, 4, 8>(g, p, st);
+    if (p.src != 0 && g.T <= 4) return mm_go<TYPE, 1, 1>(g, p, st);
+    if (p.src != 0 && g.T <= 8) return mm_go<TYPE, 1, 2>(g, p, st);
+    if (g.T <= 16) return mm_go<TYPE, 1, 4>(g, p, st);
     // 32 tokens of a work-group until 64 leave three waves for every two SIMDs (8192
     // x 2048 Q4_K: 128 rows 16.6 us against 18.4 with 64, 200 rows 31.8 against 18.9)
-    if (g.T <= 32 || p.ntiles * ((g.T + 63) / 64) < 1536) return mm_go<TYPE, 2, 4, 8>(g, p, st);
-    return mm_go<TYPE, 4, 4, 8>(g, p, st);
+    if (g.T <= 32 || p.ntiles * ((g.T + 63) / 64) < 1536) return mm_go<TYPE, 2, 4>(g, p, st);
+    return mm_go<TYPE, 4, 4>(g, p, st);
 }
 
 int launch_mm(const MmArgs &g, hipStream_t st) {
