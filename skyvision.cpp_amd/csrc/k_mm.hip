@@ -835,8 +835,9 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
         if (rc) return rc;
         p.src = 0;
     }
-    if (p.src != 0 && g.T <= 4) return mm_go<TYPE, 1, 1>(g, p, st);
-    if (p.src != 0 && g.T <= 8) return mm_go<TYPE, 1, 2>(g, p, st);
+    // (by rows alone, not by b's type: a plan's order of sums is the same for both)
+    if (g.T <= 4) return mm_go<TYPE, 1, 1>(g, p, st);
+    if (g.T < MM_PREP_T) return mm_go<TYPE, 1, 2>(g, p, st);
     if (g.T <= 16) return mm_go<TYPE, 1, 4>(g, p, st);
     // 32 tokens of a work-group until 64 leave three waves for every two SIMDs (8192
     // x 2048 Q4_K: 128 rows 16.6 us against 18.4 with 64, 200 rows 31.8 against 18.9)

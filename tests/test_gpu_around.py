@@ -551,3 +551,15 @@ def test_capacity(ctx):
     M.check("mul_mat", small.mul_mat(a.desc, Rows(30, 512, M.TYPE_Q8_0, data=np.zeros((30, 544), np.uint8)).desc, Rows(30, 8).desc))
     M.synchronize()
     small.close()
+
+
+# ------------------------------------------------------------------ where launches and plans change over
+@pytest.mark.parametrize("type_", [M.TYPE_Q4_0, M.TYPE_Q4_K], ids=["q4_0", "q4_K"])
+@pytest.mark.parametrize("T", [7, 8, 9])
+def test_mul_mat_bits_where_the_operands_are_made_elsewhere(type_, T):
+    """long rows, whose sums' order follows the operands' place in LDS: float32 rows and 8-bit rows give the same bits
+    on both sides of the batch from which the operands are made in a launch of their own"""
+    ctx = M.Context(0)
+    ctx.reserve(T, 8448, 32, 1, 1)
+    check_mul_mat(ctx, type_, T, 4096, 8448)
+    ctx.close()
