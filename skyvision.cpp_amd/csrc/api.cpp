@@ -1865,7 +1865,7 @@ int mi_add_norm(mi_moe_ctx *c, const mi_moe_norm *norm, const mi_tensor *x, cons
         if (q->type != MI_TYPE_Q8_0 && q->type != MI_TYPE_Q8_K) return MI_MOE_ERR_TYPE;
         TRY(check_rows(*q, D, T));
     }
-    if (D > ADD_NORM_MAX_D || T > 0x7fffffff) return MI_MOE_ERR_UNSUPPORTED;
+    if (D > ADD_NORM_MAX_D) return MI_MOE_ERR_UNSUPPORTED;
     if (T == 0) return MI_MOE_OK;
     // an output is apart from everything, or sum / y is x or add itself
     const mi_tensor *outs[3] = {sum, y, q}, *ins[2] = {x, add};

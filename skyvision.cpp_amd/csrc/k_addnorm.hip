@@ -251,10 +251,22 @@ static int an_launch(const AddNormArgs &a, int64_t T, int D, hipStream_t st) {
 
 int launch_add_norm(const AddNormArgs &a, int64_t T, int D, hipStream_t st) {
     if (T <= 0) return 0;
-    if (D <= 0 || D > ADD_NORM_MAX_D || T > 0x7fffffff || (a.norm.kind != NORM_RMS && a.norm.kind != NORM_LAYER)) return -6;
+    if (D <= 0 || D > ADD_NORM_MAX_D || (a.norm.kind != NORM_RMS && a.norm.kind != NORM_LAYER)) return -6;
     if (a.q && a.qtype != 8 && a.qtype != 15) return -3;
     if (a.q && D % (a.qtype == 8 ? 32 : QK)) return -2;
-    return D % 4 ? an_launch<true>(a, T, D, st) : an_launch<false>(a, T, D, st);
+    constexpr int64_t PASS = 1 << 21;   // rows of a launch (it covers fewer than 2^32 threads)
+    for (int64_t t = 0; t < T; t += PASS) {
+        AddNormArgs g = a;
+        g.x += t * a.ldx;
+        if (a.add) g.add += t * a.lda;
+        if (a.sum) g.sum += t * a.lds;
+        if (a.y) g.y += t * a.ldy;
+        if (a.q) g.q += t * a.ldq;
+        const int64_t n = T - t < PASS ? T - t : PASS;
+        const int rc = D % 4 ? an_launch<true>(g, n, D, st) : an_launch<false>(g, n, D, st);
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 // values of Q8_K blocks, one wave per block
@@ -262,7 +274,7 @@ __global__ void __launch_bounds__(256) k_dequantize_q8k(const uint8_t *__restric
     const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (b >= nblocks) return;
     const int lane = threadIdx.x & 63;
-    const uint8_t *p = src + 292 * b;
+    const uint8_t *p = src + Q8K_BYTES * b;
     const float d = *(const float *)p;
     const uint32_t c = *(const uint32_t *)(p + 4 + 4 * lane);
     float *o = dst + 256 * b + 4 * lane;
@@ -272,9 +284,15 @@ __global__ void __launch_bounds__(256) k_dequantize_q8k(const uint8_t *__restric
 
 int launch_dequantize_q8k(const void *src, float *dst, int64_t nblocks, hipStream_t st) {
     if (nblocks <= 0) return 0;
-    if ((nblocks + 3) / 4 > 0x7fffffff) return -6;
-    hipLaunchKernelGGL(k_dequantize_q8k, dim3((unsigned)((nblocks + 3) / 4)), dim3(256), 0, st, (const uint8_t *)src, dst, nblocks);
-    return hip_check_launch();
+    constexpr int64_t PASS = 1 << 24;   // blocks of a launch (it covers fewer than 2^32 threads)
+    for (int64_t b = 0; b < nblocks; b += PASS) {
+        const int64_t n = nblocks - b < PASS ? nblocks - b : PASS;
+        hipLaunchKernelGGL(k_dequantize_q8k, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, (const uint8_t *)src + Q8K_BYTES * b,
+                           dst + QK * b, n);
+        const int rc = hip_check_launch();
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 }  // namespace mimoe

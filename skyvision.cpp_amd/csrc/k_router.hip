@@ -281,7 +281,6 @@ int launch_route(const float *logits, int64_t ldl, int64_t T, int E, int K, cons
     if (T <= 0) return 0;
     if (E <= 0 || E > ROUTER_MAX_E || K <= 0 || K > ROUTER_MAX_K || K > E) return -6;
     if (p.n_group < 1 || p.n_group > ROUTER_MAX_GROUPS || E % p.n_group || p.n_kept < 1 || p.n_kept > p.n_group) return -6;
-    if ((T + RT_W - 1) / RT_W > 0x7fffffff) return -6;
     const int nper = E <= 64 ? 1 : E <= 128 ? 2 : E <= 256 ? 4 : E <= 512 ? 8 : 16;
     RoutePlan q;
     q.gs = E / p.n_group;
@@ -290,15 +289,21 @@ int launch_route(const float *logits, int64_t ldl, int64_t T, int E, int K, cons
     q.ls = 0;
     while (p.n_group << (q.ls + 1) <= 64) ++q.ls;
     q.vec = E % nper == 0;
-    const dim3 grid((unsigned)((T + RT_W - 1) / RT_W)), block(64 * RT_W);
-#define ROUTE(N) hipLaunchKernelGGL(k_route<N>, grid, block, 0, st, logits, ldl, T, E, K, p, q, sel, w)
-    if (nper == 1) ROUTE(1);
-    else if (nper == 2) ROUTE(2);
-    else if (nper == 4) ROUTE(4);
-    else if (nper == 8) ROUTE(8);
-    else ROUTE(16);
+    constexpr int64_t PASS = 1 << 24;   // tokens of a launch (it covers fewer than 2^32 threads)
+    for (int64_t t = 0; t < T; t += PASS) {
+        const int64_t n = T - t < PASS ? T - t : PASS;
+        const dim3 grid((unsigned)((n + RT_W - 1) / RT_W)), block(64 * RT_W);
+#define ROUTE(N) hipLaunchKernelGGL(k_route<N>, grid, block, 0, st, logits + t * ldl, ldl, n, E, K, p, q, sel + t * K, w + t * K)
+        if (nper == 1) ROUTE(1);
+        else if (nper == 2) ROUTE(2);
+        else if (nper == 4) ROUTE(4);
+        else if (nper == 8) ROUTE(8);
+        else ROUTE(16);
 #undef ROUTE
-    return hip_check_launch();
+        const int rc = hip_check_launch();
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 }  // namespace mimoe

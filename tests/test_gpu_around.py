@@ -563,3 +563,62 @@ def test_mul_mat_bits_where_the_operands_are_made_elsewhere(type_, T):
     ctx.reserve(T, 8448, 32, 1, 1)
     check_mul_mat(ctx, type_, T, 4096, 8448)
     ctx.close()
+
+
+def _spots(T, n):
+    """rows around the ends of what 2^32 threads cover, for any count of threads a row"""
+    s = {0, T - n} | {(1 << k) - n // 2 for k in range(20, 33) if (1 << k) + n // 2 <= T}
+    return sorted(s)
+
+
+def test_route_more_rows_than_a_launch_has_threads(ctx):
+    T, E, n = (1 << 26) + 29, 4, 8
+    rng = np.random.default_rng(11)
+    lg = M.DeviceBuffer(4 * T * E).zero()
+    sel, w = M.DeviceBuffer(4 * T), M.DeviceBuffer(4 * T)
+    M.call("mi_memset_d", sel.ptr, 0xFF, 4 * T)
+    rows = {s: rng.standard_normal((n, E)).astype(F32) for s in _spots(T, n)}
+    for s, l in rows.items():
+        lg.upload(l, 16 * s)
+    M.check("route", ctx.route(M.make_router(E, 1, M.SCORE_SIGMOID, renorm=False), M.tensor(lg, M.TYPE_F32, [E, T]), sel, w))
+    M.synchronize()
+    for s, l in rows.items():
+        assert np.array_equal(sel.download(np.int32, (n,), 4 * s), l.argmax(1))
+    for b in (lg, sel, w):
+        b.free()
+
+
+def test_add_norm_more_rows_than_a_launch_has_threads(ctx):
+    T, D, n = (1 << 25) + 29, 4, 8
+    rng = np.random.default_rng(12)
+    x, y = M.DeviceBuffer(4 * T * D).zero(), M.DeviceBuffer(4 * T * D)
+    M.call("mi_memset_d", y.ptr, 0xFF, 4 * T * D)
+    rows = {s: rng.standard_normal((n, D)).astype(F32) for s in _spots(T, n)}
+    for s, v in rows.items():
+        x.upload(v, 16 * s)
+    M.check("add_norm", ctx.add_norm(M.make_norm(M.NORM_RMS, 1e-6), M.tensor(x, M.TYPE_F32, [D, T]), None, None,
+                                     M.tensor(y, M.TYPE_F32, [D, T])))
+    M.synchronize()
+    for s, v in rows.items():
+        assert np.array_equal(y.download(F32, (n, D), 16 * s), A.add_norm(v, None, False, 1e-6)[1])
+    for b in (x, y):
+        b.free()
+
+
+def test_dequantize_q8_K_more_blocks_than_a_launch_has_threads(ctx):
+    n, T = 8, (1 << 26) + 29
+    try:
+        q, y = M.DeviceBuffer(292 * T).zero(), M.DeviceBuffer(1024 * T)
+    except M.MimoeError:
+        pytest.skip("88 GB of device memory")
+    rng = np.random.default_rng(13)
+    rows = {s: A.q8_bytes(rng.standard_normal((n, 256)).astype(F32), M.TYPE_Q8_K) for s in _spots(T, n)}
+    for s, v in rows.items():
+        q.upload(v, 292 * s)
+    M.check("dequantize", ctx.dequantize(M.TYPE_Q8_K, q, y, T, 256))
+    M.synchronize()
+    for s, v in rows.items():
+        d, c = v[:, :4].copy().view(F32), v[:, 4:260].view(np.int8)
+        assert np.array_equal(y.download(F32, (n, 256), 1024 * s), d * c.astype(F32))
+    for b in (q, y):
+        b.free()
