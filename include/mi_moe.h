@@ -189,10 +189,11 @@ typedef struct {
  * in fp64 and rounded to float32 once, and what is ranked are float32 numbers
  * (as the layer's gatings rank; without groups MI_SCORE_SIGMOID chooses as
  * MI_GATING_SIGMOID_BIAS, MI_SCORE_SOFTMAX as MI_GATING_SOFTMAX_ALL).  A c that
- * is NaN comes behind every number (a group's value is of its numbers; a group
- * of fewer than group_top of them comes behind the others); slots that no number
- * fills take the lowest ids not taken and the weight NaN.  -inf as a logit or
- * bias is a number (a mask); a softmax of nothing but -inf is NaN. */
+ * is NaN comes behind every number (a group's value is of its numbers: -inf with
+ * fewer than group_top of them; with none, or a sum that is none, the group comes
+ * behind the others); slots that no number fills take the lowest ids not taken and
+ * the weight NaN.  -inf as a logit or bias is a number (a mask); a softmax of
+ * nothing but -inf is NaN. */
 typedef enum {
     MI_SCORE_SOFTMAX = 0,
     MI_SCORE_SIGMOID = 1,
@@ -314,7 +315,8 @@ int mi_moe_forward_router(mi_moe_ctx *ctx, const mi_moe_layer *layer, const mi_m
 
 /* ids and weights of rows of logits (mi_moe_router): logits F32 ne=[E, T], any
  * row stride; sel I32 [T][K], weights F32 [T][K] device, not overlapping the
- * logits or each other.  The routing that mi_moe_expert_ffn takes; no workspace. */
+ * logits, the router's arrays or each other.  The routing that mi_moe_expert_ffn
+ * takes; no workspace. */
 int mi_moe_route(mi_moe_ctx *ctx, const mi_moe_router *router, const mi_tensor *logits, int32_t *sel, float *weights,
                  mi_stream_t stream);
 
@@ -329,11 +331,12 @@ int mi_norm(mi_moe_ctx *ctx, const mi_moe_norm *norm, const float *x, int64_t n_
  * followed by mi_norm's norm (sums in fp64, every other step rounded to
  * float32).  x, add, sum, y: F32 ne=[D, T] of any row stride; add NULL: h = x;
  * sum (NULL: not wanted) receives h, y (NULL: not wanted) the norm; either may
- * be x or add (data and strides alike), otherwise the outputs overlap nothing.
- * q (NULL: not wanted): y in Q8_0 (D % 32 == 0) or Q8_K (D % 256 == 0), byte for byte ggml's quantize_row of the float32 y, at any
- * row stride of whole 2 (Q8_0) or 4 (Q8_K) bytes, a block with a NaN or an
- * infinity being one of scale NaN and codes 0 - what mi_mul_mat takes.  y or q is
- * required.  No workspace. */
+ * be x or add (data and strides alike), otherwise the outputs overlap nothing, the
+ * norm's weight and bias included.
+ * q (NULL: not wanted): y in Q8_0 (D % 32 == 0) or Q8_K (D % 256 == 0), byte for
+ * byte ggml's quantize_row of the float32 y, at any row stride of whole 2 (Q8_0)
+ * or 4 (Q8_K) bytes, a block with a NaN or an infinity being one of scale NaN and
+ * codes 0 - what mi_mul_mat takes.  y or q is required.  No workspace. */
 int mi_add_norm(mi_moe_ctx *ctx, const mi_moe_norm *norm, const mi_tensor *x, const mi_tensor *add, mi_tensor *sum,
                 mi_tensor *y, mi_tensor *q, mi_stream_t stream);
 

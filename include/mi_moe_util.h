@@ -48,10 +48,12 @@ int mi_event_record(mi_event_t e, mi_stream_t s);
 int mi_event_synchronize(mi_event_t e);
 int mi_event_elapsed_ms(float *ms, mi_event_t start, mi_event_t stop);
 
-/* Stream capture into a replayable graph.  mi_moe_forward and
- * mi_moe_expert_ffn may be captured once their context is reserved: after
+/* Stream capture into a replayable graph.  mi_moe_forward, mi_moe_expert_ffn and
+ * mi_mul_mat may be captured once their context is reserved: after
  * reservation they allocate nothing, set no memory by memset, and wait on
- * nothing on the host (stage profiling, which records events, must be off).
+ * nothing on the host (stage profiling, which records events, must be off);
+ * mi_moe_route and mi_add_norm need no reservation.  Graphs of one context share
+ * its workspace: their launches go one after the other, like the calls.
  * Capture mode is relaxed; the stream must not be the null stream.
  * end_capture instantiates the captured work; a graph replays the captured
  * calls with their arguments (pointers, token count) as captured, so the

@@ -1840,6 +1840,8 @@ int mi_moe_route(mi_moe_ctx *c, const mi_moe_router *router, const mi_tensor *lo
     if (T == 0) return MI_MOE_OK;
     const Span in = rows_span(*logits), s = {sel, (size_t)(T * K) * 4}, w = {weights, (size_t)(T * K) * 4};
     if (overlap(in, s) || overlap(in, w) || overlap(s, w)) return MI_MOE_ERR_ARG;
+    for (const float *par : {router->sel_bias, router->expert_scale})
+        if (par && (overlap({par, (size_t)E * 4}, s) || overlap({par, (size_t)E * 4}, w))) return MI_MOE_ERR_ARG;
     HIP_TRY(hipSetDevice(c->device));
     return launch_route((const float *)logits->data, (int64_t)(logits->nb[1] / 4), T, (int)E, (int)K, p, sel, weights,
                         (hipStream_t)stream);
@@ -1871,6 +1873,8 @@ int mi_add_norm(mi_moe_ctx *c, const mi_moe_norm *norm, const mi_tensor *x, cons
     const mi_tensor *outs[3] = {sum, y, q}, *ins[2] = {x, add};
     for (int i = 0; i < 3; ++i) {
         if (!outs[i]) continue;
+        for (const float *par : {np.w, np.b})
+            if (par && overlap({par, (size_t)D * 4}, rows_span(*outs[i]))) return MI_MOE_ERR_ARG;
         for (int j = i + 1; j < 3; ++j)
             if (outs[j] && overlap(rows_span(*outs[i]), rows_span(*outs[j]))) return MI_MOE_ERR_ARG;
         for (const mi_tensor *in : ins) {
@@ -2107,6 +2111,8 @@ int mi_mul_mat(mi_moe_ctx *c, const mi_tensor *a, const mi_tensor *b, mi_tensor 
     if (N > 0x7fffffff || K > 0x7fffffff) return MI_MOE_ERR_UNSUPPORTED;
     if (b->type == MI_TYPE_F32) {
         if (!c->reserved || T > c->cap_rows || K > c->cap_kmax) return MI_MOE_ERR_CAPACITY;
+        // (3.2 bytes a value there; the operands of 8 rows, the fewest, take 2.3)
+        if (mm_ws_bytes(a->type, 0, T, K) > (size_t)((char *)c->aact.q8 - (char *)c->ax.q8)) return MI_MOE_ERR_CAPACITY;
     }
     if (T == 0) return MI_MOE_OK;
     const Span sa = {a->data, a->nb[1] * (size_t)(N - 1) + rs}, out = rows_span(*dst);

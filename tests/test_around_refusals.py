@@ -138,3 +138,17 @@ def test_mul_mat(ctx):
 
 def test_row_size():
     assert M.row_size(M.TYPE_Q8_K, 512) == 584 and M.row_size(M.TYPE_Q8_K, 300) == 0
+
+
+def test_outputs_on_parameters(ctx):
+    r = M.make_router(64, 4, M.SCORE_SIGMOID, sel_bias=A * 20, expert_scale=A * 30)
+    lg = f32([64, 5])
+    for at in (A * 20, A * 30):
+        assert ctx.route(r, lg, at + 252, A * 8) == ARG and ctx.route(r, lg, A * 8, at - 76) == ARG
+    n = M.make_norm(M.NORM_LAYER, 1e-6, weight=A * 20, bias=A * 30)
+    x = f32([256, 3])
+    for at in (A * 20, A * 30):
+        on = f32([256, 3], at=at + 1020)
+        assert ctx.add_norm(n, x, None, on, f32([256, 3], at=A * 4)) == ARG
+        assert ctx.add_norm(n, x, None, None, on) == ARG
+        assert ctx.add_norm(n, x, None, None, None, M.tensor(at, M.TYPE_Q8_0, [256, 3])) == ARG
