@@ -804,7 +804,9 @@ static int mm_go(const MmArgs &g, MmPlan p, hipStream_t st) {
     p.chunks = (p.nsets + p.cs - 1) / p.cs;
     const int lds = MT * p.cs * R::BYTES + red;
     const int wn = W / p.wk;
-    const int64_t want = (256 + slices - 1) / slices;   // work-groups of a slice: one a CU, which then makes or copies the operands once
+    // work-groups of a slice: one a CU, which then makes or copies the operands once,
+    // and none more (2048 x 2048 Q4_0, 700 rows: 24 a slice 49 us, 23 36; 160: 17.9, 15.0)
+    const int64_t want = slices < 256 ? 256 / slices : 1;
     const int64_t most = (p.ntiles + wn - 1) / wn;
     const dim3 grid((unsigned)(want < most ? want : most), (unsigned)slices), block(64 * W);
     hipLaunchKernelGGL((k_mm<TYPE, MT, NI>), grid, block, lds, st, g, p);
@@ -840,7 +842,7 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
     if (g.T < MM_PREP_T) return mm_go<TYPE, 1, 2>(g, p, st);
     if (g.T <= 16) return mm_go<TYPE, 1, 4>(g, p, st);
     // 32 tokens of a work-group until 64 leave three waves for every two SIMDs (8192
-    // x 2048 Q4_K: 128 rows 16.6 us against 18.4 with 64, 200 rows 31.8 against 18.9)
+    // x 2048 Q4_K: 128 rows 16.6 us against 18.4 with 64, 200 rows 31.8 against 19.5)
     if (g.T <= 32 || p.ntiles * ((g.T + 63) / 64) < 1536) return mm_go<TYPE, 2, 4>(g, p, st);
     return mm_go<TYPE, 4, 4>(g, p, st);
 }
