@@ -16,9 +16,10 @@
 // lanes' order (MM records) for the whole K where they fit, written once per
 // work-group, which then walks over row tiles: the matrix is read once per 16 to
 // 64 tokens.  Bound by the vector instructions that unpack codes and apply the
-// scales: 13 rows through 3712 x 2688 Q4_0 7.9 us (2.4 of them k_mm_rows), 200
-// rows through 8192 x 2048 Q4_K 19.7 us (340 TFLOP/s; matrix units busy 28 % of
-// k_mm's time, vector ones 40 %, the operands' way into LDS some 15 %).
+// scales: 13 rows through 3712 x 2688 Q4_0 8.0 us (2.4 of them k_mm_rows), 200
+// rows through 8192 x 2048 Q4_K 19.8 us (340 TFLOP/s; matrix units busy 28 % of
+// k_mm's time, vector instructions besides issued in 47 %, the operands' way into
+// LDS some 15 %).
 #include <type_traits>
 
 #include "b32.hpp"
@@ -753,9 +754,9 @@ static int mv_go(const MmArgs &g, hipStream_t st) {
 }
 
 // Rows of a lane: one where few, and work-groups of 16 waves, which share the
-// operands (8192 x 2048 Q4_0, one row of b: 4 waves 6.2 us, 16 4.4); more loads in
-// flight where many: two (16384 x 2048 Q4_0: 7.0 -> 6.4 us), four, as far as the
-// registers allow (65536 x 2048 Q4_0: two 23.7 us, four 21.8; 16384: 6.4 and 8.0)
+// operands (8192 x 2048 Q4_0, one row of b: 4 waves 6.2 us, 16 4.3); more loads in
+// flight where many: two (16384 x 2048 Q4_0: 7.0 -> 6.1 us), four, as far as the
+// registers allow (65536 x 2048 Q4_0 from memory: two 23.7 us, four 21.9; 16384: 6.1 and 8.0)
 template <int TYPE, int T>
 static int mv_launch(const MmArgs &g, hipStream_t st) {
     if constexpr (T <= 2)
@@ -777,9 +778,11 @@ static bool mv_ok(const MmArgs &g) {
 
 constexpr int64_t MM_PASS_T = 32768;   // rows of one pass (grid dimensions)
 // fp32 rows from so many on: their records in a launch of their own, else every
-// work-group makes them for itself (2048 x 2048 and 8192 x 2048 Q4_0: 13 rows 12.0
-// and 12.2 us, with the launch 8.5 and 11.8)
+// work-group makes them for itself (2048 columns, in the work-groups and with the
+// launch: 13 rows 2048 x Q4_0 9.5 and 8.4 us, Q4_K 9.2 and 7.6; 9 rows 8192 x Q4_0
+// 10.3 and 9.9, 32768 20.2 and 19.8)
 constexpr int64_t MM_PREP_T = 8;
+static_assert(MM_PREP_T <= 9, "NI 2 holds 8 rows");
 
 size_t mm_ws_bytes(int type, int btype, int64_t T, int64_t K) {
     if (btype != 0 || T < MM_PREP_T) return 0;
@@ -793,7 +796,7 @@ static int mm_go(const MmArgs &g, MmPlan p, hipStream_t st) {
     constexpr int W = MM_W;
     const int64_t slices = (g.T + 16 * MT - 1) / (16 * MT);
     // waves that share a row tile: the fewest that give every CU eight (8192 x 2048
-    // Q4_0, 16 rows: 9.9 us, for 16 waves 11.8; 128 rows Q4_K: 16.6 and 18.1)
+    // Q4_0, 16 rows: 9.9 us, sixteen 11.8; 128 rows Q4_K: 16.7 and 18.1)
     p.wk = 1;
     while (p.wk < (MT > 2 ? 1 : 8) && p.ntiles * slices * p.wk < 256 * 8) p.wk *= 2;
     const int red = p.wk > 1 ? 2 * W * MT * 64 * NI * 4 : 0;
@@ -842,7 +845,7 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
     if (g.T < MM_PREP_T) return mm_go<TYPE, 1, 2>(g, p, st);
     if (g.T <= 16) return mm_go<TYPE, 1, 4>(g, p, st);
     // 32 tokens of a work-group until 64 leave three waves for every two SIMDs (8192
-    // x 2048 Q4_K: 128 rows 16.6 us against 18.4 with 64, 200 rows 31.8 against 19.5)
+    // x 2048 Q4_K: 128 rows 16.7 us against 18.4 with 64, 200 rows 31.8 against 19.5)
     if (g.T <= 32 || p.ntiles * ((g.T + 63) / 64) < 1536) return mm_go<TYPE, 2, 4>(g, p, st);
     return mm_go<TYPE, 4, 4>(g, p, st);
 }

@@ -95,10 +95,10 @@ constexpr int RT_W = 4;   // waves (tokens) of a work-group
 // sortable integers; a group's value is found by 2^ls lanes from a copy in LDS
 // (groups of any size), the groups' places by counting, the experts by K rounds
 // of the wave's largest, each lane offering its best.
-// Bound by its vector instructions (some 650 a token of 256 experts, 130 of them
-// the sigmoids; 86 % of the time issued): 8192 tokens of 256 experts in 8 groups
-// 11.8 us, of 128 without groups (softmax) 7.6; the bytes alone would take 2 us.
-// One token 4.4 us: the rounds' latency.
+// Bound by its vector instructions (some 620 a token of 256 experts, 130 of them
+// the sigmoids; issued in 77 % of the CUs' time): 8192 tokens of 256 experts in 8
+// groups 12.0 us, of 128 without groups (softmax) 7.6; the bytes alone would take 2.
+// One token 4.5 us: the rounds' latency.
 template <int NPER>
 __global__ void __launch_bounds__(64 * RT_W) k_route(const float *__restrict__ logits, int64_t ldl, int64_t T, int E, int K,
                                                      RouterParams p, RoutePlan q, int32_t *__restrict__ sel, float *__restrict__ w) {
