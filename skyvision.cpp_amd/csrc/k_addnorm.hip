@@ -145,8 +145,8 @@ __device__ __forceinline__ void an_store4(float *x, int i, int D, const float (&
 // A work-group of W waves per row, thread i holding the values at 256 W k + 4 i,
 // k < P.
 // Bound by the memory: 4096 rows of 2048 with the sum and Q8_K codes, 110 MB in
-// 21 us (67 of them read, partly from the last-level cache); 4096 rows of 8192 in
-// fp32, 537 MB in 100 us (5.4 TB/s, a large copy 5.1).
+// 21 us, the inputs in the last-level cache; 4096 rows of 8192 in fp32, 537 MB in
+// 100 us (5.4 TB/s, a large copy 5.1).
 template <int W, int P, bool TAIL>
 __global__ void __launch_bounds__(64 * W) k_add_norm(AddNormArgs a, int D, double rD) {
     __shared__ double red[2][W];
