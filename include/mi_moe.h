@@ -391,7 +391,9 @@ int mi_mul_mat_id(mi_moe_ctx *ctx, const mi_tensor *as, const mi_tensor *b, cons
  * block whose Q8_0 scale leaves the fp16 range (|x| above 8.3e6) makes its dst
  * row NaN, a row of a with a scale that is not finite makes its column NaN or
  * infinite.  F32 rows use the context's workspace (mi_moe_ctx_reserve: T within
- * max_tokens * n_expert_used, K within the wider of n_embd and n_ff). */
+ * max_tokens * n_expert_used, K within the wider of n_embd and n_ff); rows in 8
+ * bits, 8 and more, use it where it holds them (without it: the same bits, up to
+ * twice the time). */
 int mi_mul_mat(mi_moe_ctx *ctx, const mi_tensor *a, const mi_tensor *b, mi_tensor *dst, mi_stream_t stream);
 
 /* ---- weight preparation ----------------------------------------------------

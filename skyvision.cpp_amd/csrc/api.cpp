@@ -2109,10 +2109,11 @@ int mi_mul_mat(mi_moe_ctx *c, const mi_tensor *a, const mi_tensor *b, mi_tensor 
     TRY(check_rows(*b, K, T));
     TRY(check_rows(*dst, N, T));
     if (N > 0x7fffffff || K > 0x7fffffff) return MI_MOE_ERR_UNSUPPORTED;
+    const size_t ws = c->reserved ? (size_t)((char *)c->aact.q8 - (char *)c->ax.q8) : 0;
     if (b->type == MI_TYPE_F32) {
         if (!c->reserved || T > c->cap_rows || K > c->cap_kmax) return MI_MOE_ERR_CAPACITY;
         // (3.2 bytes a value there; the operands of 8 rows, the fewest, take 2.3)
-        if (mm_ws_bytes(a->type, 0, T, K) > (size_t)((char *)c->aact.q8 - (char *)c->ax.q8)) return MI_MOE_ERR_CAPACITY;
+        if (mm_ws_bytes(a->type, T, K) > ws) return MI_MOE_ERR_CAPACITY;
     }
     if (T == 0) return MI_MOE_OK;
     const Span sa = {a->data, a->nb[1] * (size_t)(N - 1) + rs}, out = rows_span(*dst);
@@ -2123,6 +2124,7 @@ int mi_mul_mat(mi_moe_ctx *c, const mi_tensor *a, const mi_tensor *b, mi_tensor 
     g.b = b->data; g.btype = b->type; g.ldb = (int64_t)b->nb[1]; g.T = T;
     g.y = (float *)dst->data; g.ldy = (int64_t)(dst->nb[1] / 4);
     g.ws = c->ax.q8;
+    g.ws_bytes = ws;
     return launch_mm(g, (hipStream_t)stream);
 }
 

@@ -190,15 +190,15 @@ __device__ __forceinline__ void mm_put(const MmPiece<SRC> &r, int p, int m, uint
 }
 
 // records of a call's rows: ws + ((tile of 16 tokens) * nsets + set) * BYTES
-template <int TYPE>
+template <int TYPE, int SRC>
 __global__ void __launch_bounds__(256) k_mm_rows(const uint8_t *b, int64_t ldb, int64_t T, int K, int nsets, uint8_t *ws) {
     using R = MmRec<TYPE>;
     const int64_t t = blockIdx.y;
     const int p = blockIdx.x * 256 + threadIdx.x, set = p / (R::VALUES / 8);
     if (set >= nsets) return;   // whole sets of lanes
-    MmPiece<1> r;
-    mm_fetch<TYPE, 1, TYPE == 2>(r, b + t * ldb, p, 8 * (int64_t)p < K);
-    mm_put<TYPE, 1>(r, p, (int)(t & 15), ws + ((t >> 4) * nsets + set) * R::BYTES);
+    MmPiece<SRC> r;
+    mm_fetch<TYPE, SRC, TYPE == 2>(r, b + t * ldb, p, 8 * (int64_t)p < K);
+    mm_put<TYPE, SRC>(r, p, (int)(t & 15), ws + ((t >> 4) * nsets + set) * R::BYTES);
 }
 
 struct MmPlan {
@@ -777,15 +777,16 @@ static bool mv_ok(const MmArgs &g) {
 }
 
 constexpr int64_t MM_PASS_T = 32768;   // rows of one pass (grid dimensions)
-// fp32 rows from so many on: their records in a launch of their own, else every
-// work-group makes them for itself (2048 columns, in the work-groups and with the
-// launch: 13 rows 2048 x Q4_0 9.5 and 8.4 us, Q4_K 9.2 and 7.6; 9 rows 8192 x Q4_0
-// 10.3 and 9.9, 32768 20.2 and 19.8)
+// From so many rows on their records are written by a launch of their own, else
+// every work-group makes them for itself (2048 columns, in the work-groups and with
+// the launch: 13 fp32 rows 2048 x Q4_0 9.5 and 8.4 us, Q4_K 9.2 and 7.6; 9 rows 8192
+// x Q4_0 10.3 and 9.9, 32768 20.2 and 19.8; norm and product of 200 rows in 8 bits,
+// 8192 x Q4_K 32.7 and 22.3, 64 rows of 8192 columns, 2048 x Q4_0 50 and 23)
 constexpr int64_t MM_PREP_T = 8;
 static_assert(MM_PREP_T <= 9, "NI 2 holds 8 rows");
 
-size_t mm_ws_bytes(int type, int btype, int64_t T, int64_t K) {
-    if (btype != 0 || T < MM_PREP_T) return 0;
+size_t mm_ws_bytes(int type, int64_t T, int64_t K) {
+    if (T < MM_PREP_T) return 0;
     return type == 2 ? (size_t)((T + 15) / 16 * ((K + 127) / 128) * MmRec<2>::BYTES)
                      : (size_t)((T + 15) / 16 * (K / 256) * MmRec<12>::BYTES);
 }
@@ -833,9 +834,10 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
     p.nsets = (int)((g.K + R::VALUES - 1) / R::VALUES);
     p.ntiles = (int)((g.N + 15) / 16);
     p.src = g.btype != 0 ? 2 : 1;
-    if (g.btype == 0 && g.T >= MM_PREP_T) {
+    if (g.T >= MM_PREP_T && mm_ws_bytes(g.type, g.T, g.K) <= g.ws_bytes) {
         const dim3 grid((unsigned)((p.nsets * (R::VALUES / 8) + 255) / 256), (unsigned)g.T);
-        hipLaunchKernelGGL(k_mm_rows<TYPE>, grid, dim3(256), 0, st, (const uint8_t *)g.b, g.ldb, g.T, (int)g.K, p.nsets, (uint8_t *)g.ws);
+        hipLaunchKernelGGL((g.btype == 0 ? k_mm_rows<TYPE, 1> : k_mm_rows<TYPE, 2>), grid, dim3(256), 0, st, (const uint8_t *)g.b, g.ldb,
+                           g.T, (int)g.K, p.nsets, (uint8_t *)g.ws);
         const int rc = hip_check_launch();
         if (rc) return rc;
         p.src = 0;
@@ -843,7 +845,9 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
     // (by rows alone, not by b's type: a plan's order of sums is the same for both)
     if (g.T <= 4) return mm_go<TYPE, 1, 1>(g, p, st);
     if (g.T < MM_PREP_T) return mm_go<TYPE, 1, 2>(g, p, st);
-    if (g.T <= 16) return mm_go<TYPE, 1, 4>(g, p, st);
+    // 16 tokens of a work-group also while one round of the CUs takes all tiles (64
+    // rows: 1024 x 8192 Q4_0 14.5 us against 18.3 with 32 tokens, 512 x 4096 10.5 and 12.6)
+    if (g.T <= 16 || p.ntiles * ((g.T + 15) / 16) <= 256) return mm_go<TYPE, 1, 4>(g, p, st);
     // 32 tokens of a work-group until 64 leave three waves for every two SIMDs (8192
     // x 2048 Q4_K: 128 rows 16.7 us against 18.4 with 64, 200 rows 31.8 against 19.5)
     if (g.T <= 32 || p.ntiles * ((g.T + 63) / 64) < 1536) return mm_go<TYPE, 2, 4>(g, p, st);

@@ -536,7 +536,8 @@ int decode1_max_grid(int device, int *grid);
 
 // ---- dense products of 4-bit matrices (k_mm.hip)
 // y[t][n] = a[n] . b[t]: a Q4_0 (2) or Q4_K (12) rows, b rows as fp32 (0) or in
-// a's 8-bit form (Q8_0 = 8 / Q8_K = 15).  ws: mm_ws_bytes of workspace, 16-byte aligned.
+// a's 8-bit form (Q8_0 = 8 / Q8_K = 15).  ws: ws_bytes of workspace, 16-byte aligned;
+// less than mm_ws_bytes: the work-groups make the operands, the same bits, slower.
 struct MmArgs {
     const uint8_t *a;
     int type;
@@ -548,8 +549,9 @@ struct MmArgs {
     float *y;
     int64_t ldy;          // floats
     void *ws;
+    size_t ws_bytes;
 };
-size_t mm_ws_bytes(int type, int btype, int64_t T, int64_t K);
+size_t mm_ws_bytes(int type, int64_t T, int64_t K);
 int launch_mm(const MmArgs &g, hipStream_t st);
 
 }  // namespace mimoe

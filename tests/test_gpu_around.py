@@ -622,3 +622,32 @@ def test_dequantize_q8_K_more_blocks_than_a_launch_has_threads(ctx):
         assert np.array_equal(y.download(F32, (n, 256), 1024 * s), d * c.astype(F32))
     for b in (q, y):
         b.free()
+
+
+@pytest.mark.parametrize("type_", [M.TYPE_Q4_0, M.TYPE_Q4_K], ids=["q4_0", "q4_K"])
+@pytest.mark.parametrize("T,N,n", [(17, 2100, 512), (33, 2200, 512), (33, 2200, 5120), (100, 1000, 1024), (65, 12300, 512),
+                                   (70, 12297, 2816), (200, 6200, 768), (17, 40, 7936), (200, 52, 7168)])
+def test_mul_mat_tiles_of_rows(ctx, type_, T, N, n):
+    """16, 32 and 64 rows of b a work-group, their operands in LDS at once and in parts"""
+    check_mul_mat(ctx, type_, T, N, n)
+
+
+@pytest.mark.parametrize("type_", [M.TYPE_Q4_0, M.TYPE_Q4_K], ids=["q4_0", "q4_K"])
+@pytest.mark.parametrize("T,N,n", [(8, 4096, 8448), (9, 70, 512), (24, 100, 2048), (33, 2200, 5120), (70, 12297, 768), (16, 33, 8192)])
+def test_mul_mat_rows_in_8_bits_without_workspace(type_, T, N, n):
+    """the work-groups make the operands then: the same bits"""
+    rng = np.random.default_rng(T + N)
+    rows8 = A.q8_bytes(stream_rows(rng, T, n), EIGHT[type_])
+    a = Rows(N, n, type_, data=O.quantize(type_, (0.05 * rng.standard_normal((N, n))).astype(F32)).reshape(N, -1))
+    b = Rows(T, n, EIGHT[type_], data=rows8)
+    outs = []
+    for reserved in (False, True):
+        c = M.Context(0)
+        if reserved:
+            c.reserve(T, n, 32, 1, 1)
+        d = Rows(T, N)
+        M.check("mul_mat", c.mul_mat(a.desc, b.desc, d.desc))
+        M.synchronize()
+        outs.append(d.get())
+        c.close()
+    assert np.array_equal(*outs)
