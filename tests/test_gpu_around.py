@@ -651,3 +651,40 @@ def test_mul_mat_rows_in_8_bits_without_workspace(type_, T, N, n):
         outs.append(d.get())
         c.close()
     assert np.array_equal(*outs)
+
+
+@pytest.mark.parametrize("type_", [M.TYPE_Q4_0, M.TYPE_Q4_K], ids=["q4_0", "q4_K"])
+def test_dense_block_of_a_batch(ctx, type_):
+    """norm -> 8-bit rows -> matrix and float32 rows -> matrix, captured; other products of the same context, which
+    use the same workspace, between the replays"""
+    T, n, N = 45, 1024, 4300      # the operands in a launch of their own, 32 rows a work-group
+    rng = np.random.default_rng(8)
+    a = Rows(N, n, type_, data=O.quantize(type_, (0.05 * rng.standard_normal((N, n))).astype(F32)).reshape(N, -1))
+    x, y, q = Rows(T, n), Rows(T, n), Rows(T, n, EIGHT[type_])
+    d8, d32, other = Rows(T, N), Rows(T, N), Rows(T, N)
+    noise = Rows(T, n, data=stream_rows(rng, T, n))
+    norm = M.make_norm(M.NORM_RMS, 1e-6)
+
+    def step(st):
+        M.check("add_norm", ctx.add_norm(norm, x.desc, None, None, y.desc, q.desc, st.h))
+        M.check("mul_mat", ctx.mul_mat(a.desc, q.desc, d8.desc, st.h))
+        M.check("mul_mat", ctx.mul_mat(a.desc, y.desc, d32.desc, st.h))
+
+    st = M.Stream()
+    graph = M.Graph(st, step)
+    for i in range(4):
+        x.buf.upload(stream_rows(rng, T, n))
+        step(st)
+        st.synchronize()
+        want = d8.buf.download(F32, (T, N))
+        assert np.isfinite(want).all() and np.array_equal(want, d32.buf.download(F32, (T, N)))
+        M.check("mul_mat", ctx.mul_mat(a.desc, noise.desc, other.desc, st.h))
+        d8.buf.zero(), d32.buf.zero()
+        M.synchronize()
+        graph.launch(st)
+        M.check("mul_mat", ctx.mul_mat(a.desc, noise.desc, other.desc, st.h))
+        graph.launch(st)
+        st.synchronize()
+        assert np.array_equal(want, d8.buf.download(F32, (T, N))) and np.array_equal(want, d32.buf.download(F32, (T, N)))
+    graph.destroy()
+    st.destroy()
