@@ -33,7 +33,7 @@ mi_tensor as_mi(const Tensor *t) {
     return m;
 }
 
-// bytes of a row of n values (mi_row_size covers the expert-table types)
+// bytes of a row of n values, 0 where they are no whole blocks (mi_row_size: the types of tables and rows)
 size_t row_bytes(int type, int64_t n) {
     if (n <= 0) return 0;
     if (type == MI_TYPE_I32) return 4 * (size_t)n;
@@ -81,8 +81,10 @@ Tensor *Session::new_tensor(int type, int64_t ne0, int64_t ne1, int64_t ne2) {
     Tensor *t = new Tensor;
     t->type = type;
     t->ne[0] = ne0; t->ne[1] = ne1; t->ne[2] = ne2; t->ne[3] = 1;
-    t->nb[0] = type == MI_TYPE_F32 || type == MI_TYPE_I32 ? 4 : type == MI_TYPE_F16 ? 2 :
-               type == MI_TYPE_Q4_K || type == MI_TYPE_Q6_K ? row / (size_t)(ne0 / 256) : row / (size_t)(ne0 / 32);
+    // a block: the shortest row that the type has (1, 32 or 256 values)
+    t->nb[0] = row_bytes(type, 1);
+    if (!t->nb[0]) t->nb[0] = row_bytes(type, 32);
+    if (!t->nb[0]) t->nb[0] = row_bytes(type, 256);
     t->nb[1] = row;
     t->nb[2] = row * (size_t)ne1;
     t->nb[3] = t->nb[2] * (size_t)ne2;
