@@ -88,13 +88,13 @@ int scalar_bytes(uint32_t t) {
     }
 }
 
-// bytes of a ggml tensor of these dims (F32, F16, I32, Q4_0, Q5_0, Q8_0, Q4_K, Q6_K), 0 if not
-// one of them; UINT64_MAX if the product overflows (dims come from the file)
+// bytes of a ggml tensor of these dims (F32, F16, I32, Q4_0, Q5_0, Q8_0, Q4_K, Q6_K, MXFP4), 0 if
+// not one of them (Q8_K is a type of rows only: none is read from a file); UINT64_MAX if the product overflows (dims come from the file)
 uint64_t tensor_bytes(int32_t type, const int64_t ne[4]) {
     for (int d = 0; d < 4; ++d)
         if (ne[d] < 1) return UINT64_MAX;
     if ((uint64_t)ne[0] > ((uint64_t)1 << 40)) return UINT64_MAX;
-    const size_t row = type == MI_TYPE_I32 ? 4 * (size_t)ne[0] : mi_row_size(type, ne[0]);
+    const size_t row = type == MI_TYPE_I32 ? 4 * (size_t)ne[0] : type == MI_TYPE_Q8_K ? 0 : mi_row_size(type, ne[0]);
     if (!row) return 0;
     uint64_t n = row;
     for (int d = 1; d < 4; ++d) {

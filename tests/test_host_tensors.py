@@ -1,9 +1,10 @@
 """Tensors of the C++ host mirror (vqa::moe::Session::new_tensor) of every type a tensor can have: ggml's strides.  On the
-CPU: the mirror is compiled with an allocator of its own."""
+CPU: the mirror is compiled with an allocator of its own.  And Q8_K in GGUF files: a type of rows, not of stored tensors."""
 import pathlib
 import subprocess
 
 import mimoe as M
+from test_gguf import write_gguf
 
 ROOT = pathlib.Path(__file__).resolve().parents[1]
 PKG = ROOT / "skyvision.cpp_amd"
@@ -47,3 +48,17 @@ def test_new_tensor_strides(tmp_path):
         row = n // values * block
         assert [int(v) for v in strides] == [block, row, 5 * row, 10 * row], t
     assert got[len(kinds):] == [["none"]] * 3
+
+
+def test_gguf_q8_K_is_not_read(tmp_path):
+    """a file that holds a Q8_K tensor is as one with any type the library does not read: its size is 0, it may be cut
+    short, and the tensors beside it are there"""
+    p = tmp_path / "rows.gguf"
+    write_gguf(p, [], [("a", M.TYPE_F32, [4, 2], bytes(32)), ("rows", M.TYPE_Q8_K, [512, 3], bytes(3 * 584))])
+    for cut in (0, 100):
+        data = p.read_bytes()
+        p.write_bytes(data[:len(data) - cut])
+        g = M.Gguf(p)
+        assert g.tensor_info("rows") == (M.TYPE_Q8_K, [512, 3, 1, 1], 0)
+        assert g.tensor_info("a") == (M.TYPE_F32, [4, 2, 1, 1], 32)
+        g.close()
