@@ -209,7 +209,7 @@ Tensor *build_expert_ffn_res(Session &s, Tensor *x, Tensor *res, const std::vect
     for (const auto *r : roles)
         for (const Tensor *t : *r)
             if (t->type != (*r)[0]->type || t->ne[1] != (*r)[0]->ne[1] || t->ne[2] != 1 || t->ne[3] != 1 ||
-                !contiguous(t))
+                t->type == MI_TYPE_Q8_K || !contiguous(t))   // (Q8_K: rows, no table has them)
                 return nullptr;
     const int64_t T = x->ne[1];
     const int64_t K = (int64_t)n_used;
