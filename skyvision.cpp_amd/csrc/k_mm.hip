@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256) k_mm_rows(const uint8_t *b, int64_t ldb, 
 }
 
 struct MmPlan {
-    int src;       // operands: 0 records at ws, 1 fp32 rows, 2 rows in 8 bits
+    int src;       // operands: 0 records at ws, 1 fp32 rows (fewer than MM_PREP_T), 2 rows in 8 bits
     int nsets;     // sets of a row
     int chunks, cs;  // chunks of cs sets whose operands lie in LDS at a time
     int wk;        // waves that share a row tile, each taking every wk-th step of sets
@@ -418,8 +418,13 @@ __global__ void __launch_bounds__(64 * MM_W) k_mm(MmArgs g, MmPlan p) {
                     }
                 }
             };
-            if (p.src == 1) make(std::integral_constant<int, 1>{});
-            else make(std::integral_constant<int, 2>{});
+            // (fp32 rows from MM_PREP_T on always come as records)
+            if constexpr (NI < 4) {
+                if (p.src == 1) make(std::integral_constant<int, 1>{});
+                else make(std::integral_constant<int, 2>{});
+            } else {
+                make(std::integral_constant<int, 2>{});
+            }
         }
     };
 
@@ -841,6 +846,8 @@ static int mm_launch(const MmArgs &g, hipStream_t st) {
         const int rc = hip_check_launch();
         if (rc) return rc;
         p.src = 0;
+    } else if (g.T >= MM_PREP_T && g.btype == 0) {
+        return -4;   // (mi_mul_mat looks before: no such call comes here)
     }
     // (by rows alone, not by b's type: a plan's order of sums is the same for both)
     if (g.T <= 4) return mm_go<TYPE, 1, 1>(g, p, st);

@@ -537,7 +537,8 @@ int decode1_max_grid(int device, int *grid);
 // ---- dense products of 4-bit matrices (k_mm.hip)
 // y[t][n] = a[n] . b[t]: a Q4_0 (2) or Q4_K (12) rows, b rows as fp32 (0) or in
 // a's 8-bit form (Q8_0 = 8 / Q8_K = 15).  ws: ws_bytes of workspace, 16-byte aligned;
-// less than mm_ws_bytes: the work-groups make the operands, the same bits, slower.
+// less than mm_ws_bytes: the work-groups make the operands, the same bits, slower
+// (8 and more fp32 rows: refused, MI_MOE_ERR_CAPACITY).
 struct MmArgs {
     const uint8_t *a;
     int type;
