@@ -1,0 +1,47 @@
+"""Products of 4-bit matrices (mi_mul_mat) where their plans differ: a row's bits among other rows of the same plan, the
+kernels of few rows past what the dot products take, float32 rows in a captured step.
+
+Tolerances: _around.mul_mat's bound of a float32 sum of exact block parts; within a plan, and between eager and
+replayed calls, equal bits."""
+import numpy as np
+import pytest
+
+import _around as A
+import mimoe as M
+import pyoracle as O
+from test_gpu_around import EIGHT, F32, Rows, check_mul_mat, stream_rows
+
+pytestmark = pytest.mark.gpu
+TYPES = pytest.mark.parametrize("type_", [M.TYPE_Q4_0, M.TYPE_Q4_K], ids=["q4_0", "q4_K"])
+
+
+def products(ctx, a, type_, x, eight):
+    """rows of x through a, given in float32 or in 8 bits"""
+    T, n = x.shape
+    b = Rows(T, n, EIGHT[type_], data=A.q8_bytes(x, EIGHT[type_])) if eight else Rows(T, n, data=x)
+    d = Rows(T, a.T)
+    M.check("mul_mat", ctx.mul_mat(a.desc, b.desc, d.desc))
+    M.synchronize()
+    return d.get()
+
+
+@TYPES
+@pytest.mark.parametrize("eight", [False, True], ids=["f32", "8bit"])
+@pytest.mark.parametrize("lo,hi,N,n", [(9, 16, 200, 2048),       # 16 rows a work-group, waves share a tile of the matrix
+                                       (17, 32, 2100, 512),      # 32 rows
+                                       (33, 64, 24600, 256),     # 64 rows, a wave a tile
+                                       (65, 128, 12300, 512)])   # the same, two work-groups of rows
+def test_a_rows_bits_among_others(type_, eight, lo, hi, N, n):
+    """a row's result is the same bits in any batch of the plan: fewer rows, other rows around it, another place"""
+    ctx = M.Context(0)
+    ctx.reserve(hi, n, 32, 1, 1)
+    rng = np.random.default_rng(lo)
+    a = Rows(N, n, type_, data=O.quantize(type_, (0.05 * rng.standard_normal((N, n))).astype(F32)).reshape(N, -1))
+    x = stream_rows(rng, hi, n)
+    whole = products(ctx, a, type_, x, eight)
+    want, tol = A.mul_mat(a.view().copy(), type_, A.q8_bytes(x, EIGHT[type_]), n)
+    assert (np.abs(whole - want) <= tol).all()
+    for pick in (np.arange(lo), np.arange(hi - lo, hi), rng.permutation(hi), rng.permutation(hi)[:(lo + hi) // 2],
+                 np.repeat(rng.integers(0, hi), lo)):
+        assert np.array_equal(products(ctx, a, type_, x[pick], eight), whole[pick])
+    ctx.close()
