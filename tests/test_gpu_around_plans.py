@@ -45,3 +45,19 @@ def test_a_rows_bits_among_others(type_, eight, lo, hi, N, n):
                  np.repeat(rng.integers(0, hi), lo)):
         assert np.array_equal(products(ctx, a, type_, x[pick], eight), whole[pick])
     ctx.close()
+
+
+# rows of the matrix-unit kernel's forms of up to 4 and of up to 7 tokens: their operands are more than the dot
+# products' LDS holds (40 bytes a token and 32 values, 160 KB), or T N n is past 9 * 2^24 (Q4_0; Q4_K 9 * 2^23).  Q4_0
+# rows whose last set of 128 values holds 1, 2 or 3 blocks.
+@pytest.mark.parametrize("T,N,n,type_", [(1, 21, 131104, M.TYPE_Q4_0), (2, 37, 65600, M.TYPE_Q4_0), (3, 20, 43744, M.TYPE_Q4_0),
+                                         (4, 50, 40992, M.TYPE_Q4_0), (5, 9800, 3104, M.TYPE_Q4_0), (6, 8200, 3136, M.TYPE_Q4_0),
+                                         (7, 6900, 3168, M.TYPE_Q4_0), (5, 33, 32800, M.TYPE_Q4_0), (7, 50, 24032, M.TYPE_Q4_0),
+                                         (3, 10000, 2560, M.TYPE_Q4_K), (4, 9000, 2304, M.TYPE_Q4_K), (7, 5000, 2304, M.TYPE_Q4_K),
+                                         (6, 50, 28160, M.TYPE_Q4_K)])
+def test_few_rows_on_the_matrix_units(T, N, n, type_):
+    assert T * 40 * (n // 32) > 160 * 1024 or T * N * n > 9 << (24 if type_ == M.TYPE_Q4_0 else 23)
+    ctx = M.Context(0)
+    ctx.reserve(T, n, 32, 1, 1)
+    check_mul_mat(ctx, type_, T, N, n)
+    ctx.close()
