@@ -61,3 +61,49 @@ def test_few_rows_on_the_matrix_units(T, N, n, type_):
     ctx.reserve(T, n, 32, 1, 1)
     check_mul_mat(ctx, type_, T, N, n)
     ctx.close()
+
+
+@TYPES
+def test_float32_rows_in_a_captured_step(type_):
+    """residual + norm, then float32 rows of three tokens through two matrices (made into operands by the work-groups
+    themselves), each product kept: eager, replayed and from the same rows in 8 bits"""
+    rng = np.random.default_rng(23)
+    T, n, N = 3, 1536, 500
+    ctx = M.Context(0)
+    ctx.reserve(T, n, 32, 1, 1)
+    raw = [O.quantize(type_, (0.05 * rng.standard_normal((N, n))).astype(F32)).reshape(N, -1) for _ in range(2)]
+    mats = [Rows(N, n, type_, data=r) for r in raw]
+    x, add, s, y, q = Rows(T, n), Rows(T, n), Rows(T, n), Rows(T, n), Rows(T, n, EIGHT[type_])
+    rows = [(m, b) for m in mats for b in (s, y, q)]
+    outs = [Rows(T, N) for _ in rows]
+    norm = M.make_norm(M.NORM_RMS, 1e-5)
+
+    def step(st):
+        M.check("add_norm", ctx.add_norm(norm, x.desc, add.desc, s.desc, y.desc, q.desc, st.h))
+        for (m, b), o in zip(rows, outs):
+            M.check("mul_mat", ctx.mul_mat(m.desc, b.desc, o.desc, st.h))
+
+    st = M.Stream()
+    graph = M.Graph(st, step)
+    for i in range(4):
+        hx, ha = stream_rows(rng, T, n), stream_rows(rng, T, n)
+        x.buf.upload(hx), add.buf.upload(ha)
+        step(st)
+        st.synchronize()
+        eager = [o.buf.download(F32, (T, N)) for o in outs]
+        h, yh = A.add_norm(hx, ha, False, 1e-5)
+        for k, r in enumerate(raw):
+            for got, v in ((eager[3 * k], h), (eager[3 * k + 1], yh)):
+                want, tol = A.mul_mat(r, type_, A.q8_bytes(v, EIGHT[type_]), n)
+                assert (np.abs(got - want) <= tol).all()
+            assert np.array_equal(eager[3 * k + 1], eager[3 * k + 2])
+        for o in outs:
+            o.buf.zero()
+        M.synchronize()
+        graph.launch(st)
+        st.synchronize()
+        for o, e in zip(outs, eager):
+            assert np.array_equal(o.buf.download(F32, (T, N)), e)
+    graph.destroy()
+    st.destroy()
+    ctx.close()
