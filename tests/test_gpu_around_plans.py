@@ -107,3 +107,29 @@ def test_float32_rows_in_a_captured_step(type_):
     graph.destroy()
     st.destroy()
     ctx.close()
+
+
+@pytest.mark.parametrize("T", [1, 3, 7, 20, 70])
+def test_rows_that_mi_quantize_wrote(T):
+    """Q8_0 rows of mi_quantize: the bytes of mi_add_norm's blocks and the bits of the float32 rows' product, with blocks
+    of zeros, scales below fp16's and codes between two"""
+    rng = np.random.default_rng(T)
+    n, N = 736, 300
+    ctx = M.Context(0)
+    ctx.reserve(T, n, 32, 1, 1)
+    x = stream_rows(rng, T, n)
+    x[:, 32:64] = 0
+    x[:, 64:96] *= F32(1e-7)
+    x[:, 96:128] *= F32(1e-12)
+    x[:, 128:160] = np.arange(-15.5, 16.5)
+    x[:, 128] = 127
+    a = Rows(N, n, M.TYPE_Q4_0, data=O.quantize(M.TYPE_Q4_0, (0.05 * rng.standard_normal((N, n))).astype(F32)).reshape(N, -1))
+    b, q = Rows(T, n, data=x), Rows(T, n, M.TYPE_Q8_0)
+    M.check("quantize", ctx.quantize(M.TYPE_Q8_0, b.buf, q.buf, T, n))
+    outs = [Rows(T, N), Rows(T, N)]
+    for r, d in zip((b, q), outs):
+        M.check("mul_mat", ctx.mul_mat(a.desc, r.desc, d.desc))
+    M.synchronize()
+    assert np.array_equal(q.get(), A.q8_bytes(x, M.TYPE_Q8_0))
+    assert np.array_equal(outs[0].get(), outs[1].get())
+    ctx.close()
