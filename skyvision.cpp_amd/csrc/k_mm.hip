@@ -363,8 +363,11 @@ template <int TYPE> constexpr int MM_U = TYPE == 2 ? 2 : 1;
 // Work-group (x, y) of W waves: tokens 16 MT y .. (NI < 4: 4 NI tokens at most,
 // token t in row 4 (t / NI) + t % NI of the MFMA's), row tiles x (W / wk), +
 // gridDim.x (W / wk) ..
+// Waves of a SIMD: two (one work-group a CU).  Told two or three, the compiler
+// orders the steps of 64 tokens as it does with more registers in use (65536 x 2048,
+// 1024 rows, Q4_0 564 -> 543 us, Q4_K 375 -> 363; told two only, Q4_0 617).
 template <int TYPE, int MT, int NI>
-__global__ void __launch_bounds__(64 * MM_W) k_mm(MmArgs g, MmPlan p) {
+__global__ void __launch_bounds__(64 * MM_W) __attribute__((amdgpu_waves_per_eu(2, 3))) k_mm(MmArgs g, MmPlan p) {
     using R = MmRec<TYPE>;
     constexpr int U = MM_U<TYPE>, W = MM_W;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
