@@ -187,8 +187,11 @@ typedef struct {
  *   w[k] = s[ids[k]] [/ (sum_K s + eps)] * scaling [* expert_scale[ids[k]]]
  * Equal values: the lower id (group) first.  Every exp and sigmoid is evaluated
  * in fp64 and rounded to float32 once, and what is ranked are float32 numbers
- * (as the layer's gatings rank; without groups MI_SCORE_SIGMOID chooses as
- * MI_GATING_SIGMOID_BIAS, MI_SCORE_SOFTMAX as MI_GATING_SOFTMAX_ALL).  A c that
+ * (as the layer's gatings rank: without groups MI_SCORE_SIGMOID chooses as
+ * MI_GATING_SIGMOID_BIAS, MI_SCORE_SOFTMAX as MI_GATING_SOFTMAX_ALL.  The fp64
+ * steps are others - exp and reciprocal of their own, a softmax's sum in another
+ * order - so where an fp64 score lies within some 2^-52 of the border between two
+ * float32 numbers, a score's last bit can differ: none of 4e8 sigmoids did).  A c that
  * is NaN comes behind every number (a group's value is of its numbers: -inf with
  * fewer than group_top of them; with none, or a sum that is none, the group comes
  * behind the others); slots that no number fills take the lowest ids not taken and
@@ -390,10 +393,11 @@ int mi_mul_mat_id(mi_moe_ctx *ctx, const mi_tensor *as, const mi_tensor *b, cons
  * 2 bytes, Q8_K 4); dst overlaps neither.  A row of b with a NaN, an infinity or a
  * block whose Q8_0 scale leaves the fp16 range (|x| above 8.3e6) makes its dst
  * row NaN, a row of a with a scale that is not finite makes its column NaN or
- * infinite.  F32 rows use the context's workspace (mi_moe_ctx_reserve: T within
- * max_tokens * n_expert_used, K within the wider of n_embd and n_ff); rows in 8
- * bits, 8 and more, use it where it holds them (without it: the same bits, up to
- * twice the time). */
+ * infinite (mi_add_norm's blocks keep a NaN, mi_quantize's Q8_0 blocks do not).
+ * F32 rows need the context's reservation, one row too (mi_moe_ctx_reserve: T
+ * within max_tokens * n_expert_used, K within the wider of n_embd and n_ff), and
+ * 8 and more of them use its workspace; rows in 8 bits, 8 and more, use it where
+ * it holds them (without it: the same bits, up to twice the time). */
 int mi_mul_mat(mi_moe_ctx *ctx, const mi_tensor *a, const mi_tensor *b, mi_tensor *dst, mi_stream_t stream);
 
 /* ---- weight preparation ----------------------------------------------------

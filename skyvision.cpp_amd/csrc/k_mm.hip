@@ -2,11 +2,12 @@
 //   y[t][n] = sum over blocks of (a's block . b's block), b in a's 8-bit form.
 //   Q4_0 . Q8_0: d_a d_b sum (q - 8) c                                      (32 values)
 //   Q4_K . Q8_K: d_b (d sum_j sc_j sum_j q c - dmin sum_j m_j sum_j c)     (256, j: 32 values)
-// The sums over codes are exact integers, the blocks are added in fp32.
+// The sums over codes are exact integers (of a Q4_K block up to 63 * 15 * 127 * 256,
+// 3.07e7: rounded once on the way to fp32), the blocks are added in fp32.
 //
 // Two kernels.  k_mv (up to 8 rows of b): a lane per 32 values of whole rows of
 // the matrix on v_dot4_i32_i8, bound by the stream of the matrix: one row through
-// 65536 x 2048 Q4_K (75 MB) 16.8 us = 4.5 TB/s out of the last-level cache, 18.5 us
+// 65536 x 2048 Q4_K (75 MB) 17.0 us = 4.5 TB/s out of the last-level cache, 18.6 us
 // from memory (a large copy moves 5.1 TB/s); 2048 x 2048 3.6 us, of which the call's
 // latency is most.
 // k_mm (more): the codes' products on the int8 MFMA, whose 32 (16x16x32) or 64
@@ -16,8 +17,8 @@
 // lanes' order (MM records) for the whole K where they fit, written once per
 // work-group, which then walks over row tiles: the matrix is read once per 16 to
 // 64 tokens.  Bound by the vector instructions that unpack codes and apply the
-// scales: 13 rows through 3712 x 2688 Q4_0 8.0 us (2.4 of them k_mm_rows), 200
-// rows through 8192 x 2048 Q4_K 19.8 us (340 TFLOP/s; matrix units busy 28 % of
+// scales: 13 rows through 3712 x 2688 Q4_0 8.3 us (2.3 of them k_mm_rows), 200
+// rows through 8192 x 2048 Q4_K 19.5 us (344 TFLOP/s; matrix units busy 28 % of
 // k_mm's time, vector instructions besides issued in 47 %, the operands' way into
 // LDS some 15 %).
 #include <type_traits>
@@ -785,11 +786,12 @@ static bool mv_ok(const MmArgs &g) {
 }
 
 constexpr int64_t MM_PASS_T = 32768;   // rows of one pass (grid dimensions)
-// From so many rows on their records are written by a launch of their own, else
-// every work-group makes them for itself (2048 columns, in the work-groups and with
-// the launch: 13 fp32 rows 2048 x Q4_0 9.5 and 8.4 us, Q4_K 9.2 and 7.6; 9 rows 8192
-// x Q4_0 10.3 and 9.9, 32768 20.2 and 19.8; norm and product of 200 rows in 8 bits,
-// 8192 x Q4_K 32.7 and 22.3, 64 rows of 8192 columns, 2048 x Q4_0 50 and 23)
+// From so many rows on (8 rows: where k_mv does not take them) their records are
+// written by a launch of their own, else every work-group makes them for itself (2048
+// columns, in the work-groups and with the launch: 13 fp32 rows 2048 x Q4_0 9.5 and
+// 8.4 us, Q4_K 9.2 and 7.6; 9 rows 8192 x Q4_0 10.3 and 9.9, 32768 20.2 and 19.8; norm
+// and product of 200 rows in 8 bits, 8192 x Q4_K 32.7 and 22.3, 64 rows of 8192
+// columns, 2048 x Q4_0 50 and 23)
 constexpr int64_t MM_PREP_T = 8;
 static_assert(MM_PREP_T <= 9, "NI 2 holds 8 rows");
 
@@ -817,7 +819,9 @@ static int mm_go(const MmArgs &g, MmPlan p, hipStream_t st) {
     const int lds = MT * p.cs * R::BYTES + red;
     const int wn = W / p.wk;
     // work-groups of a slice: one a CU, which then makes or copies the operands once,
-    // and none more (2048 x 2048 Q4_0, 700 rows: 24 a slice 49 us, 23 36; 160: 17.9, 15.0)
+    // and none more (2048 x 2048 Q4_0, 700 rows: 24 a slice 49 us, 23 36; 160: 17.9, 15.0).
+    // A slice's share is a whole number: of long batches it leaves up to half the CUs
+    // idle (8192 x 2048 Q4_0: 8192 rows, 128 slices of two, 575 us; 8193, 129 of one, 1082)
     const int64_t want = slices < 256 ? 256 / slices : 1;
     const int64_t most = (p.ntiles + wn - 1) / wn;
     const dim3 grid((unsigned)(want < most ? want : most), (unsigned)slices), block(64 * W);

@@ -3,7 +3,8 @@
 // which the best are kept, top-k, renormalized weights.
 //
 //   s = fl32(1 / (1 + exp(-l))) or the softmax over all E as ggml_soft_max
-//   (e = fl32(exp(fl32(l - max))), p = e * fl32(1 / sum)), every exp in fp64;
+//   (e = fl32(exp(fl32(l - max))), p = e * fl32(1 / sum)), every exp and sum in fp64
+//   (the sum over the lanes, not in expert order);
 //   c = s + bias; a group's value: the sum of its 1 or 2 largest c; the best
 //   groups stay; K rounds of the largest c left, lowest id on ties;
 //   w = s [/ (fl32(sum of the K in fp64, slot order) + eps)] * scaling [* scale].
@@ -99,7 +100,7 @@ constexpr int RT_W = 4;   // waves (tokens) of a work-group
 // of the wave's largest, each lane offering its best.
 // Bound by its vector instructions (some 620 a token of 256 experts, 130 of them
 // the sigmoids; issued in 77 % of the CUs' time): 8192 tokens of 256 experts in 8
-// groups 12.0 us, of 128 without groups (softmax) 7.6; the bytes alone would take 2.
+// groups 12.7 us, of 128 without groups (softmax) 7.6; the bytes alone would take 2.
 // One token 4.5 us: the rounds' latency.
 template <int NPER>
 __global__ void __launch_bounds__(64 * RT_W) k_route(const float *__restrict__ logits, int64_t ldl, int64_t T, int E, int K,
